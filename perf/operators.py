@@ -229,20 +229,22 @@ def _plain(st):
 def run(state):
     if not own:
         return _plain(state)
-    from lookatmyquant_b200 import attention, embedding, orthogonal
     case = state["case"]
+    if case["op"].startswith("lookup"):
+        from lookatmyquant_b200 import embedding
+        if case["op"] == "lookup":
+            return embedding.lookup(state["table"], state["ids"], scale=state["scale"], padding_idx=state["padding"])
+        return embedding.lookup_gradient(state["dy"], state["ids"], case["V"], scale=state["scale"],
+                                         padding_idx=state["padding"])
+    if case["op"] == "newton_schulz":
+        from lookatmyquant_b200 import orthogonal
+        return orthogonal.newton_schulz(state["G"], steps=NS_STEPS, coefficients=NS_COEFFICIENTS)
+    from lookatmyquant_b200 import attention
     if case["op"] == "attention_forward":
         return attention.forward(state["q"], state["k"], state["v"], causal=case["causal"], key_start=state["start"],
                                  key_end=state["end"])
-    if case["op"] == "attention_backward":
-        return attention.backward(state["do"], state["q"], state["k"], state["v"], state["o"], state["lse"],
-                                  causal=case["causal"], key_start=state["start"], key_end=state["end"])
-    if case["op"] == "lookup":
-        return embedding.lookup(state["table"], state["ids"], scale=state["scale"], padding_idx=state["padding"])
-    if case["op"] == "lookup_gradient":
-        return embedding.lookup_gradient(state["dy"], state["ids"], case["V"], scale=state["scale"],
-                                         padding_idx=state["padding"])
-    return orthogonal.newton_schulz(state["G"], steps=NS_STEPS, coefficients=NS_COEFFICIENTS)
+    return attention.backward(state["do"], state["q"], state["k"], state["v"], state["o"], state["lse"],
+                              causal=case["causal"], key_start=state["start"], key_end=state["end"])
 
 
 def work(case):

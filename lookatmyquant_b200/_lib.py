@@ -1,4 +1,4 @@
-"""ctypes bindings to liblamq_b200.so (the C ABI declared in include/lamq_b200.h).
+"""ctypes bindings to liblamq_b200.so (the C ABI declared in include/lamq_b200.h and include/lamq_b200_train.h).
 
 The library is the product's only compute path: if it is missing or cannot load, every entry point raises — there is
 no CPU or PyTorch fallback. `torch` tensors are passed as raw device pointers on the current CUDA stream.
@@ -21,7 +21,7 @@ LAMQ_F32, LAMQ_BF16, LAMQ_F64 = 0, 1, 2
 _c = ctypes
 _P, _I64, _I32, _SZ, _D = _c.c_void_p, _c.c_int64, _c.c_int, _c.c_size_t, _c.c_double
 
-# name -> (restype, argtypes): every symbol include/lamq_b200.h declares
+# name -> (restype, argtypes): every symbol include/lamq_b200.h and include/lamq_b200_train.h declare
 SIGNATURES = {
     "lamq_abi_version": (_I32, []),
     "lamq_kernel_launches": (_c.c_uint64, []),
@@ -67,6 +67,10 @@ SIGNATURES = {
     "lamq_ldlq_rowtrellis_workspace_size": (_SZ, [_I64, _I32]),
     "lamq_ldlq_rowtrellis": (_I32, [_P, _I64, _I64, _I32, _P, _I64, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32,
                                     _P, _P, _P, _SZ, _P]),
+    "lamq_embedding_lookup": (_I32, [_P, _I32, _I64, _I64, _I32, _P, _I32, _I64, _c.c_float, _I64, _P, _I64, _P, _P]),
+    "lamq_embedding_gradient_workspace_size": (_SZ, [_I64, _I32]),
+    "lamq_embedding_gradient": (_I32, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I32, _c.c_float, _I64, _I32, _P, _I64,
+                                       _P, _SZ, _P, _P]),
 }
 
 
@@ -129,3 +133,30 @@ def ptr(t) -> int | None:
 def stream_ptr(device=None) -> int:
     import torch
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class StatusWord:
+    """One device int per GPU that an operator's kernels set on an error (a status argument of the C ABI). Calls only
+    pass it on; `check` reads it, which waits for the device."""
+
+    def __init__(self, what: str):
+        self.what = what
+        self.words = {}
+
+    def on(self, device):
+        word = self.words.get(device)
+        if word is None:
+            import torch
+            with torch.cuda.device(device):
+                word = torch.zeros(1, dtype=torch.int32, device=device)
+                torch.cuda.synchronize(device)  # zero before any stream's kernel can set it
+            self.words[device] = word
+        return word
+
+    def check(self):
+        """Raises if a kernel of any call so far set a word, and clears it."""
+        for word in self.words.values():
+            st = int(word.item())
+            if st:
+                word.zero_()
+                raise (ValueError if st == LAMQ_ERR_INVALID else LamqError)(f"{self.what} (status {st})")

@@ -36,7 +36,7 @@ def nvcc() -> str:
 
 
 def _deps(src: Path) -> list[Path]:
-    return [src] + sorted(CSRC.glob("*.cuh")) + [INCLUDE / "lamq_b200.h"]
+    return [src] + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
 
 
 def _stale(obj: Path, src: Path) -> bool:

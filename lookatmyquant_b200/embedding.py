@@ -10,13 +10,17 @@ zero rows to whole runs of 256 and dropped after. The compute runs in liblamq_b2
 Hadamard factors (lamq_rht_rows), the environment (lamq_env_factor), the column-trellis sweep (lamq_ldlq_coltrellis)
 or the Viterbi (lamq_viterbi). `lm`/`ter` scalar-code buckets and sliced (per-layer-input) tables are not on this
 path and raise NotImplementedError.
+
+A training step's side of a table is here too: `lookup` (rows by token id, scaled), `lookup_gradient` (the table's
+gradient, summed in the tokens' order: bit-reproducible) and `scaled_embedding`, the two under autograd.
 """
 
 from __future__ import annotations
 
 import torch
 
-from . import codes
+from . import _lib, codes
+from ._lib import check, ptr, stream_ptr
 from .quantize import Dense, parse
 from .rotation import Rotation
 
@@ -92,3 +96,103 @@ def quantize_embedding(E: torch.Tensor, spec: dict, H: torch.Tensor | None, orde
         bits += net.rate_bits()
         lo += size
     return bits, E.numel()
+
+
+_STATUS = _lib.StatusWord("embedding ids outside the table")
+_DTYPES = {torch.float32: _lib.LAMQ_F32, torch.bfloat16: _lib.LAMQ_BF16}
+
+
+def check_status():
+    """Raises ValueError if a lookup or gradient so far met an id outside its table (its row is taken as zero). Waits
+    for the device."""
+    _STATUS.check()
+
+
+def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
+    if x.dtype not in _DTYPES or not x.is_cuda:
+        raise TypeError(f"{what} must be a float32 or bfloat16 CUDA tensor")
+    if x.stride(-1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        x = x.contiguous()
+    return x
+
+
+def _ids(ids: torch.Tensor, device) -> torch.Tensor:
+    if ids.dtype not in (torch.int64, torch.int32) or ids.device != device:
+        raise TypeError("ids must be an int64 or int32 tensor on the table's device")
+    return ids if ids.is_contiguous() else ids.contiguous()
+
+
+def _padding(padding_idx: int | None, rows: int) -> int:
+    if padding_idx is None:
+        return -1
+    if not 0 <= padding_idx < rows:
+        raise ValueError(f"padding_idx {padding_idx} outside the table's {rows} rows")
+    return padding_idx
+
+
+def lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None) -> torch.Tensor:
+    """scale · table[ids] (ids of any shape; table V x d fp32 or bf16; the result in the table's type, the product in
+    fp32). Tokens with id `padding_idx` get zero rows. An id outside the table gets a zero row and is reported by
+    `check_status()`."""
+    if table.ndim != 2:
+        raise ValueError("the table must be a matrix")
+    table = _matrix(table, "the table")
+    dev = table.device
+    ids = _ids(ids, dev)
+    V, d = table.shape
+    out = torch.empty(*ids.shape, d, dtype=table.dtype, device=dev)
+    with torch.cuda.device(dev):
+        check(_lib.load().lamq_embedding_lookup(
+            ptr(table), _DTYPES[table.dtype], max(table.stride(0), d), V, d, ptr(ids), ids.dtype == torch.int64,
+            ids.numel(), scale, _padding(padding_idx, V), ptr(out), d, ptr(_STATUS.on(dev)),
+            stream_ptr(dev)), "lamq_embedding_lookup")
+    return out
+
+
+def lookup_gradient(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: float = 1.0,
+                    padding_idx: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of `lookup` in a table of `rows` rows: row v is scale · the sum of `grad` (ids.shape + (d,), fp32
+    or bf16) over the tokens with id v, in fp32, rounded once to grad's type. With `out` (rows x d, grad's type) the
+    gradient is added to it and rows without a token are left alone. Equal calls give equal bits."""
+    if grad.shape[:-1] != ids.shape or grad.ndim < 1:
+        raise ValueError(f"one gradient row per id: gradient {tuple(grad.shape)}, ids {tuple(ids.shape)}")
+    if rows < 0:
+        raise ValueError("rows must not be negative")
+    d = grad.shape[-1]
+    grad = _matrix(grad.reshape(-1, d), "the gradient")
+    dev = grad.device
+    ids = _ids(ids, dev)
+    accumulate = out is not None
+    if accumulate:
+        if out.shape != (rows, d) or out.dtype != grad.dtype or out.device != dev or out.stride(-1) != 1 or (
+                rows > 1 and out.stride(0) < d):
+            raise ValueError(f"out must be a {rows} x {d} {grad.dtype} matrix with contiguous rows on {dev}")
+    else:
+        out = torch.empty(rows, d, dtype=grad.dtype, device=dev)
+    lib = _lib.load()
+    n = ids.numel()
+    ws = torch.empty(lib.lamq_embedding_gradient_workspace_size(n, d), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        check(lib.lamq_embedding_gradient(
+            ptr(grad), _DTYPES[grad.dtype], max(grad.stride(0), d), ptr(ids), ids.dtype == torch.int64, n, rows, d,
+            scale, _padding(padding_idx, rows), accumulate, ptr(out), max(out.stride(0), d), ptr(ws),
+            ws.numel(), ptr(_STATUS.on(dev)), stream_ptr(dev)), "lamq_embedding_gradient")
+    return out
+
+
+class _ScaledEmbedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, ids, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.rows, ctx.scale, ctx.padding_idx = table.shape[0], scale, padding_idx
+        return lookup(table, ids, scale, padding_idx)
+
+    @staticmethod
+    def backward(ctx, grad):
+        (ids,) = ctx.saved_tensors
+        return lookup_gradient(grad, ids, ctx.rows, ctx.scale, ctx.padding_idx), None, None, None
+
+
+def scaled_embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None):
+    """`lookup` under autograd: the table's gradient is `lookup_gradient`."""
+    return _ScaledEmbedding.apply(table, ids, float(scale), padding_idx)

@@ -1,0 +1,74 @@
+"""The training operators' C ABI (include/lamq_b200_train.h): every declared symbol is exported and bound, arguments
+are checked before the device is touched, and empty inputs are a successful no-op (no GPU needed)."""
+
+import re
+from pathlib import Path
+
+import pytest
+
+from lookatmyquant_b200 import _lib
+from lookatmyquant_b200.build import LIB, build
+
+HEADER = Path(__file__).resolve().parents[1] / "include" / "lamq_b200_train.h"
+N, P = None, 4096  # P: a non-null pointer that the checks never dereference
+
+
+def declared():
+    text = re.sub(r"/\*.*?\*/", "", HEADER.read_text(), flags=re.S)
+    return sorted(set(re.findall(r"\b(lamq_[a-z0-9_]+)\s*\(", text)))
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not LIB.exists():
+        build()
+    return _lib.load()
+
+
+INVALID = [
+    ("lamq_embedding_lookup", (P, 0, 4, 10, 8, P, 1, 5, 1.0, -1, P, 8, P, N), b"bad shape"),
+    ("lamq_embedding_lookup", (P, 2, 8, 10, 8, P, 1, 5, 1.0, -1, P, 8, P, N), b"dtype"),
+    ("lamq_embedding_lookup", (P, 0, 8, 10, 8, N, 1, 5, 1.0, -1, P, 8, P, N), b"null pointer"),
+    ("lamq_embedding_lookup", (P, 0, 8, 10, 8, P, 1, 5, 1.0, -1, P, 8, N, N), b"null pointer"),
+    ("lamq_embedding_lookup", (P, 0, 8, 10, 8, P, 1, 2**40, 1.0, -1, P, 8, P, N), b"too many tokens"),
+    ("lamq_embedding_gradient", (P, 0, 8, P, 1, -1, 10, 8, 1.0, -1, 0, P, 8, P, 0, P, N), b"bad shape"),
+    ("lamq_embedding_gradient", (P, 7, 8, P, 1, 4, 10, 8, 1.0, -1, 0, P, 8, P, 0, P, N), b"dtype"),
+    ("lamq_embedding_gradient", (P, 0, 8, P, 1, 2**33, 10, 8, 1.0, -1, 0, P, 8, P, 0, P, N), b"more than 2^31"),
+    ("lamq_embedding_gradient", (N, 0, 8, P, 1, 4, 10, 8, 1.0, -1, 0, P, 8, P, 0, P, N), b"null pointer"),
+    ("lamq_embedding_gradient", (P, 0, 8, P, 1, 4, 10, 8, 1.0, -1, 0, P, 8, P, 16, P, N), b"workspace"),
+]
+
+EMPTY = [
+    ("lamq_embedding_lookup", (N, 0, 8, 10, 8, N, 1, 0, 1.0, -1, N, 8, N, N)),
+    ("lamq_embedding_gradient", (N, 0, 8, N, 1, 4, 0, 8, 1.0, -1, 0, N, 8, N, 0, N, N)),
+]
+
+
+def test_every_declared_symbol_is_exported(lib):
+    for name in declared():
+        assert hasattr(lib, name) and name in _lib.SIGNATURES, name
+
+
+@pytest.mark.parametrize("name,args,text", INVALID, ids=[f"{c[0]}-{i}" for i, c in enumerate(INVALID)])
+def test_entry_point_rejects_bad_arguments(lib, name, args, text):
+    before = lib.lamq_kernel_launches()
+    assert getattr(lib, name)(*args) == _lib.LAMQ_ERR_INVALID
+    assert text in lib.lamq_last_error()
+    assert lib.lamq_kernel_launches() == before
+
+
+@pytest.mark.parametrize("name,args", EMPTY, ids=[f"{c[0]}-{i}" for i, c in enumerate(EMPTY)])
+def test_entry_point_accepts_empty_input(lib, name, args):
+    before = lib.lamq_kernel_launches()
+    assert getattr(lib, name)(*args) == _lib.LAMQ_OK
+    assert lib.lamq_kernel_launches() == before
+
+
+def test_tables_cover_every_compute_entry_point():
+    compute = {n for n in declared() if not n.endswith("_workspace_size")}
+    assert compute <= {c[0] for c in INVALID} & {c[0] for c in EMPTY}
+
+
+def test_gradient_workspace_size(lib):
+    assert lib.lamq_embedding_gradient_workspace_size(0, 64) == 0
+    assert lib.lamq_embedding_gradient_workspace_size(100, 64) >= 4 * 400 + 2 * 13 * 64 * 4

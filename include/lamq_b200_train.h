@@ -36,6 +36,55 @@ int lamq_embedding_gradient(const void *dy, int dtype, int64_t ldy, const void *
                             int d, float scale, int64_t padding, int accumulate, void *dE, int64_t lde, void *workspace,
                             size_t workspace_bytes, int *status, lamq_stream_t stream);
 
+/*
+ * A (batch, heads, length, head_dim) bf16 tensor: its first element (16-byte aligned) and the strides in elements of
+ * the first three axes (positive multiples of 8 where the axis has more than one entry; head_dim is contiguous).
+ */
+typedef struct lamq_heads {
+    void *data;
+    int64_t batch, head, row;
+} lamq_heads;
+
+/*
+ * The operands of an attention call. Query head h reads key head h / (heads / kv_heads). Query i of text b sees the
+ * keys j with key_start[b] <= j < key_end[b] (device int32 arrays of `batch` entries, clamped to [0, kv_len); NULL:
+ * from 0, to kv_len) and, with causal != 0, j <= i + kv_len − q_len (the last query sees the last key). head_dim is a
+ * multiple of 8 up to 128; lengths are arbitrary, zero included. q, k, v: read. o and lse (batch x heads x q_len fp32,
+ * contiguous): written by the forward, read by the backward. d_o is read and dq, dk, dv are written by the backward
+ * only. Outputs are written whole and overlap no input. 328 bytes, no padding (`reserved` is ignored).
+ */
+typedef struct lamq_attention_args {
+    int64_t batch;
+    int heads, kv_heads, head_dim, causal;
+    int64_t q_len, kv_len;
+    float scale;
+    int reserved;
+    const int32_t *key_start, *key_end;
+    lamq_heads q, k, v, o;
+    float *lse;
+    lamq_heads d_o, dq, dk, dv;
+} lamq_attention_args;
+
+/*
+ * o = softmax(scale·q·kᵀ)·v over each query's allowed keys (bf16, the softmax in fp32) and lse, the natural logarithm
+ * of the sum of exponentials. A query without a key gets o = 0 and lse = −inf. Keys outside a text's range are not
+ * used, whatever they hold; a NaN or infinity inside it spreads to the queries of its tile, as in a matrix product.
+ * *status becomes LAMQ_ERR_TIMEOUT if a bounded device wait gives up. `args` is host memory, read before the call
+ * returns.
+ */
+int lamq_attention_forward(const lamq_attention_args *args, int *status, lamq_stream_t stream);
+
+/*
+ * The gradients of lamq_attention_forward from d_o, recomputing the probabilities from q, k and lse (o and lse as the
+ * forward wrote them): dq, dk, dv (bf16, summed in fp32; a key head's gradient is the sum over its query heads).
+ * Queries without a key get a zero gradient and add none, whatever their rows of q and d_o hold; keys that no query
+ * sees get zeros. Every sum has a fixed order: equal calls give equal bits. Workspace:
+ * lamq_attention_backward_workspace_size(batch, heads, q_len) bytes, 16-byte aligned.
+ */
+size_t lamq_attention_backward_workspace_size(int64_t batch, int heads, int64_t q_len);
+int lamq_attention_backward(const lamq_attention_args *args, void *workspace, size_t workspace_bytes, int *status,
+                            lamq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,7 @@ no CPU or PyTorch fallback. `torch` tensors are passed as raw device pointers on
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -71,7 +72,14 @@ SIGNATURES = {
     "lamq_embedding_gradient_workspace_size": (_SZ, [_I64, _I32]),
     "lamq_embedding_gradient": (_I32, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I32, _c.c_float, _I64, _I32, _P, _I64,
                                        _P, _SZ, _P, _P]),
+    "lamq_attention_forward": (_I32, [_P, _P, _P]),
+    "lamq_attention_backward_workspace_size": (_SZ, [_I64, _I32, _I64]),
+    "lamq_attention_backward": (_I32, [_P, _P, _SZ, _P, _P]),
 }
+
+# lamq_attention_args (328 bytes): batch; heads, kv_heads, head_dim, causal; q_len, kv_len; scale, reserved; key_start,
+# key_end; q, k, v, o; lse; d_o, dq, dk, dv (a lamq_heads is a pointer and three strides)
+ATTENTION_ARGS = struct.Struct("=q4i2qfi2Q16qQ16q")
 
 
 class ProductGroup(_c.Structure):

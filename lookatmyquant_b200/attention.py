@@ -1,0 +1,155 @@
+"""Attention for training steps on B200 (liblamq_b200: lamq_attention_forward, lamq_attention_backward).
+
+The model passes this package runs gradients through (importance.row_importance, importance.guided_weights, and a
+fine-tuning step around trellis-coded matrices) spend their attention here: `forward` keeps, beside the output, one
+number per query (lse, the logarithm of the sum of exponentials); `backward` recomputes the probabilities from it, so
+that nothing of size queries x keys is ever stored. `attention` is the two under autograd, and `use_in_transformers`
+makes it an attention implementation of Hugging Face models ("lamq").
+
+Tensors are (batch, heads, length, head_dim) bf16 views with contiguous head_dim (a projection's (batch, length, heads,
+head_dim) output transposed is read in place); outputs come in that memory order too. Heads may be shared: query head h
+reads key head h // (heads // kv_heads). Query i of text b sees keys key_start[b] <= j < key_end[b] and, when causal,
+j <= i + kv_len - q_len. A query that sees no key gives a zero output, lse -inf and no gradient.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._lib import ATTENTION_ARGS, check, ptr, stream_ptr
+
+_STATUS = _lib.StatusWord("attention")
+
+
+def check_status():
+    """Raises if a kernel of any call so far gave up on a device wait (its results are then invalid). Waits for the
+    device."""
+    _STATUS.check()
+
+
+def _heads(x: torch.Tensor, what: str) -> torch.Tensor:
+    if x.dtype != torch.bfloat16 or not x.is_cuda:
+        raise TypeError(f"{what} must be a bfloat16 CUDA tensor")
+    if x.ndim != 4:
+        raise ValueError(f"{what} must be (batch, heads, length, head_dim)")
+    if x.numel() and (x.stride(3) != 1 or x.data_ptr() % 16 or
+                      any(n > 1 and (s % 8 or s <= 0) for n, s in zip(x.shape[:3], x.stride()[:3]))):
+        x = x.contiguous()
+    return x
+
+
+def _like_projection(B: int, H: int, L: int, D: int, device) -> torch.Tensor:
+    """An empty (B, H, L, D) tensor in the memory order of a projection's (B, L, H·D) output."""
+    return torch.empty(B, L, H, D, dtype=torch.bfloat16, device=device).transpose(1, 2)
+
+
+def _bounds(x: torch.Tensor | None, what: str, batch: int, device):
+    if x is None:
+        return None
+    if x.dtype != torch.int32 or x.device != device or x.shape != (batch,):
+        raise ValueError(f"{what} must be an int32 tensor of {batch} entries on {device}")
+    return x.contiguous()
+
+
+def _pack(x: torch.Tensor | None):
+    if x is None:
+        return (0, 0, 0, 0)
+    s = x.stride()
+    return (x.data_ptr(), s[0], s[1], s[2])
+
+
+def _shapes(q, k, v, scale):
+    B, Hq, Lq, D = q.shape
+    Hkv, Lk = k.shape[1], k.shape[2]
+    if k.shape != (B, Hkv, Lk, D) or v.shape != k.shape or k.device != q.device or v.device != q.device:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    return B, Hq, Hkv, D, Lq, Lk, D ** -0.5 if scale is None else float(scale)
+
+
+def forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None, causal: bool = True,
+            key_start: torch.Tensor | None = None, key_end: torch.Tensor | None = None):
+    """softmax(scale·q·kᵀ)·v over each query's keys (scale: head_dim^-1/2 by default): (output, lse), the output bf16
+    like q and lse (batch, heads, q length) fp32."""
+    q, k, v = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
+    B, Hq, Hkv, D, Lq, Lk, scale = _shapes(q, k, v, scale)
+    dev = q.device
+    start, end = _bounds(key_start, "key_start", B, dev), _bounds(key_end, "key_end", B, dev)
+    o = _like_projection(B, Hq, Lq, D, dev)
+    lse = torch.empty(B, Hq, Lq, dtype=torch.float32, device=dev)
+    none = (0,) * 16
+    args = ATTENTION_ARGS.pack(B, Hq, Hkv, D, causal, Lq, Lk, scale, 0, ptr(start) or 0, ptr(end) or 0, *_pack(q),
+                               *_pack(k), *_pack(v), *_pack(o), lse.data_ptr(), *none)
+    with torch.cuda.device(dev):
+        check(_lib.load().lamq_attention_forward(args, ptr(_STATUS.on(dev)), stream_ptr(dev)),
+              "lamq_attention_forward")
+    return o, lse
+
+
+def backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor,
+             scale: float | None = None, causal: bool = True, key_start: torch.Tensor | None = None,
+             key_end: torch.Tensor | None = None):
+    """(dq, dk, dv) of `forward` for the output's gradient `do`, with the o and lse that `forward` returned for the
+    same q, k, v, scale, causal and key ranges. Equal calls give equal bits."""
+    q, k, v, o, do = _heads(q, "q"), _heads(k, "k"), _heads(v, "v"), _heads(o, "o"), _heads(do, "do")
+    B, Hq, Hkv, D, Lq, Lk, scale = _shapes(q, k, v, scale)
+    dev = q.device
+    if o.shape != q.shape or do.shape != q.shape or o.device != dev or do.device != dev:
+        raise ValueError(f"o {tuple(o.shape)} and do {tuple(do.shape)} must be like q {tuple(q.shape)}")
+    if lse.shape != (B, Hq, Lq) or lse.dtype != torch.float32 or lse.device != dev:
+        raise ValueError(f"lse must be a float32 tensor of shape {(B, Hq, Lq)}")
+    lse = lse.contiguous()
+    start, end = _bounds(key_start, "key_start", B, dev), _bounds(key_end, "key_end", B, dev)
+    dq, dk, dv = (_like_projection(B, H, L, D, dev) for H, L in ((Hq, Lq), (Hkv, Lk), (Hkv, Lk)))
+    lib = _lib.load()
+    ws = torch.empty(lib.lamq_attention_backward_workspace_size(B, Hq, Lq), dtype=torch.uint8, device=dev)
+    args = ATTENTION_ARGS.pack(B, Hq, Hkv, D, causal, Lq, Lk, scale, 0, ptr(start) or 0, ptr(end) or 0, *_pack(q),
+                               *_pack(k), *_pack(v), *_pack(o), lse.data_ptr(), *_pack(do), *_pack(dq), *_pack(dk),
+                               *_pack(dv))
+    with torch.cuda.device(dev):
+        check(lib.lamq_attention_backward(args, ptr(ws), ws.numel(), ptr(_STATUS.on(dev)), stream_ptr(dev)),
+              "lamq_attention_backward")
+    return dq, dk, dv
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, scale, causal, key_start, key_end):
+        o, lse = forward(q, k, v, scale, causal, key_start, key_end)
+        ctx.save_for_backward(q, k, v, o, lse, key_start, key_end)
+        ctx.scale, ctx.causal = scale, causal
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        q, k, v, o, lse, start, end = ctx.saved_tensors
+        return (*backward(do, q, k, v, o, lse, ctx.scale, ctx.causal, start, end), None, None, None, None)
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None, causal: bool = True,
+              key_start: torch.Tensor | None = None, key_end: torch.Tensor | None = None) -> torch.Tensor:
+    """`forward`'s output under autograd: its gradients are `backward`'s."""
+    return _Attention.apply(q, k, v, scale, causal, key_start, key_end)
+
+
+def _transformers_attention(module, query, key, value, attention_mask, scaling=None, dropout=0.0, **kwargs):
+    if attention_mask is not None or dropout:
+        raise NotImplementedError("the lamq attention takes whole windows: no mask and no dropout")
+    causal = getattr(module, "is_causal", True)
+    return attention(query, key, value, scaling, causal).transpose(1, 2), None
+
+
+def use_in_transformers(name: str = "lamq") -> str:
+    """Registers `attention` with Hugging Face transformers under `name` (returned): a model whose config has
+    `_attn_implementation = name` runs its attention forwards and backwards on these kernels. Windows are whole (no
+    padding mask); bf16 models."""
+    from transformers import AttentionInterface, AttentionMaskInterface
+    AttentionInterface.register(name, _transformers_attention)
+    AttentionMaskInterface.register(name, _no_mask)
+    return name
+
+
+def _no_mask(*args, attention_mask=None, **kwargs):
+    if attention_mask is not None and not bool(attention_mask.all()):
+        raise NotImplementedError("the lamq attention takes whole windows: no padding")
+    return None

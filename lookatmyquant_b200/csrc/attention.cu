@@ -1,0 +1,1062 @@
+// Attention of a training step on tcgen05: the forward, which keeps one number per query (lse), and the backward, which
+// recomputes the probabilities from it.
+//
+//   S_ij = scale · q_i·k_j over the allowed pairs (keys of the text's range; j <= i + Lk − Lq when causal),
+//   lse_i = log Σ_j exp S_ij,  P_ij = exp(S_ij − lse_i),  O = P·V          (a row without a key: O = 0, lse = −inf)
+//   D_i = Σ_d dO_id·O_id,  dV = Pᵀ·dO,  dS = P ∘ (dO·Vᵀ − D),  dQ = scale·dS·K,  dK = scale·dSᵀ·Q
+//
+// Nothing of size Lq x Lk is written. bf16 operands, fp32 accumulators in TMEM; the softmax's maximum, sum, lse, D and
+// dS are fp32, and P and dS are rounded to bf16 once, as operands of the second product (the precision of the inputs).
+//
+// forward: a CTA takes two tiles of 128 queries over the keys in tiles of 128; each tile has a warpgroup (a thread per
+// query row), so one tile's softmax runs while the tensor core works for the other. P goes back to TMEM as the A operand
+// of P·V. O is rescaled only when a row's maximum grows by more than 2^8.
+// backward: two kernels, so that every sum has one writer and one order (no atomics; equal calls give equal bits):
+//   dq: a CTA per 128 queries walks the keys and sums dS·K in TMEM;
+//   dkv: a CTA per 128 keys walks the queries of every head of its group and sums Pᵀ·dO and dSᵀ·Q in TMEM, so a shared
+//        K/V head's gradient needs no join. It computes Sᵀ and dPᵀ (keys as rows): Pᵀ and dSᵀ come out as A operands.
+//   The recomputation of S and dP in both costs two of seven products, against a dQ of fp32 sums in memory.
+// A first small kernel computes D and stores lse and D by padded rows (lse = +inf where there is no row: P = 0).
+//
+// Rows of K, V, Q or dO that no allowed pair touches (outside a text's key range; queries before its first key) are
+// zeroed in shared memory before a product would sum over them, so what they hold (NaN included) reaches nothing.
+//
+// Warp roles (320 threads): warp 0 issues TMA loads, warp 1 the MMAs, warps 2-9 the elementwise work. One thread issues
+// all MMAs of a CTA and the tensor core runs them in issue order, so a product may overwrite TMEM that the product
+// issued before it reads.
+#include <algorithm>
+#include <climits>
+#include <mutex>
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include "../../include/lamq_b200_train.h"
+#include "lamq_common.cuh"
+#include "sm100.cuh"
+
+namespace lamq {
+namespace {
+
+using namespace sm100;
+
+constexpr int kTile = 128;
+constexpr int kThreads = 320;
+constexpr uint32_t kTmemCols = 512;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct Rows {  // where a thread writes: element (b, h, row, 0) of a (B, H, L, D) tensor
+    __nv_bfloat16 *p;
+    int64_t batch, head, row;
+};
+
+struct Shape {
+    int B, Hq, Hkv, group, D;
+    int Lq, Lk, off;  // off = Lk − Lq
+    int lq_pad;       // Lq rounded up to whole tiles
+    int causal;
+    float scale, sl;  // sl = scale·log2 e
+    const int32_t *ks, *ke;
+    int *status;
+};
+
+template <int HD>
+struct Sizes {
+    static constexpr int NC = HD / 64;                  // 64-wide chunks of a row
+    static constexpr int CHUNK = kTile * 128;           // bytes of a chunk of 128 rows
+    static constexpr int TILE = NC * CHUNK;             // bytes of a 128 x HD tile
+    static constexpr int FWD_STAGES = HD == 128 ? 4 : 6;
+    static constexpr int BWD_STAGES = 2;
+    static constexpr int ROWSTATS = 2 * kTile * 4;      // lse and D of a query tile
+    static constexpr size_t FWD_SMEM = 1024 + 2 * TILE + FWD_STAGES * TILE + 256;
+    static constexpr size_t DQ_SMEM = 1024 + 2 * TILE + 2 * BWD_STAGES * TILE + 256;
+    static constexpr size_t DKV_SMEM = 1024 + 2 * TILE + BWD_STAGES * (2 * TILE + ROWSTATS) + 256;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ void key_range(const Shape &s, int b, int &lo, int &hi) {
+    lo = s.ks ? max(0, s.ks[b]) : 0;
+    hi = s.ke ? min(s.Lk, s.ke[b]) : s.Lk;
+    if (lo >= hi) lo = hi = 0;
+}
+
+// A tile of 128 rows from row `row` of head (b, h): NC boxes of 64 x 128, zero past the tensor's end.
+template <int HD>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap *map, int row, int h, int b, uint32_t bar) {
+#pragma unroll
+    for (int c = 0; c < Sizes<HD>::NC; ++c) tma_load_4d(dst + c * Sizes<HD>::CHUNK, map, 64 * c, row, h, b, bar);
+}
+
+// D (+)= A·Bᵀ over HD, both tiles 128 x HD (K-major).
+template <int HD>
+__device__ __forceinline__ void mma_rows_rows(uint32_t d, uint32_t a, uint32_t b) {
+    constexpr uint32_t idesc = idesc_bf16_f32(kTile, kTile, false, false);
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk) {
+        const uint32_t at = (kk / 4) * Sizes<HD>::CHUNK + (kk % 4) * 32;
+        mma_f16_ss(d, smem_desc_sw128(a + at, 16, 1024), smem_desc_sw128(b + at, 16, 1024), idesc, kk > 0);
+    }
+}
+
+// D (+)= A·B, A 128 x 128 bf16 in TMEM (its columns 64.. from a + hi_cols), B a tile of 128 rows x HD.
+template <int HD>
+__device__ __forceinline__ void mma_tmem_rows(uint32_t d, uint32_t a, uint32_t hi_cols, uint32_t b, bool accumulate) {
+    constexpr uint32_t idesc = idesc_bf16_f32(kTile, HD, false, true);
+#pragma unroll
+    for (int kk = 0; kk < kTile / 16; ++kk) {
+        const uint32_t at = a + (kk < 4 ? kk * 8 : hi_cols + (kk - 4) * 8);
+        mma_f16_ts(d, at, smem_desc_sw128(b + kk * 2048, Sizes<HD>::CHUNK, 1024), idesc, accumulate || kk > 0);
+    }
+}
+
+// A warp zeroes the rows of a tile outside [lo, hi) (whole rows: the swizzle stays inside a row).
+template <int HD>
+__device__ __forceinline__ void zero_rows(uint32_t tile, int lo, int hi) {
+    const int lane = threadIdx.x & 31;
+    for (int i = lane; i < Sizes<HD>::NC * kTile * 8; i += 32) {
+        const int row = (i >> 3) & (kTile - 1);
+        if (row < lo || row >= hi)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + i * 16), "r"(0) : "memory");
+    }
+    fence_async_smem();
+    __syncwarp();
+}
+
+__device__ __forceinline__ void wait_bounded(uint32_t bar, uint32_t parity) {
+    const unsigned long long t0 = globaltimer();
+    while (!mbar_try_wait(bar, parity) && globaltimer() - t0 < kWaitTimeoutNs) {
+    }
+}
+
+__device__ __forceinline__ uint8_t *align_smem(uint8_t *p) {
+    return reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(p) + 1023) & ~uintptr_t(1023));
+}
+
+// A thread's row of an accumulator, times `f`, as bf16 (cols < D; D is a multiple of 8).
+template <int COLS>
+__device__ __forceinline__ void store_row(__nv_bfloat16 *dst, uint32_t taddr, int col0, int D, float f, bool live) {
+#pragma unroll
+    for (int c = 0; c < COLS; c += 32) {
+        uint32_t r[32];
+        tmem_load32(taddr + c, r);
+        tmem_ld_wait();
+        if (!live) continue;
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+            if (col0 + c + e >= D) break;
+            uint4 v;
+            v.x = pack_bf16(__uint_as_float(r[e]) * f, __uint_as_float(r[e + 1]) * f);
+            v.y = pack_bf16(__uint_as_float(r[e + 2]) * f, __uint_as_float(r[e + 3]) * f);
+            v.z = pack_bf16(__uint_as_float(r[e + 4]) * f, __uint_as_float(r[e + 5]) * f);
+            v.w = pack_bf16(__uint_as_float(r[e + 6]) * f, __uint_as_float(r[e + 7]) * f);
+            *reinterpret_cast<uint4 *>(dst + col0 + c + e) = v;
+        }
+    }
+}
+
+__device__ __forceinline__ void zero_row(__nv_bfloat16 *dst, int D) {
+    for (int e = 0; e < D; e += 8) *reinterpret_cast<uint4 *>(dst + e) = make_uint4(0, 0, 0, 0);
+}
+
+// ------------------------------------------------------------------------------------------------------------ forward
+
+// The key tiles [j0, j0 + n) that the queries row0 .. row0 + 127 meet.
+__device__ __forceinline__ int key_tiles(const Shape &s, int row0, int lo, int hi) {
+    if (row0 >= s.Lq) return 0;
+    const int last = min(row0 + kTile, s.Lq) - 1;
+    const int end = s.causal ? min(hi, last + s.off + 1) : hi;
+    return end <= lo ? 0 : (end + kTile - 1) / kTile - lo / kTile;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
+                             const __grid_constant__ CUtensorMap mapV, Shape s, Rows out, float *__restrict__ lse) {
+    using Z = Sizes<HD>;
+    constexpr int STAGES = Z::FWD_STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = align_smem(smem_raw);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + STAGES) * Z::TILE);
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 8);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), q_full = smem_u32(bars + 2 * STAGES);
+    const uint32_t s_full0 = q_full + 8, p_ready0 = q_full + 24, pv_done0 = q_full + 40, drain = q_full + 56;
+    const uint32_t sq = smem_u32(smem), skv = sq + 2 * Z::TILE;
+
+    const int pairs = s.lq_pad / kTile / 2 + (s.lq_pad / kTile & 1), heads = s.Hq * s.B;
+    const int qp = pairs - 1 - (int)(blockIdx.x / heads);  // the longest rows of a causal mask first
+    const int bh = (int)(blockIdx.x % heads), b = bh / s.Hq, h = bh % s.Hq, hk = h / s.group;
+    int lo, hi;
+    key_range(s, b, lo, hi);
+    const int n0 = key_tiles(s, (2 * qp) * kTile, lo, hi), n1 = key_tiles(s, (2 * qp + 1) * kTile, lo, hi);
+    const int n = max(n0, n1), j0 = lo / kTile;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2 * STAGES + 1; ++i) mbar_init(full0 + 8 * i, 1);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(s_full0 + 8 * t, 1);
+            mbar_init(p_ready0 + 8 * t, 128);
+            mbar_init(pv_done0 + 8 * t, 1);
+        }
+        mbar_init(drain, 1);
+        fence_mbar_init();
+        prefetch_tmap(&mapQ);
+        prefetch_tmap(&mapK);
+        prefetch_tmap(&mapV);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_holder), kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_holder;
+
+    if (warp == 0) {
+        if (lane == 0 && n > 0) {  // ---- TMA producer: Q once, then K, V, K, V, ... through the ring
+            mbar_expect_tx(q_full, 2 * Z::TILE);
+            load_tile<HD>(sq, &mapQ, 2 * qp * kTile, h, b, q_full);
+            load_tile<HD>(sq + Z::TILE, &mapQ, (2 * qp + 1) * kTile, h, b, q_full);
+            int issued = 0;
+            bool ok = true;
+            for (; issued < 2 * n; ++issued) {
+                const int st = issued % STAGES;
+                ok = mbar_wait(empty0 + 8 * st, ((issued / STAGES) & 1) ^ 1, s.status);
+                if (!ok) break;
+                mbar_expect_tx(full0 + 8 * st, Z::TILE);
+                load_tile<HD>(skv + st * Z::TILE, (issued & 1) ? &mapV : &mapK, (j0 + issued / 2) * kTile, hk, b,
+                              full0 + 8 * st);
+            }
+            if (!ok) {  // error path: let the copies in flight land before the CTA exits
+                wait_bounded(q_full, 0);
+                for (int i = max(0, issued - STAGES); i < issued; ++i)
+                    wait_bounded(full0 + 8 * (i % STAGES), (i / STAGES) & 1);
+            }
+        }
+    } else if (warp == 1) {
+        if (n > 0) {  // ---- MMA issuer (the whole warp walks along: it zeroes rows of V outside the key range)
+            bool ok = mbar_wait(q_full, 0, s.status) && mbar_wait(full0, 0, s.status);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+            if (ok && lane == 0) {
+                for (int t = 0; t < 2; ++t)
+                    if ((t ? n1 : n0) > 0) {
+                        mma_rows_rows<HD>(tmem + t * kTile, sq + t * Z::TILE, skv);
+                        mma_commit(s_full0 + 8 * t);
+                    }
+                mma_commit(empty0);
+            }
+            for (int j = 0; ok && j < n; ++j) {
+                const int iv = 2 * j + 1, sv = iv % STAGES, ik = iv + 1, sk = ik % STAGES;
+                ok = mbar_wait(full0 + 8 * sv, (iv / STAGES) & 1, s.status);
+                if (ok && j + 1 < n) ok = mbar_wait(full0 + 8 * sk, (ik / STAGES) & 1, s.status);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const int key0 = (j0 + j) * kTile;
+                if (key0 < lo || key0 + kTile > hi) zero_rows<HD>(skv + sv * Z::TILE, lo - key0, hi - key0);
+                for (int t = 0; t < 2; ++t) {
+                    const int nt = t ? n1 : n0;
+                    if (j < nt) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(p_ready0 + 8 * t, j & 1, s.status));
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (lane == 0) {
+                            mma_tmem_rows<HD>(tmem + 2 * kTile + t * HD, tmem + t * kTile, 32, skv + sv * Z::TILE, j > 0);
+                            mma_commit(pv_done0 + 8 * t);
+                        }
+                    }
+                    if (t == 1 && lane == 0) mma_commit(empty0 + 8 * sv);
+                    if (j + 1 < nt && lane == 0) {
+                        mma_rows_rows<HD>(tmem + t * kTile, sq + t * Z::TILE, skv + sk * Z::TILE);
+                        mma_commit(s_full0 + 8 * t);
+                    }
+                    if (t == 1 && j + 1 < n && lane == 0) mma_commit(empty0 + 8 * sk);
+                }
+            }
+            if (lane == 0) {  // every MMA this thread issued completes before TMEM is released
+                mma_commit(drain);
+                wait_bounded(drain, 0);
+            }
+            __syncwarp();
+        }
+    } else {  // ---- softmax: warps 2-5 tile 0, warps 6-9 tile 1, a thread per query
+        const int t = (warp - 2) >> 2, quad = warp & 3, nt = t ? n1 : n0;
+        const int row0 = (2 * qp + t) * kTile, i = row0 + 32 * quad + lane;
+        const bool live = i < s.Lq;
+        const int row_hi = s.causal ? min(hi, i + s.off + 1) : hi;
+        const uint32_t lanes = (uint32_t)(32 * quad) << 16;
+        const uint32_t ts = tmem + lanes + t * kTile, to = tmem + lanes + 2 * kTile + t * HD;
+        float m = -INFINITY, sum = 0.f;  // m: the maximum that the exponentials are taken against
+        bool ok = true;
+        for (int j = 0; j < nt; ++j) {
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * t, j & 1, s.status));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t r[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_load32(ts + 32 * c, r[c]);
+            tmem_ld_wait();
+            const int key0 = (j0 + j) * kTile;
+            if (key0 < lo || key0 + kTile > hi || (s.causal && key0 + kTile - 1 > row0 + s.off)) {
+                const int clo = lo - key0, chi = row_hi - key0;
+#pragma unroll
+                for (int c = 0; c < kTile; ++c)
+                    if (c < clo || c >= chi) r[c >> 5][c & 31] = 0xff800000u;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < kTile; ++c) mx = fmaxf(mx, __uint_as_float(r[c >> 5][c & 31]));
+            // O and the sum are rescaled only when the maximum has grown by more than 8 binary orders: until then P
+            // stays below 2^8, exact enough in fp32 and bf16 alike
+            const bool grow = mx > m && (m == -INFINITY || (mx - m) * s.sl > 8.f);
+            if (__any_sync(0xffffffffu, grow)) {
+                const float f = grow ? ex2((m - mx) * s.sl) : 1.f;
+                if (grow) m = mx;
+                sum *= f;
+                if (j > 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * t, (j - 1) & 1, s.status));
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t o[32];
+                        tmem_load32(to + c, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_store32(to + c, o);
+                    }
+                }
+            }
+            const float base = m == -INFINITY ? 0.f : m * s.sl;
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                uint32_t pk[32];
+#pragma unroll
+                for (int c = 0; c < 64; c += 2) {
+                    const float p0 = ex2(fmaf(__uint_as_float(r[2 * g + (c >> 5)][c & 31]), s.sl, -base));
+                    const float p1 = ex2(fmaf(__uint_as_float(r[2 * g + (c >> 5)][(c & 31) + 1]), s.sl, -base));
+                    part[(c >> 1) & 3] += p0 + p1;
+                    pk[c >> 1] = pack_bf16(p0, p1);
+                }
+                tmem_store32(ts + 32 * g, pk);
+            }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(p_ready0 + 8 * t);
+        }
+        if (ok && nt > 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * t, (nt - 1) & 1, s.status));
+            tc_fence_after();
+        }
+        if (ok) {
+            __nv_bfloat16 *dst = out.p + b * out.batch + h * out.head + (int64_t)i * out.row;
+            if (nt > 0) store_row<HD>(dst, to, 0, s.D, sum > 0.f || sum != sum ? 1.f / sum : 0.f, live);
+            else if (live) zero_row(dst, s.D);
+            if (live)
+                lse[((int64_t)b * s.Hq + h) * s.Lq + i] =
+                    sum == 0.f ? -INFINITY : ((m == -INFINITY ? 0.f : m * s.sl) + log2f(sum)) * kLn2;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+}
+
+// ----------------------------------------------------------------------------------------------------------- backward
+
+// D = Σ dO·O per query and lse in units of log 2, by rows padded to whole tiles: half a warp per row.
+__global__ void __launch_bounds__(256)
+    attention_rowstats_kernel(const Rows o, const Rows g, Shape s, const float *__restrict__ lse,
+                              float *__restrict__ lse2, float *__restrict__ Dr) {
+    const int sub = threadIdx.x & 15;
+    const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 4;
+    const int64_t total = (int64_t)s.B * s.Hq * s.lq_pad;
+    if (row >= total) return;  // whole half warps: total is a multiple of 128
+    const int i = (int)(row % s.lq_pad);
+    const int64_t bh = row / s.lq_pad;
+    const int b = (int)(bh / s.Hq), h = (int)(bh % s.Hq);
+    float l = -INFINITY, d = 0.f;
+    if (i < s.Lq) l = lse[bh * s.Lq + i];
+    if (l != -INFINITY && 8 * sub < s.D) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(o.p + b * o.batch + h * o.head + (int64_t)i * o.row + 8 * sub);
+        const uint4 y = *reinterpret_cast<const uint4 *>(g.p + b * g.batch + h * g.head + (int64_t)i * g.row + 8 * sub);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            d = fmaf(__uint_as_float(xs[e] << 16), __uint_as_float(ys[e] << 16), d);
+            d = fmaf(__uint_as_float(xs[e] & 0xffff0000u), __uint_as_float(ys[e] & 0xffff0000u), d);
+        }
+    }
+#pragma unroll
+    for (int k = 8; k > 0; k >>= 1) d += __shfl_xor_sync(0xffffffffu, d, k);
+    if (sub == 0) {
+        lse2[row] = l == -INFINITY ? INFINITY : l * kLog2e;
+        Dr[row] = d;
+    }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
+                        const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapG, Shape s,
+                        const float *__restrict__ lse2, const float *__restrict__ Dr, Rows dq) {
+    using Z = Sizes<HD>;
+    constexpr int STAGES = Z::BWD_STAGES;
+    constexpr uint32_t kDQ = 0, kS = 128, kP = 256, kDS = 384;  // TMEM columns
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = align_smem(smem_raw);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + 2 * STAGES) * Z::TILE);
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 4 * STAGES + 9);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // K stages 0.., V stages STAGES..
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + 2 * STAGES), q_full = smem_u32(bars + 4 * STAGES);
+    const uint32_t s_full = q_full + 8, s_free = q_full + 16, p_full = q_full + 24, p_free = q_full + 32;
+    const uint32_t ds_ready = q_full + 40, ds_free = q_full + 48, drain = q_full + 56;
+    const uint32_t sq = smem_u32(smem), sg = sq + Z::TILE, sk = sg + Z::TILE, sv = sk + STAGES * Z::TILE;
+
+    const int tiles = s.lq_pad / kTile, heads = s.Hq * s.B;
+    const int qt = tiles - 1 - (int)(blockIdx.x / heads);
+    const int bh = (int)(blockIdx.x % heads), b = bh / s.Hq, h = bh % s.Hq, hk = h / s.group;
+    const int row0 = qt * kTile;
+    int lo, hi;
+    key_range(s, b, lo, hi);
+    const int n = key_tiles(s, row0, lo, hi), j0 = lo / kTile;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 4 * STAGES + 1; ++i) mbar_init(full0 + 8 * i, 1);
+        mbar_init(s_full, 1);
+        mbar_init(s_free, 256);
+        mbar_init(p_full, 1);
+        mbar_init(p_free, 256);
+        mbar_init(ds_ready, 256);
+        mbar_init(ds_free, 1);
+        mbar_init(drain, 1);
+        fence_mbar_init();
+        prefetch_tmap(&mapQ);
+        prefetch_tmap(&mapK);
+        prefetch_tmap(&mapV);
+        prefetch_tmap(&mapG);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_holder), kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_holder;
+
+    if (warp == 0) {
+        if (lane == 0 && n > 0) {
+            mbar_expect_tx(q_full, 2 * Z::TILE);
+            load_tile<HD>(sq, &mapQ, row0, h, b, q_full);
+            load_tile<HD>(sg, &mapG, row0, h, b, q_full);
+            int issued = 0;
+            bool ok = true;
+            for (; issued < n; ++issued) {
+                const int st = issued % STAGES;
+                const uint32_t par = ((issued / STAGES) & 1) ^ 1;
+                ok = mbar_wait(empty0 + 8 * st, par, s.status);
+                if (!ok) break;
+                mbar_expect_tx(full0 + 8 * st, Z::TILE);
+                load_tile<HD>(sk + st * Z::TILE, &mapK, (j0 + issued) * kTile, hk, b, full0 + 8 * st);
+                // V's stage is released by an earlier product than K's of the same key tile
+                ok = mbar_wait(empty0 + 8 * (STAGES + st), par, s.status);
+                if (!ok) break;
+                mbar_expect_tx(full0 + 8 * (STAGES + st), Z::TILE);
+                load_tile<HD>(sv + st * Z::TILE, &mapV, (j0 + issued) * kTile, hk, b, full0 + 8 * (STAGES + st));
+            }
+            if (!ok) {
+                wait_bounded(q_full, 0);
+                for (int i = max(0, issued - STAGES); i < issued; ++i)
+                    for (int w = 0; w < 2; ++w) wait_bounded(full0 + 8 * (w * STAGES + i % STAGES), (i / STAGES) & 1);
+                wait_bounded(full0 + 8 * (issued % STAGES), (issued / STAGES) & 1);
+            }
+        }
+    } else if (warp == 1) {
+        if (n > 0) {
+            bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, s.status));
+            // S and dP of key tile j run while the warps work on tile j − 1; then dQ of tile j − 1
+            for (int j = 0; ok && j <= n; ++j) {
+                if (j < n) {
+                    const int st = j % STAGES;
+                    const uint32_t par = (j / STAGES) & 1;
+                    ok = mbar_wait(full0 + 8 * st, par, s.status) && mbar_wait(s_free, (j & 1) ^ 1, s.status);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const int key0 = (j0 + j) * kTile;
+                    if (key0 < lo || key0 + kTile > hi) zero_rows<HD>(sk + st * Z::TILE, lo - key0, hi - key0);
+                    tc_fence_after();
+                    if (lane == 0) {
+                        mma_rows_rows<HD>(tmem + kS, sq, sk + st * Z::TILE);
+                        mma_commit(s_full);
+                    }
+                    ok = mbar_wait(full0 + 8 * (STAGES + st), par, s.status) && mbar_wait(p_free, (j & 1) ^ 1, s.status);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        mma_rows_rows<HD>(tmem + kP, sg, sv + st * Z::TILE);
+                        mma_commit(p_full);
+                        mma_commit(empty0 + 8 * (STAGES + st));
+                    }
+                }
+                if (j > 0) {
+                    const int st = (j - 1) % STAGES;
+                    ok = __all_sync(0xffffffffu, mbar_wait(ds_ready, (j - 1) & 1, s.status));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        mma_tmem_rows<HD>(tmem + kDQ, tmem + kDS, 32, sk + st * Z::TILE, j > 1);
+                        mma_commit(ds_free);
+                        mma_commit(empty0 + 8 * st);
+                    }
+                }
+            }
+            if (lane == 0) {
+                mma_commit(drain);
+                wait_bounded(drain, 0);
+            }
+            __syncwarp();
+        }
+    } else {  // two threads per query: columns 64·half ..
+        const int half = (warp - 2) >> 2, quad = warp & 3;
+        const int i = row0 + 32 * quad + lane;
+        const bool live = i < s.Lq;
+        const int row_hi = s.causal ? min(hi, i + s.off + 1) : hi;
+        const uint32_t lanes = (uint32_t)(32 * quad) << 16;
+        const float l2 = lse2[(int64_t)bh * s.lq_pad + i], Di = Dr[(int64_t)bh * s.lq_pad + i];
+        bool ok = true;
+        for (int j = 0; j < n; ++j) {
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full, j & 1, s.status));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t r[2][32], d[2][32];
+            tmem_load32(tmem + lanes + kS + 64 * half, r[0]);
+            tmem_load32(tmem + lanes + kS + 64 * half + 32, r[1]);
+            tmem_ld_wait();
+            tc_fence_before();
+            mbar_arrive(s_free);
+            const int key0 = (j0 + j) * kTile;
+            const bool edge = key0 < lo || key0 + kTile > hi || (s.causal && key0 + kTile - 1 > row0 + s.off);
+            const int clo = lo - key0 - 64 * half, chi = row_hi - key0 - 64 * half;
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+                r[c >> 5][c & 31] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c >> 5][c & 31]), s.sl, -l2)));
+            ok = __all_sync(0xffffffffu, mbar_wait(p_full, j & 1, s.status));
+            if (!ok) break;
+            tc_fence_after();
+            tmem_load32(tmem + lanes + kP + 64 * half, d[0]);
+            tmem_load32(tmem + lanes + kP + 64 * half + 32, d[1]);
+            tmem_ld_wait();
+            tc_fence_before();
+            mbar_arrive(p_free);
+#pragma unroll
+            for (int c = 0; c < 64; ++c) {
+                const float x = __uint_as_float(r[c >> 5][c & 31]) * (__uint_as_float(d[c >> 5][c & 31]) - Di);
+                r[c >> 5][c & 31] = __float_as_uint(x);
+            }
+            if (edge) {
+#pragma unroll
+                for (int c = 0; c < 64; ++c)
+                    if (c < clo || c >= chi) r[c >> 5][c & 31] = 0u;
+            }
+            uint32_t pk[32];
+#pragma unroll
+            for (int c = 0; c < 64; c += 2)
+                pk[c >> 1] = pack_bf16(__uint_as_float(r[c >> 5][c & 31]), __uint_as_float(r[c >> 5][(c & 31) + 1]));
+            ok = __all_sync(0xffffffffu, mbar_wait(ds_free, (j & 1) ^ 1, s.status));
+            if (!ok) break;
+            tc_fence_after();
+            tmem_store32(tmem + lanes + kDS + 32 * half, pk);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(ds_ready);
+        }
+        if (ok && n > 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait(ds_free, (n - 1) & 1, s.status));
+            tc_fence_after();
+        }
+        if (ok) {
+            __nv_bfloat16 *dst = dq.p + b * dq.batch + h * dq.head + (int64_t)i * dq.row;
+            if (n > 0) store_row<HD / 2>(dst, tmem + lanes + kDQ + half * (HD / 2), half * (HD / 2), s.D, s.scale, live);
+            else if (live && half == 0) zero_row(dst, s.D);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
+                         const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapG, Shape s,
+                         const float *__restrict__ lse2, const float *__restrict__ Dr, Rows dk, Rows dv) {
+    using Z = Sizes<HD>;
+    constexpr int STAGES = Z::BWD_STAGES;
+    // TMEM columns. Pᵀ and dSᵀ (bf16) lie over Sᵀ and dPᵀ: the threads of columns 0..63 write columns 0..31 of them,
+    // those of columns 64..127 write 64..95, so that no thread overwrites what another has yet to read
+    constexpr uint32_t kS = 0, kP = 128, kDV = 256, kDK = 384;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = align_smem(smem_raw);
+    float *stats = reinterpret_cast<float *>(smem + (2 + 2 * STAGES) * Z::TILE);  // per stage: lse2, D
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + 2 * STAGES) * Z::TILE + STAGES * Z::ROWSTATS);
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 4 * STAGES + 7);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // Q stages (with lse2) 0.., dO stages (with D) STAGES..
+    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + 2 * STAGES), kv_full = smem_u32(bars + 4 * STAGES);
+    const uint32_t s_full = kv_full + 8, p_full = kv_full + 16, p_ready = kv_full + 24, ds_ready = kv_full + 32;
+    const uint32_t done = kv_full + 40;
+    const uint32_t sk = smem_u32(smem), sv = sk + Z::TILE, sq = sv + Z::TILE, sg = sq + STAGES * Z::TILE;
+
+    const int heads = s.Hkv * s.B;
+    const int kt = (int)(blockIdx.x / heads);  // the first keys are seen by the most queries: they come first
+    const int bh = (int)(blockIdx.x % heads), b = bh / s.Hkv, hk = bh % s.Hkv;
+    const int key0 = kt * kTile;
+    int lo, hi;
+    key_range(s, b, lo, hi);
+    const int q_lo = s.causal ? max(0, lo - s.off) : 0;  // the queries before see no key
+    const int first = s.causal ? max(q_lo, key0 - s.off) : 0;
+    const int t0 = first / kTile, tiles = s.lq_pad / kTile;
+    const int nq = key0 >= hi || key0 + kTile <= lo || first >= s.Lq ? 0 : tiles - t0;
+    const int n = nq * s.group;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 4 * STAGES + 1; ++i) mbar_init(full0 + 8 * i, 1);
+        mbar_init(s_full, 1);
+        mbar_init(p_full, 1);
+        mbar_init(p_ready, 256);
+        mbar_init(ds_ready, 256);
+        mbar_init(done, 1);
+        fence_mbar_init();
+        prefetch_tmap(&mapQ);
+        prefetch_tmap(&mapK);
+        prefetch_tmap(&mapV);
+        prefetch_tmap(&mapG);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(tmem_holder), kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_holder;
+
+    if (warp == 0) {
+        if (lane == 0 && n > 0) {
+            mbar_expect_tx(kv_full, 2 * Z::TILE);
+            load_tile<HD>(sk, &mapK, key0, hk, b, kv_full);
+            load_tile<HD>(sv, &mapV, key0, hk, b, kv_full);
+            int issued = 0;
+            bool ok = true;
+            for (; issued < n; ++issued) {
+                const int st = issued % STAGES, h = hk * s.group + issued / nq, row = (t0 + issued % nq) * kTile;
+                const int64_t at = ((int64_t)b * s.Hq + h) * s.lq_pad + row;
+                const uint32_t par = ((issued / STAGES) & 1) ^ 1;
+                float *st_stats = stats + st * 2 * kTile;
+                // dO's stage is released by an earlier product than Q's of the same query tile
+                ok = mbar_wait(empty0 + 8 * st, par, s.status);
+                if (!ok) break;
+                mbar_expect_tx(full0 + 8 * st, Z::TILE + kTile * 4);
+                load_tile<HD>(sq + st * Z::TILE, &mapQ, row, h, b, full0 + 8 * st);
+                bulk_load(smem_u32(st_stats), lse2 + at, kTile * 4, full0 + 8 * st);
+                ok = mbar_wait(empty0 + 8 * (STAGES + st), par, s.status);
+                if (!ok) break;
+                mbar_expect_tx(full0 + 8 * (STAGES + st), Z::TILE + kTile * 4);
+                load_tile<HD>(sg + st * Z::TILE, &mapG, row, h, b, full0 + 8 * (STAGES + st));
+                bulk_load(smem_u32(st_stats + kTile), Dr + at, kTile * 4, full0 + 8 * (STAGES + st));
+            }
+            if (!ok) {
+                wait_bounded(kv_full, 0);
+                for (int i = max(0, issued - STAGES); i < issued; ++i)
+                    for (int w = 0; w < 2; ++w) wait_bounded(full0 + 8 * (w * STAGES + i % STAGES), (i / STAGES) & 1);
+                wait_bounded(full0 + 8 * (issued % STAGES), (issued / STAGES) & 1);
+            }
+        }
+    } else if (warp == 1) {
+        if (n > 0) {
+            bool ok = __all_sync(0xffffffffu, mbar_wait(kv_full, 0, s.status));
+            // in issue order: S(0) dP(0) | dV(j) S(j + 1) | dK(j) dP(j + 1) | ...: the warps form P(j) while dK(j − 1)
+            // and dP(j) run, and dS(j) while dV(j) and S(j + 1) run
+            for (int j = -1; ok && j < n; ++j) {
+                const int st = j % STAGES, nx = (j + 1) % STAGES;
+                const uint32_t npar = ((j + 1) / STAGES) & 1;
+                const int qrow = (t0 + (j + 1) % nq) * kTile;
+                if (j >= 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(p_ready, j & 1, s.status));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        mma_tmem_rows<HD>(tmem + kDV, tmem + kS, 64, sg + st * Z::TILE, j > 0);
+                    }
+                }
+                if (j + 1 < n) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * nx, npar, s.status));
+                    if (!ok) break;
+                    if (qrow < q_lo) zero_rows<HD>(sq + nx * Z::TILE, q_lo - qrow, kTile);
+                    if (lane == 0) {
+                        mma_rows_rows<HD>(tmem + kS, sk, sq + nx * Z::TILE);
+                        mma_commit(s_full);
+                    }
+                }
+                if (j >= 0) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(ds_ready, j & 1, s.status));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        mma_commit(empty0 + 8 * (STAGES + st));  // D(j) was read before ds_ready, dO(j) by dV(j)
+                        mma_tmem_rows<HD>(tmem + kDK, tmem + kP, 64, sq + st * Z::TILE, j > 0);
+                        mma_commit(empty0 + 8 * st);
+                    }
+                }
+                if (j + 1 < n) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * (STAGES + nx), npar, s.status));
+                    if (!ok) break;
+                    if (qrow < q_lo) zero_rows<HD>(sg + nx * Z::TILE, q_lo - qrow, kTile);
+                    if (lane == 0) {
+                        mma_rows_rows<HD>(tmem + kP, sv, sg + nx * Z::TILE);
+                        mma_commit(p_full);
+                    }
+                }
+            }
+            if (lane == 0) {
+                mma_commit(done);
+                wait_bounded(done, 0);
+            }
+            __syncwarp();
+        }
+    } else {  // two threads per key: queries 64·half .. of each tile
+        const int half = (warp - 2) >> 2, quad = warp & 3;
+        const int key = key0 + 32 * quad + lane;
+        const bool in = key >= lo && key < hi;
+        const uint32_t lanes = (uint32_t)(32 * quad) << 16;
+        const bool edge_keys = key0 < lo || key0 + kTile > hi;
+        bool ok = true;
+        for (int j = 0; j < n; ++j) {
+            const int st = j % STAGES, row0 = (t0 + j % nq) * kTile;
+            const float4 *l4 = reinterpret_cast<const float4 *>(stats + st * 2 * kTile + 64 * half);
+            const float4 *d4 = reinterpret_cast<const float4 *>(stats + st * 2 * kTile + kTile + 64 * half);
+            const bool edge = edge_keys || (s.causal && key0 + kTile - 1 > row0 + s.off);
+            const int clo = !in ? 64 : s.causal ? key - s.off - row0 - 64 * half : 0;  // columns before are masked
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full, j & 1, s.status));
+            // the tile's statistics came with Q and dO: their barriers make them visible to this thread
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(full0 + 8 * st, (j / STAGES) & 1, s.status));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t r[2][32], pk[32];
+            tmem_load32(tmem + lanes + kS + 64 * half, r[0]);
+            tmem_load32(tmem + lanes + kS + 64 * half + 32, r[1]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < 64; c += 4) {
+                const float4 l = l4[c >> 2];
+                const float ls[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float p = ex2(fmaf(__uint_as_float(r[(c + e) >> 5][(c + e) & 31]), s.sl, -ls[e]));
+                    r[(c + e) >> 5][(c + e) & 31] = __float_as_uint(p);
+                }
+            }
+            if (edge) {
+#pragma unroll
+                for (int c = 0; c < 64; ++c)
+                    if (c < clo) r[c >> 5][c & 31] = 0u;
+            }
+#pragma unroll
+            for (int c = 0; c < 64; c += 2)
+                pk[c >> 1] = pack_bf16(__uint_as_float(r[c >> 5][c & 31]), __uint_as_float(r[c >> 5][(c & 31) + 1]));
+            tmem_store32(tmem + lanes + kS + 64 * half, pk);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(p_ready);
+
+            ok = __all_sync(0xffffffffu, mbar_wait(p_full, j & 1, s.status));
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(full0 + 8 * (STAGES + st), (j / STAGES) & 1, s.status));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t d[2][32];
+            tmem_load32(tmem + lanes + kP + 64 * half, d[0]);
+            tmem_load32(tmem + lanes + kP + 64 * half + 32, d[1]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < 64; c += 4) {
+                const float4 l = d4[c >> 2];
+                const float ds[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = __uint_as_float(r[(c + e) >> 5][(c + e) & 31]) *
+                                    (__uint_as_float(d[(c + e) >> 5][(c + e) & 31]) - ds[e]);
+                    d[(c + e) >> 5][(c + e) & 31] = __float_as_uint(x);
+                }
+            }
+            if (edge) {
+#pragma unroll
+                for (int c = 0; c < 64; ++c)
+                    if (c < clo) d[c >> 5][c & 31] = 0u;
+            }
+#pragma unroll
+            for (int c = 0; c < 64; c += 2)
+                pk[c >> 1] = pack_bf16(__uint_as_float(d[c >> 5][c & 31]), __uint_as_float(d[c >> 5][(c & 31) + 1]));
+            tmem_store32(tmem + lanes + kP + 64 * half, pk);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(ds_ready);
+        }
+        const bool live = key < s.Lk;
+        if (ok && n > 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait(done, 0, s.status));
+            tc_fence_after();
+        }
+        if (ok) {  // columns half·HD/2 .. of the thread's key
+            const int c0 = half * (HD / 2);
+            __nv_bfloat16 *pk_ = dk.p + b * dk.batch + hk * dk.head + (int64_t)key * dk.row;
+            __nv_bfloat16 *pv_ = dv.p + b * dv.batch + hk * dv.head + (int64_t)key * dv.row;
+            if (n > 0) {
+                store_row<HD / 2>(pk_, tmem + lanes + kDK + c0, c0, s.D, s.scale, live);
+                store_row<HD / 2>(pv_, tmem + lanes + kDV + c0, c0, s.D, 1.f, live);
+            } else if (live) {
+                zero_row(half ? pv_ : pk_, s.D);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+}
+
+// --------------------------------------------------------------------------------------------------------------- host
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_fn() {
+    static std::once_flag once;
+    static EncodeTiled fn = nullptr;
+    std::call_once(once, [] {
+        void *ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiled>(ptr);
+    });
+    return fn;
+}
+
+// A (B, H, L, D) bf16 tensor in boxes of 64 x 128 rows, 128-byte swizzle, zero outside.
+int tile_map(CUtensorMap *m, const lamq_heads &t, int B, int H, int64_t L, int D) {
+    EncodeTiled enc = encode_fn();
+    if (enc == nullptr) {
+        set_error("lamq_attention: cuTensorMapEncodeTiled is unavailable");
+        return LAMQ_ERR_CUDA;
+    }
+    const auto stride = [](int64_t n, int64_t s, int64_t other) { return (cuuint64_t)(n > 1 ? s : other) * 2; };
+    const int64_t dense = (D + 7) / 8 * 8;  // the stride of an axis of one entry is not used: any valid value
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)L, (cuuint64_t)H, (cuuint64_t)B};
+    const cuuint64_t strides[3] = {stride(L, t.row, dense), stride(H, t.head, dense), stride(B, t.batch, dense)};
+    const cuuint32_t box[4] = {64, kTile, 1, 1}, step[4] = {1, 1, 1, 1};
+    const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, t.data, dims, strides, box, step,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("lamq_attention: cuTensorMapEncodeTiled failed (%d)", (int)r);
+        return LAMQ_ERR_CUDA;
+    }
+    return LAMQ_OK;
+}
+
+int check_heads(const char *fn, const char *name, const lamq_heads &t, int64_t B, int64_t H, int64_t L) {
+    LAMQ_REQUIRE(t.data != nullptr, "%s: null pointer (%s)", fn, name);
+    const auto fits = [](int64_t n, int64_t s) { return n <= 1 || (s > 0 && s % 8 == 0 && s < (1ll << 38)); };
+    LAMQ_REQUIRE(reinterpret_cast<uintptr_t>(t.data) % 16 == 0 && fits(B, t.batch) && fits(H, t.head) && fits(L, t.row),
+                 "%s: %s must be 16-byte aligned with positive strides that are multiples of 8", fn, name);
+    return LAMQ_OK;
+}
+
+int shape_of(const char *fn, const lamq_attention_args &a, int *status, Shape &s, bool &empty) {
+    LAMQ_REQUIRE(a.batch >= 0 && a.heads >= 0 && a.kv_heads >= 0 && a.q_len >= 0 && a.kv_len >= 0, "%s: bad shape", fn);
+    LAMQ_REQUIRE(a.head_dim >= 8 && a.head_dim <= 128 && a.head_dim % 8 == 0,
+                 "%s: head_dim must be a multiple of 8 in 8..128 (got %d)", fn, a.head_dim);
+    LAMQ_REQUIRE(a.heads == 0 || (a.kv_heads > 0 && a.heads % a.kv_heads == 0),
+                 "%s: %d query heads are not a multiple of %d key heads", fn, a.heads, a.kv_heads);
+    LAMQ_REQUIRE(a.scale > 0.f && a.scale < INFINITY, "%s: the scale must be positive and finite", fn);
+    LAMQ_REQUIRE(a.q_len <= (1 << 30) && a.kv_len <= (1 << 30) && a.batch * (int64_t)a.heads <= (1 << 20),
+                 "%s: lengths up to 2^30 and up to 2^20 heads in all", fn);
+    empty = a.batch == 0 || a.heads == 0;
+    if (empty) return LAMQ_OK;
+    LAMQ_REQUIRE(status != nullptr, "%s: null pointer (status)", fn);
+    s.B = (int)a.batch;
+    s.Hq = a.heads;
+    s.Hkv = a.kv_heads;
+    s.group = a.heads / a.kv_heads;
+    s.D = a.head_dim;
+    s.Lq = (int)a.q_len;
+    s.Lk = (int)a.kv_len;
+    s.off = s.Lk - s.Lq;
+    s.lq_pad = (s.Lq + kTile - 1) / kTile * kTile;
+    s.causal = a.causal;
+    s.scale = a.scale;
+    s.sl = a.scale * kLog2e;
+    s.ks = a.key_start;
+    s.ke = a.key_end;
+    s.status = status;
+    return LAMQ_OK;
+}
+
+Rows rows_of(const lamq_heads &t) { return {reinterpret_cast<__nv_bfloat16 *>(t.data), t.batch, t.head, t.row}; }
+
+int launch_failed(const char *what, cudaError_t e) {
+    set_error("%s: %s", what, cudaGetErrorString(e));
+    return LAMQ_ERR_CUDA;
+}
+
+// The tensor maps are made by a driver call, which needs the device's context bound to the calling thread; a thread that
+// has made no runtime call yet (autograd's) has none.
+int bind_context(const char *fn) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaSetDevice(dev);
+    return e == cudaSuccess ? LAMQ_OK : launch_failed(fn, e);
+}
+
+template <int HD>
+int run_forward(const lamq_attention_args &a, const Shape &s, cudaStream_t st) {
+    CUtensorMap mq, mk, mv;
+    if (int e = tile_map(&mq, a.q, s.B, s.Hq, s.Lq, s.D)) return e;
+    if (s.Lk > 0) {
+        if (int e = tile_map(&mk, a.k, s.B, s.Hkv, s.Lk, s.D)) return e;
+        if (int e = tile_map(&mv, a.v, s.B, s.Hkv, s.Lk, s.D)) return e;
+    } else {
+        mk = mv = mq;  // not read: no query meets a key tile
+    }
+    const int64_t pairs = (s.lq_pad / kTile + 1) / 2, blocks = pairs * s.Hq * s.B;
+    LAMQ_REQUIRE(blocks <= INT_MAX, "lamq_attention_forward: too many query tiles");
+    auto *k = attention_forward_kernel<HD>;
+    if (cudaError_t e = smem_limit_once((const void *)k, (int)Sizes<HD>::FWD_SMEM))
+        return launch_failed("lamq_attention_forward", e);
+    k<<<(unsigned)blocks, kThreads, Sizes<HD>::FWD_SMEM, st>>>(mq, mk, mv, s, rows_of(a.o), a.lse);
+    LAMQ_CHECK_LAUNCH("lamq_attention_forward");
+    return LAMQ_OK;
+}
+
+template <int HD>
+int run_backward(const lamq_attention_args &a, const Shape &s, float *lse2, float *D, cudaStream_t st) {
+    CUtensorMap mq, mk, mv, mg;
+    const bool queries = s.Lq > 0, keys = s.Lk > 0;
+    if (queries) {
+        if (int e = tile_map(&mq, a.q, s.B, s.Hq, s.Lq, s.D)) return e;
+        if (int e = tile_map(&mg, a.d_o, s.B, s.Hq, s.Lq, s.D)) return e;
+    }
+    if (keys) {
+        if (int e = tile_map(&mk, a.k, s.B, s.Hkv, s.Lk, s.D)) return e;
+        if (int e = tile_map(&mv, a.v, s.B, s.Hkv, s.Lk, s.D)) return e;
+    }
+    if (!keys) mk = mv = mq;   // not read: no query meets a key tile
+    if (!queries) mq = mg = mk;
+    if (queries) {
+        const int64_t rows = (int64_t)s.B * s.Hq * s.lq_pad, blocks = rows / 16;
+        LAMQ_REQUIRE(blocks <= INT_MAX, "lamq_attention_backward: too many queries");
+        attention_rowstats_kernel<<<(unsigned)blocks, 256, 0, st>>>(rows_of(a.o), rows_of(a.d_o), s, a.lse, lse2, D);
+        LAMQ_CHECK_LAUNCH("lamq_attention_backward statistics");
+        const int64_t tiles = (int64_t)(s.lq_pad / kTile) * s.Hq * s.B;
+        auto *k = attention_dq_kernel<HD>;
+        if (cudaError_t e = smem_limit_once((const void *)k, (int)Sizes<HD>::DQ_SMEM))
+            return launch_failed("lamq_attention_backward", e);
+        k<<<(unsigned)tiles, kThreads, Sizes<HD>::DQ_SMEM, st>>>(mq, mk, mv, mg, s, lse2, D, rows_of(a.dq));
+        LAMQ_CHECK_LAUNCH("lamq_attention_backward dq");
+    }
+    if (keys) {
+        const int64_t tiles = (int64_t)((s.Lk + kTile - 1) / kTile) * s.Hkv * s.B;
+        LAMQ_REQUIRE(tiles <= INT_MAX, "lamq_attention_backward: too many key tiles");
+        auto *k = attention_dkv_kernel<HD>;
+        if (cudaError_t e = smem_limit_once((const void *)k, (int)Sizes<HD>::DKV_SMEM))
+            return launch_failed("lamq_attention_backward", e);
+        k<<<(unsigned)tiles, kThreads, Sizes<HD>::DKV_SMEM, st>>>(mq, mk, mv, mg, s, lse2, D, rows_of(a.dk),
+                                                                 rows_of(a.dv));
+        LAMQ_CHECK_LAUNCH("lamq_attention_backward dkv");
+    }
+    return LAMQ_OK;
+}
+
+}  // namespace
+}  // namespace lamq
+
+using namespace lamq;
+
+static_assert(sizeof(lamq_heads) == 32 && sizeof(lamq_attention_args) == 328, "lamq_attention_args' layout in the C ABI");
+
+extern "C" int lamq_attention_forward(const lamq_attention_args *args, int *status, lamq_stream_t stream) {
+    const char *fn = "lamq_attention_forward";
+    LAMQ_REQUIRE(args != nullptr, "%s: null pointer", fn);
+    const lamq_attention_args &a = *args;
+    Shape s{};
+    bool empty = false;
+    if (int e = shape_of(fn, a, status, s, empty)) return e;
+    if (empty || s.Lq == 0) return LAMQ_OK;
+    if (int e = check_heads(fn, "q", a.q, s.B, s.Hq, s.Lq)) return e;
+    if (int e = check_heads(fn, "o", a.o, s.B, s.Hq, s.Lq)) return e;
+    if (s.Lk > 0) {
+        if (int e = check_heads(fn, "k", a.k, s.B, s.Hkv, s.Lk)) return e;
+        if (int e = check_heads(fn, "v", a.v, s.B, s.Hkv, s.Lk)) return e;
+    }
+    LAMQ_REQUIRE(a.lse != nullptr, "%s: null pointer (lse)", fn);
+    if (int e = bind_context(fn)) return e;
+    return s.D <= 64 ? run_forward<64>(a, s, (cudaStream_t)stream) : run_forward<128>(a, s, (cudaStream_t)stream);
+}
+
+extern "C" size_t lamq_attention_backward_workspace_size(int64_t batch, int heads, int64_t q_len) {
+    if (batch <= 0 || heads <= 0 || q_len <= 0) return 0;
+    return (size_t)batch * (size_t)heads * (size_t)((q_len + kTile - 1) / kTile * kTile) * 2 * sizeof(float);
+}
+
+extern "C" int lamq_attention_backward(const lamq_attention_args *args, void *workspace, size_t workspace_bytes,
+                                       int *status, lamq_stream_t stream) {
+    const char *fn = "lamq_attention_backward";
+    LAMQ_REQUIRE(args != nullptr, "%s: null pointer", fn);
+    const lamq_attention_args &a = *args;
+    Shape s{};
+    bool empty = false;
+    if (int e = shape_of(fn, a, status, s, empty)) return e;
+    if (empty || (s.Lq == 0 && s.Lk == 0)) return LAMQ_OK;
+    if (s.Lq > 0) {
+        if (int e = check_heads(fn, "q", a.q, s.B, s.Hq, s.Lq)) return e;
+        if (int e = check_heads(fn, "o", a.o, s.B, s.Hq, s.Lq)) return e;
+        if (int e = check_heads(fn, "do", a.d_o, s.B, s.Hq, s.Lq)) return e;
+        if (int e = check_heads(fn, "dq", a.dq, s.B, s.Hq, s.Lq)) return e;
+        LAMQ_REQUIRE(a.lse != nullptr, "%s: null pointer (lse)", fn);
+    }
+    if (s.Lk > 0) {
+        if (int e = check_heads(fn, "k", a.k, s.B, s.Hkv, s.Lk)) return e;
+        if (int e = check_heads(fn, "v", a.v, s.B, s.Hkv, s.Lk)) return e;
+        if (int e = check_heads(fn, "dk", a.dk, s.B, s.Hkv, s.Lk)) return e;
+        if (int e = check_heads(fn, "dv", a.dv, s.B, s.Hkv, s.Lk)) return e;
+    }
+    const size_t need = lamq_attention_backward_workspace_size(s.B, s.Hq, s.Lq);
+    LAMQ_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 16 == 0)),
+                 "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", fn, need, workspace_bytes);
+    if (int e = bind_context(fn)) return e;
+    float *lse2 = reinterpret_cast<float *>(workspace);
+    float *D = lse2 + need / (2 * sizeof(float));
+    return s.D <= 64 ? run_backward<64>(a, s, lse2, D, (cudaStream_t)stream)
+                     : run_backward<128>(a, s, lse2, D, (cudaStream_t)stream);
+}

@@ -38,7 +38,38 @@ INVALID = [
     ("lamq_embedding_gradient", (P, 0, 8, P, 1, 4, 10, 8, 1.0, -1, 0, P, 8, P, 16, P, N), b"workspace"),
 ]
 
+
+
+def heads(data=P, batch=4096, head=128, row=512):
+    return (data, batch, head, row)
+
+
+def attention(batch=2, heads_=4, kv=2, D=64, Lq=9, Lk=9, scale=0.125, q=heads(), k=heads(), v=heads(), o=heads(), lse=P,
+              d_o=heads(), dq=heads(), dk=heads(), dv=heads()):
+    return _lib.ATTENTION_ARGS.pack(batch, heads_, kv, D, 1, Lq, Lk, scale, 0, 0, 0, *q, *k, *v, *o, lse, *d_o, *dq, *dk,
+                                    *dv)
+
+
+INVALID += [(f"lamq_attention_{way}", (a, *rest), text)
+            for way, rest in (("forward", (P, N)), ("backward", (P, 0, P, N)))
+            for a, text in [(N, b"null pointer"), (attention(Lq=-1), b"bad shape"), (attention(D=12), b"head_dim"),
+                            (attention(D=136), b"head_dim"), (attention(kv=3), b"not a multiple of 3"),
+                            (attention(scale=0.0), b"scale"), (attention(scale=float("nan")), b"scale"),
+                            (attention(Lk=2**31), b"lengths up to"), (attention(batch=2**20), b"heads in all"),
+                            (attention(q=heads(0)), b"null pointer (q)"), (attention(k=heads(P + 8)), b"aligned"),
+                            (attention(v=heads(row=60)), b"multiples of 8"), (attention(o=heads(head=0)), b"positive"),
+                            (attention(lse=0), b"null pointer (lse)")]]
+INVALID += [("lamq_attention_forward", (attention(), N, N), b"null pointer (status)"),
+            ("lamq_attention_backward", (attention(), P, 0, N, N), b"null pointer (status)"),
+            ("lamq_attention_backward", (attention(d_o=heads(0)), P, 0, P, N), b"null pointer (do)"),
+            ("lamq_attention_backward", (attention(dv=heads(row=-8)), P, 0, P, N), b"positive"),
+            ("lamq_attention_backward", (attention(), P, 100, P, N), b"workspace of 8192 bytes")]
+
 EMPTY = [
+    ("lamq_attention_forward", (attention(batch=0), N, N)),
+    ("lamq_attention_forward", (attention(Lq=0, q=heads(0), o=heads(0)), P, N)),
+    ("lamq_attention_backward", (attention(heads_=0), N, 0, N, N)),
+    ("lamq_attention_backward", (attention(Lq=0, Lk=0), N, 0, P, N)),
     ("lamq_embedding_lookup", (N, 0, 8, 10, 8, N, 1, 0, 1.0, -1, N, 8, N, N)),
     ("lamq_embedding_gradient", (N, 0, 8, N, 1, 4, 0, 8, 1.0, -1, 0, N, 8, N, 0, N, N)),
 ]

@@ -85,6 +85,22 @@ size_t lamq_attention_backward_workspace_size(int64_t batch, int heads, int64_t 
 int lamq_attention_backward(const lamq_attention_args *args, void *workspace, size_t workspace_bytes, int *status,
                             lamq_stream_t stream);
 
+/*
+ * The orthogonalised update of each of `batch` matrices G (m x n, leading dimension ldg, batch_stride elements apart;
+ * dtype LAMQ_F32 or LAMQ_BF16): X = G / (|G|_F + eps), then for each of `steps` (1..16) steps, with (a, b, c) the
+ * step's coefficients (host memory, 3·steps floats, read before the call returns), X <- (aI + bA + cA²)·X, A = X·Xᵀ
+ * (on the smaller side of G: for m > n, X <- X·(aI + bA + cA²), A = Xᵀ·X). out: batch x m x n bf16, contiguous.
+ * X, A and B are held in 22 bits, products take fp16 operands where their rounding cannot grow, fp16 pairs elsewhere,
+ * with fp32 accumulation: the relative error is about the bf16 output's rounding (2^-9) again. Coefficients that take singular values of [0, 1] above 5, or the polynomial of A above 32, are
+ * rejected. A zero matrix gives zeros; a matrix with a NaN or an infinity gives NaN. Workspace:
+ * lamq_newton_schulz_workspace_size(batch, m, n) bytes, 16-byte aligned. One cooperative kernel; *status becomes
+ * LAMQ_ERR_TIMEOUT if a bounded device wait gives up. Equal calls give equal bits.
+ */
+size_t lamq_newton_schulz_workspace_size(int batch, int m, int n);
+int lamq_newton_schulz(const void *G, int dtype, int64_t ldg, int64_t batch_stride, int batch, int m, int n, int steps,
+                       const float *coefficients, float eps, uint16_t *out, void *workspace, size_t workspace_bytes,
+                       int *status, lamq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -75,6 +75,8 @@ SIGNATURES = {
     "lamq_attention_forward": (_I32, [_P, _P, _P]),
     "lamq_attention_backward_workspace_size": (_SZ, [_I64, _I32, _I64]),
     "lamq_attention_backward": (_I32, [_P, _P, _SZ, _P, _P]),
+    "lamq_newton_schulz_workspace_size": (_SZ, [_I32, _I32, _I32]),
+    "lamq_newton_schulz": (_I32, [_P, _I32, _I64, _I64, _I32, _I32, _I32, _I32, _P, _c.c_float, _P, _P, _SZ, _P, _P]),
 }
 
 # lamq_attention_args (328 bytes): batch; heads, kv_heads, head_dim, causal; q_len, kv_len; scale, reserved; key_start,

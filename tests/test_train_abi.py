@@ -1,7 +1,9 @@
 """The training operators' C ABI (include/lamq_b200_train.h): every declared symbol is exported and bound, arguments
 are checked before the device is touched, and empty inputs are a successful no-op (no GPU needed)."""
 
+import ctypes
 import re
+import struct
 from pathlib import Path
 
 import pytest
@@ -65,7 +67,19 @@ INVALID += [("lamq_attention_forward", (attention(), N, N), b"null pointer (stat
             ("lamq_attention_backward", (attention(dv=heads(row=-8)), P, 0, P, N), b"positive"),
             ("lamq_attention_backward", (attention(), P, 100, P, N), b"workspace of 8192 bytes")]
 
+C3 = struct.pack("3f", 3.4445, -4.7750, 2.0315)
+INVALID += [("lamq_newton_schulz", (P, dt, ld, 64, b, m, n, steps, coef, eps, out, ws, 0, P, N), text)
+            for dt, ld, b, m, n, steps, coef, eps, out, ws, text in [
+                (0, 8, 1, -1, 8, 1, C3, 0.0, P, P, b"bad shape"), (0, 7, 1, 8, 8, 1, C3, 0.0, P, P, b"bad shape"),
+                (2, 8, 1, 8, 8, 1, C3, 0.0, P, P, b"dtype"), (0, 8, 1, 8, 8, 0, C3, 0.0, P, P, b"1 to 16 steps"),
+                (0, 8, 1, 8, 8, 17, C3, 0.0, P, P, b"1 to 16 steps"), (0, 8, 1, 8, 8, 1, C3, -1.0, P, P, b"eps"),
+                (0, 8, 2, 9, 8, 1, C3, 0.0, P, P, b"overlap"), (0, 8, 1, 8, 8, 1, N, 0.0, P, P, b"null pointer"),
+                (0, 2**24, 65535, 2**24, 2**24, 1, C3, 0.0, P, P, b"too large"),
+                (0, 8, 1, 8, 8, 1, C3, 0.0, N, P, b"null pointer"), (0, 8, 1, 8, 8, 1, C3, 0.0, P, P, b"workspace")]]
+
 EMPTY = [
+    ("lamq_newton_schulz", (N, 0, 8, 0, 0, 8, 8, 1, N, 0.0, N, N, 0, N, N)),
+    ("lamq_newton_schulz", (N, 0, 8, 0, 1, 0, 8, 1, N, 0.0, N, N, 0, N, N)),
     ("lamq_attention_forward", (attention(batch=0), N, N)),
     ("lamq_attention_forward", (attention(Lq=0, q=heads(0), o=heads(0)), P, N)),
     ("lamq_attention_backward", (attention(heads_=0), N, 0, N, N)),
@@ -103,3 +117,25 @@ def test_tables_cover_every_compute_entry_point():
 def test_gradient_workspace_size(lib):
     assert lib.lamq_embedding_gradient_workspace_size(0, 64) == 0
     assert lib.lamq_embedding_gradient_workspace_size(100, 64) >= 4 * 400 + 2 * 13 * 64 * 4
+
+
+def test_newton_schulz_coefficients_that_leave_the_range(lib):
+    """Checked after the workspace (whose size is right here) and before the device: sizes and pointers stand in."""
+    need = lib.lamq_newton_schulz_workspace_size(1, 8, 8)
+    for c in ((40.0, 0.0, 0.0), (6.0, 0.0, 0.0), (0.0, 0.0, 33.0), (float("nan"), 0.0, 0.0)):
+        st = lib.lamq_newton_schulz(P, 0, 8, 64, 1, 8, 8, 1, struct.pack("3f", *c), 0.0, P, P, need, P, None)
+        assert st == _lib.LAMQ_ERR_INVALID and b"leave the range" in lib.lamq_last_error(), c
+
+
+def test_attention_args_layout_matches_the_header(lib):
+    """The packed lamq_attention_args reaches the library field for field: the checks name the tensor that breaks."""
+    assert _lib.ATTENTION_ARGS.size == 328
+    for name in ("q", "k", "v", "o"):
+        args = attention(**{name: heads(0)})
+        assert lib.lamq_attention_forward(args, P, None) == _lib.LAMQ_ERR_INVALID
+        assert f"({name})".encode() in lib.lamq_last_error()
+    for name, key in (("do", "d_o"), ("dq", "dq"), ("dk", "dk"), ("dv", "dv")):
+        args = attention(**{key: heads(0)})
+        assert lib.lamq_attention_backward(args, P, 0, P, None) == _lib.LAMQ_ERR_INVALID
+        assert f"({name})".encode() in lib.lamq_last_error()
+    assert ctypes.sizeof(ctypes.c_void_p) == 8

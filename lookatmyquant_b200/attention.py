@@ -133,23 +133,30 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | 
 
 
 def _transformers_attention(module, query, key, value, attention_mask, scaling=None, dropout=0.0, **kwargs):
+    for what in ("sliding_window", "softcap", "s_aux"):
+        if kwargs.get(what) is not None:
+            raise NotImplementedError(f"the lamq attention has no {what}")
     if attention_mask is not None or dropout:
         raise NotImplementedError("the lamq attention takes whole windows: no mask and no dropout")
-    causal = getattr(module, "is_causal", True)
+    causal = kwargs.get("is_causal")
+    causal = getattr(module, "is_causal", True) if causal is None else causal
     return attention(query, key, value, scaling, causal).transpose(1, 2), None
+
+
+def _transformers_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_function=None,
+                       attention_mask=None, **kwargs):
+    from transformers.masking_utils import causal_mask_function
+    if mask_function not in (None, causal_mask_function) or kv_offset or int(q_offset) + q_length != kv_length or (
+            attention_mask is not None and not bool(attention_mask.all())):
+        raise NotImplementedError("the lamq attention takes whole windows: no padding, packing or windowed mask")
+    return None
 
 
 def use_in_transformers(name: str = "lamq") -> str:
     """Registers `attention` with Hugging Face transformers under `name` (returned): a model whose config has
-    `_attn_implementation = name` runs its attention forwards and backwards on these kernels. Windows are whole (no
-    padding mask); bf16 models."""
+    `_attn_implementation = name` runs its attention forwards and backwards on these kernels. bf16 models on whole
+    windows: a padded, packed or windowed mask raises NotImplementedError."""
     from transformers import AttentionInterface, AttentionMaskInterface
     AttentionInterface.register(name, _transformers_attention)
-    AttentionMaskInterface.register(name, _no_mask)
+    AttentionMaskInterface.register(name, _transformers_mask)
     return name
-
-
-def _no_mask(*args, attention_mask=None, **kwargs):
-    if attention_mask is not None and not bool(attention_mask.all()):
-        raise NotImplementedError("the lamq attention takes whole windows: no padding")
-    return None

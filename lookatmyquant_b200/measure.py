@@ -34,20 +34,21 @@ STAGES = [("self_attn", ["self_attn.q_proj", "self_attn.k_proj", "self_attn.v_pr
 BLOCK_SEED = {"self_attn": 2, "mlp": 3}  # compiler_arch.block_seed for the Llama blocks
 
 
-def smollm2_config(layers: int = 32):
+def smollm2_config(layers: int = 32, attention: str = "sdpa"):
     from transformers import LlamaConfig
     cfg = LlamaConfig(hidden_size=960, intermediate_size=2560, num_hidden_layers=layers, num_attention_heads=15,
                       num_key_value_heads=5, vocab_size=49152, rms_norm_eps=1e-5, rope_theta=1e5,
                       tie_word_embeddings=True, max_position_embeddings=8192, initializer_range=0.02)
-    cfg._attn_implementation = "sdpa"
+    cfg._attn_implementation = attention
     return cfg
 
 
-def build_model(layers: int = 32, seed: int = 0, device="cuda"):
-    """A SmolLM2-360M-architecture model with random N(0, 0.02²) weights, bf16, on the device."""
+def build_model(layers: int = 32, seed: int = 0, device="cuda", attention: str = "sdpa"):
+    """A SmolLM2-360M-architecture model with random N(0, 0.02²) weights, bf16, on the device. `attention` is its
+    attention implementation ("lamq" after attention.use_in_transformers())."""
     from transformers import LlamaForCausalLM
     torch.manual_seed(seed)
-    model = LlamaForCausalLM(smollm2_config(layers))
+    model = LlamaForCausalLM(smollm2_config(layers, attention))
     return model.to(device=device, dtype=torch.bfloat16).eval()
 
 

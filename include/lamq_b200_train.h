@@ -27,9 +27,10 @@ int lamq_embedding_lookup(const void *table, int dtype, int64_t ldt, int64_t row
 /*
  * The lookup's gradient: dE[v] = scale · Σ_{t: ids[t] = v} dy[t] for every v < rows (dE: rows x d, lde, of dy's dtype),
  * or dE[v] += that with accumulate != 0 (rows without a token are then left alone). Tokens with id == padding or an
- * invalid id (which sets *status to LAMQ_ERR_INVALID) add nothing. Sums are fp32 in the order of the tokens within
- * fixed chunks of the sorted tokens: equal calls give equal bits. Workspace:
- * lamq_embedding_gradient_workspace_size(n, d) bytes, 16-byte aligned.
+ * invalid id (which sets *status to LAMQ_ERR_INVALID) add nothing. Sums are fp32 in the order of the tokens (above 2048
+ * tokens, within fixed chunks of the sorted tokens, then chunk by chunk): equal calls give equal bits. Workspace:
+ * lamq_embedding_gradient_workspace_size(n, d) bytes, 16-byte aligned (0, and NULL allowed, up to 2048 tokens). *status
+ * becomes LAMQ_ERR_TIMEOUT if a bounded device wait gives up.
  */
 size_t lamq_embedding_gradient_workspace_size(int64_t n, int d);
 int lamq_embedding_gradient(const void *dy, int dtype, int64_t ldy, const void *ids, int ids64, int64_t n, int64_t rows,

@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import ATTENTION_ARGS, check, ptr, stream_ptr
+from ._lib import ATTENTION_ARGS, check, launch_on, ptr
 
 _STATUS = _lib.StatusWord("attention")
 
@@ -28,20 +28,29 @@ def check_status():
     _STATUS.check()
 
 
-def _heads(x: torch.Tensor, what: str) -> torch.Tensor:
-    if x.dtype != torch.bfloat16 or not x.is_cuda:
+def _heads(x: torch.Tensor, what: str):
+    """(x, what lamq_heads holds of it), x copied where TMA cannot read it in place."""
+    if x.dtype is not torch.bfloat16 or not x.is_cuda:
         raise TypeError(f"{what} must be a bfloat16 CUDA tensor")
     if x.ndim != 4:
         raise ValueError(f"{what} must be (batch, heads, length, head_dim)")
-    if x.numel() and (x.stride(3) != 1 or x.data_ptr() % 16 or
-                      any(n > 1 and (s % 8 or s <= 0) for n, s in zip(x.shape[:3], x.stride()[:3]))):
-        x = x.contiguous()
-    return x
+    b, h, r, one = x.stride()
+    p = x.data_ptr()
+    if one != 1 or (b | h | r) & 7 or p & 15 or b <= 0 or h <= 0 or r <= 0:
+        n, m, k, d = x.shape  # the stride of an axis of one entry does not matter
+        if d and ((one != 1 and d > 1) or p & 15 or (n > 1 and (b & 7 or b <= 0)) or (m > 1 and (h & 7 or h <= 0)) or
+                  (k > 1 and (r & 7 or r <= 0))):
+            x = x.contiguous()
+            b, h, r, one = x.stride()
+            p = x.data_ptr()
+    return x, (p, b, h, r)
 
 
-def _like_projection(B: int, H: int, L: int, D: int, device) -> torch.Tensor:
-    """An empty (B, H, L, D) tensor in the memory order of a projection's (B, L, H·D) output."""
-    return torch.empty(B, L, H, D, dtype=torch.bfloat16, device=device).transpose(1, 2)
+def _like_projection(B: int, H: int, L: int, D: int, device):
+    """An empty (B, H, L, D) tensor in the memory order of a projection's (B, L, H·D) output, as _heads gives it."""
+    strides = (L * H * D, D, H * D)
+    x = torch.empty_strided((B, H, L, D), (*strides, 1), dtype=torch.bfloat16, device=device)
+    return x, (x.data_ptr(), *strides)
 
 
 def _bounds(x: torch.Tensor | None, what: str, batch: int, device):
@@ -52,17 +61,11 @@ def _bounds(x: torch.Tensor | None, what: str, batch: int, device):
     return x.contiguous()
 
 
-def _pack(x: torch.Tensor | None):
-    if x is None:
-        return (0, 0, 0, 0)
-    s = x.stride()
-    return (x.data_ptr(), s[0], s[1], s[2])
-
-
 def _shapes(q, k, v, scale):
     B, Hq, Lq, D = q.shape
     Hkv, Lk = k.shape[1], k.shape[2]
-    if k.shape != (B, Hkv, Lk, D) or v.shape != k.shape or k.device != q.device or v.device != q.device:
+    shape = (B, Hkv, Lk, D)
+    if k.shape != shape or v.shape != shape or k.device != q.device or v.device != q.device:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
     return B, Hq, Hkv, D, Lq, Lk, D ** -0.5 if scale is None else float(scale)
 
@@ -71,18 +74,17 @@ def forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | No
             key_start: torch.Tensor | None = None, key_end: torch.Tensor | None = None):
     """softmax(scale·q·kᵀ)·v over each query's keys (scale: head_dim^-1/2 by default): (output, lse), the output bf16
     like q and lse (batch, heads, q length) fp32."""
-    q, k, v = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
+    (q, qh), (k, kh), (v, vh) = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
     B, Hq, Hkv, D, Lq, Lk, scale = _shapes(q, k, v, scale)
     dev = q.device
     start, end = _bounds(key_start, "key_start", B, dev), _bounds(key_end, "key_end", B, dev)
-    o = _like_projection(B, Hq, Lq, D, dev)
-    lse = torch.empty(B, Hq, Lq, dtype=torch.float32, device=dev)
-    none = (0,) * 16
-    args = ATTENTION_ARGS.pack(B, Hq, Hkv, D, causal, Lq, Lk, scale, 0, ptr(start) or 0, ptr(end) or 0, *_pack(q),
-                               *_pack(k), *_pack(v), *_pack(o), lse.data_ptr(), *none)
-    with torch.cuda.device(dev):
-        check(_lib.load().lamq_attention_forward(args, ptr(_STATUS.on(dev)), stream_ptr(dev)),
-              "lamq_attention_forward")
+    o, oh = _like_projection(B, Hq, Lq, D, dev)
+    lse = torch.empty((B, Hq, Lq), dtype=torch.float32, device=dev)
+    args = ATTENTION_ARGS.pack(B, Hq, Hkv, D, causal, Lq, Lk, scale, 0, ptr(start) or 0, ptr(end) or 0, *qh, *kh, *vh,
+                               *oh, lse.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    here, stream = launch_on(dev)
+    with here:
+        check(_lib.load().lamq_attention_forward(args, _STATUS.on(dev).data_ptr(), stream), "lamq_attention_forward")
     return o, lse
 
 
@@ -91,23 +93,27 @@ def backward(do: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor
              key_end: torch.Tensor | None = None):
     """(dq, dk, dv) of `forward` for the output's gradient `do`, with the o and lse that `forward` returned for the
     same q, k, v, scale, causal and key ranges. Equal calls give equal bits."""
-    q, k, v, o, do = _heads(q, "q"), _heads(k, "k"), _heads(v, "v"), _heads(o, "o"), _heads(do, "do")
+    (q, qh), (k, kh), (v, vh) = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
+    (o, oh), (do, doh) = _heads(o, "o"), _heads(do, "do")
     B, Hq, Hkv, D, Lq, Lk, scale = _shapes(q, k, v, scale)
     dev = q.device
     if o.shape != q.shape or do.shape != q.shape or o.device != dev or do.device != dev:
         raise ValueError(f"o {tuple(o.shape)} and do {tuple(do.shape)} must be like q {tuple(q.shape)}")
-    if lse.shape != (B, Hq, Lq) or lse.dtype != torch.float32 or lse.device != dev:
+    if lse.shape != (B, Hq, Lq) or lse.dtype is not torch.float32 or lse.device != dev:
         raise ValueError(f"lse must be a float32 tensor of shape {(B, Hq, Lq)}")
     lse = lse.contiguous()
     start, end = _bounds(key_start, "key_start", B, dev), _bounds(key_end, "key_end", B, dev)
-    dq, dk, dv = (_like_projection(B, H, L, D, dev) for H, L in ((Hq, Lq), (Hkv, Lk), (Hkv, Lk)))
+    dq, dqh = _like_projection(B, Hq, Lq, D, dev)
+    dk, dkh = _like_projection(B, Hkv, Lk, D, dev)
+    dv, dvh = _like_projection(B, Hkv, Lk, D, dev)
     lib = _lib.load()
-    ws = torch.empty(lib.lamq_attention_backward_workspace_size(B, Hq, Lq), dtype=torch.uint8, device=dev)
-    args = ATTENTION_ARGS.pack(B, Hq, Hkv, D, causal, Lq, Lk, scale, 0, ptr(start) or 0, ptr(end) or 0, *_pack(q),
-                               *_pack(k), *_pack(v), *_pack(o), lse.data_ptr(), *_pack(do), *_pack(dq), *_pack(dk),
-                               *_pack(dv))
-    with torch.cuda.device(dev):
-        check(lib.lamq_attention_backward(args, ptr(ws), ws.numel(), ptr(_STATUS.on(dev)), stream_ptr(dev)),
+    size = lib.lamq_attention_backward_workspace_size(B, Hq, Lq)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    args = ATTENTION_ARGS.pack(B, Hq, Hkv, D, causal, Lq, Lk, scale, 0, ptr(start) or 0, ptr(end) or 0, *qh, *kh, *vh,
+                               *oh, lse.data_ptr(), *doh, *dqh, *dkh, *dvh)
+    here, stream = launch_on(dev)
+    with here:
+        check(lib.lamq_attention_backward(args, ws.data_ptr(), size, _STATUS.on(dev).data_ptr(), stream),
               "lamq_attention_backward")
     return dq, dk, dv
 

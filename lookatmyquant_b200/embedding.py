@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib, codes
-from ._lib import check, ptr, stream_ptr
+from ._lib import check, launch_on, ptr
 from .quantize import Dense, parse
 from .rotation import Rotation
 
@@ -140,12 +140,13 @@ def lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_i
     dev = table.device
     ids = _ids(ids, dev)
     V, d = table.shape
-    out = torch.empty(*ids.shape, d, dtype=table.dtype, device=dev)
-    with torch.cuda.device(dev):
+    out = torch.empty((*ids.shape, d), dtype=table.dtype, device=dev)
+    here, stream = launch_on(dev)
+    with here:
         check(_lib.load().lamq_embedding_lookup(
             ptr(table), _DTYPES[table.dtype], max(table.stride(0), d), V, d, ptr(ids), ids.dtype == torch.int64,
             ids.numel(), scale, _padding(padding_idx, V), ptr(out), d, ptr(_STATUS.on(dev)),
-            stream_ptr(dev)), "lamq_embedding_lookup")
+            stream), "lamq_embedding_lookup")
     return out
 
 
@@ -171,12 +172,14 @@ def lookup_gradient(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: flo
         out = torch.empty(rows, d, dtype=grad.dtype, device=dev)
     lib = _lib.load()
     n = ids.numel()
-    ws = torch.empty(lib.lamq_embedding_gradient_workspace_size(n, d), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
+    size = lib.lamq_embedding_gradient_workspace_size(n, d)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    here, stream = launch_on(dev)
+    with here:
         check(lib.lamq_embedding_gradient(
             ptr(grad), _DTYPES[grad.dtype], max(grad.stride(0), d), ptr(ids), ids.dtype == torch.int64, n, rows, d,
             scale, _padding(padding_idx, rows), accumulate, ptr(out), max(out.stride(0), d), ptr(ws),
-            ws.numel(), ptr(_STATUS.on(dev)), stream_ptr(dev)), "lamq_embedding_gradient")
+            size, ptr(_STATUS.on(dev)), stream), "lamq_embedding_gradient")
     return out
 
 

@@ -15,7 +15,7 @@ import struct
 import torch
 
 from . import _lib
-from ._lib import check, ptr, stream_ptr
+from ._lib import check, launch_on, ptr
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # Muon's quintic: steep at zero, singular values end within about [0.7, 1.2]
 
@@ -58,10 +58,11 @@ def newton_schulz(G: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS, ep
     out = torch.empty(G.shape, dtype=torch.bfloat16, device=dev)
     lib = _lib.load()
     ws = torch.empty(lib.lamq_newton_schulz_workspace_size(batch, m, n), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
+    here, stream = launch_on(dev)
+    with here:
         check(lib.lamq_newton_schulz(ptr(X), _DTYPES[X.dtype], max(X.stride(-2), n) if X.numel() else n,
                                      X.stride(0) if X.ndim == 3 else 0, batch, m, n, steps, coef, eps, ptr(out),
-                                     ptr(ws), ws.numel(), ptr(_STATUS.on(dev)), stream_ptr(dev)), "lamq_newton_schulz")
+                                     ptr(ws), ws.numel(), ptr(_STATUS.on(dev)), stream), "lamq_newton_schulz")
     return out
 
 

@@ -66,11 +66,14 @@ struct Sizes {
     static constexpr int CHUNK = kTile * 128;           // bytes of a chunk of 128 rows
     static constexpr int TILE = NC * CHUNK;             // bytes of a 128 x HD tile
     static constexpr int FWD_STAGES = HD == 128 ? 4 : 6;
-    static constexpr int BWD_STAGES = 2;
-    static constexpr int ROWSTATS = 2 * kTile * 4;      // lse and D of a query tile
-    static constexpr size_t FWD_SMEM = 1024 + 2 * TILE + FWD_STAGES * TILE + 256;
-    static constexpr size_t DQ_SMEM = 1024 + 2 * TILE + 2 * BWD_STAGES * TILE + 256;
-    static constexpr size_t DKV_SMEM = 1024 + 2 * TILE + BWD_STAGES * (2 * TILE + ROWSTATS) + 256;
+    // backward: stages of the operand that two products read (K for dQ, Q for dK and dV) and of the one that the first
+    // product alone reads early (V, dO). The former is released a whole tile later: with two stages for both, its next
+    // load came a TMA latency too late and S waited 1100 of 3300 cycles a tile.
+    static constexpr int LATE_STAGES = HD == 128 ? 3 : 4, EARLY_STAGES = HD == 128 ? 2 : 4;
+    static constexpr int ROW = kTile * 4;               // bytes of lse (or D) of a query tile
+    static constexpr size_t FWD_SMEM = 2 * TILE + FWD_STAGES * TILE + 256;
+    static constexpr size_t DQ_SMEM = 2 * TILE + (LATE_STAGES + EARLY_STAGES) * TILE + 256;
+    static constexpr size_t DKV_SMEM = 2 * TILE + (LATE_STAGES + EARLY_STAGES) * (TILE + ROW) + 256;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -98,26 +101,33 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap *map, 
     for (int c = 0; c < Sizes<HD>::NC; ++c) tma_load_4d(dst + c * Sizes<HD>::CHUNK, map, 64 * c, row, h, b, bar);
 }
 
+// Descriptors of a tile's first K step: K-major (rows as M or N) and as 128 rows of K by HD columns of N. Later steps add
+// constants to them (a shared-memory address below 256 KiB never carries out of the address field): the issuing thread
+// has a few cycles per MMA, and computing whole descriptors there held the tensor core up.
+__device__ __forceinline__ uint64_t rows_desc(uint32_t tile) { return smem_desc_sw128(tile, 16, 1024); }
+
+template <int HD>
+__device__ __forceinline__ uint64_t cols_desc(uint32_t tile) { return smem_desc_sw128(tile, Sizes<HD>::CHUNK, 1024); }
+
 // D (+)= A·Bᵀ over HD, both tiles 128 x HD (K-major).
 template <int HD>
-__device__ __forceinline__ void mma_rows_rows(uint32_t d, uint32_t a, uint32_t b) {
+__device__ __forceinline__ void mma_rows_rows(uint32_t d, uint64_t a, uint64_t b) {
     constexpr uint32_t idesc = idesc_bf16_f32(kTile, kTile, false, false);
 #pragma unroll
     for (int kk = 0; kk < HD / 16; ++kk) {
-        const uint32_t at = (kk / 4) * Sizes<HD>::CHUNK + (kk % 4) * 32;
-        mma_f16_ss(d, smem_desc_sw128(a + at, 16, 1024), smem_desc_sw128(b + at, 16, 1024), idesc, kk > 0);
+        const uint32_t at = ((kk / 4) * Sizes<HD>::CHUNK + (kk % 4) * 32) >> 4;
+        mma_f16_ss(d, a + at, b + at, idesc, kk > 0);
     }
 }
 
 // D (+)= A·B, A 128 x 128 bf16 in TMEM (its columns 64.. from a + hi_cols), B a tile of 128 rows x HD.
 template <int HD>
-__device__ __forceinline__ void mma_tmem_rows(uint32_t d, uint32_t a, uint32_t hi_cols, uint32_t b, bool accumulate) {
+__device__ __forceinline__ void mma_tmem_rows(uint32_t d, uint32_t a, uint32_t hi_cols, uint64_t b, bool accumulate) {
     constexpr uint32_t idesc = idesc_bf16_f32(kTile, HD, false, true);
 #pragma unroll
-    for (int kk = 0; kk < kTile / 16; ++kk) {
-        const uint32_t at = a + (kk < 4 ? kk * 8 : hi_cols + (kk - 4) * 8);
-        mma_f16_ts(d, at, smem_desc_sw128(b + kk * 2048, Sizes<HD>::CHUNK, 1024), idesc, accumulate || kk > 0);
-    }
+    for (int kk = 0; kk < kTile / 16; ++kk)
+        mma_f16_ts(d, a + (kk < 4 ? kk * 8 : hi_cols + (kk - 4) * 8), b + ((kk * 2048) >> 4), idesc,
+                   kk > 0 ? 1u : (uint32_t)accumulate);
 }
 
 // A warp zeroes the rows of a tile outside [lo, hi) (whole rows: the swizzle stays inside a row).
@@ -139,8 +149,11 @@ __device__ __forceinline__ void wait_bounded(uint32_t bar, uint32_t parity) {
     }
 }
 
-__device__ __forceinline__ uint8_t *align_smem(uint8_t *p) {
-    return reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(p) + 1023) & ~uintptr_t(1023));
+// One arrival for the warp, after its TMEM reads and writes.
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
 // A thread's row of an accumulator, times `f`, as bf16 (cols < D; D is a multiple of 8).
@@ -185,8 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                              const __grid_constant__ CUtensorMap mapV, Shape s, Rows out, float *__restrict__ lse) {
     using Z = Sizes<HD>;
     constexpr int STAGES = Z::FWD_STAGES;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = align_smem(smem_raw);
+    extern __shared__ __align__(1024) uint8_t smem[];  // swizzled tiles start at multiples of 1024 bytes
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + STAGES) * Z::TILE);
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 8);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -206,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 2 * STAGES + 1; ++i) mbar_init(full0 + 8 * i, 1);
         for (int t = 0; t < 2; ++t) {
             mbar_init(s_full0 + 8 * t, 1);
-            mbar_init(p_ready0 + 8 * t, 128);
+            mbar_init(p_ready0 + 8 * t, 4);
             mbar_init(pv_done0 + 8 * t, 1);
         }
         mbar_init(drain, 1);
@@ -247,13 +259,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 1) {
         if (n > 0) {  // ---- MMA issuer (the whole warp walks along: it zeroes rows of V outside the key range)
+            const uint64_t q_desc = rows_desc(sq), kv_desc = rows_desc(skv), v_desc = cols_desc<HD>(skv);
             bool ok = mbar_wait(q_full, 0, s.status) && mbar_wait(full0, 0, s.status);
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
             if (ok && lane == 0) {
                 for (int t = 0; t < 2; ++t)
                     if ((t ? n1 : n0) > 0) {
-                        mma_rows_rows<HD>(tmem + t * kTile, sq + t * Z::TILE, skv);
+                        mma_rows_rows<HD>(tmem + t * kTile, q_desc + t * (Z::TILE >> 4), kv_desc);
                         mma_commit(s_full0 + 8 * t);
                     }
                 mma_commit(empty0);
@@ -273,13 +286,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (!ok) break;
                         tc_fence_after();
                         if (lane == 0) {
-                            mma_tmem_rows<HD>(tmem + 2 * kTile + t * HD, tmem + t * kTile, 32, skv + sv * Z::TILE, j > 0);
+                            mma_tmem_rows<HD>(tmem + 2 * kTile + t * HD, tmem + t * kTile, 32, v_desc + sv * (Z::TILE >> 4), j > 0);
                             mma_commit(pv_done0 + 8 * t);
                         }
                     }
                     if (t == 1 && lane == 0) mma_commit(empty0 + 8 * sv);
                     if (j + 1 < nt && lane == 0) {
-                        mma_rows_rows<HD>(tmem + t * kTile, sq + t * Z::TILE, skv + sk * Z::TILE);
+                        mma_rows_rows<HD>(tmem + t * kTile, q_desc + t * (Z::TILE >> 4), kv_desc + sk * (Z::TILE >> 4));
                         mma_commit(s_full0 + 8 * t);
                     }
                     if (t == 1 && j + 1 < n && lane == 0) mma_commit(empty0 + 8 * sk);
@@ -356,8 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             sum += (part[0] + part[1]) + (part[2] + part[3]);
             tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(p_ready0 + 8 * t);
+            warp_arrive(p_ready0 + 8 * t);
         }
         if (ok && nt > 0) {
             ok = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * t, (nt - 1) & 1, s.status));
@@ -417,18 +429,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapG, Shape s,
                         const float *__restrict__ lse2, const float *__restrict__ Dr, Rows dq) {
     using Z = Sizes<HD>;
-    constexpr int STAGES = Z::BWD_STAGES;
+    constexpr int KS = Z::LATE_STAGES, VS = Z::EARLY_STAGES;
     constexpr uint32_t kDQ = 0, kS = 128, kP = 256, kDS = 384;  // TMEM columns
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = align_smem(smem_raw);
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + 2 * STAGES) * Z::TILE);
-    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 4 * STAGES + 9);
+    extern __shared__ __align__(1024) uint8_t smem[];  // swizzled tiles start at multiples of 1024 bytes
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + KS + VS) * Z::TILE);
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 2 * (KS + VS) + 9);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // K stages 0.., V stages STAGES..
-    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + 2 * STAGES), q_full = smem_u32(bars + 4 * STAGES);
+    const uint32_t k_full0 = smem_u32(bars), v_full0 = k_full0 + 8 * KS, k_empty0 = v_full0 + 8 * VS,
+                   v_empty0 = k_empty0 + 8 * KS, q_full = v_empty0 + 8 * VS;
     const uint32_t s_full = q_full + 8, s_free = q_full + 16, p_full = q_full + 24, p_free = q_full + 32;
     const uint32_t ds_ready = q_full + 40, ds_free = q_full + 48, drain = q_full + 56;
-    const uint32_t sq = smem_u32(smem), sg = sq + Z::TILE, sk = sg + Z::TILE, sv = sk + STAGES * Z::TILE;
+    const uint32_t sq = smem_u32(smem), sg = sq + Z::TILE, sk = sg + Z::TILE, sv = sk + KS * Z::TILE;
 
     const int tiles = s.lq_pad / kTile, heads = s.Hq * s.B;
     const int qt = tiles - 1 - (int)(blockIdx.x / heads);
@@ -439,12 +450,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int n = key_tiles(s, row0, lo, hi), j0 = lo / kTile;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 4 * STAGES + 1; ++i) mbar_init(full0 + 8 * i, 1);
+        for (int i = 0; i < 2 * (KS + VS) + 1; ++i) mbar_init(k_full0 + 8 * i, 1);
         mbar_init(s_full, 1);
-        mbar_init(s_free, 256);
+        mbar_init(s_free, 8);
         mbar_init(p_full, 1);
-        mbar_init(p_free, 256);
-        mbar_init(ds_ready, 256);
+        mbar_init(p_free, 8);
+        mbar_init(ds_ready, 8);
         mbar_init(ds_free, 1);
         mbar_init(drain, 1);
         fence_mbar_init();
@@ -467,65 +478,65 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_expect_tx(q_full, 2 * Z::TILE);
             load_tile<HD>(sq, &mapQ, row0, h, b, q_full);
             load_tile<HD>(sg, &mapG, row0, h, b, q_full);
-            int issued = 0;
+            int k_issued = 0, v_issued = 0;
             bool ok = true;
-            for (; issued < n; ++issued) {
-                const int st = issued % STAGES;
-                const uint32_t par = ((issued / STAGES) & 1) ^ 1;
-                ok = mbar_wait(empty0 + 8 * st, par, s.status);
+            for (int j = 0; j < n; ++j) {  // V's stage is released by an earlier product than K's of the same key tile
+                const int ks = j % KS, vs = j % VS, row = (j0 + j) * kTile;
+                ok = mbar_wait(k_empty0 + 8 * ks, ((j / KS) & 1) ^ 1, s.status);
                 if (!ok) break;
-                mbar_expect_tx(full0 + 8 * st, Z::TILE);
-                load_tile<HD>(sk + st * Z::TILE, &mapK, (j0 + issued) * kTile, hk, b, full0 + 8 * st);
-                // V's stage is released by an earlier product than K's of the same key tile
-                ok = mbar_wait(empty0 + 8 * (STAGES + st), par, s.status);
+                mbar_expect_tx(k_full0 + 8 * ks, Z::TILE);
+                load_tile<HD>(sk + ks * Z::TILE, &mapK, row, hk, b, k_full0 + 8 * ks);
+                ++k_issued;
+                ok = mbar_wait(v_empty0 + 8 * vs, ((j / VS) & 1) ^ 1, s.status);
                 if (!ok) break;
-                mbar_expect_tx(full0 + 8 * (STAGES + st), Z::TILE);
-                load_tile<HD>(sv + st * Z::TILE, &mapV, (j0 + issued) * kTile, hk, b, full0 + 8 * (STAGES + st));
+                mbar_expect_tx(v_full0 + 8 * vs, Z::TILE);
+                load_tile<HD>(sv + vs * Z::TILE, &mapV, row, hk, b, v_full0 + 8 * vs);
+                ++v_issued;
             }
             if (!ok) {
                 wait_bounded(q_full, 0);
-                for (int i = max(0, issued - STAGES); i < issued; ++i)
-                    for (int w = 0; w < 2; ++w) wait_bounded(full0 + 8 * (w * STAGES + i % STAGES), (i / STAGES) & 1);
-                wait_bounded(full0 + 8 * (issued % STAGES), (issued / STAGES) & 1);
+                for (int i = max(0, k_issued - KS); i < k_issued; ++i) wait_bounded(k_full0 + 8 * (i % KS), (i / KS) & 1);
+                for (int i = max(0, v_issued - VS); i < v_issued; ++i) wait_bounded(v_full0 + 8 * (i % VS), (i / VS) & 1);
             }
         }
     } else if (warp == 1) {
         if (n > 0) {
+            const uint64_t q_desc = rows_desc(sq), g_desc = rows_desc(sg), k_desc = rows_desc(sk), v_desc = rows_desc(sv),
+                           kc_desc = cols_desc<HD>(sk);
             bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, s.status));
             // S and dP of key tile j run while the warps work on tile j − 1; then dQ of tile j − 1
             for (int j = 0; ok && j <= n; ++j) {
                 if (j < n) {
-                    const int st = j % STAGES;
-                    const uint32_t par = (j / STAGES) & 1;
-                    ok = mbar_wait(full0 + 8 * st, par, s.status) && mbar_wait(s_free, (j & 1) ^ 1, s.status);
+                    const int ks = j % KS, vs = j % VS;
+                    ok = mbar_wait(k_full0 + 8 * ks, (j / KS) & 1, s.status) && mbar_wait(s_free, (j & 1) ^ 1, s.status);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     const int key0 = (j0 + j) * kTile;
-                    if (key0 < lo || key0 + kTile > hi) zero_rows<HD>(sk + st * Z::TILE, lo - key0, hi - key0);
+                    if (key0 < lo || key0 + kTile > hi) zero_rows<HD>(sk + ks * Z::TILE, lo - key0, hi - key0);
                     tc_fence_after();
                     if (lane == 0) {
-                        mma_rows_rows<HD>(tmem + kS, sq, sk + st * Z::TILE);
+                        mma_rows_rows<HD>(tmem + kS, q_desc, k_desc + ks * (Z::TILE >> 4));
                         mma_commit(s_full);
                     }
-                    ok = mbar_wait(full0 + 8 * (STAGES + st), par, s.status) && mbar_wait(p_free, (j & 1) ^ 1, s.status);
+                    ok = mbar_wait(v_full0 + 8 * vs, (j / VS) & 1, s.status) && mbar_wait(p_free, (j & 1) ^ 1, s.status);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after();
                     if (lane == 0) {
-                        mma_rows_rows<HD>(tmem + kP, sg, sv + st * Z::TILE);
+                        mma_rows_rows<HD>(tmem + kP, g_desc, v_desc + vs * (Z::TILE >> 4));
                         mma_commit(p_full);
-                        mma_commit(empty0 + 8 * (STAGES + st));
+                        mma_commit(v_empty0 + 8 * vs);
                     }
                 }
                 if (j > 0) {
-                    const int st = (j - 1) % STAGES;
+                    const int ks = (j - 1) % KS;
                     ok = __all_sync(0xffffffffu, mbar_wait(ds_ready, (j - 1) & 1, s.status));
                     if (!ok) break;
                     tc_fence_after();
                     if (lane == 0) {
-                        mma_tmem_rows<HD>(tmem + kDQ, tmem + kDS, 32, sk + st * Z::TILE, j > 1);
+                        mma_tmem_rows<HD>(tmem + kDQ, tmem + kDS, 32, kc_desc + ks * (Z::TILE >> 4), j > 1);
                         mma_commit(ds_free);
-                        mma_commit(empty0 + 8 * st);
+                        mma_commit(k_empty0 + 8 * ks);
                     }
                 }
             }
@@ -551,8 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_load32(tmem + lanes + kS + 64 * half, r[0]);
             tmem_load32(tmem + lanes + kS + 64 * half + 32, r[1]);
             tmem_ld_wait();
-            tc_fence_before();
-            mbar_arrive(s_free);
+            warp_arrive(s_free);
             const int key0 = (j0 + j) * kTile;
             const bool edge = key0 < lo || key0 + kTile > hi || (s.causal && key0 + kTile - 1 > row0 + s.off);
             const int clo = lo - key0 - 64 * half, chi = row_hi - key0 - 64 * half;
@@ -565,8 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_load32(tmem + lanes + kP + 64 * half, d[0]);
             tmem_load32(tmem + lanes + kP + 64 * half + 32, d[1]);
             tmem_ld_wait();
-            tc_fence_before();
-            mbar_arrive(p_free);
+            warp_arrive(p_free);
 #pragma unroll
             for (int c = 0; c < 64; ++c) {
                 const float x = __uint_as_float(r[c >> 5][c & 31]) * (__uint_as_float(d[c >> 5][c & 31]) - Di);
@@ -586,8 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             tmem_store32(tmem + lanes + kDS + 32 * half, pk);
             tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(ds_ready);
+            warp_arrive(ds_ready);
         }
         if (ok && n > 0) {
             ok = __all_sync(0xffffffffu, mbar_wait(ds_free, (n - 1) & 1, s.status));
@@ -611,21 +619,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                          const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapG, Shape s,
                          const float *__restrict__ lse2, const float *__restrict__ Dr, Rows dk, Rows dv) {
     using Z = Sizes<HD>;
-    constexpr int STAGES = Z::BWD_STAGES;
+    constexpr int QS = Z::LATE_STAGES, GS = Z::EARLY_STAGES;  // Q (with lse), dO (with D)
     // TMEM columns. Pᵀ and dSᵀ (bf16) lie over Sᵀ and dPᵀ: the threads of columns 0..63 write columns 0..31 of them,
     // those of columns 64..127 write 64..95, so that no thread overwrites what another has yet to read
     constexpr uint32_t kS = 0, kP = 128, kDV = 256, kDK = 384;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = align_smem(smem_raw);
-    float *stats = reinterpret_cast<float *>(smem + (2 + 2 * STAGES) * Z::TILE);  // per stage: lse2, D
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + 2 * STAGES) * Z::TILE + STAGES * Z::ROWSTATS);
-    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 4 * STAGES + 7);
+    extern __shared__ __align__(1024) uint8_t smem[];  // swizzled tiles start at multiples of 1024 bytes
+    float *row_lse = reinterpret_cast<float *>(smem + (2 + QS + GS) * Z::TILE), *row_d = row_lse + QS * kTile;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(row_d + GS * kTile);
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 2 * (QS + GS) + 7);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // Q stages (with lse2) 0.., dO stages (with D) STAGES..
-    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + 2 * STAGES), kv_full = smem_u32(bars + 4 * STAGES);
+    const uint32_t q_full0 = smem_u32(bars), g_full0 = q_full0 + 8 * QS, q_empty0 = g_full0 + 8 * GS,
+                   g_empty0 = q_empty0 + 8 * QS, kv_full = g_empty0 + 8 * GS;
     const uint32_t s_full = kv_full + 8, p_full = kv_full + 16, p_ready = kv_full + 24, ds_ready = kv_full + 32;
     const uint32_t done = kv_full + 40;
-    const uint32_t sk = smem_u32(smem), sv = sk + Z::TILE, sq = sv + Z::TILE, sg = sq + STAGES * Z::TILE;
+    const uint32_t sk = smem_u32(smem), sv = sk + Z::TILE, sq = sv + Z::TILE, sg = sq + QS * Z::TILE;
 
     const int heads = s.Hkv * s.B;
     const int kt = (int)(blockIdx.x / heads);  // the first keys are seen by the most queries: they come first
@@ -640,11 +647,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int n = nq * s.group;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 4 * STAGES + 1; ++i) mbar_init(full0 + 8 * i, 1);
+        for (int i = 0; i < 2 * (QS + GS) + 1; ++i) mbar_init(q_full0 + 8 * i, 1);
         mbar_init(s_full, 1);
         mbar_init(p_full, 1);
-        mbar_init(p_ready, 256);
-        mbar_init(ds_ready, 256);
+        mbar_init(p_ready, 8);
+        mbar_init(ds_ready, 8);
         mbar_init(done, 1);
         fence_mbar_init();
         prefetch_tmap(&mapQ);
@@ -666,55 +673,54 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_expect_tx(kv_full, 2 * Z::TILE);
             load_tile<HD>(sk, &mapK, key0, hk, b, kv_full);
             load_tile<HD>(sv, &mapV, key0, hk, b, kv_full);
-            int issued = 0;
+            int q_issued = 0, g_issued = 0;
             bool ok = true;
-            for (; issued < n; ++issued) {
-                const int st = issued % STAGES, h = hk * s.group + issued / nq, row = (t0 + issued % nq) * kTile;
+            for (int j = 0; j < n; ++j) {  // dO's stage is released by an earlier product than Q's of the same query tile
+                const int qs = j % QS, gs = j % GS, h = hk * s.group + j / nq, row = (t0 + j % nq) * kTile;
                 const int64_t at = ((int64_t)b * s.Hq + h) * s.lq_pad + row;
-                const uint32_t par = ((issued / STAGES) & 1) ^ 1;
-                float *st_stats = stats + st * 2 * kTile;
-                // dO's stage is released by an earlier product than Q's of the same query tile
-                ok = mbar_wait(empty0 + 8 * st, par, s.status);
+                ok = mbar_wait(q_empty0 + 8 * qs, ((j / QS) & 1) ^ 1, s.status);
                 if (!ok) break;
-                mbar_expect_tx(full0 + 8 * st, Z::TILE + kTile * 4);
-                load_tile<HD>(sq + st * Z::TILE, &mapQ, row, h, b, full0 + 8 * st);
-                bulk_load(smem_u32(st_stats), lse2 + at, kTile * 4, full0 + 8 * st);
-                ok = mbar_wait(empty0 + 8 * (STAGES + st), par, s.status);
+                mbar_expect_tx(q_full0 + 8 * qs, Z::TILE + Z::ROW);
+                load_tile<HD>(sq + qs * Z::TILE, &mapQ, row, h, b, q_full0 + 8 * qs);
+                bulk_load(smem_u32(row_lse + qs * kTile), lse2 + at, Z::ROW, q_full0 + 8 * qs);
+                ++q_issued;
+                ok = mbar_wait(g_empty0 + 8 * gs, ((j / GS) & 1) ^ 1, s.status);
                 if (!ok) break;
-                mbar_expect_tx(full0 + 8 * (STAGES + st), Z::TILE + kTile * 4);
-                load_tile<HD>(sg + st * Z::TILE, &mapG, row, h, b, full0 + 8 * (STAGES + st));
-                bulk_load(smem_u32(st_stats + kTile), Dr + at, kTile * 4, full0 + 8 * (STAGES + st));
+                mbar_expect_tx(g_full0 + 8 * gs, Z::TILE + Z::ROW);
+                load_tile<HD>(sg + gs * Z::TILE, &mapG, row, h, b, g_full0 + 8 * gs);
+                bulk_load(smem_u32(row_d + gs * kTile), Dr + at, Z::ROW, g_full0 + 8 * gs);
+                ++g_issued;
             }
             if (!ok) {
                 wait_bounded(kv_full, 0);
-                for (int i = max(0, issued - STAGES); i < issued; ++i)
-                    for (int w = 0; w < 2; ++w) wait_bounded(full0 + 8 * (w * STAGES + i % STAGES), (i / STAGES) & 1);
-                wait_bounded(full0 + 8 * (issued % STAGES), (issued / STAGES) & 1);
+                for (int i = max(0, q_issued - QS); i < q_issued; ++i) wait_bounded(q_full0 + 8 * (i % QS), (i / QS) & 1);
+                for (int i = max(0, g_issued - GS); i < g_issued; ++i) wait_bounded(g_full0 + 8 * (i % GS), (i / GS) & 1);
             }
         }
     } else if (warp == 1) {
         if (n > 0) {
+            const uint64_t k_desc = rows_desc(sk), v_desc = rows_desc(sv), q_desc = rows_desc(sq), g_desc = rows_desc(sg),
+                           qc_desc = cols_desc<HD>(sq), gc_desc = cols_desc<HD>(sg);
             bool ok = __all_sync(0xffffffffu, mbar_wait(kv_full, 0, s.status));
             // in issue order: S(0) dP(0) | dV(j) S(j + 1) | dK(j) dP(j + 1) | ...: the warps form P(j) while dK(j − 1)
             // and dP(j) run, and dS(j) while dV(j) and S(j + 1) run
             for (int j = -1; ok && j < n; ++j) {
-                const int st = j % STAGES, nx = (j + 1) % STAGES;
-                const uint32_t npar = ((j + 1) / STAGES) & 1;
+                const int qs = j % QS, gs = j % GS, qn = (j + 1) % QS, gn = (j + 1) % GS;
                 const int qrow = (t0 + (j + 1) % nq) * kTile;
                 if (j >= 0) {
                     ok = __all_sync(0xffffffffu, mbar_wait(p_ready, j & 1, s.status));
                     if (!ok) break;
                     tc_fence_after();
                     if (lane == 0) {
-                        mma_tmem_rows<HD>(tmem + kDV, tmem + kS, 64, sg + st * Z::TILE, j > 0);
+                        mma_tmem_rows<HD>(tmem + kDV, tmem + kS, 64, gc_desc + gs * (Z::TILE >> 4), j > 0);
                     }
                 }
                 if (j + 1 < n) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * nx, npar, s.status));
+                    ok = __all_sync(0xffffffffu, mbar_wait(q_full0 + 8 * qn, ((j + 1) / QS) & 1, s.status));
                     if (!ok) break;
-                    if (qrow < q_lo) zero_rows<HD>(sq + nx * Z::TILE, q_lo - qrow, kTile);
+                    if (qrow < q_lo) zero_rows<HD>(sq + qn * Z::TILE, q_lo - qrow, kTile);
                     if (lane == 0) {
-                        mma_rows_rows<HD>(tmem + kS, sk, sq + nx * Z::TILE);
+                        mma_rows_rows<HD>(tmem + kS, k_desc, q_desc + qn * (Z::TILE >> 4));
                         mma_commit(s_full);
                     }
                 }
@@ -723,17 +729,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!ok) break;
                     tc_fence_after();
                     if (lane == 0) {
-                        mma_commit(empty0 + 8 * (STAGES + st));  // D(j) was read before ds_ready, dO(j) by dV(j)
-                        mma_tmem_rows<HD>(tmem + kDK, tmem + kP, 64, sq + st * Z::TILE, j > 0);
-                        mma_commit(empty0 + 8 * st);
+                        mma_commit(g_empty0 + 8 * gs);  // D(j) was read before ds_ready, dO(j) by dV(j)
+                        mma_tmem_rows<HD>(tmem + kDK, tmem + kP, 64, qc_desc + qs * (Z::TILE >> 4), j > 0);
+                        mma_commit(q_empty0 + 8 * qs);
                     }
                 }
                 if (j + 1 < n) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * (STAGES + nx), npar, s.status));
+                    ok = __all_sync(0xffffffffu, mbar_wait(g_full0 + 8 * gn, ((j + 1) / GS) & 1, s.status));
                     if (!ok) break;
-                    if (qrow < q_lo) zero_rows<HD>(sg + nx * Z::TILE, q_lo - qrow, kTile);
+                    if (qrow < q_lo) zero_rows<HD>(sg + gn * Z::TILE, q_lo - qrow, kTile);
                     if (lane == 0) {
-                        mma_rows_rows<HD>(tmem + kP, sv, sg + nx * Z::TILE);
+                        mma_rows_rows<HD>(tmem + kP, v_desc, g_desc + gn * (Z::TILE >> 4));
                         mma_commit(p_full);
                     }
                 }
@@ -752,14 +758,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool edge_keys = key0 < lo || key0 + kTile > hi;
         bool ok = true;
         for (int j = 0; j < n; ++j) {
-            const int st = j % STAGES, row0 = (t0 + j % nq) * kTile;
-            const float4 *l4 = reinterpret_cast<const float4 *>(stats + st * 2 * kTile + 64 * half);
-            const float4 *d4 = reinterpret_cast<const float4 *>(stats + st * 2 * kTile + kTile + 64 * half);
+            const int qs = j % QS, gs = j % GS, row0 = (t0 + j % nq) * kTile;
+            const float4 *l4 = reinterpret_cast<const float4 *>(row_lse + qs * kTile + 64 * half);
+            const float4 *d4 = reinterpret_cast<const float4 *>(row_d + gs * kTile + 64 * half);
             const bool edge = edge_keys || (s.causal && key0 + kTile - 1 > row0 + s.off);
             const int clo = !in ? 64 : s.causal ? key - s.off - row0 - 64 * half : 0;  // columns before are masked
             ok = __all_sync(0xffffffffu, mbar_wait(s_full, j & 1, s.status));
             // the tile's statistics came with Q and dO: their barriers make them visible to this thread
-            ok = ok && __all_sync(0xffffffffu, mbar_wait(full0 + 8 * st, (j / STAGES) & 1, s.status));
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(q_full0 + 8 * qs, (j / QS) & 1, s.status));
             if (!ok) break;
             tc_fence_after();
             uint32_t r[2][32], pk[32];
@@ -786,11 +792,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 pk[c >> 1] = pack_bf16(__uint_as_float(r[c >> 5][c & 31]), __uint_as_float(r[c >> 5][(c & 31) + 1]));
             tmem_store32(tmem + lanes + kS + 64 * half, pk);
             tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(p_ready);
+            warp_arrive(p_ready);
 
             ok = __all_sync(0xffffffffu, mbar_wait(p_full, j & 1, s.status));
-            ok = ok && __all_sync(0xffffffffu, mbar_wait(full0 + 8 * (STAGES + st), (j / STAGES) & 1, s.status));
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(g_full0 + 8 * gs, (j / GS) & 1, s.status));
             if (!ok) break;
             tc_fence_after();
             uint32_t d[2][32];
@@ -818,8 +823,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 pk[c >> 1] = pack_bf16(__uint_as_float(d[c >> 5][c & 31]), __uint_as_float(d[c >> 5][(c & 31) + 1]));
             tmem_store32(tmem + lanes + kP + 64 * half, pk);
             tmem_st_wait();
-            tc_fence_before();
-            mbar_arrive(ds_ready);
+            warp_arrive(ds_ready);
         }
         const bool live = key < s.Lk;
         if (ok && n > 0) {

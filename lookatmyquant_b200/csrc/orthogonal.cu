@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 2 * SLOTS; ++i) mbar_init(full0 + 8 * i, 1);
         for (int a = 0; a < 2; ++a) {
             mbar_init(tfull0 + 8 * a, 1);
-            mbar_init(tempty0 + 8 * a, 256);
+            mbar_init(tempty0 + 8 * a, 8);
         }
         mbar_init(drain, 1);
         fence_mbar_init();
@@ -487,7 +487,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 tc_fence_before();
-                mbar_arrive(tempty0 + 8 * acc);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(tempty0 + 8 * acc);
             }
         }
         go = grid_barrier(p, target += gridDim.x, shared_ok);

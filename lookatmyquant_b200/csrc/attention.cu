@@ -23,7 +23,9 @@
 //
 // Warp roles (320 threads): warp 0 issues TMA loads, warp 1 the MMAs, warps 2-9 the elementwise work. One thread issues
 // all MMAs of a CTA and the tensor core runs them in issue order, so a product may overwrite TMEM that the product
-// issued before it reads.
+// issued before it reads. That thread does nothing else and waits alone: it runs hardly ahead of the tensor core, and
+// where its warp takes part (a vote after each wait, MMAs predicated by lane) a group of 24 MMAs takes 2475 cycles
+// instead of 1847. Two issuing warps were slower still (their MMAs alternate between accumulators).
 #include <algorithm>
 #include <climits>
 #include <mutex>
@@ -120,6 +122,27 @@ __device__ __forceinline__ void mma_rows_rows(uint32_t d, uint64_t a, uint64_t b
     }
 }
 
+// D = A·Bᵀ over HD, A 128 x HD bf16 in TMEM, B a tile (K-major).
+template <int HD>
+__device__ __forceinline__ void mma_tmem_rows_t(uint32_t d, uint32_t a, uint64_t b) {
+    constexpr uint32_t idesc = idesc_bf16_f32(kTile, kTile, false, false);
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk)
+        mma_f16_ts(d, a + kk * 8, b + (((kk / 4) * Sizes<HD>::CHUNK + (kk % 4) * 32) >> 4), idesc, kk > 0);
+}
+
+// A thread's row of a tile's 64-wide chunk (swizzled: 16-byte piece c of row r lies at c ^ (r mod 8)) into 32 TMEM columns
+// of its lane, as an A operand.
+__device__ __forceinline__ void chunk_to_tmem(uint32_t chunk, int row, uint32_t taddr) {
+    uint32_t r[32];
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[4 * c]), "=r"(r[4 * c + 1]), "=r"(r[4 * c + 2]), "=r"(r[4 * c + 3])
+                     : "r"(chunk + row * 128 + ((c ^ (row & 7)) << 4)));
+    tmem_store32(taddr, r);
+}
+
 // D (+)= A·B, A 128 x 128 bf16 in TMEM (its columns 64.. from a + hi_cols), B a tile of 128 rows x HD.
 template <int HD>
 __device__ __forceinline__ void mma_tmem_rows(uint32_t d, uint32_t a, uint32_t hi_cols, uint64_t b, bool accumulate) {
@@ -130,17 +153,16 @@ __device__ __forceinline__ void mma_tmem_rows(uint32_t d, uint32_t a, uint32_t h
                    kk > 0 ? 1u : (uint32_t)accumulate);
 }
 
-// A warp zeroes the rows of a tile outside [lo, hi) (whole rows: the swizzle stays inside a row).
+// Threads `me` of `threads` zero the rows of a tile outside [lo, hi) (whole rows: the swizzle stays inside a row), for
+// products issued after the barrier on which they arrive next.
 template <int HD>
-__device__ __forceinline__ void zero_rows(uint32_t tile, int lo, int hi) {
-    const int lane = threadIdx.x & 31;
-    for (int i = lane; i < Sizes<HD>::NC * kTile * 8; i += 32) {
+__device__ __forceinline__ void zero_rows(uint32_t tile, int lo, int hi, int me, int threads) {
+    for (int i = me; i < Sizes<HD>::NC * kTile * 8; i += threads) {
         const int row = (i >> 3) & (kTile - 1);
         if (row < lo || row >= hi)
             asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(tile + i * 16), "r"(0) : "memory");
     }
     fence_async_smem();
-    __syncwarp();
 }
 
 __device__ __forceinline__ void wait_bounded(uint32_t bar, uint32_t parity) {
@@ -258,12 +280,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else if (warp == 1) {
-        if (n > 0) {  // ---- MMA issuer (the whole warp walks along: it zeroes rows of V outside the key range)
+        if (lane == 0 && n > 0) {  // ---- MMA issuer. P lies over S: P·V of key tile j goes before S of tile j + 1
             const uint64_t q_desc = rows_desc(sq), kv_desc = rows_desc(skv), v_desc = cols_desc<HD>(skv);
             bool ok = mbar_wait(q_full, 0, s.status) && mbar_wait(full0, 0, s.status);
-            ok = __all_sync(0xffffffffu, ok);
-            tc_fence_after();
-            if (ok && lane == 0) {
+            if (ok) {
                 for (int t = 0; t < 2; ++t)
                     if ((t ? n1 : n0) > 0) {
                         mma_rows_rows<HD>(tmem + t * kTile, q_desc + t * (Z::TILE >> 4), kv_desc);
@@ -273,37 +293,30 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             for (int j = 0; ok && j < n; ++j) {
                 const int iv = 2 * j + 1, sv = iv % STAGES, ik = iv + 1, sk = ik % STAGES;
-                ok = mbar_wait(full0 + 8 * sv, (iv / STAGES) & 1, s.status);
-                if (ok && j + 1 < n) ok = mbar_wait(full0 + 8 * sk, (ik / STAGES) & 1, s.status);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                const int key0 = (j0 + j) * kTile;
-                if (key0 < lo || key0 + kTile > hi) zero_rows<HD>(skv + sv * Z::TILE, lo - key0, hi - key0);
-                for (int t = 0; t < 2; ++t) {
+                ok = mbar_wait(full0 + 8 * sv, (iv / STAGES) & 1, s.status) &&
+                     (j + 1 == n || mbar_wait(full0 + 8 * sk, (ik / STAGES) & 1, s.status));
+                for (int t = 0; ok && t < 2; ++t) {
                     const int nt = t ? n1 : n0;
                     if (j < nt) {
-                        ok = __all_sync(0xffffffffu, mbar_wait(p_ready0 + 8 * t, j & 1, s.status));
+                        ok = mbar_wait(p_ready0 + 8 * t, j & 1, s.status);
                         if (!ok) break;
                         tc_fence_after();
-                        if (lane == 0) {
-                            mma_tmem_rows<HD>(tmem + 2 * kTile + t * HD, tmem + t * kTile, 32, v_desc + sv * (Z::TILE >> 4), j > 0);
-                            mma_commit(pv_done0 + 8 * t);
-                        }
+                        mma_tmem_rows<HD>(tmem + 2 * kTile + t * HD, tmem + t * kTile, 32, v_desc + sv * (Z::TILE >> 4), j > 0);
+                        mma_commit(pv_done0 + 8 * t);
                     }
-                    if (t == 1 && lane == 0) mma_commit(empty0 + 8 * sv);
-                    if (j + 1 < nt && lane == 0) {
+                    if (j + 1 < nt) {
                         mma_rows_rows<HD>(tmem + t * kTile, q_desc + t * (Z::TILE >> 4), kv_desc + sk * (Z::TILE >> 4));
                         mma_commit(s_full0 + 8 * t);
                     }
-                    if (t == 1 && j + 1 < n && lane == 0) mma_commit(empty0 + 8 * sk);
                 }
+                if (!ok) break;
+                mma_commit(empty0 + 8 * sv);
+                if (j + 1 < n) mma_commit(empty0 + 8 * sk);
             }
-            if (lane == 0) {  // every MMA this thread issued completes before TMEM is released
-                mma_commit(drain);
-                wait_bounded(drain, 0);
-            }
-            __syncwarp();
+            mma_commit(drain);  // every MMA this thread issued completes before TMEM is released
+            wait_bounded(drain, 0);
         }
+        __syncwarp();
     } else {  // ---- softmax: warps 2-5 tile 0, warps 6-9 tile 1, a thread per query
         const int t = (warp - 2) >> 2, quad = warp & 3, nt = t ? n1 : n0;
         const int row0 = (2 * qp + t) * kTile, i = row0 + 32 * quad + lane;
@@ -327,6 +340,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int c = 0; c < kTile; ++c)
                     if (c < clo || c >= chi) r[c >> 5][c & 31] = 0xff800000u;
+                if (key0 < lo || key0 + kTile > hi) {  // (both tiles' warps do: the same zeros)
+                    const int sv = (2 * j + 1) % STAGES;
+                    ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * sv, ((2 * j + 1) / STAGES) & 1, s.status));
+                    if (!ok) break;
+                    zero_rows<HD>(skv + sv * Z::TILE, lo - key0, hi - key0, threadIdx.x - 64 - 128 * t, 128);
+                }
             }
             float mx = -INFINITY;
 #pragma unroll
@@ -430,15 +449,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const float *__restrict__ lse2, const float *__restrict__ Dr, Rows dq) {
     using Z = Sizes<HD>;
     constexpr int KS = Z::LATE_STAGES, VS = Z::EARLY_STAGES;
-    constexpr uint32_t kDQ = 0, kS = 128, kP = 256, kDS = 384;  // TMEM columns
+    // TMEM columns. Q and dO lie there as A operands: from shared memory they would take, with the key tile's rows, all
+    // of its bandwidth. dS (bf16) lies over dP, as in the dkv kernel.
+    constexpr uint32_t kDQ = 0, kS = 128, kP = 256, kQ = 384, kG = 448;
     extern __shared__ __align__(1024) uint8_t smem[];  // swizzled tiles start at multiples of 1024 bytes
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + KS + VS) * Z::TILE);
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 2 * (KS + VS) + 9);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t k_full0 = smem_u32(bars), v_full0 = k_full0 + 8 * KS, k_empty0 = v_full0 + 8 * VS,
                    v_empty0 = k_empty0 + 8 * KS, q_full = v_empty0 + 8 * VS;
-    const uint32_t s_full = q_full + 8, s_free = q_full + 16, p_full = q_full + 24, p_free = q_full + 32;
-    const uint32_t ds_ready = q_full + 40, ds_free = q_full + 48, drain = q_full + 56;
+    const uint32_t q_ready = q_full + 8, s_full = q_full + 16, s_free = q_full + 24, p_full = q_full + 32;
+    const uint32_t ds_ready = q_full + 40, done = q_full + 48;
     const uint32_t sq = smem_u32(smem), sg = sq + Z::TILE, sk = sg + Z::TILE, sv = sk + KS * Z::TILE;
 
     const int tiles = s.lq_pad / kTile, heads = s.Hq * s.B;
@@ -451,13 +472,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2 * (KS + VS) + 1; ++i) mbar_init(k_full0 + 8 * i, 1);
+        mbar_init(q_ready, 8);
         mbar_init(s_full, 1);
         mbar_init(s_free, 8);
         mbar_init(p_full, 1);
-        mbar_init(p_free, 8);
         mbar_init(ds_ready, 8);
-        mbar_init(ds_free, 1);
-        mbar_init(drain, 1);
+        mbar_init(done, 1);
         fence_mbar_init();
         prefetch_tmap(&mapQ);
         prefetch_tmap(&mapK);
@@ -500,52 +520,40 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else if (warp == 1) {
-        if (n > 0) {
-            const uint64_t q_desc = rows_desc(sq), g_desc = rows_desc(sg), k_desc = rows_desc(sk), v_desc = rows_desc(sv),
-                           kc_desc = cols_desc<HD>(sk);
-            bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, 0, s.status));
-            // S and dP of key tile j run while the warps work on tile j − 1; then dQ of tile j − 1
-            for (int j = 0; ok && j <= n; ++j) {
-                if (j < n) {
-                    const int ks = j % KS, vs = j % VS;
-                    ok = mbar_wait(k_full0 + 8 * ks, (j / KS) & 1, s.status) && mbar_wait(s_free, (j & 1) ^ 1, s.status);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    const int key0 = (j0 + j) * kTile;
-                    if (key0 < lo || key0 + kTile > hi) zero_rows<HD>(sk + ks * Z::TILE, lo - key0, hi - key0);
-                    tc_fence_after();
-                    if (lane == 0) {
-                        mma_rows_rows<HD>(tmem + kS, q_desc, k_desc + ks * (Z::TILE >> 4));
-                        mma_commit(s_full);
-                    }
-                    ok = mbar_wait(v_full0 + 8 * vs, (j / VS) & 1, s.status) && mbar_wait(p_free, (j & 1) ^ 1, s.status);
-                    ok = __all_sync(0xffffffffu, ok);
+        if (lane == 0 && n > 0) {
+            const uint64_t k_desc = rows_desc(sk), v_desc = rows_desc(sv), kc_desc = cols_desc<HD>(sk);
+            bool ok = mbar_wait(q_ready, 0, s.status);
+            // in issue order: S(0) dP(0) | S(j + 1) | dQ(j) dP(j + 1) | ...: while the warps form P(j), S(j + 1) runs; while
+            // they go on to P(j + 1), dQ(j) and, over the dS(j) that it read, dP(j + 1) run
+            for (int j = -1; ok && j < n; ++j) {
+                const int kn = (j + 1) % KS, vn = (j + 1) % VS;
+                if (j + 1 < n) {
+                    ok = mbar_wait(k_full0 + 8 * kn, ((j + 1) / KS) & 1, s.status) &&
+                         (j < 0 || mbar_wait(s_free, j & 1, s.status));
                     if (!ok) break;
                     tc_fence_after();
-                    if (lane == 0) {
-                        mma_rows_rows<HD>(tmem + kP, g_desc, v_desc + vs * (Z::TILE >> 4));
-                        mma_commit(p_full);
-                        mma_commit(v_empty0 + 8 * vs);
-                    }
+                    mma_tmem_rows_t<HD>(tmem + kS, tmem + kQ, k_desc + kn * (Z::TILE >> 4));
+                    mma_commit(s_full);
+                    ok = mbar_wait(v_full0 + 8 * vn, ((j + 1) / VS) & 1, s.status);
+                    if (!ok) break;
                 }
-                if (j > 0) {
-                    const int ks = (j - 1) % KS;
-                    ok = __all_sync(0xffffffffu, mbar_wait(ds_ready, (j - 1) & 1, s.status));
+                if (j >= 0) {
+                    ok = mbar_wait(ds_ready, j & 1, s.status);
                     if (!ok) break;
                     tc_fence_after();
-                    if (lane == 0) {
-                        mma_tmem_rows<HD>(tmem + kDQ, tmem + kDS, 32, kc_desc + ks * (Z::TILE >> 4), j > 1);
-                        mma_commit(ds_free);
-                        mma_commit(k_empty0 + 8 * ks);
-                    }
+                    mma_tmem_rows<HD>(tmem + kDQ, tmem + kP, 64, kc_desc + (j % KS) * (Z::TILE >> 4), j > 0);
+                    mma_commit(k_empty0 + 8 * (j % KS));
+                }
+                if (j + 1 < n) {
+                    mma_tmem_rows_t<HD>(tmem + kP, tmem + kG, v_desc + vn * (Z::TILE >> 4));
+                    mma_commit(p_full);
+                    mma_commit(v_empty0 + 8 * vn);
                 }
             }
-            if (lane == 0) {
-                mma_commit(drain);
-                wait_bounded(drain, 0);
-            }
-            __syncwarp();
+            mma_commit(done);
+            wait_bounded(done, 0);
         }
+        __syncwarp();
     } else {  // two threads per query: columns 64·half ..
         const int half = (warp - 2) >> 2, quad = warp & 3;
         const int i = row0 + 32 * quad + lane;
@@ -553,8 +561,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int row_hi = s.causal ? min(hi, i + s.off + 1) : hi;
         const uint32_t lanes = (uint32_t)(32 * quad) << 16;
         const float l2 = lse2[(int64_t)bh * s.lq_pad + i], Di = Dr[(int64_t)bh * s.lq_pad + i];
-        bool ok = true;
-        for (int j = 0; j < n; ++j) {
+        bool ok = n > 0 && __all_sync(0xffffffffu, mbar_wait(q_full, 0, s.status));
+        if (ok) {
+            if (HD == 64) {
+                chunk_to_tmem(half ? sg : sq, 32 * quad + lane, tmem + lanes + (half ? kG : kQ));
+            } else {
+                chunk_to_tmem(sq + half * Z::CHUNK, 32 * quad + lane, tmem + lanes + kQ + 32 * half);
+                chunk_to_tmem(sg + half * Z::CHUNK, 32 * quad + lane, tmem + lanes + kG + 32 * half);
+            }
+            tmem_st_wait();
+            warp_arrive(q_ready);
+        }
+        for (int j = 0; ok && j < n; ++j) {
             ok = __all_sync(0xffffffffu, mbar_wait(s_full, j & 1, s.status));
             if (!ok) break;
             tc_fence_after();
@@ -575,7 +593,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_load32(tmem + lanes + kP + 64 * half, d[0]);
             tmem_load32(tmem + lanes + kP + 64 * half + 32, d[1]);
             tmem_ld_wait();
-            warp_arrive(p_free);
 #pragma unroll
             for (int c = 0; c < 64; ++c) {
                 const float x = __uint_as_float(r[c >> 5][c & 31]) * (__uint_as_float(d[c >> 5][c & 31]) - Di);
@@ -590,18 +607,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int c = 0; c < 64; c += 2)
                 pk[c >> 1] = pack_bf16(__uint_as_float(r[c >> 5][c & 31]), __uint_as_float(r[c >> 5][(c & 31) + 1]));
-            ok = __all_sync(0xffffffffu, mbar_wait(ds_free, (j & 1) ^ 1, s.status));
-            if (!ok) break;
-            tc_fence_after();
-            tmem_store32(tmem + lanes + kDS + 32 * half, pk);
+            if (key0 < lo || key0 + kTile > hi)  // S(j), the other reader of K(j), is done
+                zero_rows<HD>(sk + (j % KS) * Z::TILE, lo - key0, hi - key0, threadIdx.x - 64, 256);
+            tmem_store32(tmem + lanes + kP + 64 * half, pk);
             tmem_st_wait();
             warp_arrive(ds_ready);
         }
-        if (ok && n > 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait(ds_free, (n - 1) & 1, s.status));
+        if (ok) {
+            ok = __all_sync(0xffffffffu, mbar_wait(done, 0, s.status));
             tc_fence_after();
         }
-        if (ok) {
+        if (ok || n == 0) {
             __nv_bfloat16 *dst = dq.p + b * dq.batch + h * dq.head + (int64_t)i * dq.row;
             if (n > 0) store_row<HD / 2>(dst, tmem + lanes + kDQ + half * (HD / 2), half * (HD / 2), s.D, s.scale, live);
             else if (live && half == 0) zero_row(dst, s.D);
@@ -698,58 +714,45 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     } else if (warp == 1) {
-        if (n > 0) {
+        if (lane == 0 && n > 0) {
             const uint64_t k_desc = rows_desc(sk), v_desc = rows_desc(sv), q_desc = rows_desc(sq), g_desc = rows_desc(sg),
                            qc_desc = cols_desc<HD>(sq), gc_desc = cols_desc<HD>(sg);
-            bool ok = __all_sync(0xffffffffu, mbar_wait(kv_full, 0, s.status));
+            bool ok = mbar_wait(kv_full, 0, s.status);
             // in issue order: S(0) dP(0) | dV(j) S(j + 1) | dK(j) dP(j + 1) | ...: the warps form P(j) while dK(j − 1)
             // and dP(j) run, and dS(j) while dV(j) and S(j + 1) run
             for (int j = -1; ok && j < n; ++j) {
                 const int qs = j % QS, gs = j % GS, qn = (j + 1) % QS, gn = (j + 1) % GS;
-                const int qrow = (t0 + (j + 1) % nq) * kTile;
+                if (j + 1 < n) ok = mbar_wait(q_full0 + 8 * qn, ((j + 1) / QS) & 1, s.status);
                 if (j >= 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(p_ready, j & 1, s.status));
+                    ok = ok && mbar_wait(p_ready, j & 1, s.status);
                     if (!ok) break;
                     tc_fence_after();
-                    if (lane == 0) {
-                        mma_tmem_rows<HD>(tmem + kDV, tmem + kS, 64, gc_desc + gs * (Z::TILE >> 4), j > 0);
-                    }
+                    mma_tmem_rows<HD>(tmem + kDV, tmem + kS, 64, gc_desc + gs * (Z::TILE >> 4), j > 0);
                 }
                 if (j + 1 < n) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(q_full0 + 8 * qn, ((j + 1) / QS) & 1, s.status));
                     if (!ok) break;
-                    if (qrow < q_lo) zero_rows<HD>(sq + qn * Z::TILE, q_lo - qrow, kTile);
-                    if (lane == 0) {
-                        mma_rows_rows<HD>(tmem + kS, k_desc, q_desc + qn * (Z::TILE >> 4));
-                        mma_commit(s_full);
-                    }
+                    mma_rows_rows<HD>(tmem + kS, k_desc, q_desc + qn * (Z::TILE >> 4));
+                    mma_commit(s_full);
+                    ok = mbar_wait(g_full0 + 8 * gn, ((j + 1) / GS) & 1, s.status);
                 }
                 if (j >= 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(ds_ready, j & 1, s.status));
+                    ok = ok && mbar_wait(ds_ready, j & 1, s.status);
                     if (!ok) break;
                     tc_fence_after();
-                    if (lane == 0) {
-                        mma_commit(g_empty0 + 8 * gs);  // D(j) was read before ds_ready, dO(j) by dV(j)
-                        mma_tmem_rows<HD>(tmem + kDK, tmem + kP, 64, qc_desc + qs * (Z::TILE >> 4), j > 0);
-                        mma_commit(q_empty0 + 8 * qs);
-                    }
+                    mma_commit(g_empty0 + 8 * gs);  // D(j) was read before ds_ready, dO(j) by dV(j)
+                    mma_tmem_rows<HD>(tmem + kDK, tmem + kP, 64, qc_desc + qs * (Z::TILE >> 4), j > 0);
+                    mma_commit(q_empty0 + 8 * qs);
                 }
                 if (j + 1 < n) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(g_full0 + 8 * gn, ((j + 1) / GS) & 1, s.status));
                     if (!ok) break;
-                    if (qrow < q_lo) zero_rows<HD>(sg + gn * Z::TILE, q_lo - qrow, kTile);
-                    if (lane == 0) {
-                        mma_rows_rows<HD>(tmem + kP, v_desc, g_desc + gn * (Z::TILE >> 4));
-                        mma_commit(p_full);
-                    }
+                    mma_rows_rows<HD>(tmem + kP, v_desc, g_desc + gn * (Z::TILE >> 4));
+                    mma_commit(p_full);
                 }
             }
-            if (lane == 0) {
-                mma_commit(done);
-                wait_bounded(done, 0);
-            }
-            __syncwarp();
+            mma_commit(done);
+            wait_bounded(done, 0);
         }
+        __syncwarp();
     } else {  // two threads per key: queries 64·half .. of each tile
         const int half = (warp - 2) >> 2, quad = warp & 3;
         const int key = key0 + 32 * quad + lane;
@@ -790,6 +793,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int c = 0; c < 64; c += 2)
                 pk[c >> 1] = pack_bf16(__uint_as_float(r[c >> 5][c & 31]), __uint_as_float(r[c >> 5][(c & 31) + 1]));
+            if (row0 < q_lo) {  // dV sums over dO's rows, dK over Q's: those of queries without a key
+                ok = __all_sync(0xffffffffu, mbar_wait(g_full0 + 8 * gs, (j / GS) & 1, s.status));
+                if (!ok) break;
+                zero_rows<HD>(sg + gs * Z::TILE, q_lo - row0, kTile, threadIdx.x - 64, 256);
+                zero_rows<HD>(sq + qs * Z::TILE, q_lo - row0, kTile, threadIdx.x - 64, 256);
+            }
             tmem_store32(tmem + lanes + kS + 64 * half, pk);
             tmem_st_wait();
             warp_arrive(p_ready);

@@ -347,9 +347,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     zero_rows<HD>(skv + sv * Z::TILE, lo - key0, hi - key0, threadIdx.x - 64 - 128 * t, 128);
                 }
             }
-            float mx = -INFINITY;
+            float top[8];  // eight chains: one of 128 comparisons would take 500 cycles of latency
 #pragma unroll
-            for (int c = 0; c < kTile; ++c) mx = fmaxf(mx, __uint_as_float(r[c >> 5][c & 31]));
+            for (int c = 0; c < 8; ++c) top[c] = __uint_as_float(r[0][c]);
+#pragma unroll
+            for (int c = 8; c < kTile; ++c) top[c & 7] = fmaxf(top[c & 7], __uint_as_float(r[c >> 5][c & 31]));
+            const float mx = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])),
+                                   fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
             // O and the sum are rescaled only when the maximum has grown by more than 8 binary orders: until then P
             // stays below 2^8, exact enough in fp32 and bf16 alike
             const bool grow = mx > m && (m == -INFINITY || (mx - m) * s.sl > 8.f);

@@ -18,7 +18,7 @@
 //
 // One persistent cooperative kernel runs all phases (sum of squares, X_0, then A, B, X per step) with a grid barrier
 // between two of them: a small matrix would otherwise spend its time in launches. A phase's products are tiles of
-// 128 x 256, or of 128 x 64 where the wider ones would leave SMs idle, handed out over the CTAs; A and B are symmetric,
+// 128 x 256, or of 128 x 128 where the wider ones would leave SMs idle, handed out over the CTAs; A and B are symmetric,
 // so only the tiles that reach the diagonal are computed and each is also written mirrored. Operands are read by TMA in the major order in which they lie, so nothing is
 // transposed in memory.
 //
@@ -48,19 +48,24 @@ template <int BN>
 struct Tile {
     static constexpr int A_BYTES = 2 * BOX, B_BYTES = BN / 64 * BOX;
     static constexpr int SLOT = A_BYTES + B_BYTES;       // the hi (or the lo) operands of 64 entries of K
-    static constexpr int SLOTS = BN == 256 ? 4 : 8;      // the ring; split products take two slots a step
-    static constexpr size_t SMEM = 1024 + SLOTS * SLOT + 512;
+    static constexpr int SLOTS = BN == 256 ? 4 : 6;      // the ring; split products take two slots a step
+    static constexpr int STAGING = 8 * 32 * 128;         // the epilogue warps': 32 rows of 64 fp16 each
+    static constexpr size_t SMEM = SLOTS * SLOT + STAGING + 512;
     static constexpr int EPI = BN / 2;                   // columns per epilogue warp
+    static constexpr bool HALF = BN == 256;              // of A and B only the tiles that reach the diagonal (the narrow
+                                                         // tiles leave SMs idle: mirroring would cost more than it saves)
 };
 
 constexpr int kThreads = 320;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kScale = 1024.f;
 constexpr int kMaxSteps = 16;
-constexpr int kParts = 296;                      // parts of a matrix in the sum of squares (fewer for a batch)
+constexpr int kParts = 296;                      // parts of a batch in the sum of squares, at most
+constexpr int kSplitUnits = 148;                 // pieces of A's products over all of K, at most
 
 struct Maps {
-    CUtensorMap x[2][2];  // X of even and odd steps, hi and lo
+    CUtensorMap x[2][2];     // X of even and odd steps, hi and lo: boxes of 128 rows by 64 columns
+    CUtensorMap xt[2][2];    // the same in boxes of 64 rows by two blocks of 64 columns: X as the transposed operand
     CUtensorMap gram[2], poly[2];
 };
 
@@ -72,10 +77,12 @@ struct Params {
     __nv_bfloat16 *out;
     int batch, m, n;      // G is batch x m x n
     int s, l, tall;       // the smaller and the larger side
-    int64_t ldx, lds;     // leading dimensions of X (m x n) and of A and B (s x s)
+    int64_t ldx, lds;     // leading dimensions of X (m x n) and of A and B (s x s): whole 64s, zeros past the end
     __half *x[2][2], *gram[2], *poly[2];
     double *partial;      // batch x parts sums of squares
     int parts;
+    float *pieces;        // A's tiles over a part of K each (ksplit > 1), columns of 128 rows
+    int ksplit;
     float eps;
     int steps;
     float coef[kMaxSteps][3];
@@ -119,16 +126,16 @@ __device__ __forceinline__ Phase phase_of(const Params &p, int index) {
     f.b_mn = (f.kind == kGram && p.tall) || (f.kind == kApply && !p.tall);
     f.tm = (f.M + BM - 1) / BM;
     f.tn = (f.N + BN - 1) / BN;
-    f.tiles = f.kind == kApply ? f.tm * f.tn : symmetric_tiles<BN>(f.tm, f.tn);
+    f.tiles = f.kind == kApply || !Tile<BN>::HALF ? f.tm * f.tn : symmetric_tiles<BN>(f.tm, f.tn);
     return f;
 }
 
 // Unit u: matrix z, tile (ti, tj). The tiles that share rows or columns of X follow one another.
 template <int BN>
-__device__ __forceinline__ void tile_of(const Params &p, const Phase &f, int64_t u, int &z, int &ti, int &tj) {
-    z = (int)(u / f.tiles);
-    int t = (int)(u - (int64_t)z * f.tiles);
-    if (f.kind == kApply) {
+__device__ __forceinline__ void tile_of(const Params &p, const Phase &f, int u, int &z, int &ti, int &tj) {
+    z = u / f.tiles;
+    int t = u - z * f.tiles;
+    if (f.kind == kApply || !Tile<BN>::HALF) {
         if (p.tall) {
             ti = t / f.tn;
             tj = t - ti * f.tn;
@@ -150,11 +157,9 @@ __device__ __forceinline__ void tile_of(const Params &p, const Phase &f, int64_t
 // an error has been recorded.
 __device__ __forceinline__ bool grid_barrier(const Params &p, unsigned target, int *shared_ok) {
     asm volatile("fence.proxy.async.global;" ::: "memory");  // this thread's writes before other SMs' TMA reads
-    __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
-        __threadfence();
-        atomicAdd(p.barrier, 1u);
+        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(p.barrier) : "memory");
         const unsigned long long t0 = globaltimer();
         int ok = 1;
         for (unsigned it = 1;; ++it) {
@@ -170,7 +175,6 @@ __device__ __forceinline__ bool grid_barrier(const Params &p, unsigned target, i
                 if (!ok) break;
             }
         }
-        __threadfence();
         *shared_ok = ok;
     }
     __syncthreads();
@@ -216,40 +220,71 @@ __device__ __forceinline__ double block_sum(double v, double *red) {
 }
 
 // v as hi + lo, both fp16.
-__device__ __forceinline__ void split8(const float (&v)[8], __half (&h)[8], __half (&l)[8]) {
+__device__ __forceinline__ void split8(const float *v, uint4 &hi, uint4 &lo) {
+    uint32_t h[4], l[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        h[e] = __float2half_rn(v[e]);
-        l[e] = __float2half_rn(v[e] - __half2float(h[e]));
+    for (int e = 0; e < 4; ++e) {
+        const __half2 a = __floats2half2_rn(v[2 * e], v[2 * e + 1]);
+        const float2 f = __half22float2(a);
+        const __half2 b = __floats2half2_rn(v[2 * e] - f.x, v[2 * e + 1] - f.y);
+        h[e] = *reinterpret_cast<const uint32_t *>(&a);
+        l[e] = *reinterpret_cast<const uint32_t *>(&b);
+    }
+    hi = make_uint4(h[0], h[1], h[2], h[3]);
+    lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+// v[e] += the eight fp16 of q.
+__device__ __forceinline__ void add8(uint4 q, float *v) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[e]));
+        v[2 * e] += f.x;
+        v[2 * e + 1] += f.y;
     }
 }
 
-// Eight (or, at a row's end, `left`) fp16 values to p; rows start at multiples of 16 bytes.
-__device__ __forceinline__ void store8(__half *p, const __half (&h)[8], int left) {
-    if (left >= 8) {
-        union { __half h[8]; uint4 q; } u;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) u.h[e] = h[e];
-        *reinterpret_cast<uint4 *>(p) = u.q;
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (e < left) p[e] = h[e];
+// A warp's 32 x 64 block of 16-bit values between rows (a lane holds a row) and pieces of 16 bytes in memory order (a
+// warp's access covers whole 128-byte rows: a lane's own row in 16-byte stores took 14,000 cycles a tile). Piece c of
+// row r lies at c ^ (r mod 8).
+__device__ __forceinline__ uint4 *staged(uint8_t *buf, int row, int c) {
+    return reinterpret_cast<uint4 *>(buf + row * 128 + ((c ^ (row & 7)) << 4));
 }
 
-// hi + lo of eight (or `left`) values.
-__device__ __forceinline__ void load8(const __half *hi, const __half *lo, int left, float (&v)[8]) {
-    if (left >= 8) {
-        union { uint4 q; __half h[8]; } a, b;
-        a.q = *reinterpret_cast<const uint4 *>(hi);
-        b.q = *reinterpret_cast<const uint4 *>(lo);
+// Rows [0, rows) of the block at `base` into the lanes' pieces (piece i of a lane: row 4i + lane / 8, piece lane % 8).
+__device__ __forceinline__ void load_block(const __half *base, int64_t ld, int rows, uint4 (&q)[8]) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = __half2float(a.h[e]) + __half2float(b.h[e]);
-        return;
+    for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        q[i] = r < rows ? *reinterpret_cast<const uint4 *>(base + r * ld + 8 * (lane & 7)) : make_uint4(0, 0, 0, 0);
     }
+}
+
+__device__ __forceinline__ void pieces_to_rows(uint8_t *buf, const uint4 (&q)[8], float (&v)[64]) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = e < left ? __half2float(hi[e]) + __half2float(lo[e]) : 0.f;
+    for (int i = 0; i < 8; ++i) *staged(buf, 4 * i + (lane >> 3), lane & 7) = q[i];
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 8; ++c) add8(*staged(buf, lane, c), v + 8 * c);
+}
+
+// The lanes' rows (8 pieces each) to the block at `base`.
+template <typename T>
+__device__ __forceinline__ void store_block(uint8_t *buf, const uint4 (&q)[8], T *base, int64_t ld, int rows) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 8; ++c) *staged(buf, lane, c) = q[c];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3);
+        if (r < rows) *reinterpret_cast<uint4 *>(base + r * ld + 8 * (lane & 7)) = *staged(buf, r, lane & 7);
+    }
 }
 
 template <int BN>
@@ -257,9 +292,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
     using Z = Tile<BN>;
     constexpr int SLOT = Z::SLOT, SLOTS = Z::SLOTS, A_BYTES = Z::A_BYTES, EPI = Z::EPI;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + SLOTS * SLOT);
+    extern __shared__ __align__(1024) uint8_t smem[];  // swizzled boxes start at multiples of 1024 bytes
+    uint8_t *const staging = smem + SLOTS * SLOT;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(staging + Z::STAGING);
     double *red = reinterpret_cast<double *>(bars + 2 * SLOTS + 6);
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(red + kThreads / 32);
     int *shared_ok = reinterpret_cast<int *>(tmem_holder + 1);
@@ -275,6 +310,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mbar_init(drain, 1);
         fence_mbar_init();
+        for (int i = 0; i < 2; ++i) {
+            for (int q = 0; q < 2; ++q) {
+                prefetch_tmap(&maps.x[i][q]);
+                prefetch_tmap(&maps.xt[i][q]);
+            }
+            prefetch_tmap(&maps.gram[i]);
+            prefetch_tmap(&maps.poly[i]);
+        }
     }
     if (warp == 1) {
         tmem_alloc(smem_u32(tmem_holder), kTmemCols);
@@ -287,16 +330,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     unsigned target = 0;
 
     // ---- |G|_F: fixed parts of each matrix, summed in 64 bits; then X_0 by the same parts
-    const int row_groups = (p.n + 7) / 8;
-    const int64_t groups = (int64_t)p.m * row_groups;
-    for (int64_t u = blockIdx.x; u < (int64_t)p.batch * p.parts; u += gridDim.x) {
-        const int z = (int)(u / p.parts), part = (int)(u % p.parts);
-        const int64_t g1 = groups * (part + 1) / p.parts;
+    const uint32_t row_groups = (uint32_t)(p.ldx / 8), groups = (uint32_t)p.m * row_groups;
+    for (int u = blockIdx.x; u < p.batch * p.parts; u += gridDim.x) {
+        const int z = u / p.parts, part = u % p.parts;
+        const uint32_t g1 = (uint32_t)((uint64_t)groups * (part + 1) / p.parts);
         double acc = 0.0;
-        for (int64_t g = groups * part / p.parts + threadIdx.x; g < g1; g += kThreads) {
-            const int r = (int)(g / row_groups);
+        for (uint32_t g = (uint32_t)((uint64_t)groups * part / p.parts) + threadIdx.x; g < g1; g += kThreads) {
+            const uint32_t r = g / row_groups;
             float v[8];
-            load_g8(p, z, r, (int)(g - (int64_t)r * row_groups) * 8, v);
+            load_g8(p, z, (int)r, (int)(g - r * row_groups) * 8, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc += (double)v[e] * (double)v[e];
         }
@@ -304,65 +346,67 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (threadIdx.x == 0) p.partial[u] = acc;
     }
     bool go = grid_barrier(p, target += gridDim.x, shared_ok);
-    for (int64_t u = blockIdx.x; go && u < (int64_t)p.batch * p.parts; u += gridDim.x) {
-        const int z = (int)(u / p.parts), part = (int)(u % p.parts);
+    for (int u = blockIdx.x; go && u < p.batch * p.parts; u += gridDim.x) {
+        const int z = u / p.parts, part = u % p.parts;
         double acc = 0.0;
         for (int i = threadIdx.x; i < p.parts; i += kThreads)
             acc += *reinterpret_cast<volatile double *>(p.partial + (int64_t)z * p.parts + i);
         const float inv = (float)((double)kScale / (sqrt(block_sum(acc, red)) + (double)p.eps));
-        const int64_t g1 = groups * (part + 1) / p.parts;
-        for (int64_t g = groups * part / p.parts + threadIdx.x; g < g1; g += kThreads) {
-            const int r = (int)(g / row_groups), c = (int)(g - (int64_t)r * row_groups) * 8;
+        const uint32_t g1 = (uint32_t)((uint64_t)groups * (part + 1) / p.parts);
+        for (uint32_t g = (uint32_t)((uint64_t)groups * part / p.parts) + threadIdx.x; g < g1; g += kThreads) {
+            const uint32_t r = g / row_groups, c = (g - r * row_groups) * 8;
             float v[8];
-            load_g8(p, z, r, c, v);
+            load_g8(p, z, (int)r, (int)c, v);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] *= inv;
-            __half h[8], l[8];
-            split8(v, h, l);
             const int64_t at = ((int64_t)z * p.m + r) * p.ldx + c;
-            store8(p.x[0][0] + at, h, p.n - c);
-            store8(p.x[0][1] + at, l, p.n - c);
+            split8(v, *reinterpret_cast<uint4 *>(p.x[0][0] + at), *reinterpret_cast<uint4 *>(p.x[0][1] + at));
         }
     }
     if (go) go = grid_barrier(p, target += gridDim.x, shared_ok);
 
     // ---- the products. Ring slots and accumulators are counted through all phases, by each role alike
-    int64_t slots = 0;
-    int accs = 0;
+    uint32_t slots = 0, accs = 0;
     bool ok = true;
     for (int ph = 0; go && ph < 3 * p.steps; ++ph) {
         const Phase f = phase_of<BN>(p, ph);
         const int step = ph / 3, cur = step & 1, parts = f.split ? 2 : 1;
         const int kblocks = (f.K + BK - 1) / BK;
-        const int64_t units = (int64_t)p.batch * f.tiles;
+        const int splits = !Z::HALF && f.kind == kGram ? p.ksplit : 1, units = p.batch * f.tiles * splits;
+        const auto k_range = [&](int u, int &k0, int &k1) {
+            const int part = Z::HALF ? 0 : u % splits;
+            k0 = Z::HALF ? 0 : kblocks * part / splits;
+            k1 = Z::HALF ? kblocks : kblocks * (part + 1) / splits;
+        };
         if (warp == 0) {
             if (lane == 0) {  // ---- TMA producer
-                const CUtensorMap *ma = f.kind == kGram || (f.kind == kApply && p.tall) ? maps.x[cur]
+                const CUtensorMap *ma = f.a_mn                                          ? maps.xt[cur]
+                                        : f.kind == kGram || (f.kind == kApply && p.tall) ? maps.x[cur]
                                         : f.kind == kPoly                               ? maps.gram
                                                                                         : maps.poly;
-                const CUtensorMap *mb = f.kind == kGram || (f.kind == kApply && !p.tall) ? maps.x[cur]
-                                        : f.kind == kPoly                                ? maps.gram
-                                                                                         : maps.poly;
-                for (int64_t u = blockIdx.x; ok && u < units; u += gridDim.x) {
-                    int z, ti, tj;
-                    tile_of<BN>(p, f, u, z, ti, tj);
-                    for (int kb = 0; ok && kb < kblocks; ++kb)
+                const CUtensorMap *mb = f.b_mn                                          ? maps.xt[cur]
+                                        : f.kind == kGram                               ? maps.x[cur]
+                                        : f.kind == kPoly                               ? maps.gram
+                                                                                        : maps.poly;
+                for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+                    int z, ti, tj, k0, k1;
+                    tile_of<BN>(p, f, Z::HALF ? u : u / splits, z, ti, tj);
+                    k_range(u, k0, k1);
+                    for (int kb = k0; ok && kb < k1; ++kb)
                         for (int q = 0; q < parts; ++q, ++slots) {
-                            const int st = (int)(slots % SLOTS);
-                            ok = mbar_wait(empty0 + 8 * st, (uint32_t)((slots / SLOTS) & 1) ^ 1, p.status);
+                            const uint32_t st = slots % SLOTS;
+                            ok = mbar_wait(empty0 + 8 * st, ((slots / SLOTS) & 1) ^ 1, p.status);
                             if (!ok) break;
                             const uint32_t bar = full0 + 8 * st, sa = ring + st * SLOT, sb = sa + A_BYTES;
-                            const int k = kb * BK;
                             mbar_expect_tx(bar, SLOT);
+                            // few large boxes: six of 8 KiB a slot kept the issuing thread behind the tensor core
+                            if (f.a_mn) tma_load_4d(sa, ma + q, 0, kb * BK, ti * 2, z, bar);
+                            else tma_load_3d(sa, ma + q, kb * BK, ti * BM, z, bar);
 #pragma unroll
-                            for (int c = 0; c < 2; ++c) {
-                                const int mn = ti * BM + 64 * c;
-                                tma_load_3d(sa + c * BOX, ma + q, f.a_mn ? mn : k, f.a_mn ? k : mn, z, bar);
-                            }
-#pragma unroll
-                            for (int c = 0; c < BN / 64; ++c) {
-                                const int mn = tj * BN + 64 * c;
-                                tma_load_3d(sb + c * BOX, mb + q, f.b_mn ? mn : k, f.b_mn ? k : mn, z, bar);
+                            for (int c = 0; c < BN / 128; ++c) {
+                                const uint32_t to = sb + c * 2 * BOX;
+                                if (f.b_mn) tma_load_4d(to, mb + q, 0, kb * BK, tj * (BN / 64) + 2 * c, z, bar);
+                                else tma_load_3d(to, mb + q, kb * BK, tj * BN + 128 * c, z, bar);
                             }
                         }
                 }
@@ -371,33 +415,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else if (warp == 1) {
             if (lane == 0) {  // ---- MMA issuer
                 const uint32_t idesc = idesc_f16_f32(BM, BN, f.a_mn, f.b_mn);
-                const uint32_t a_step = f.a_mn ? 2048 : 32, b_step = f.b_mn ? 2048 : 32;
+                const uint32_t a_step = (f.a_mn ? 2048 : 32) >> 4, b_step = (f.b_mn ? 2048 : 32) >> 4;  // descriptor units
                 const uint32_t a_lbo = f.a_mn ? BOX : 16, b_lbo = f.b_mn ? BOX : 16;
-                for (int64_t u = blockIdx.x; ok && u < units; u += gridDim.x, ++accs) {
+                for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++accs) {
                     const int acc = accs & 1;
-                    ok = mbar_wait(tempty0 + 8 * acc, (uint32_t)((accs >> 1) & 1) ^ 1, p.status);
+                    ok = mbar_wait(tempty0 + 8 * acc, ((accs >> 1) & 1) ^ 1, p.status);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t d = tmem + acc * BN;
-                    for (int kb = 0; ok && kb < kblocks; ++kb, slots += parts) {
-                        uint32_t sa[2];
+                    int k0, k1;
+                    k_range(u, k0, k1);
+                    for (int kb = k0; ok && kb < k1; ++kb, slots += parts) {
+                        uint64_t da[2], db[2];
                         for (int q = 0; q < parts; ++q) {
-                            const int64_t i = slots + q;
-                            ok = ok && mbar_wait(full0 + 8 * (int)(i % SLOTS), (uint32_t)((i / SLOTS) & 1), p.status);
-                            sa[q] = ring + (int)(i % SLOTS) * SLOT;
+                            const uint32_t st = (slots + q) % SLOTS;
+                            ok = ok && mbar_wait(full0 + 8 * st, ((slots + q) / SLOTS) & 1, p.status);
+                            da[q] = smem_desc_sw128(ring + st * SLOT, a_lbo, 1024);
+                            db[q] = smem_desc_sw128(ring + st * SLOT + A_BYTES, b_lbo, 1024);
                         }
                         if (!ok) break;
                         tc_fence_after();
-                        const int products = f.split ? 3 : 1;  // hi·hi, hi·lo, lo·hi
-                        for (int q = 0; q < products; ++q) {
-                            const uint32_t at = sa[q == 2 ? 1 : 0], bt = sa[q == 1 ? 1 : 0] + A_BYTES;
+#pragma unroll
+                        for (int kk = 0; kk < BK / 16; ++kk)
+                            mma_f16_ss(d, da[0] + kk * a_step, db[0] + kk * b_step, idesc, (kb > k0 || kk > 0) ? 1u : 0u);
+                        if (f.split) {
 #pragma unroll
                             for (int kk = 0; kk < BK / 16; ++kk)
-                                mma_f16_ss(d, smem_desc_sw128(at + kk * a_step, a_lbo, 1024),
-                                           smem_desc_sw128(bt + kk * b_step, b_lbo, 1024), idesc,
-                                           (kb > 0 || kk > 0 || q > 0) ? 1u : 0u);
+                                mma_f16_ss(d, da[0] + kk * a_step, db[1] + kk * b_step, idesc, 1u);
+#pragma unroll
+                            for (int kk = 0; kk < BK / 16; ++kk)
+                                mma_f16_ss(d, da[1] + kk * a_step, db[0] + kk * b_step, idesc, 1u);
                         }
-                        for (int q = 0; q < parts; ++q) mma_commit(empty0 + 8 * (int)((slots + q) % SLOTS));
+                        for (int q = 0; q < parts; ++q) mma_commit(empty0 + 8 * ((slots + q) % SLOTS));
                     }
                     if (ok) mma_commit(tfull0 + 8 * acc);
                 }
@@ -412,91 +461,144 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float f_old = f.kind == kApply ? coef[0] : coef[1];
             const float f_acc = (f.kind == kPoly ? coef[2] : 1.f) / kScale;
             const int64_t ld = f.kind == kApply ? p.ldx : p.lds;
-            for (int64_t u = blockIdx.x; ok && u < units; u += gridDim.x, ++accs) {
+            for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++accs) {
                 int z, ti, tj;
-                tile_of<BN>(p, f, u, z, ti, tj);
+                tile_of<BN>(p, f, Z::HALF ? u : u / splits, z, ti, tj);
                 const int acc = accs & 1;
-                ok = __all_sync(0xffffffffu, mbar_wait(tfull0 + 8 * acc, (uint32_t)((accs >> 1) & 1), p.status));
+                const int i0 = ti * BM + 32 * quad, i = i0 + lane, j0 = tj * BN + EPI * half;
+                const int rows = f.M - i0;  // of the warp's 32 that exist
+                uint4 early_h[8], early_l[8];
+                // the exact terms' operands come while the products run (a wide tile's warps are busy with the last tile)
+                if (!Z::HALF && f.kind != kGram && rows > 0 && j0 < ld) {
+                    const int64_t at0 = ((int64_t)z * f.M + i0) * ld + j0;
+                    load_block(old[0] + at0, ld, rows, early_h);
+                    load_block(old[1] + at0, ld, rows, early_l);
+                }
+                ok = __all_sync(0xffffffffu, mbar_wait(tfull0 + 8 * acc, (accs >> 1) & 1, p.status));
                 if (!ok) break;
                 tc_fence_after();
-                const int i0 = ti * BM + 32 * quad, i = i0 + lane, j0 = tj * BN + EPI * half;
                 // (j, i) lies in no computed tile (EPI columns share a row tile, a warp's rows a column tile)
-                const bool mirror = f.kind != kApply && j0 / BM >= column_tiles<BN>(f.tm, i0 / BN);
+                const bool mirror = Z::HALF && f.kind != kApply && j0 / BM >= column_tiles<BN>(f.tm, i0 / BN);
                 const uint32_t t = tmem + ((uint32_t)(32 * quad) << 16) + acc * BN + EPI * half;
+                if (!Z::HALF && splits > 1) {  // the piece as it is, column by column
+                    float *const piece = p.pieces + ((int64_t)u * BN + EPI * half) * BM + 32 * quad + lane;
 #pragma unroll 1
-                for (int c = 0; c < EPI; c += 32) {
-                    if (j0 + c >= f.N) break;
-                    const int64_t at0 = ((int64_t)z * f.M + i) * ld + j0 + c;
-                    const bool live = i < f.M;
-                    float o[32];
-                    if (f.kind != kGram && live) {
+                    for (int c = 0; c < EPI; c += 32) {
+                        uint32_t r[32];
+                        tmem_load32(t + c, r);
+                        tmem_ld_wait();
 #pragma unroll
-                        for (int e0 = 0; e0 < 32; e0 += 8) {
-                            float v[8];
-                            load8(old[0] + at0 + e0, old[1] + at0 + e0, f.N - j0 - c - e0, v);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) o[e0 + e] = v[e];
-                        }
+                        for (int e = 0; e < 32; ++e) piece[(int64_t)(c + e) * BM] = __uint_as_float(r[e]);
                     }
-                    uint32_t r[32];
-                    tmem_load32(t + c, r);
-                    tmem_ld_wait();
-                    if (!live) continue;
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(tempty0 + 8 * acc);
+                    continue;
+                }
+                uint8_t *const buf = staging + (warp - 2) * 4096;
+#pragma unroll 1
+                for (int c = 0; c < EPI; c += 64) {
+                    if (j0 + c >= ld || rows <= 0) break;
+                    const int64_t at0 = ((int64_t)z * f.M + i0) * ld + j0 + c;
+                    uint4 qh[8], ql[8];
+                    float v[64];
 #pragma unroll
-                    for (int e0 = 0; e0 < 32; e0 += 8) {
-                        const int j = j0 + c + e0, left = f.N - j;
-                        if (left <= 0) break;
-                        float v[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[e0 + e]) * f_acc;
-                        if (f.kind != kGram) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) v[e] = fmaf(f_old, o[e0 + e], v[e]);
+                    for (int e = 0; e < 64; ++e) v[e] = 0.f;
+                    if (f.kind != kGram) {
+                        static_assert(Z::HALF || EPI == 64, "a narrow tile's warp has one block of columns");
+                        if (Z::HALF) {
+                            load_block(old[0] + at0, ld, rows, qh);
+                            load_block(old[1] + at0, ld, rows, ql);
                         }
-                        if (f.kind == kApply && f.last) {
-                            __nv_bfloat16 *to = p.out + ((int64_t)z * p.m + i) * p.n + j;
-                            if (p.out_vec && left >= 8) {
+                        pieces_to_rows(buf, Z::HALF ? qh : early_h, v);
+                        pieces_to_rows(buf, Z::HALF ? ql : early_l, v);
+                    }
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        uint32_t r[32];
+                        tmem_load32(t + c + 32 * g, r);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            v[32 * g + e] = fmaf(f_old, v[32 * g + e], __uint_as_float(r[e]) * f_acc);
+                    }
+                    if (f.kind == kApply && f.last) {
+                        __nv_bfloat16 *to = p.out + ((int64_t)z * p.m + i0) * p.n + j0 + c;
+                        if (p.out_vec && j0 + c + 64 <= p.n) {
+#pragma unroll
+                            for (int g = 0; g < 8; ++g) {
                                 uint32_t w[4];
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
-                                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * e] * (1.f / kScale),
-                                                                                   v[2 * e + 1] * (1.f / kScale));
+                                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[8 * g + 2 * e] * (1.f / kScale),
+                                                                                   v[8 * g + 2 * e + 1] * (1.f / kScale));
                                     w[e] = *reinterpret_cast<const uint32_t *>(&b);
                                 }
-                                *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 8; ++e)
-                                    if (e < left) to[e] = __float2bfloat16_rn(v[e] * (1.f / kScale));
+                                qh[g] = make_uint4(w[0], w[1], w[2], w[3]);
                             }
-                            continue;
+                            store_block(buf, qh, to, p.n, rows);
+                        } else if (i < f.M) {
+#pragma unroll
+                            for (int e = 0; e < 64; ++e)
+                                if (j0 + c + e < p.n) to[(int64_t)lane * p.n + e] = __float2bfloat16_rn(v[e] * (1.f / kScale));
                         }
-                        __half h[8], l[8];
-                        split8(v, h, l);
-                        store8(dst[0] + at0 + e0, h, left);
-                        store8(dst[1] + at0 + e0, l, left);
-                        if (mirror) {
+                        continue;
+                    }
+#pragma unroll
+                    for (int g = 0; g < 8; ++g) {
+                        split8(v + 8 * g, qh[g], ql[g]);
+                        if (mirror && i < f.M) {
+                            union { uint4 q; __half h[8]; } hi, lo;
+                            hi.q = qh[g];
+                            lo.q = ql[g];
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
-                                if (e >= left) break;
-                                const int64_t back = ((int64_t)z * f.M + j + e) * ld + i;
-                                dst[0][back] = h[e];
-                                dst[1][back] = l[e];
+                                const int j = j0 + c + 8 * g + e;
+                                if (j < f.M) {
+                                    dst[0][((int64_t)z * f.M + j) * ld + i] = hi.h[e];
+                                    dst[1][((int64_t)z * f.M + j) * ld + i] = lo.h[e];
+                                }
                             }
                         }
                     }
+                    store_block(buf, qh, dst[0] + at0, ld, rows);
+                    store_block(buf, ql, dst[1] + at0, ld, rows);
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(tempty0 + 8 * acc);
             }
         }
-        go = grid_barrier(p, target += gridDim.x, shared_ok);
+        if (!Z::HALF && splits > 1) {  // the pieces added in order; A is symmetric, so its columns are written as rows
+            go = grid_barrier(p, target += gridDim.x, shared_ok);
+            const int total = p.batch * f.tiles * BN * (BM / 4);
+            for (int e = blockIdx.x * kThreads + threadIdx.x; go && e < total; e += gridDim.x * kThreads) {
+                const int row = e % (BM / 4) * 4, col = e / (BM / 4) % BN, tile = e / (BM / 4 * BN);
+                int z, ti, tj;
+                tile_of<BN>(p, f, tile, z, ti, tj);
+                const int i = ti * BM + row, j = tj * BN + col;
+                if (j >= f.M || i >= p.lds) continue;  // (lds is a multiple of four)
+                const float *piece = p.pieces + ((int64_t)tile * splits * BN + col) * BM + row;
+                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                for (int q = 0; q < splits; ++q) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(piece + (int64_t)q * BN * BM));
+                    acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+                }
+                const float v[8] = {acc.x / kScale, acc.y / kScale, acc.z / kScale, acc.w / kScale, 0.f, 0.f, 0.f, 0.f};
+                uint4 hi, lo;
+                split8(v, hi, lo);
+                const int64_t at = ((int64_t)z * f.M + j) * p.lds + i;
+                *reinterpret_cast<uint2 *>(p.gram[0] + at) = make_uint2(hi.x, hi.y);
+                *reinterpret_cast<uint2 *>(p.gram[1] + at) = make_uint2(lo.x, lo.y);
+            }
+        }
+        if (go) go = grid_barrier(p, target += gridDim.x, shared_ok);
     }
     if (warp == 0 && lane == 0) {  // after an error, copies may still be in flight: they land before the CTA exits
-        for (int64_t i = slots > SLOTS ? slots - SLOTS : 0; i < slots; ++i) {
+        for (uint32_t i = slots > SLOTS ? slots - SLOTS : 0; i < slots; ++i) {
             const unsigned long long t0 = globaltimer();
-            while (!mbar_try_wait(full0 + 8 * (int)(i % SLOTS), (uint32_t)((i / SLOTS) & 1)) &&
+            while (!mbar_try_wait(full0 + 8 * (i % SLOTS), (i / SLOTS) & 1) &&
                    globaltimer() - t0 < kWaitTimeoutNs) {
             }
         }
@@ -533,17 +635,20 @@ EncodeTiled encode_fn() {
     return fn;
 }
 
-// A batch of rows x cols fp16 matrices in boxes of 64 x 64, 128-byte swizzle, zero outside each matrix.
-int matrix_map(CUtensorMap *m, const __half *base, int batch, int rows, int cols, int64_t ld) {
+// A batch of rows x ld fp16 matrices, 128-byte swizzle, zero past the rows: boxes of 128 rows by 64 columns, or (blocks)
+// of 64 rows by two blocks of 64 columns, one block after the other.
+int matrix_map(CUtensorMap *m, const __half *base, int batch, int rows, int64_t ld, bool blocks) {
     EncodeTiled enc = encode_fn();
     if (enc == nullptr) {
         set_error("lamq_newton_schulz: cuTensorMapEncodeTiled is unavailable");
         return LAMQ_ERR_CUDA;
     }
-    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batch};
-    const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)ld * 2 * (cuuint64_t)rows};
-    const cuuint32_t box[3] = {64, 64, 1}, step[3] = {1, 1, 1};
-    const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half *>(base), dims, strides, box, step,
+    const cuuint64_t row = (cuuint64_t)ld * 2, all = row * (cuuint64_t)rows;
+    const cuuint64_t dims3[3] = {(cuuint64_t)ld, (cuuint64_t)rows, (cuuint64_t)batch}, strides3[2] = {row, all};
+    const cuuint64_t dims4[4] = {64, (cuuint64_t)rows, (cuuint64_t)ld / 64, (cuuint64_t)batch}, strides4[3] = {row, 128, all};
+    const cuuint32_t box3[3] = {64, 128, 1}, box4[4] = {64, 64, 2, 1}, step[4] = {1, 1, 1, 1};
+    const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, blocks ? 4 : 3, const_cast<__half *>(base),
+                           blocks ? dims4 : dims3, blocks ? strides4 : strides3, blocks ? box4 : box3, step,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
@@ -553,22 +658,36 @@ int matrix_map(CUtensorMap *m, const __half *base, int batch, int rows, int cols
     return LAMQ_OK;
 }
 
-int64_t up8(int64_t v) { return (v + 7) / 8 * 8; }
+int64_t up64(int64_t v) { return (v + 63) / 64 * 64; }
 size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-int parts_of(int batch) { return std::max(1, kParts / batch); }
+int64_t tiles_of(int64_t n, int tile) { return (n + tile - 1) / tile; }
 
-struct Layout {
-    size_t x, square, partial, total;  // bytes of one X, of one A or B, of the partial sums, and of all
+// How a batch of m x n matrices is cut up: by its sizes alone, so that equal calls sum in equal order everywhere.
+struct Plan {
+    bool wide;     // tiles of 128 x 256, else of 128 x 128
+    int parts;     // of each matrix in the sum of squares
+    int ksplit;    // parts of K in A's products
+    size_t x, square, partial, pieces, total;  // bytes of one X, of one A or B, of the partial sums, the pieces, and all
 };
 
-Layout layout_of(int batch, int m, int n) {
-    Layout L;
-    const int s = std::min(m, n);
-    L.x = up256((size_t)batch * m * up8(n) * 2);
-    L.square = up256((size_t)batch * s * up8(s) * 2);
-    L.partial = up256((size_t)batch * parts_of(batch) * 8);
-    L.total = 4 * L.x + 4 * L.square + L.partial + 256;
+Plan plan_of(int batch, int m, int n) {
+    Plan L;
+    const int s = std::min(m, n), l = std::max(m, n);
+    // The wide tiles have the better ratio of products to operand bytes, the narrow ones half of the latency (narrower
+    // still would not: an MMA of 64 columns takes as long as one of 128). Wide ones as soon as the larger phase (B·X)
+    // fills the device with them.
+    L.wide = batch * (m > n ? tiles_of(l, BM) * tiles_of(s, 256) : tiles_of(s, BM) * tiles_of(l, 256)) >= kSplitUnits;
+    L.parts = (int)std::max<int64_t>(1, std::min<int64_t>(kParts / batch, (int64_t)m * up64(n) / 16384));
+    // A is s x s over K = l: of a skinny matrix few tiles, each a long sum. Cut K, in parts of four steps or more, where
+    // SMs would be idle (16 x 9728: 152 steps of some 700 cycles on one SM otherwise)
+    const int64_t tiles = batch * tiles_of(s, BM) * tiles_of(s, 128), steps = tiles_of(l, BK);
+    L.ksplit = L.wide ? 1 : (int)std::max<int64_t>(1, std::min(kSplitUnits / tiles, steps / 4));
+    L.x = up256((size_t)batch * m * up64(n) * 2);
+    L.square = up256((size_t)batch * s * up64(s) * 2);
+    L.partial = up256((size_t)batch * L.parts * 8);
+    L.pieces = L.ksplit > 1 ? (size_t)tiles * L.ksplit * BM * 128 * 4 : 0;
+    L.total = 4 * L.x + 4 * L.square + L.partial + L.pieces + 256;
     return L;
 }
 
@@ -595,7 +714,7 @@ using namespace lamq;
 
 extern "C" size_t lamq_newton_schulz_workspace_size(int batch, int m, int n) {
     if (batch <= 0 || m <= 0 || n <= 0) return 0;
-    return layout_of(batch, m, n).total;
+    return plan_of(batch, m, n).total;
 }
 
 extern "C" int lamq_newton_schulz(const void *G, int dtype, int64_t ldg, int64_t batch_stride, int batch, int m, int n,
@@ -610,7 +729,7 @@ extern "C" int lamq_newton_schulz(const void *G, int dtype, int64_t ldg, int64_t
     if (batch == 0 || m == 0 || n == 0) return LAMQ_OK;
     LAMQ_REQUIRE(batch == 1 || batch_stride >= (int64_t)(m - 1) * ldg + n, "lamq_newton_schulz: matrices overlap");
     LAMQ_REQUIRE(G && coefficients && out && status, "lamq_newton_schulz: null pointer");
-    const Layout L = layout_of(batch, m, n);
+    const Plan L = plan_of(batch, m, n);
     LAMQ_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= L.total,
                  "lamq_newton_schulz: workspace of %zu bytes (16-byte aligned) needed, %zu given", L.total,
                  workspace_bytes);
@@ -651,9 +770,10 @@ extern "C" int lamq_newton_schulz(const void *G, int dtype, int64_t ldg, int64_t
     p.tall = m > n;
     p.s = std::min(m, n);
     p.l = std::max(m, n);
-    p.ldx = up8(n);
-    p.lds = up8(p.s);
-    p.parts = parts_of(batch);
+    p.ldx = up64(n);
+    p.lds = up64(p.s);
+    p.parts = L.parts;
+    p.ksplit = L.ksplit;
     p.eps = eps;
     p.steps = steps;
     p.status = status;
@@ -662,23 +782,23 @@ extern "C" int lamq_newton_schulz(const void *G, int dtype, int64_t ldg, int64_t
     for (int i = 0; i < 2; ++i) {
         for (int q = 0; q < 2; ++q) {
             p.x[i][q] = reinterpret_cast<__half *>(ws + (2 * i + q) * L.x);
-            if (int st = matrix_map(&maps.x[i][q], p.x[i][q], batch, m, n, p.ldx)) return st;
+            if (int st = matrix_map(&maps.x[i][q], p.x[i][q], batch, m, p.ldx, false)) return st;
+            if (int st = matrix_map(&maps.xt[i][q], p.x[i][q], batch, m, p.ldx, true)) return st;
         }
         p.gram[i] = reinterpret_cast<__half *>(ws + 4 * L.x + i * L.square);
         p.poly[i] = reinterpret_cast<__half *>(ws + 4 * L.x + (2 + i) * L.square);
-        if (int st = matrix_map(&maps.gram[i], p.gram[i], batch, p.s, p.s, p.lds)) return st;
-        if (int st = matrix_map(&maps.poly[i], p.poly[i], batch, p.s, p.s, p.lds)) return st;
+        if (int st = matrix_map(&maps.gram[i], p.gram[i], batch, p.s, p.lds, false)) return st;
+        if (int st = matrix_map(&maps.poly[i], p.poly[i], batch, p.s, p.lds, false)) return st;
     }
     p.partial = reinterpret_cast<double *>(ws + 4 * L.x + 4 * L.square);
-    p.barrier = reinterpret_cast<unsigned *>(ws + 4 * L.x + 4 * L.square + L.partial);
+    p.pieces = reinterpret_cast<float *>(ws + 4 * L.x + 4 * L.square + L.partial);
+    p.barrier = reinterpret_cast<unsigned *>(ws + 4 * L.x + 4 * L.square + L.partial + L.pieces);
     e = cudaMemsetAsync(p.barrier, 0, sizeof(unsigned), s);
     if (e != cudaSuccess) return cuda_failed(e);
-    // The wide tiles have the better ratio of products to operand bytes; the narrow ones a quarter of the latency. Wide
-    // ones as soon as the larger phase (B·X) fills the device with them.
-    const int64_t ts = (p.s + BM - 1) / BM, tl = (p.l + BM - 1) / BM;
-    const bool wide = (int64_t)batch * (p.tall ? tl * ((p.s + 255) / 256) : ts * ((p.l + 255) / 256)) >= sms;
-    // a CTA per tile of the phase with the most of them, at most one per SM
-    const int grid = (int)std::min<int64_t>(sms, std::max<int64_t>((int64_t)batch * ts * tl * 2,
-                                                                  std::min<int64_t>(sms, (int64_t)m * n / 4096 + 1)));
-    return wide ? launch<256>(maps, p, grid, s) : launch<64>(maps, p, grid, s);
+    // a CTA per unit of the phase with the most of them, at most one per SM
+    const int bn = L.wide ? 256 : 128;
+    const int64_t apply = batch * (p.tall ? tiles_of(p.l, BM) * tiles_of(p.s, bn) : tiles_of(p.s, BM) * tiles_of(p.l, bn));
+    const int64_t gram = batch * tiles_of(p.s, BM) * tiles_of(p.s, bn) * L.ksplit;
+    const int grid = (int)std::min<int64_t>(sms, std::max<int64_t>({apply, gram, (int64_t)batch * L.parts, L.ksplit > 1 ? sms : 1}));
+    return L.wide ? launch<256>(maps, p, grid, s) : launch<128>(maps, p, grid, s);
 }

@@ -16,7 +16,7 @@
 //   dkv: a CTA per 128 keys walks the queries of every head of its group and sums Pᵀ·dO and dSᵀ·Q in TMEM, so a shared
 //        K/V head's gradient needs no join. It computes Sᵀ and dPᵀ (keys as rows): Pᵀ and dSᵀ come out as A operands.
 //   The recomputation of S and dP in both costs two of seven products, against a dQ of fp32 sums in memory.
-// A first small kernel computes D and stores lse and D by padded rows (lse = +inf where there is no row: P = 0).
+// The dq kernel, which holds dO's rows, also computes D and keeps lse and D by padded rows for the dkv kernel.
 //
 // Rows of K, V, Q or dO that no allowed pair touches (outside a text's key range; queries before its first key) are
 // zeroed in shared memory before a product would sum over them, so what they hold (NaN included) reaches nothing.
@@ -74,7 +74,7 @@ struct Sizes {
     static constexpr int LATE_STAGES = HD == 128 ? 3 : 4, EARLY_STAGES = HD == 128 ? 2 : 4;
     static constexpr int ROW = kTile * 4;               // bytes of lse (or D) of a query tile
     static constexpr size_t FWD_SMEM = 2 * TILE + FWD_STAGES * TILE + 256;
-    static constexpr size_t DQ_SMEM = 2 * TILE + (LATE_STAGES + EARLY_STAGES) * TILE + 256;
+    static constexpr size_t DQ_SMEM = 2 * TILE + (LATE_STAGES + EARLY_STAGES) * TILE + 256 + 2 * ROW;
     static constexpr size_t DKV_SMEM = 2 * TILE + (LATE_STAGES + EARLY_STAGES) * (TILE + ROW) + 256;
 };
 
@@ -415,42 +415,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ----------------------------------------------------------------------------------------------------------- backward
 
-// D = Σ dO·O per query and lse in units of log 2, by rows padded to whole tiles: half a warp per row.
-__global__ void __launch_bounds__(256)
-    attention_rowstats_kernel(const Rows o, const Rows g, Shape s, const float *__restrict__ lse,
-                              float *__restrict__ lse2, float *__restrict__ Dr) {
-    const int sub = threadIdx.x & 15;
-    const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 4;
-    const int64_t total = (int64_t)s.B * s.Hq * s.lq_pad;
-    if (row >= total) return;  // whole half warps: total is a multiple of 128
-    const int i = (int)(row % s.lq_pad);
-    const int64_t bh = row / s.lq_pad;
-    const int b = (int)(bh / s.Hq), h = (int)(bh % s.Hq);
-    float l = -INFINITY, d = 0.f;
-    if (i < s.Lq) l = lse[bh * s.Lq + i];
-    if (l != -INFINITY && 8 * sub < s.D) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(o.p + b * o.batch + h * o.head + (int64_t)i * o.row + 8 * sub);
-        const uint4 y = *reinterpret_cast<const uint4 *>(g.p + b * g.batch + h * g.head + (int64_t)i * g.row + 8 * sub);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+// Sum of the products of two 16-byte pieces of bf16.
+__device__ __forceinline__ float dot8(uint4 x, uint4 y, float d) {
+    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            d = fmaf(__uint_as_float(xs[e] << 16), __uint_as_float(ys[e] << 16), d);
-            d = fmaf(__uint_as_float(xs[e] & 0xffff0000u), __uint_as_float(ys[e] & 0xffff0000u), d);
-        }
+    for (int e = 0; e < 4; ++e) {
+        d = fmaf(__uint_as_float(xs[e] << 16), __uint_as_float(ys[e] << 16), d);
+        d = fmaf(__uint_as_float(xs[e] & 0xffff0000u), __uint_as_float(ys[e] & 0xffff0000u), d);
     }
-#pragma unroll
-    for (int k = 8; k > 0; k >>= 1) d += __shfl_xor_sync(0xffffffffu, d, k);
-    if (sub == 0) {
-        lse2[row] = l == -INFINITY ? INFINITY : l * kLog2e;
-        Dr[row] = d;
-    }
+    return d;
 }
 
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
                         const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapG, Shape s,
-                        const float *__restrict__ lse2, const float *__restrict__ Dr, Rows dq) {
+                        const float *__restrict__ lse, float *__restrict__ lse2, float *__restrict__ Dr, Rows o, Rows dq) {
     using Z = Sizes<HD>;
     constexpr int KS = Z::LATE_STAGES, VS = Z::EARLY_STAGES;
     // TMEM columns. Q and dO lie there as A operands: from shared memory they would take, with the key tile's rows, all
@@ -464,6 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                    v_empty0 = k_empty0 + 8 * KS, q_full = v_empty0 + 8 * VS;
     const uint32_t q_ready = q_full + 8, s_full = q_full + 16, s_free = q_full + 24, p_full = q_full + 32;
     const uint32_t ds_ready = q_full + 40, done = q_full + 48;
+    float *half_d = reinterpret_cast<float *>(smem + Z::DQ_SMEM - 2 * Z::ROW);  // each half's sum of dO·O
     const uint32_t sq = smem_u32(smem), sg = sq + Z::TILE, sk = sg + Z::TILE, sv = sk + KS * Z::TILE;
 
     const int tiles = s.lq_pad / kTile, heads = s.Hq * s.B;
@@ -564,8 +545,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool live = i < s.Lq;
         const int row_hi = s.causal ? min(hi, i + s.off + 1) : hi;
         const uint32_t lanes = (uint32_t)(32 * quad) << 16;
-        const float l2 = lse2[(int64_t)bh * s.lq_pad + i], Di = Dr[(int64_t)bh * s.lq_pad + i];
+        // lse in units of log 2 (+inf where there is no row or it is empty: P = 0) and D = Σ dO·O, half of the row each;
+        // kept by padded rows for the dkv kernel
+        const float l = live ? lse[(int64_t)bh * s.Lq + i] : -INFINITY, l2 = l == -INFINITY ? INFINITY : l * kLog2e;
+        const bool some = l != -INFINITY;
+        uint4 orow[HD / 16];
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) {
+            const int col = half * (HD / 2) + 8 * c;
+            orow[c] = some && col < s.D ? *reinterpret_cast<const uint4 *>(o.p + b * o.batch + h * o.head + (int64_t)i * o.row + col)
+                                        : make_uint4(0, 0, 0, 0);
+        }
         bool ok = n > 0 && __all_sync(0xffffffffu, mbar_wait(q_full, 0, s.status));
+        float Di = 0.f;
+        if (ok && some) {
+            const int row = 32 * quad + lane;
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) {
+                const int piece = (HD == 64 ? 4 * half : 0) + c;
+                uint4 g;
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(g.x), "=r"(g.y), "=r"(g.z), "=r"(g.w)
+                             : "r"(sg + (HD == 64 ? 0 : half * Z::CHUNK) + row * 128 + ((piece ^ (row & 7)) << 4)));
+                Di = dot8(orow[c], g, Di);
+            }
+        }
+        half_d[half * kTile + 32 * quad + lane] = Di;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        Di = half_d[32 * quad + lane] + half_d[kTile + 32 * quad + lane];
+        if (half == 0) {
+            lse2[(int64_t)bh * s.lq_pad + i] = l2;
+            Dr[(int64_t)bh * s.lq_pad + i] = Di;
+        }
         if (ok) {
             if (HD == 64) {
                 chunk_to_tmem(half ? sg : sq, 32 * quad + lane, tmem + lanes + (half ? kG : kQ));
@@ -991,15 +1002,13 @@ int run_backward(const lamq_attention_args &a, const Shape &s, float *lse2, floa
     if (!keys) mk = mv = mq;   // not read: no query meets a key tile
     if (!queries) mq = mg = mk;
     if (queries) {
-        const int64_t rows = (int64_t)s.B * s.Hq * s.lq_pad, blocks = rows / 16;
-        LAMQ_REQUIRE(blocks <= INT_MAX, "lamq_attention_backward: too many queries");
-        attention_rowstats_kernel<<<(unsigned)blocks, 256, 0, st>>>(rows_of(a.o), rows_of(a.d_o), s, a.lse, lse2, D);
-        LAMQ_CHECK_LAUNCH("lamq_attention_backward statistics");
         const int64_t tiles = (int64_t)(s.lq_pad / kTile) * s.Hq * s.B;
+        LAMQ_REQUIRE(tiles <= INT_MAX, "lamq_attention_backward: too many query tiles");
         auto *k = attention_dq_kernel<HD>;
         if (cudaError_t e = smem_limit_once((const void *)k, (int)Sizes<HD>::DQ_SMEM))
             return launch_failed("lamq_attention_backward", e);
-        k<<<(unsigned)tiles, kThreads, Sizes<HD>::DQ_SMEM, st>>>(mq, mk, mv, mg, s, lse2, D, rows_of(a.dq));
+        k<<<(unsigned)tiles, kThreads, Sizes<HD>::DQ_SMEM, st>>>(mq, mk, mv, mg, s, a.lse, lse2, D, rows_of(a.o),
+                                                                 rows_of(a.dq));
         LAMQ_CHECK_LAUNCH("lamq_attention_backward dq");
     }
     if (keys) {

@@ -18,9 +18,9 @@
 //
 // One persistent cooperative kernel runs all phases (sum of squares, X_0, then A, B, X per step) with a grid barrier
 // between two of them: a small matrix would otherwise spend its time in launches. A phase's products are tiles of
-// 128 x 256, or of 128 x 128 where the wider ones would leave SMs idle, handed out over the CTAs; A and B are symmetric,
-// so only the tiles that reach the diagonal are computed and each is also written mirrored. Operands are read by TMA in the major order in which they lie, so nothing is
-// transposed in memory.
+// 256 x 256 on pairs of CTAs, or of 128 x 128 on single ones where the larger would leave SMs idle, handed out over the
+// device. A and B are symmetric: of the large tiles only those that reach the diagonal are computed, and each is also
+// written mirrored. Operands are read by TMA in the major order in which they lie, so nothing is transposed in memory.
 //
 // Warp roles (320 threads): warp 0 issues TMA loads, warp 1 the MMAs into two TMEM accumulators, warps 2-9 drain one
 // while the next fills.
@@ -46,13 +46,15 @@ constexpr int BOX = 64 * 128;                    // bytes of a 64 x 64 fp16 box
 
 template <int BN>
 struct Tile {
-    static constexpr int A_BYTES = 2 * BOX, B_BYTES = BN / 64 * BOX;
+    static constexpr bool PAIR = BN == 256;              // two CTAs (a cluster) compute 256 x 256 with cta_group::2 MMAs
+    static constexpr int ROWS = PAIR ? 256 : 128;        // of a tile
+    static constexpr int A_BYTES = 2 * BOX, B_BYTES = 2 * BOX;  // a CTA loads 128 rows of either operand
     static constexpr int SLOT = A_BYTES + B_BYTES;       // the hi (or the lo) operands of 64 entries of K
-    static constexpr int SLOTS = BN == 256 ? 4 : 6;      // the ring; split products take two slots a step
+    static constexpr int SLOTS = 6;                      // the ring; split products take two slots a step
     static constexpr int STAGING = 8 * 32 * 128;         // the epilogue warps': 32 rows of 64 fp16 each
     static constexpr size_t SMEM = SLOTS * SLOT + STAGING + 512;
     static constexpr int EPI = BN / 2;                   // columns per epilogue warp
-    static constexpr bool HALF = BN == 256;              // of A and B only the tiles that reach the diagonal (the narrow
+    static constexpr bool HALF = PAIR;                   // of A and B only the tiles that reach the diagonal (the narrow
                                                          // tiles leave SMs idle: mirroring would cost more than it saves)
 };
 
@@ -101,7 +103,7 @@ struct Phase {
 // The row tiles of column tile tj of a symmetric C that reach the diagonal: those that start at or before its last column.
 template <int BN>
 __host__ __device__ __forceinline__ int column_tiles(int tm, int tj) {
-    const int c = ((tj + 1) * BN - 1) / BM + 1;
+    const int c = ((tj + 1) * BN - 1) / Tile<BN>::ROWS + 1;
     return c < tm ? c : tm;
 }
 
@@ -124,7 +126,7 @@ __device__ __forceinline__ Phase phase_of(const Params &p, int index) {
     f.K = f.kind == kGram ? p.l : p.s;
     f.a_mn = f.kind == kGram && p.tall;
     f.b_mn = (f.kind == kGram && p.tall) || (f.kind == kApply && !p.tall);
-    f.tm = (f.M + BM - 1) / BM;
+    f.tm = (f.M + Tile<BN>::ROWS - 1) / Tile<BN>::ROWS;
     f.tn = (f.N + BN - 1) / BN;
     f.tiles = f.kind == kApply || !Tile<BN>::HALF ? f.tm * f.tn : symmetric_tiles<BN>(f.tm, f.tn);
     return f;
@@ -292,6 +294,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
     using Z = Tile<BN>;
     constexpr int SLOT = Z::SLOT, SLOTS = Z::SLOTS, A_BYTES = Z::A_BYTES, EPI = Z::EPI;
+    constexpr bool PAIR = Z::PAIR;
+    const int rank = PAIR ? (int)cluster_rank() : 0, worker = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
+    const int workers = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;  // what computes tiles: pairs, or CTAs
     extern __shared__ __align__(1024) uint8_t smem[];  // swizzled boxes start at multiples of 1024 bytes
     uint8_t *const staging = smem + SLOTS * SLOT;
     uint64_t *bars = reinterpret_cast<uint64_t *>(staging + Z::STAGING);
@@ -306,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 2 * SLOTS; ++i) mbar_init(full0 + 8 * i, 1);
         for (int a = 0; a < 2; ++a) {
             mbar_init(tfull0 + 8 * a, 1);
-            mbar_init(tempty0 + 8 * a, 8);
+            mbar_init(tempty0 + 8 * a, PAIR ? 16 : 8);  // a pair's warps all arrive on the even CTA's
         }
         mbar_init(drain, 1);
         fence_mbar_init();
@@ -320,11 +325,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     if (warp == 1) {
-        tmem_alloc(smem_u32(tmem_holder), kTmemCols);
-        tmem_relinquish();
+        if (PAIR) {
+            tmem_alloc_pair(smem_u32(tmem_holder), kTmemCols);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(smem_u32(tmem_holder), kTmemCols);
+            tmem_relinquish();
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync_all();  // both CTAs' barriers exist before either signals the other
     tc_fence_after();
     const uint32_t tmem = *tmem_holder;
     unsigned target = 0;
@@ -388,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                         : f.kind == kGram                               ? maps.x[cur]
                                         : f.kind == kPoly                               ? maps.gram
                                                                                         : maps.poly;
-                for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+                for (int u = worker; ok && u < units; u += workers) {
                     int z, ti, tj, k0, k1;
                     tile_of<BN>(p, f, Z::HALF ? u : u / splits, z, ti, tj);
                     k_range(u, k0, k1);
@@ -397,27 +408,34 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const uint32_t st = slots % SLOTS;
                             ok = mbar_wait(empty0 + 8 * st, ((slots / SLOTS) & 1) ^ 1, p.status);
                             if (!ok) break;
-                            const uint32_t bar = full0 + 8 * st, sa = ring + st * SLOT, sb = sa + A_BYTES;
-                            mbar_expect_tx(bar, SLOT);
-                            // few large boxes: six of 8 KiB a slot kept the issuing thread behind the tensor core
-                            if (f.a_mn) tma_load_4d(sa, ma + q, 0, kb * BK, ti * 2, z, bar);
-                            else tma_load_3d(sa, ma + q, kb * BK, ti * BM, z, bar);
-#pragma unroll
-                            for (int c = 0; c < BN / 128; ++c) {
-                                const uint32_t to = sb + c * 2 * BOX;
-                                if (f.b_mn) tma_load_4d(to, mb + q, 0, kb * BK, tj * (BN / 64) + 2 * c, z, bar);
-                                else tma_load_3d(to, mb + q, kb * BK, tj * BN + 128 * c, z, bar);
+                            const uint32_t sa = ring + st * SLOT, sb = sa + A_BYTES, bar = full0 + 8 * st;
+                            const int k = kb * BK, ra = ti * Z::ROWS + 128 * rank, rb = tj * BN + 128 * rank;
+                            // two boxes of 16 KiB (six of 8 KiB kept the issuing thread behind the tensor core). A pair's
+                            // loads all complete on the even CTA's barrier
+                            if (PAIR) {
+                                const uint32_t pb = map_to_rank(bar, 0);
+                                if (rank == 0) mbar_expect_tx(bar, 2 * SLOT);
+                                if (f.a_mn) tma_load_4d_pair(sa, ma + q, 0, k, ra / 64, z, pb);
+                                else tma_load_3d_pair(sa, ma + q, k, ra, z, pb);
+                                if (f.b_mn) tma_load_4d_pair(sb, mb + q, 0, k, rb / 64, z, pb);
+                                else tma_load_3d_pair(sb, mb + q, k, rb, z, pb);
+                            } else {
+                                mbar_expect_tx(bar, SLOT);
+                                if (f.a_mn) tma_load_4d(sa, ma + q, 0, k, ra / 64, z, bar);
+                                else tma_load_3d(sa, ma + q, k, ra, z, bar);
+                                if (f.b_mn) tma_load_4d(sb, mb + q, 0, k, rb / 64, z, bar);
+                                else tma_load_3d(sb, mb + q, k, rb, z, bar);
                             }
                         }
                 }
             }
             __syncwarp();
         } else if (warp == 1) {
-            if (lane == 0) {  // ---- MMA issuer
-                const uint32_t idesc = idesc_f16_f32(BM, BN, f.a_mn, f.b_mn);
+            if (lane == 0 && rank == 0) {  // ---- MMA issuer (of a pair: the even CTA)
+                const uint32_t idesc = idesc_f16_f32(Z::ROWS, BN, f.a_mn, f.b_mn);
                 const uint32_t a_step = (f.a_mn ? 2048 : 32) >> 4, b_step = (f.b_mn ? 2048 : 32) >> 4;  // descriptor units
                 const uint32_t a_lbo = f.a_mn ? BOX : 16, b_lbo = f.b_mn ? BOX : 16;
-                for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++accs) {
+                for (int u = worker; ok && u < units; u += workers, ++accs) {
                     const int acc = accs & 1;
                     ok = mbar_wait(tempty0 + 8 * acc, ((accs >> 1) & 1) ^ 1, p.status);
                     if (!ok) break;
@@ -435,20 +453,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                         if (!ok) break;
                         tc_fence_after();
+                        const auto product = [&](int qa, int qb, bool first) {
 #pragma unroll
-                        for (int kk = 0; kk < BK / 16; ++kk)
-                            mma_f16_ss(d, da[0] + kk * a_step, db[0] + kk * b_step, idesc, (kb > k0 || kk > 0) ? 1u : 0u);
+                            for (int kk = 0; kk < BK / 16; ++kk) {
+                                const uint64_t ad = da[qa] + kk * a_step, bd = db[qb] + kk * b_step;
+                                const uint32_t add = first && kk == 0 ? 0u : 1u;
+                                if (PAIR) mma_f16_ss_pair(d, ad, bd, idesc, add);
+                                else mma_f16_ss(d, ad, bd, idesc, add);
+                            }
+                        };
+                        product(0, 0, kb == k0);
                         if (f.split) {
-#pragma unroll
-                            for (int kk = 0; kk < BK / 16; ++kk)
-                                mma_f16_ss(d, da[0] + kk * a_step, db[1] + kk * b_step, idesc, 1u);
-#pragma unroll
-                            for (int kk = 0; kk < BK / 16; ++kk)
-                                mma_f16_ss(d, da[1] + kk * a_step, db[0] + kk * b_step, idesc, 1u);
+                            product(0, 1, false);
+                            product(1, 0, false);
                         }
-                        for (int q = 0; q < parts; ++q) mma_commit(empty0 + 8 * ((slots + q) % SLOTS));
+                        for (int q = 0; q < parts; ++q) {
+                            const uint32_t bar = empty0 + 8 * ((slots + q) % SLOTS);
+                            if (PAIR) mma_commit_pair_multicast(bar, 0x3);
+                            else mma_commit(bar);
+                        }
                     }
-                    if (ok) mma_commit(tfull0 + 8 * acc);
+                    if (ok) {
+                        if (PAIR) mma_commit_pair_multicast(tfull0 + 8 * acc, 0x3);
+                        else mma_commit(tfull0 + 8 * acc);
+                    }
                 }
             }
             __syncwarp();
@@ -461,11 +489,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float f_old = f.kind == kApply ? coef[0] : coef[1];
             const float f_acc = (f.kind == kPoly ? coef[2] : 1.f) / kScale;
             const int64_t ld = f.kind == kApply ? p.ldx : p.lds;
-            for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++accs) {
+            for (int u = worker; ok && u < units; u += workers, ++accs) {
                 int z, ti, tj;
                 tile_of<BN>(p, f, Z::HALF ? u : u / splits, z, ti, tj);
                 const int acc = accs & 1;
-                const int i0 = ti * BM + 32 * quad, i = i0 + lane, j0 = tj * BN + EPI * half;
+                const int i0 = ti * Z::ROWS + 128 * rank + 32 * quad, i = i0 + lane, j0 = tj * BN + EPI * half;
                 const int rows = f.M - i0;  // of the warp's 32 that exist
                 uint4 early_h[8], early_l[8];
                 // the exact terms' operands come while the products run (a wide tile's warps are busy with the last tile)
@@ -478,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!ok) break;
                 tc_fence_after();
                 // (j, i) lies in no computed tile (EPI columns share a row tile, a warp's rows a column tile)
-                const bool mirror = Z::HALF && f.kind != kApply && j0 / BM >= column_tiles<BN>(f.tm, i0 / BN);
+                const bool mirror = Z::HALF && f.kind != kApply && j0 / Z::ROWS >= column_tiles<BN>(f.tm, i0 / BN);
                 const uint32_t t = tmem + ((uint32_t)(32 * quad) << 16) + acc * BN + EPI * half;
                 if (!Z::HALF && splits > 1) {  // the piece as it is, column by column
                     float *const piece = p.pieces + ((int64_t)u * BN + EPI * half) * BM + 32 * quad + lane;
@@ -566,7 +594,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(tempty0 + 8 * acc);
+                if (lane == 0) {
+                    if (rank) mbar_arrive_cluster(map_to_rank(tempty0 + 8 * acc, 0));
+                    else mbar_arrive(tempty0 + 8 * acc);
+                }
             }
         }
         if (!Z::HALF && splits > 1) {  // the pieces added in order; A is symmetric, so its columns are written as rows
@@ -595,16 +626,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (go) go = grid_barrier(p, target += gridDim.x, shared_ok);
     }
-    if (warp == 0 && lane == 0) {  // after an error, copies may still be in flight: they land before the CTA exits
-        for (uint32_t i = slots > SLOTS ? slots - SLOTS : 0; i < slots; ++i) {
+    if (warp == 0 && lane == 0 && !ok) {  // after an error, copies may still be in flight: they land before the CTA exits
+        if (PAIR) __nanosleep(200000);  // (their barrier is the even CTA's)
+        for (uint32_t i = slots > SLOTS ? slots - SLOTS : 0; !PAIR && i < slots; ++i) {
             const unsigned long long t0 = globaltimer();
-            while (!mbar_try_wait(full0 + 8 * (i % SLOTS), (i / SLOTS) & 1) &&
-                   globaltimer() - t0 < kWaitTimeoutNs) {
+            while (!mbar_try_wait(full0 + 8 * (i % SLOTS), (i / SLOTS) & 1) && globaltimer() - t0 < kWaitTimeoutNs) {
             }
         }
     }
-    if (warp == 1 && lane == 0) {  // every MMA completes before TMEM is released
-        mma_commit(drain);
+    if (warp == 1 && lane == 0 && rank == 0) {  // every MMA completes before TMEM is released
+        if (PAIR) mma_commit_pair(drain);
+        else mma_commit(drain);
         const unsigned long long t0 = globaltimer();
         while (!mbar_try_wait(drain, 0) && globaltimer() - t0 < kWaitTimeoutNs) {
         }
@@ -612,8 +644,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync_all();  // neither CTA leaves while the pair's MMAs or arrivals may still touch it
     tc_fence_after();
-    if (warp == 1) tmem_dealloc(tmem, kTmemCols);
+    if (warp == 1) {
+        if (PAIR) tmem_dealloc_pair(tmem, kTmemCols);
+        else tmem_dealloc(tmem, kTmemCols);
+    }
 }
 
 // --------------------------------------------------------------------------------------------------------------- host
@@ -665,7 +701,7 @@ int64_t tiles_of(int64_t n, int tile) { return (n + tile - 1) / tile; }
 
 // How a batch of m x n matrices is cut up: by its sizes alone, so that equal calls sum in equal order everywhere.
 struct Plan {
-    bool wide;     // tiles of 128 x 256, else of 128 x 128
+    bool wide;     // tiles of 256 x 256 on pairs of CTAs, else of 128 x 128
     int parts;     // of each matrix in the sum of squares
     int ksplit;    // parts of K in A's products
     size_t x, square, partial, pieces, total;  // bytes of one X, of one A or B, of the partial sums, the pieces, and all
@@ -674,10 +710,10 @@ struct Plan {
 Plan plan_of(int batch, int m, int n) {
     Plan L;
     const int s = std::min(m, n), l = std::max(m, n);
-    // The wide tiles have the better ratio of products to operand bytes, the narrow ones half of the latency (narrower
-    // still would not: an MMA of 64 columns takes as long as one of 128). Wide ones as soon as the larger phase (B·X)
-    // fills the device with them.
-    L.wide = batch * (m > n ? tiles_of(l, BM) * tiles_of(s, 256) : tiles_of(s, BM) * tiles_of(l, 256)) >= kSplitUnits;
+    // The wide tiles have the better ratio of products to operand bytes (single CTAs of 128 x 256 waited for L2: 9728 x
+    // 2560 took 1.57 ms), the narrow ones half of the latency (narrower still would not: an MMA of 64 columns takes as
+    // long as one of 128). Wide ones as soon as the larger phase (B·X) gives every pair of SMs a tile.
+    L.wide = batch * tiles_of(l, 256) * tiles_of(s, 256) >= kSplitUnits / 2;
     L.parts = (int)std::max<int64_t>(1, std::min<int64_t>(kParts / batch, (int64_t)m * up64(n) / 16384));
     // A is s x s over K = l: of a skinny matrix few tiles, each a long sum. Cut K, in parts of four steps or more, where
     // SMs would be idle (16 x 9728: 152 steps of some 700 cycles on one SM otherwise)
@@ -698,10 +734,33 @@ int cuda_failed(cudaError_t e) {
 
 template <int BN>
 int launch(Maps &maps, Params &p, int grid, cudaStream_t s) {
-    const void *k = (const void *)newton_schulz_kernel<BN>;
-    cudaError_t e = smem_limit_once(k, (int)Tile<BN>::SMEM);
-    void *args[] = {&maps, &p};
-    if (e == cudaSuccess) e = cudaLaunchCooperativeKernel(k, dim3(grid), dim3(kThreads), args, Tile<BN>::SMEM, s);
+    const auto k = newton_schulz_kernel<BN>;
+    cudaError_t e = smem_limit_once((const void *)k, (int)Tile<BN>::SMEM);
+    if (e != cudaSuccess) return cuda_failed(e);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Tile<BN>::SMEM;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = Tile<BN>::PAIR ? 2 : 1;
+    if (Tile<BN>::PAIR) {  // pairs that fit at once
+        int pairs = 0;
+        cfg.attrs = attr + 1;
+        cfg.numAttrs = 1;
+        e = cudaOccupancyMaxActiveClusters(&pairs, (const void *)k, &cfg);
+        if (e != cudaSuccess) return cuda_failed(e);
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+        cfg.gridDim = dim3((unsigned)std::min(grid / 2, pairs) * 2);
+    }
+    e = cudaLaunchKernelEx(&cfg, k, maps, p);
     if (e != cudaSuccess) return cuda_failed(e);
     LAMQ_CHECK_LAUNCH("lamq_newton_schulz");
     return LAMQ_OK;
@@ -797,8 +856,8 @@ extern "C" int lamq_newton_schulz(const void *G, int dtype, int64_t ldg, int64_t
     if (e != cudaSuccess) return cuda_failed(e);
     // a CTA per unit of the phase with the most of them, at most one per SM
     const int bn = L.wide ? 256 : 128;
-    const int64_t apply = batch * (p.tall ? tiles_of(p.l, BM) * tiles_of(p.s, bn) : tiles_of(p.s, BM) * tiles_of(p.l, bn));
-    const int64_t gram = batch * tiles_of(p.s, BM) * tiles_of(p.s, bn) * L.ksplit;
-    const int grid = (int)std::min<int64_t>(sms, std::max<int64_t>({apply, gram, (int64_t)batch * L.parts, L.ksplit > 1 ? sms : 1}));
+    const int64_t apply = batch * tiles_of(p.l, bn) * tiles_of(p.s, bn), gram = batch * tiles_of(p.s, bn) * tiles_of(p.s, bn);
+    const int grid = (int)std::min<int64_t>(sms, std::max<int64_t>({apply * (L.wide ? 2 : 1), gram * L.ksplit,
+                                                                   (int64_t)batch * L.parts, L.ksplit > 1 ? sms : 1}));
     return L.wide ? launch<256>(maps, p, grid, s) : launch<128>(maps, p, grid, s);
 }

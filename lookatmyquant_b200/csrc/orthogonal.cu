@@ -289,6 +289,30 @@ __device__ __forceinline__ void store_block(uint8_t *buf, const uint4 (&q)[8], T
     }
 }
 
+// The same block transposed: 64 rows (of which `rows` exist) of 32 values (pieces up to column `cols`).
+__device__ __forceinline__ void store_transposed(uint8_t *buf, const uint4 (&q)[8], __half *base, int64_t ld, int rows,
+                                                 int cols) {
+    const int lane = threadIdx.x & 31;
+    uint16_t *t = reinterpret_cast<uint16_t *>(buf) + lane;
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        const uint32_t w[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            t[(8 * c + 2 * e) * 32] = (uint16_t)w[e];
+            t[(8 * c + 2 * e + 1) * 32] = (uint16_t)(w[e] >> 16);
+        }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = 8 * i + (lane >> 2), c = 8 * (lane & 3);
+        if (r < rows && c < cols)
+            *reinterpret_cast<uint4 *>(base + r * ld + c) = *reinterpret_cast<const uint4 *>(buf + r * 64 + 2 * c);
+    }
+}
+
 template <int BN>
 __global__ void __launch_bounds__(kThreads, 1)
     newton_schulz_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
@@ -575,22 +599,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int g = 0; g < 8; ++g) {
                         split8(v + 8 * g, qh[g], ql[g]);
-                        if (mirror && i < f.M) {
-                            union { uint4 q; __half h[8]; } hi, lo;
-                            hi.q = qh[g];
-                            lo.q = ql[g];
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const int j = j0 + c + 8 * g + e;
-                                if (j < f.M) {
-                                    dst[0][((int64_t)z * f.M + j) * ld + i] = hi.h[e];
-                                    dst[1][((int64_t)z * f.M + j) * ld + i] = lo.h[e];
-                                }
-                            }
-                        }
                     }
                     store_block(buf, qh, dst[0] + at0, ld, rows);
                     store_block(buf, ql, dst[1] + at0, ld, rows);
+                    if (mirror) {
+                        const int64_t back = ((int64_t)z * f.M + j0 + c) * ld + i0;
+                        store_transposed(buf, qh, dst[0] + back, ld, f.M - j0 - c, (int)ld - i0);
+                        store_transposed(buf, ql, dst[1] + back, ld, f.M - j0 - c, (int)ld - i0);
+                    }
                 }
                 tc_fence_before();
                 __syncwarp();

@@ -903,9 +903,18 @@ int tile_map(CUtensorMap *m, const lamq_heads &t, int B, int H, int64_t L, int D
     const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)L, (cuuint64_t)H, (cuuint64_t)B};
     const cuuint64_t strides[3] = {stride(L, t.row, dense), stride(H, t.head, dense), stride(B, t.batch, dense)};
     const cuuint32_t box[4] = {64, kTile, 1, 1}, step[4] = {1, 1, 1, 1};
-    const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, t.data, dims, strides, box, step,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const auto make = [&] {
+        return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, t.data, dims, strides, box, step,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = make();
+    if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+        // a driver call needs the device's context bound to the thread, and one that has made no runtime call yet
+        // (autograd's) has none: bind it
+        int dev = 0;
+        if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = make();
+    }
     if (r != CUDA_SUCCESS) {
         set_error("lamq_attention: cuTensorMapEncodeTiled failed (%d)", (int)r);
         return LAMQ_ERR_CUDA;
@@ -956,15 +965,6 @@ Rows rows_of(const lamq_heads &t) { return {reinterpret_cast<__nv_bfloat16 *>(t.
 int launch_failed(const char *what, cudaError_t e) {
     set_error("%s: %s", what, cudaGetErrorString(e));
     return LAMQ_ERR_CUDA;
-}
-
-// The tensor maps are made by a driver call, which needs the device's context bound to the calling thread; a thread that
-// has made no runtime call yet (autograd's) has none.
-int bind_context(const char *fn) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess) e = cudaSetDevice(dev);
-    return e == cudaSuccess ? LAMQ_OK : launch_failed(fn, e);
 }
 
 template <int HD>
@@ -1046,7 +1046,6 @@ extern "C" int lamq_attention_forward(const lamq_attention_args *args, int *stat
         if (int e = check_heads(fn, "v", a.v, s.B, s.Hkv, s.Lk)) return e;
     }
     LAMQ_REQUIRE(a.lse != nullptr, "%s: null pointer (lse)", fn);
-    if (int e = bind_context(fn)) return e;
     return s.D <= 64 ? run_forward<64>(a, s, (cudaStream_t)stream) : run_forward<128>(a, s, (cudaStream_t)stream);
 }
 
@@ -1080,7 +1079,6 @@ extern "C" int lamq_attention_backward(const lamq_attention_args *args, void *wo
     const size_t need = lamq_attention_backward_workspace_size(s.B, s.Hq, s.Lq);
     LAMQ_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (uintptr_t)workspace % 16 == 0)),
                  "%s: workspace of %zu bytes (16-byte aligned) needed, %zu given", fn, need, workspace_bytes);
-    if (int e = bind_context(fn)) return e;
     float *lse2 = reinterpret_cast<float *>(workspace);
     float *D = lse2 + need / (2 * sizeof(float));
     return s.D <= 64 ? run_backward<64>(a, s, lse2, D, (cudaStream_t)stream)

@@ -108,12 +108,26 @@ def check_status():
     _STATUS.check()
 
 
-def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
-    if x.dtype not in _DTYPES or not x.is_cuda:
+def _matrix(x: torch.Tensor, what: str):
+    """(x, its leading dimension, its type in the C ABI), x copied where its rows are not contiguous."""
+    code = _DTYPES.get(x.dtype)
+    if code is None or not x.is_cuda:
         raise TypeError(f"{what} must be a float32 or bfloat16 CUDA tensor")
-    if x.stride(-1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
-        x = x.contiguous()
-    return x
+    ld, one = x.stride()
+    rows, d = x.shape
+    if one != 1 or ld < d:
+        if (one != 1 and d > 1) or (ld < d and rows > 1):
+            x = x.contiguous()
+            ld = x.stride(0)
+        ld = max(ld, d)  # of a single row or column: any
+    return x, ld, code
+
+
+def _rows_like(shape, d: int, x: torch.Tensor) -> torch.Tensor:
+    """An empty contiguous tensor of shape + (d,), of x's type and device."""
+    if len(shape) == 1:
+        return torch.empty_strided((shape[0], d), (d, 1), dtype=x.dtype, device=x.device)
+    return torch.empty((*shape, d), dtype=x.dtype, device=x.device)
 
 
 def _ids(ids: torch.Tensor, device) -> torch.Tensor:
@@ -136,17 +150,16 @@ def lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_i
     `check_status()`."""
     if table.ndim != 2:
         raise ValueError("the table must be a matrix")
-    table = _matrix(table, "the table")
+    table, ld, code = _matrix(table, "the table")
     dev = table.device
     ids = _ids(ids, dev)
     V, d = table.shape
-    out = torch.empty((*ids.shape, d), dtype=table.dtype, device=dev)
+    out = _rows_like(ids.shape, d, table)
     here, stream = launch_on(dev)
     with here:
         check(_lib.load().lamq_embedding_lookup(
-            ptr(table), _DTYPES[table.dtype], max(table.stride(0), d), V, d, ptr(ids), ids.dtype == torch.int64,
-            ids.numel(), scale, _padding(padding_idx, V), ptr(out), d, ptr(_STATUS.on(dev)),
-            stream), "lamq_embedding_lookup")
+            table.data_ptr(), code, ld, V, d, ids.data_ptr(), ids.dtype is torch.int64, ids.numel(), scale,
+            _padding(padding_idx, V), out.data_ptr(), d, _STATUS.on(dev).data_ptr(), stream), "lamq_embedding_lookup")
     return out
 
 
@@ -160,7 +173,7 @@ def lookup_gradient(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: flo
     if rows < 0:
         raise ValueError("rows must not be negative")
     d = grad.shape[-1]
-    grad = _matrix(grad.reshape(-1, d), "the gradient")
+    grad, ld, code = _matrix(grad if grad.ndim == 2 else grad.reshape(-1, d), "the gradient")
     dev = grad.device
     ids = _ids(ids, dev)
     accumulate = out is not None
@@ -169,7 +182,7 @@ def lookup_gradient(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: flo
                 rows > 1 and out.stride(0) < d):
             raise ValueError(f"out must be a {rows} x {d} {grad.dtype} matrix with contiguous rows on {dev}")
     else:
-        out = torch.empty(rows, d, dtype=grad.dtype, device=dev)
+        out = _rows_like((rows,), d, grad)
     lib = _lib.load()
     n = ids.numel()
     size = lib.lamq_embedding_gradient_workspace_size(n, d)
@@ -177,9 +190,9 @@ def lookup_gradient(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: flo
     here, stream = launch_on(dev)
     with here:
         check(lib.lamq_embedding_gradient(
-            ptr(grad), _DTYPES[grad.dtype], max(grad.stride(0), d), ptr(ids), ids.dtype == torch.int64, n, rows, d,
-            scale, _padding(padding_idx, rows), accumulate, ptr(out), max(out.stride(0), d), ptr(ws),
-            size, ptr(_STATUS.on(dev)), stream), "lamq_embedding_gradient")
+            grad.data_ptr(), code, ld, ids.data_ptr(), ids.dtype is torch.int64, n, rows, d, scale,
+            _padding(padding_idx, rows), accumulate, out.data_ptr(), max(out.stride(0), d), ptr(ws), size,
+            _STATUS.on(dev).data_ptr(), stream), "lamq_embedding_gradient")
     return out
 
 

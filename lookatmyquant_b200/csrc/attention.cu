@@ -44,6 +44,7 @@ using namespace sm100;
 
 constexpr int kTile = 128;
 constexpr int kThreads = 320;
+constexpr int kFill = 148;  // CTAs that fill the device
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -73,7 +74,7 @@ struct Sizes {
     // load came a TMA latency too late and S waited 1100 of 3300 cycles a tile.
     static constexpr int LATE_STAGES = HD == 128 ? 3 : 4, EARLY_STAGES = HD == 128 ? 2 : 4;
     static constexpr int ROW = kTile * 4;               // bytes of lse (or D) of a query tile
-    static constexpr size_t FWD_SMEM = 2 * TILE + FWD_STAGES * TILE + 256;
+    static constexpr size_t FWD_SMEM = 2 * TILE + FWD_STAGES * TILE + 256 + 4 * ROW;
     static constexpr size_t DQ_SMEM = 2 * TILE + (LATE_STAGES + EARLY_STAGES) * TILE + 256 + 2 * ROW;
     static constexpr size_t DKV_SMEM = 2 * TILE + (LATE_STAGES + EARLY_STAGES) * (TILE + ROW) + 256;
 };
@@ -171,6 +172,11 @@ __device__ __forceinline__ void wait_bounded(uint32_t bar, uint32_t parity) {
     }
 }
 
+__device__ __forceinline__ uint4 pack8(const float (&x)[8], float f) {
+    return make_uint4(pack_bf16(x[0] * f, x[1] * f), pack_bf16(x[2] * f, x[3] * f), pack_bf16(x[4] * f, x[5] * f),
+                      pack_bf16(x[6] * f, x[7] * f));
+}
+
 // One arrival for the warp, after its TMEM reads and writes.
 __device__ __forceinline__ void warp_arrive(uint32_t bar) {
     tc_fence_before();
@@ -206,6 +212,13 @@ __device__ __forceinline__ void zero_row(__nv_bfloat16 *dst, int D) {
 
 // ------------------------------------------------------------------------------------------------------------ forward
 
+// A float of another CTA's shared memory.
+__device__ __forceinline__ float load_cluster(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
+}
+
 // The key tiles [j0, j0 + n) that the queries row0 .. row0 + 127 meet.
 __device__ __forceinline__ int key_tiles(const Shape &s, int row0, int lo, int hi) {
     if (row0 >= s.Lq) return 0;
@@ -217,24 +230,30 @@ __device__ __forceinline__ int key_tiles(const Shape &s, int row0, int lo, int h
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
-                             const __grid_constant__ CUtensorMap mapV, Shape s, Rows out, float *__restrict__ lse) {
+                             const __grid_constant__ CUtensorMap mapV, Shape s, Rows out, float *__restrict__ lse, int split) {
     using Z = Sizes<HD>;
     constexpr int STAGES = Z::FWD_STAGES;
     extern __shared__ __align__(1024) uint8_t smem[];  // swizzled tiles start at multiples of 1024 bytes
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + STAGES) * Z::TILE);
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 8);
+    float *const parts = reinterpret_cast<float *>(smem + 2 * Z::TILE);
+    float *const row_max = reinterpret_cast<float *>(smem + Z::FWD_SMEM - 4 * Z::ROW), *const row_sum = row_max + 2 * kTile;
+    static_assert(2 * HD * kTile * 4 <= STAGES * Z::TILE, "the parts of O fit into the stages");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), q_full = smem_u32(bars + 2 * STAGES);
     const uint32_t s_full0 = q_full + 8, p_ready0 = q_full + 24, pv_done0 = q_full + 40, drain = q_full + 56;
     const uint32_t sq = smem_u32(smem), skv = sq + 2 * Z::TILE;
 
     const int pairs = s.lq_pad / kTile / 2 + (s.lq_pad / kTile & 1), heads = s.Hq * s.B;
-    const int qp = pairs - 1 - (int)(blockIdx.x / heads);  // the longest rows of a causal mask first
-    const int bh = (int)(blockIdx.x % heads), b = bh / s.Hq, h = bh % s.Hq, hk = h / s.group;
+    // `split` CTAs (a cluster) share a pair of query tiles where there would be too few: each takes a part of the keys
+    const int unit = (int)blockIdx.x / split, rank = (int)blockIdx.x % split;
+    const int qp = pairs - 1 - unit / heads;  // the longest rows of a causal mask first
+    const int bh = unit % heads, b = bh / s.Hq, h = bh % s.Hq, hk = h / s.group;
     int lo, hi;
     key_range(s, b, lo, hi);
-    const int n0 = key_tiles(s, (2 * qp) * kTile, lo, hi), n1 = key_tiles(s, (2 * qp + 1) * kTile, lo, hi);
-    const int n = max(n0, n1), j0 = lo / kTile;
+    const int all0 = key_tiles(s, (2 * qp) * kTile, lo, hi), all1 = key_tiles(s, (2 * qp + 1) * kTile, lo, hi);
+    const int n_all = max(all0, all1), first = n_all * rank / split, n = n_all * (rank + 1) / split - first;
+    const int n0 = min(n, max(0, all0 - first)), n1 = min(n, max(0, all1 - first)), j0 = lo / kTile + first;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2 * STAGES + 1; ++i) mbar_init(full0 + 8 * i, 1);
@@ -398,7 +417,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * t, (nt - 1) & 1, s.status));
             tc_fence_after();
         }
-        if (ok) {
+        if (split > 1 && n > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(drain, 0, s.status));  // the other tile's too
+        if (ok && split > 1 && n_all > 0) {  // to the cluster: columns of 128 rows over the stages, which are done with
+            row_max[t * kTile + 32 * quad + lane] = m;
+            row_sum[t * kTile + 32 * quad + lane] = sum;
+            float *const mine = parts + t * HD * kTile + 32 * quad + lane;
+#pragma unroll 1
+            for (int c = 0; nt > 0 && c < HD; c += 32) {
+                uint32_t r[32];
+                tmem_load32(to + c, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int x = 0; x < 32; ++x) mine[(c + x) * kTile] = __uint_as_float(r[x]);
+            }
+        } else if (ok && rank == 0) {
             __nv_bfloat16 *dst = out.p + b * out.batch + h * out.head + (int64_t)i * out.row;
             if (nt > 0) store_row<HD>(dst, to, 0, s.D, sum > 0.f || sum != sum ? 1.f / sum : 0.f, live);
             else if (live) zero_row(dst, s.D);
@@ -406,6 +438,36 @@ __global__ void __launch_bounds__(kThreads, 1)
                 lse[((int64_t)b * s.Hq + h) * s.Lq + i] =
                     sum == 0.f ? -INFINITY : ((m == -INFINITY ? 0.f : m * s.sl) + log2f(sum)) * kLn2;
         }
+    }
+    if (split > 1 && n_all > 0) {  // the parts joined by their maxima, in the order of the keys, a share of the columns each
+        cluster_sync_all();
+        if (warp >= 2) {
+            const int pieces = 2 * HD / 8, p0 = pieces * rank / split, p1 = pieces * (rank + 1) / split;
+            for (int e = p0 * kTile + (int)threadIdx.x - 64; e < p1 * kTile; e += 256) {
+                const int row = e % kTile, col = e / kTile * 8 % HD, t = e / kTile * 8 / HD;
+                const int i = (2 * qp + t) * kTile + row;
+                if (i >= s.Lq || col >= s.D) continue;
+                const uint32_t at_max = smem_u32(row_max + t * kTile + row), at_sum = smem_u32(row_sum + t * kTile + row);
+                const uint32_t at = smem_u32(parts + (t * HD + col) * kTile + row);
+                float m = -INFINITY, sum = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                for (int q = 0; q < split; ++q) m = fmaxf(m, load_cluster(map_to_rank(at_max, q)));
+                for (int q = 0; q < split; ++q) {
+                    const float mq = load_cluster(map_to_rank(at_max, q)), sq = load_cluster(map_to_rank(at_sum, q));
+                    if (sq == 0.f) continue;  // no key of this part (its columns may not even be written)
+                    const float w = mq == m ? 1.f : ex2((mq - m) * s.sl);
+                    sum = fmaf(w, sq, sum);
+                    const uint32_t from = map_to_rank(at, q);
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) acc[x] = fmaf(w, load_cluster(from + x * kTile * 4), acc[x]);
+                }
+                *reinterpret_cast<uint4 *>(out.p + b * out.batch + h * out.head + (int64_t)i * out.row + col) =
+                    pack8(acc, sum == 0.f ? 0.f : 1.f / sum);
+                if (col == 0)
+                    lse[((int64_t)b * s.Hq + h) * s.Lq + i] =
+                        sum == 0.f ? -INFINITY : ((m == -INFINITY ? 0.f : m * s.sl) + log2f(sum)) * kLn2;
+            }
+        }
+        cluster_sync_all();  // a CTA's shared memory stays until all have read it
     }
     tc_fence_before();
     __syncthreads();
@@ -430,7 +492,7 @@ template <int HD>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
                         const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapG, Shape s,
-                        const float *__restrict__ lse, float *__restrict__ lse2, float *__restrict__ Dr, Rows o, Rows dq) {
+                        const float *__restrict__ lse, float *__restrict__ lse2, float *__restrict__ Dr, Rows o, Rows dq, int split) {
     using Z = Sizes<HD>;
     constexpr int KS = Z::LATE_STAGES, VS = Z::EARLY_STAGES;
     // TMEM columns. Q and dO lie there as A operands: from shared memory they would take, with the key tile's rows, all
@@ -439,6 +501,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ __align__(1024) uint8_t smem[];  // swizzled tiles start at multiples of 1024 bytes
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + KS + VS) * Z::TILE);
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 2 * (KS + VS) + 9);
+    float *const parts = reinterpret_cast<float *>(smem + 2 * Z::TILE);
+    static_assert(HD * kTile * 4 <= (KS + VS) * Z::TILE, "the part of dQ fits into the stages");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t k_full0 = smem_u32(bars), v_full0 = k_full0 + 8 * KS, k_empty0 = v_full0 + 8 * VS,
                    v_empty0 = k_empty0 + 8 * KS, q_full = v_empty0 + 8 * VS;
@@ -448,12 +512,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t sq = smem_u32(smem), sg = sq + Z::TILE, sk = sg + Z::TILE, sv = sk + KS * Z::TILE;
 
     const int tiles = s.lq_pad / kTile, heads = s.Hq * s.B;
-    const int qt = tiles - 1 - (int)(blockIdx.x / heads);
-    const int bh = (int)(blockIdx.x % heads), b = bh / s.Hq, h = bh % s.Hq, hk = h / s.group;
+    const int unit = (int)blockIdx.x / split, rank = (int)blockIdx.x % split;  // as in the forward
+    const int qt = tiles - 1 - unit / heads;
+    const int bh = unit % heads, b = bh / s.Hq, h = bh % s.Hq, hk = h / s.group;
     const int row0 = qt * kTile;
     int lo, hi;
     key_range(s, b, lo, hi);
-    const int n = key_tiles(s, row0, lo, hi), j0 = lo / kTile;
+    const int n_all = key_tiles(s, row0, lo, hi), first = n_all * rank / split, n = n_all * (rank + 1) / split - first;
+    const int j0 = lo / kTile + first;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2 * (KS + VS) + 1; ++i) mbar_init(k_full0 + 8 * i, 1);
@@ -573,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         half_d[half * kTile + 32 * quad + lane] = Di;
         asm volatile("bar.sync 1, 256;" ::: "memory");
         Di = half_d[32 * quad + lane] + half_d[kTile + 32 * quad + lane];
-        if (half == 0) {
+        if (half == 0 && rank == split - 1) {  // (the last part is never without keys where there are any)
             lse2[(int64_t)bh * s.lq_pad + i] = l2;
             Dr[(int64_t)bh * s.lq_pad + i] = Di;
         }
@@ -632,11 +698,40 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = __all_sync(0xffffffffu, mbar_wait(done, 0, s.status));
             tc_fence_after();
         }
-        if (ok || n == 0) {
+        if (split > 1 && n_all > 0) {  // to the cluster: columns of 128 rows over the stages, which are done with
+            float *const mine = parts + half * (HD / 2) * kTile + 32 * quad + lane;
+#pragma unroll 1
+            for (int c = 0; c < HD / 2; c += 32) {
+                uint32_t r[32];
+                tmem_load32(tmem + lanes + kDQ + half * (HD / 2) + c, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int x = 0; x < 32; ++x) mine[(c + x) * kTile] = n > 0 ? __uint_as_float(r[x]) : 0.f;
+            }
+        } else if ((ok || n == 0) && rank == 0) {
             __nv_bfloat16 *dst = dq.p + b * dq.batch + h * dq.head + (int64_t)i * dq.row;
             if (n > 0) store_row<HD / 2>(dst, tmem + lanes + kDQ + half * (HD / 2), half * (HD / 2), s.D, s.scale, live);
             else if (live && half == 0) zero_row(dst, s.D);
         }
+    }
+    if (split > 1 && n_all > 0) {  // the parts added in the order of the keys, a share of the columns each
+        cluster_sync_all();
+        if (warp >= 2) {
+            const int pieces = HD / 8, p0 = pieces * rank / split, p1 = pieces * (rank + 1) / split;
+            for (int e = p0 * kTile + (int)threadIdx.x - 64; e < p1 * kTile; e += 256) {
+                const int row = e % kTile, col = e / kTile * 8;
+                if (row0 + row >= s.Lq || col >= s.D) continue;
+                float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                for (int q = 0; q < split; ++q) {
+                    const uint32_t from = map_to_rank(smem_u32(parts + col * kTile + row), q);
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) acc[x] += load_cluster(from + x * kTile * 4);
+                }
+                *reinterpret_cast<uint4 *>(dq.p + b * dq.batch + h * dq.head + (int64_t)(row0 + row) * dq.row + col) =
+                    pack8(acc, s.scale);
+            }
+        }
+        cluster_sync_all();
     }
     tc_fence_before();
     __syncthreads();
@@ -648,7 +743,7 @@ template <int HD>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
                          const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapG, Shape s,
-                         const float *__restrict__ lse2, const float *__restrict__ Dr, Rows dk, Rows dv) {
+                         const float *__restrict__ lse2, const float *__restrict__ Dr, Rows dk, Rows dv, int split) {
     using Z = Sizes<HD>;
     constexpr int QS = Z::LATE_STAGES, GS = Z::EARLY_STAGES;  // Q (with lse), dO (with D)
     // TMEM columns. Pᵀ and dSᵀ (bf16) lie over Sᵀ and dPᵀ: the threads of columns 0..63 write columns 0..31 of them,
@@ -658,6 +753,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     float *row_lse = reinterpret_cast<float *>(smem + (2 + QS + GS) * Z::TILE), *row_d = row_lse + QS * kTile;
     uint64_t *bars = reinterpret_cast<uint64_t *>(row_d + GS * kTile);
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 2 * (QS + GS) + 7);
+    float *const parts = reinterpret_cast<float *>(smem + 2 * Z::TILE);
+    static_assert(2 * HD * kTile * 4 <= (QS + GS) * Z::TILE, "the parts of dK and dV fit into the stages");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t q_full0 = smem_u32(bars), g_full0 = q_full0 + 8 * QS, q_empty0 = g_full0 + 8 * GS,
                    g_empty0 = q_empty0 + 8 * QS, kv_full = g_empty0 + 8 * GS;
@@ -665,9 +762,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t done = kv_full + 40;
     const uint32_t sk = smem_u32(smem), sv = sk + Z::TILE, sq = sv + Z::TILE, sg = sq + QS * Z::TILE;
 
-    const int heads = s.Hkv * s.B;
-    const int kt = (int)(blockIdx.x / heads);  // the first keys are seen by the most queries: they come first
-    const int bh = (int)(blockIdx.x % heads), b = bh / s.Hkv, hk = bh % s.Hkv;
+    // `split` CTAs (a cluster) share a key tile where there would be too few: each takes a part of the group's query heads
+    const int heads = s.Hkv * s.B, unit = (int)blockIdx.x / split, rank = (int)blockIdx.x % split;
+    const int kt = unit / heads;  // the first keys are seen by the most queries: they come first
+    const int bh = unit % heads, b = bh / s.Hkv, hk = bh % s.Hkv, h0 = hk * s.group + rank * (s.group / split);
     const int key0 = kt * kTile;
     int lo, hi;
     key_range(s, b, lo, hi);
@@ -675,7 +773,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int first = s.causal ? max(q_lo, key0 - s.off) : 0;
     const int t0 = first / kTile, tiles = s.lq_pad / kTile;
     const int nq = key0 >= hi || key0 + kTile <= lo || first >= s.Lq ? 0 : tiles - t0;
-    const int n = nq * s.group;
+    const int n = nq * (s.group / split);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2 * (QS + GS) + 1; ++i) mbar_init(q_full0 + 8 * i, 1);
@@ -707,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             int q_issued = 0, g_issued = 0;
             bool ok = true;
             for (int j = 0; j < n; ++j) {  // dO's stage is released by an earlier product than Q's of the same query tile
-                const int qs = j % QS, gs = j % GS, h = hk * s.group + j / nq, row = (t0 + j % nq) * kTile;
+                const int qs = j % QS, gs = j % GS, h = h0 + j / nq, row = (t0 + j % nq) * kTile;
                 const int64_t at = ((int64_t)b * s.Hq + h) * s.lq_pad + row;
                 ok = mbar_wait(q_empty0 + 8 * qs, ((j / QS) & 1) ^ 1, s.status);
                 if (!ok) break;
@@ -858,13 +956,45 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int c0 = half * (HD / 2);
             __nv_bfloat16 *pk_ = dk.p + b * dk.batch + hk * dk.head + (int64_t)key * dk.row;
             __nv_bfloat16 *pv_ = dv.p + b * dv.batch + hk * dv.head + (int64_t)key * dv.row;
-            if (n > 0) {
+            if (split > 1 && n > 0) {  // to the cluster: columns of 128 rows over the stages, which are done with
+                float *const mine = parts + c0 * kTile + 32 * quad + lane;
+#pragma unroll 1
+                for (int m = 0; m < 2; ++m)
+#pragma unroll 1
+                    for (int c = 0; c < HD / 2; c += 32) {
+                        uint32_t r[32];
+                        tmem_load32(tmem + lanes + (m ? kDV : kDK) + c0 + c, r);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) mine[(m * HD + c + x) * kTile] = __uint_as_float(r[x]);
+                    }
+            } else if (n > 0) {
                 store_row<HD / 2>(pk_, tmem + lanes + kDK + c0, c0, s.D, s.scale, live);
                 store_row<HD / 2>(pv_, tmem + lanes + kDV + c0, c0, s.D, 1.f, live);
-            } else if (live) {
+            } else if (live && rank == 0) {
                 zero_row(half ? pv_ : pk_, s.D);
             }
         }
+    }
+    if (split > 1 && n > 0) {  // each CTA adds its share of the columns over the cluster, in the order of the heads
+        cluster_sync_all();
+        if (warp >= 2) {
+            const int pieces = 2 * HD / 8, p0 = pieces * rank / split, p1 = pieces * (rank + 1) / split;
+            for (int i = p0 * kTile + (int)threadIdx.x - 64; i < p1 * kTile; i += 256) {
+                const int row = i % kTile, col = i / kTile * 8 % HD, m = i / kTile * 8 / HD;
+                if (key0 + row >= s.Lk || col >= s.D) continue;
+                float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                for (int q = 0; q < split; ++q) {
+                    const uint32_t from = map_to_rank(smem_u32(parts + (m * HD + col) * kTile + row), q);
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) acc[x] += load_cluster(from + x * kTile * 4);
+                }
+                const Rows &to = m ? dv : dk;
+                *reinterpret_cast<uint4 *>(to.p + b * to.batch + hk * to.head + (int64_t)(key0 + row) * to.row + col) =
+                    pack8(acc, m ? 1.f : s.scale);
+            }
+        }
+        cluster_sync_all();  // a CTA's shared memory stays until all have read it
     }
     tc_fence_before();
     __syncthreads();
@@ -967,6 +1097,43 @@ int launch_failed(const char *what, cudaError_t e) {
     return LAMQ_ERR_CUDA;
 }
 
+// A launch of `units` clusters of `split` CTAs.
+template <typename K, typename... A>
+cudaError_t launch_split(K *kernel, int64_t units, int split, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(units * split));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = split > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// CTAs per pair of query tiles (forward) or query tile (dq): 1, or where the device would hold more the largest power of
+// two up to 8 that it holds at once, in parts of four key tiles or more. 32/8 heads of 128, one query over 4096 keys:
+// forward 57 us whole, 26 in parts; dq 44 and 18. (A second wave of parts costs more than it gains: 32/8 heads, 512
+// queries and keys, dq 13 us whole, 23 in 256 CTAs.)
+int split_keys(int64_t units, int Lk) {
+    int split = 1;
+    while (split < 8 && units * split * 2 <= kFill && (Lk + kTile - 1) / kTile >= 8 * split) split *= 2;
+    return split;
+}
+
+// CTAs per key tile (dkv): 1, or where the tiles leave SMs idle the part of the group's query heads, up to 8, with which
+// they fill it; beyond one wave only if a CTA keeps eight query tiles or more. 2048 queries and keys, 15/5 heads of 64 (80
+// tiles): 86 us whole, 43 by heads; 1000 of 8/1 heads of 96 (8 tiles): 119 and 25; one query over 2048 keys: 10 and 20.
+int split_heads(int64_t units, int group, int q_tiles) {
+    int split = 1;
+    for (int c = 2; c <= 8 && units * split < kFill; ++c)
+        if (group % c == 0 && (units * c <= kFill || group / c * q_tiles >= 8)) split = c;
+    return split;
+}
+
 template <int HD>
 int run_forward(const lamq_attention_args &a, const Shape &s, cudaStream_t st) {
     CUtensorMap mq, mk, mv;
@@ -982,7 +1149,9 @@ int run_forward(const lamq_attention_args &a, const Shape &s, cudaStream_t st) {
     auto *k = attention_forward_kernel<HD>;
     if (cudaError_t e = smem_limit_once((const void *)k, (int)Sizes<HD>::FWD_SMEM))
         return launch_failed("lamq_attention_forward", e);
-    k<<<(unsigned)blocks, kThreads, Sizes<HD>::FWD_SMEM, st>>>(mq, mk, mv, s, rows_of(a.o), a.lse);
+    const int split = split_keys(blocks, s.Lk);
+    if (cudaError_t e = launch_split(k, blocks, split, Sizes<HD>::FWD_SMEM, st, mq, mk, mv, s, rows_of(a.o), a.lse, split))
+        return launch_failed("lamq_attention_forward", e);
     LAMQ_CHECK_LAUNCH("lamq_attention_forward");
     return LAMQ_OK;
 }
@@ -1007,8 +1176,10 @@ int run_backward(const lamq_attention_args &a, const Shape &s, float *lse2, floa
         auto *k = attention_dq_kernel<HD>;
         if (cudaError_t e = smem_limit_once((const void *)k, (int)Sizes<HD>::DQ_SMEM))
             return launch_failed("lamq_attention_backward", e);
-        k<<<(unsigned)tiles, kThreads, Sizes<HD>::DQ_SMEM, st>>>(mq, mk, mv, mg, s, a.lse, lse2, D, rows_of(a.o),
-                                                                 rows_of(a.dq));
+        const int split = split_keys(tiles, s.Lk);
+        if (cudaError_t e = launch_split(k, tiles, split, Sizes<HD>::DQ_SMEM, st, mq, mk, mv, mg, s,
+                                         (const float *)a.lse, lse2, D, rows_of(a.o), rows_of(a.dq), split))
+            return launch_failed("lamq_attention_backward", e);
         LAMQ_CHECK_LAUNCH("lamq_attention_backward dq");
     }
     if (keys) {
@@ -1017,8 +1188,10 @@ int run_backward(const lamq_attention_args &a, const Shape &s, float *lse2, floa
         auto *k = attention_dkv_kernel<HD>;
         if (cudaError_t e = smem_limit_once((const void *)k, (int)Sizes<HD>::DKV_SMEM))
             return launch_failed("lamq_attention_backward", e);
-        k<<<(unsigned)tiles, kThreads, Sizes<HD>::DKV_SMEM, st>>>(mq, mk, mv, mg, s, lse2, D, rows_of(a.dk),
-                                                                 rows_of(a.dv));
+        const int split = split_heads(tiles, s.group, s.lq_pad / kTile);
+        if (cudaError_t e = launch_split(k, tiles, split, Sizes<HD>::DKV_SMEM, st, mq, mk, mv, mg, s,
+                                         (const float *)lse2, (const float *)D, rows_of(a.dk), rows_of(a.dv), split))
+            return launch_failed("lamq_attention_backward", e);
         LAMQ_CHECK_LAUNCH("lamq_attention_backward dkv");
     }
     return LAMQ_OK;

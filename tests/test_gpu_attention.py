@@ -94,7 +94,10 @@ SHAPES = [  # B, Hq, Hkv, Lq, Lk, D
     (1, 2, 1, 128, 128, 128), (1, 2, 1, 129, 129, 128), (2, 3, 3, 256, 256, 96), (1, 6, 2, 257, 257, 64),
     (1, 2, 2, 385, 385, 80), (3, 8, 1, 300, 300, 128), (1, 2, 1, 1, 700, 128), (1, 4, 2, 5, 1000, 64),
     (2, 2, 1, 130, 517, 128), (1, 2, 2, 513, 129, 64), (1, 3, 1, 200, 3, 128), (1, 15, 5, 1100, 1100, 64),
-    (1, 2, 1, 1, 1, 128), (1, 1, 1, 640, 640, 72)]
+    (1, 2, 1, 1, 1, 128), (1, 1, 1, 640, 640, 72),
+    # few tiles: their work is split over a cluster, by query heads (groups of every kind) and by keys
+    (1, 16, 1, 260, 260, 64), (1, 7, 1, 200, 333, 128), (1, 11, 1, 140, 140, 64), (2, 12, 2, 130, 130, 96),
+    (1, 2, 1, 3, 1500, 64), (1, 1, 1, 1, 2048, 128), (1, 2, 2, 300, 1290, 128), (1, 1, 1, 129, 640, 40)]
 
 
 @pytest.mark.parametrize("causal", [True, False])

@@ -222,6 +222,23 @@ def test_gradient_against_differences():
             assert abs(quotient - float((got[name].double() * d).sum())) <= bound
 
 
+def test_offsets_past_32_bits():
+    """Keys beyond 2^31 elements (2^32 bytes) of their tensors: the last 300 of 2.2 million, and their gradients."""
+    B, Hq, Hkv, Lq, Lk, D, used = 1, 8, 8, 70, 2_200_000, 128, 300
+    g = torch.Generator("cuda").manual_seed(9)
+    k = torch.zeros(B, Lk, Hkv, D, dtype=torch.bfloat16, device="cuda").transpose(1, 2)
+    v = torch.zeros_like(k)
+    q, do, tail_k, tail_v = (heads(B, H, L, D, g) for H, L in ((Hq, Lq), (Hq, Lq), (Hkv, used), (Hkv, used)))
+    k[:, :, -used:], v[:, :, -used:] = tail_k, tail_v
+    start = torch.tensor([Lk - used], dtype=torch.int32, device="cuda")
+    got = both(q, k, v, do, False, start, None)
+    want, tol = exact(q, tail_k, tail_v, do, D ** -0.5, allowed(B, Lq, used, False))
+    for name in ("dk", "dv"):
+        assert not bool(got[name][:, :, :-used].any())
+        got[name] = got[name][:, :, -used:]
+    check(got, want, tol)
+
+
 def test_no_queries_or_no_keys():
     from lookatmyquant_b200 import attention as A
     e = lambda H, L: torch.randn(2, H, L, 64, device="cuda").bfloat16()

@@ -198,3 +198,25 @@ def test_autograd():
     c = torch.randn(3, 50, 24, generator=g).cuda()
     (E.scaled_embedding(t, ids, 4.0, 0) * c).sum().backward()
     check_gradient(t.grad, c.reshape(-1, 24), ids.reshape(-1), 40, 4.0, 0)
+
+
+def test_offsets_past_32_bits():
+    """Rows that lie beyond 2^31 elements (2^32 bytes) of the table, of the gradient and of the tokens' rows."""
+    from lookatmyquant_b200 import embedding as E
+    V, d = 2_200_000, 1024
+    table = torch.zeros(V, d, dtype=torch.bfloat16, device="cuda")
+    rows = torch.tensor([0, V // 2, V - 2, V - 1], device="cuda")
+    g = torch.Generator("cuda").manual_seed(1)
+    table[rows] = torch.randn(4, d, device="cuda", generator=g).bfloat16()
+    ids = rows[torch.randint(0, 4, (3000,), device="cuda", generator=g)]
+    assert torch.equal(E.lookup(table, ids, 2.0), table[ids] * 2)
+    dy = torch.randn(3000, d, device="cuda", generator=g).bfloat16()
+    for n in (1000, 3000):  # both ways to the gradient
+        dE = E.lookup_gradient(dy[:n], ids[:n], V, 0.5)
+        for r in rows:
+            mine = dy[:n][ids[:n] == r].double()
+            tol = (len(mine) + 2) * 2.0**-24 * 0.5 * mine.abs().sum(0) + 2.0**-8 * 0.5 * mine.sum(0).abs() * (1 + 1e-6)
+            assert bool(((dE[r].double() - 0.5 * mine.sum(0)).abs() <= tol).all())
+        dE[rows] = 0
+        assert not bool(dE.any())
+    E.check_status()

@@ -10,7 +10,8 @@
 //
 // forward: a CTA takes two tiles of 128 queries over the keys in tiles of 128; each tile has a warpgroup (a thread per
 // query row), so one tile's softmax runs while the tensor core works for the other. P goes back to TMEM as the A operand
-// of P·V. O is rescaled only when a row's maximum grows by more than 2^8.
+// of P·V. O is rescaled only when a row's maximum grows by more than 2^8. The (key tile, query tile) steps take turns in
+// the S buffers; with head_dim 64 there is a third one, and a warpgroup finds its next S ready when it has stored P.
 // backward: two kernels, so that every sum has one writer and one order (no atomics; equal calls give equal bits):
 //   dq: a CTA per 128 queries walks the keys and sums dS·K in TMEM;
 //   dkv: a CTA per 128 keys walks the queries of every head of its group and sums Pᵀ·dO and dSᵀ·Q in TMEM, so a shared
@@ -68,14 +69,15 @@ struct Sizes {
     static constexpr int NC = HD / 64;                  // 64-wide chunks of a row
     static constexpr int CHUNK = kTile * 128;           // bytes of a chunk of 128 rows
     static constexpr int TILE = NC * CHUNK;             // bytes of a 128 x HD tile
-    static constexpr int FWD_STAGES = HD == 128 ? 4 : 6;
+    static constexpr int FWD_STAGES = HD == 128 ? 4 : 6;  // half of them K's, half V's
+    static constexpr int FWD_S = HD == 128 ? 2 : 3;     // buffers of S in the forward: what TMEM holds beside O
     // backward: stages of the operand that two products read (K for dQ, Q for dK and dV) and of the one that the first
     // product alone reads early (V, dO). The former is released a whole tile later: with two stages for both, its next
     // load came a TMA latency too late and S waited 1100 of 3300 cycles a tile.
     static constexpr int LATE_STAGES = HD == 128 ? 3 : 4, EARLY_STAGES = HD == 128 ? 2 : 4;
     static constexpr int ROW = kTile * 4;               // bytes of lse (or D) of a query tile
     static constexpr size_t FWD_SMEM = 2 * TILE + FWD_STAGES * TILE + 256 + 4 * ROW;
-    static constexpr size_t DQ_SMEM = 2 * TILE + (LATE_STAGES + EARLY_STAGES) * TILE + 256 + 2 * ROW;
+    static constexpr size_t DQ_SMEM = 2 * TILE + (LATE_STAGES + EARLY_STAGES) * TILE + 256 + ROW;
     static constexpr size_t DKV_SMEM = 2 * TILE + (LATE_STAGES + EARLY_STAGES) * (TILE + ROW) + 256;
 };
 
@@ -184,25 +186,48 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar) {
     if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-// A thread's row of an accumulator, times `f`, as bf16 (cols < D; D is a multiple of 8).
+// A warp's 32 rows of an accumulator, each thread's times its `f`, as bf16 to rows dst, dst + stride, ... (`live` of them;
+// columns below D, a multiple of 8), through 4 KB of shared memory of the warp's: in whole lines. A thread that stored
+// its own row, 16 bytes at a time, took 4000 cycles for 64 columns and 8000 to 9000 for 128, a third of the time of 8 key
+// tiles.
 template <int COLS>
-__device__ __forceinline__ void store_row(__nv_bfloat16 *dst, uint32_t taddr, int col0, int D, float f, bool live) {
+__device__ __forceinline__ void store_rows(__nv_bfloat16 *dst, int64_t stride, uint32_t taddr, int col0, int D, float f,
+                                           int live, uint32_t stage) {
+    constexpr int W = COLS < 64 ? COLS : 64, PIECES = W / 8, ROWS = 32 / PIECES;  // columns, 16-byte pieces, rows at once
+    const int lane = threadIdx.x & 31;
+    const auto at = [&](int row, int piece) {
+        return stage + row * (W * 2) + ((piece ^ (W == 64 ? row & 7 : (row >> 1) & 3)) << 4);
+    };
+#pragma unroll 1
+    for (int c = 0; c < COLS; c += W) {
 #pragma unroll
-    for (int c = 0; c < COLS; c += 32) {
-        uint32_t r[32];
-        tmem_load32(taddr + c, r);
-        tmem_ld_wait();
-        if (!live) continue;
+        for (int g = 0; g < W; g += 32) {
+            uint32_t r[32];
+            tmem_load32(taddr + c + g, r);
+            tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-            if (col0 + c + e >= D) break;
-            uint4 v;
-            v.x = pack_bf16(__uint_as_float(r[e]) * f, __uint_as_float(r[e + 1]) * f);
-            v.y = pack_bf16(__uint_as_float(r[e + 2]) * f, __uint_as_float(r[e + 3]) * f);
-            v.z = pack_bf16(__uint_as_float(r[e + 4]) * f, __uint_as_float(r[e + 5]) * f);
-            v.w = pack_bf16(__uint_as_float(r[e + 6]) * f, __uint_as_float(r[e + 7]) * f);
-            *reinterpret_cast<uint4 *>(dst + col0 + c + e) = v;
+            for (int e = 0; e < 32; e += 8) {
+                float x[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(r[e + k]);
+                const uint4 v = pack8(x, f);
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at(lane, (g + e) / 8)), "r"(v.x), "r"(v.y),
+                             "r"(v.z), "r"(v.w)
+                             : "memory");
+            }
         }
+        __syncwarp();
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += ROWS) {
+            const int row = r0 + lane / PIECES, piece = lane % PIECES, col = col0 + c + 8 * piece;
+            uint4 v;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                         : "r"(at(row, piece))
+                         : "memory");
+            if (row < live && col < D) *reinterpret_cast<uint4 *>(dst + row * stride + col) = v;
+        }
+        __syncwarp();
     }
 }
 
@@ -211,6 +236,29 @@ __device__ __forceinline__ void zero_row(__nv_bfloat16 *dst, int D) {
 }
 
 // ------------------------------------------------------------------------------------------------------------ forward
+
+// The order of the forward's steps (key tile j, query tile t) where the two query tiles meet n0 and n1 key tiles: by key
+// tiles, and by query tiles where both meet one.
+struct Steps {
+    int n0, n1;
+    __device__ __forceinline__ int both() const { return min(n0, n1); }
+    __device__ __forceinline__ int count() const { return n0 + n1; }
+    __device__ __forceinline__ int index(int j, int t) const { return min(2 * j + t, both() + j); }
+    __device__ __forceinline__ int query_tile(int u) const { return u < 2 * both() ? u & 1 : (int)(n1 > n0); }
+    __device__ __forceinline__ bool begins(int u) const { return u >= 2 * both() || !(u & 1); }  // a key tile's first step
+    __device__ __forceinline__ bool ends(int u) const { return u >= 2 * both() || (u & 1); }
+};
+
+// A stage of a ring and the parity of its barrier: counted up, since a remainder costs the issuing thread time in which
+// the tensor core idles.
+struct Turn {
+    int at = 0;
+    uint32_t parity = 0;
+    template <int N>
+    __device__ __forceinline__ void next() {
+        if (++at == N) at = 0, parity ^= 1;
+    }
+};
 
 // A float of another CTA's shared memory.
 __device__ __forceinline__ float load_cluster(uint32_t addr) {
@@ -232,17 +280,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     attention_forward_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
                              const __grid_constant__ CUtensorMap mapV, Shape s, Rows out, float *__restrict__ lse, int split) {
     using Z = Sizes<HD>;
-    constexpr int STAGES = Z::FWD_STAGES;
+    constexpr int STAGES = Z::FWD_STAGES, RING = STAGES / 2, NB = Z::FWD_S;
     extern __shared__ __align__(1024) uint8_t smem[];  // swizzled tiles start at multiples of 1024 bytes
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + STAGES) * Z::TILE);
-    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 8);
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 2 * NB + 2);
     float *const parts = reinterpret_cast<float *>(smem + 2 * Z::TILE);
     float *const row_max = reinterpret_cast<float *>(smem + Z::FWD_SMEM - 4 * Z::ROW), *const row_sum = row_max + 2 * kTile;
     static_assert(2 * HD * kTile * 4 <= STAGES * Z::TILE, "the parts of O fit into the stages");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES), q_full = smem_u32(bars + 2 * STAGES);
-    const uint32_t s_full0 = q_full + 8, p_ready0 = q_full + 24, pv_done0 = q_full + 40, drain = q_full + 56;
-    const uint32_t sq = smem_u32(smem), skv = sq + 2 * Z::TILE;
+    const uint32_t k_full0 = smem_u32(bars), v_full0 = k_full0 + 8 * RING, k_empty0 = v_full0 + 8 * RING,
+                   v_empty0 = k_empty0 + 8 * RING, q_full = v_empty0 + 8 * RING;
+    // a buffer's s_full completes for step u when S(u) is there, and once more when P·V of the step has read it
+    const uint32_t s_full0 = q_full + 8, p_ready0 = s_full0 + 8 * NB, drain = p_ready0 + 8 * NB;
+    const uint32_t sq = smem_u32(smem), sk = sq + 2 * Z::TILE, sv = sk + RING * Z::TILE;
 
     const int pairs = s.lq_pad / kTile / 2 + (s.lq_pad / kTile & 1), heads = s.Hq * s.B;
     // `split` CTAs (a cluster) share a pair of query tiles where there would be too few: each takes a part of the keys
@@ -254,13 +304,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int all0 = key_tiles(s, (2 * qp) * kTile, lo, hi), all1 = key_tiles(s, (2 * qp + 1) * kTile, lo, hi);
     const int n_all = max(all0, all1), first = n_all * rank / split, n = n_all * (rank + 1) / split - first;
     const int n0 = min(n, max(0, all0 - first)), n1 = min(n, max(0, all1 - first)), j0 = lo / kTile + first;
+    const Steps steps{n0, n1};
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2 * STAGES + 1; ++i) mbar_init(full0 + 8 * i, 1);
-        for (int t = 0; t < 2; ++t) {
-            mbar_init(s_full0 + 8 * t, 1);
-            mbar_init(p_ready0 + 8 * t, 4);
-            mbar_init(pv_done0 + 8 * t, 1);
+        for (int i = 0; i < 2 * STAGES + 1; ++i) mbar_init(k_full0 + 8 * i, 1);
+        for (int i = 0; i < NB; ++i) {
+            mbar_init(s_full0 + 8 * i, 1);
+            mbar_init(p_ready0 + 8 * i, 4);
         }
         mbar_init(drain, 1);
         fence_mbar_init();
@@ -278,59 +328,65 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = *tmem_holder;
 
     if (warp == 0) {
-        if (lane == 0 && n > 0) {  // ---- TMA producer: Q once, then K, V, K, V, ... through the ring
+        if (lane == 0 && n > 0) {  // ---- TMA producer: Q once, then K and V through the ring
             mbar_expect_tx(q_full, 2 * Z::TILE);
             load_tile<HD>(sq, &mapQ, 2 * qp * kTile, h, b, q_full);
             load_tile<HD>(sq + Z::TILE, &mapQ, (2 * qp + 1) * kTile, h, b, q_full);
-            int issued = 0;
+            int k_issued = 0, v_issued = 0;
             bool ok = true;
-            for (; issued < 2 * n; ++issued) {
-                const int st = issued % STAGES;
-                ok = mbar_wait(empty0 + 8 * st, ((issued / STAGES) & 1) ^ 1, s.status);
+            for (int i = 0; i < 2 * n; ++i) {  // K0 K1 V0 K2 V1 ...: as the products want them
+                const bool is_k = k_issued < n && k_issued <= v_issued + 1 && (i == 0 || (i & 1));
+                int &issued = is_k ? k_issued : v_issued;
+                const int st = issued % RING;
+                const uint32_t full = (is_k ? k_full0 : v_full0) + 8 * st;
+                ok = mbar_wait((is_k ? k_empty0 : v_empty0) + 8 * st, ((issued / RING) & 1) ^ 1, s.status);
                 if (!ok) break;
-                mbar_expect_tx(full0 + 8 * st, Z::TILE);
-                load_tile<HD>(skv + st * Z::TILE, (issued & 1) ? &mapV : &mapK, (j0 + issued / 2) * kTile, hk, b,
-                              full0 + 8 * st);
+                mbar_expect_tx(full, Z::TILE);
+                load_tile<HD>((is_k ? sk : sv) + st * Z::TILE, is_k ? &mapK : &mapV, (j0 + issued) * kTile, hk, b, full);
+                ++issued;
             }
             if (!ok) {  // error path: let the copies in flight land before the CTA exits
                 wait_bounded(q_full, 0);
-                for (int i = max(0, issued - STAGES); i < issued; ++i)
-                    wait_bounded(full0 + 8 * (i % STAGES), (i / STAGES) & 1);
+                for (int i = max(0, k_issued - RING); i < k_issued; ++i) wait_bounded(k_full0 + 8 * (i % RING), (i / RING) & 1);
+                for (int i = max(0, v_issued - RING); i < v_issued; ++i) wait_bounded(v_full0 + 8 * (i % RING), (i / RING) & 1);
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && n > 0) {  // ---- MMA issuer. P lies over S: P·V of key tile j goes before S of tile j + 1
-            const uint64_t q_desc = rows_desc(sq), kv_desc = rows_desc(skv), v_desc = cols_desc<HD>(skv);
-            bool ok = mbar_wait(q_full, 0, s.status) && mbar_wait(full0, 0, s.status);
-            if (ok) {
-                for (int t = 0; t < 2; ++t)
-                    if ((t ? n1 : n0) > 0) {
-                        mma_rows_rows<HD>(tmem + t * kTile, q_desc + t * (Z::TILE >> 4), kv_desc);
-                        mma_commit(s_full0 + 8 * t);
-                    }
-                mma_commit(empty0);
-            }
-            for (int j = 0; ok && j < n; ++j) {
-                const int iv = 2 * j + 1, sv = iv % STAGES, ik = iv + 1, sk = ik % STAGES;
-                ok = mbar_wait(full0 + 8 * sv, (iv / STAGES) & 1, s.status) &&
-                     (j + 1 == n || mbar_wait(full0 + 8 * sk, (ik / STAGES) & 1, s.status));
-                for (int t = 0; ok && t < 2; ++t) {
-                    const int nt = t ? n1 : n0;
-                    if (j < nt) {
-                        ok = mbar_wait(p_ready0 + 8 * t, j & 1, s.status);
-                        if (!ok) break;
-                        tc_fence_after();
-                        mma_tmem_rows<HD>(tmem + 2 * kTile + t * HD, tmem + t * kTile, 32, v_desc + sv * (Z::TILE >> 4), j > 0);
-                        mma_commit(pv_done0 + 8 * t);
-                    }
-                    if (j + 1 < nt) {
-                        mma_rows_rows<HD>(tmem + t * kTile, q_desc + t * (Z::TILE >> 4), kv_desc + sk * (Z::TILE >> 4));
-                        mma_commit(s_full0 + 8 * t);
-                    }
+        if (lane == 0 && n > 0) {  // ---- MMA issuer. P lies over S: P·V of a step goes before the buffer's next S
+            const uint64_t q_desc = rows_desc(sq), k_desc = rows_desc(sk), v_desc = cols_desc<HD>(sv);
+            const int count = steps.count();
+            Turn k, v, buf;
+            bool ok = mbar_wait(q_full, 0, s.status);
+            const auto issue_s = [&](int u, int to) {
+                if (steps.begins(u)) ok = mbar_wait(k_full0 + 8 * k.at, k.parity, s.status);
+                if (!ok) return;
+                mma_rows_rows<HD>(tmem + to * kTile, q_desc + steps.query_tile(u) * (Z::TILE >> 4), k_desc + k.at * (Z::TILE >> 4));
+                if (steps.ends(u)) {
+                    mma_commit(k_empty0 + 8 * k.at);
+                    k.next<RING>();
                 }
+            };
+            // few commits: one takes this thread 85 cycles
+            for (int u = 0; ok && u < min(NB, count); ++u) {
+                issue_s(u, u);
+                if (ok) mma_commit(s_full0 + 8 * u);
+            }
+            uint32_t first_of = 3;  // the query tiles (bits) whose O holds nothing yet
+            for (int u = 0; ok && u < count; ++u, buf.next<NB>()) {
+                const int t = steps.query_tile(u);
+                ok = (!steps.begins(u) || mbar_wait(v_full0 + 8 * v.at, v.parity, s.status)) &&
+                     mbar_wait(p_ready0 + 8 * buf.at, buf.parity, s.status);
                 if (!ok) break;
-                mma_commit(empty0 + 8 * sv);
-                if (j + 1 < n) mma_commit(empty0 + 8 * sk);
+                tc_fence_after();
+                mma_tmem_rows<HD>(tmem + NB * kTile + t * HD, tmem + buf.at * kTile, 32, v_desc + v.at * (Z::TILE >> 4),
+                                  !(first_of >> t & 1));
+                first_of &= ~(1u << t);
+                if (steps.ends(u)) {
+                    mma_commit(v_empty0 + 8 * v.at);
+                    v.next<RING>();
+                }
+                if (u + NB < count) issue_s(u + NB, buf.at);
+                if (ok) mma_commit(s_full0 + 8 * buf.at);
             }
             mma_commit(drain);  // every MMA this thread issued completes before TMEM is released
             wait_bounded(drain, 0);
@@ -341,12 +397,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int row0 = (2 * qp + t) * kTile, i = row0 + 32 * quad + lane;
         const bool live = i < s.Lq;
         const int row_hi = s.causal ? min(hi, i + s.off + 1) : hi;
+        const int whole = s.causal ? min(hi, row0 + s.off + 1) : hi;  // a key tile from lo to here needs no mask
         const uint32_t lanes = (uint32_t)(32 * quad) << 16;
-        const uint32_t ts = tmem + lanes + t * kTile, to = tmem + lanes + 2 * kTile + t * HD;
+        const uint32_t to = tmem + lanes + NB * kTile + t * HD;
         float m = -INFINITY, sum = 0.f;  // m: the maximum that the exponentials are taken against
         bool ok = true;
         for (int j = 0; j < nt; ++j) {
-            ok = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * t, j & 1, s.status));
+            const int u = steps.index(j, t), buf = u % NB;
+            const uint32_t ts = tmem + lanes + buf * kTile;
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * buf, (u / NB) & 1, s.status));
             if (!ok) break;
             tc_fence_after();
             uint32_t r[4][32];
@@ -354,16 +413,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 0; c < 4; ++c) tmem_load32(ts + 32 * c, r[c]);
             tmem_ld_wait();
             const int key0 = (j0 + j) * kTile;
-            if (key0 < lo || key0 + kTile > hi || (s.causal && key0 + kTile - 1 > row0 + s.off)) {
+            if (key0 < lo || key0 + kTile > whole) {
                 const int clo = lo - key0, chi = row_hi - key0;
 #pragma unroll
                 for (int c = 0; c < kTile; ++c)
                     if (c < clo || c >= chi) r[c >> 5][c & 31] = 0xff800000u;
                 if (key0 < lo || key0 + kTile > hi) {  // (both tiles' warps do: the same zeros)
-                    const int sv = (2 * j + 1) % STAGES;
-                    ok = __all_sync(0xffffffffu, mbar_wait(full0 + 8 * sv, ((2 * j + 1) / STAGES) & 1, s.status));
+                    ok = __all_sync(0xffffffffu, mbar_wait(v_full0 + 8 * (j % RING), (j / RING) & 1, s.status));
                     if (!ok) break;
-                    zero_rows<HD>(skv + sv * Z::TILE, lo - key0, hi - key0, threadIdx.x - 64 - 128 * t, 128);
+                    zero_rows<HD>(sv + (j % RING) * Z::TILE, lo - key0, hi - key0, threadIdx.x - 64 - 128 * t, 128);
                 }
             }
             float top[8];  // eight chains: one of 128 comparisons would take 500 cycles of latency
@@ -381,7 +439,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (grow) m = mx;
                 sum *= f;
                 if (j > 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * t, (j - 1) & 1, s.status));
+                    const int before = steps.index(j - 1, t);
+                    ok = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * (before % NB), (before / NB + 1) & 1, s.status));
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
@@ -411,10 +470,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             sum += (part[0] + part[1]) + (part[2] + part[3]);
             tmem_st_wait();
-            warp_arrive(p_ready0 + 8 * t);
+            warp_arrive(p_ready0 + 8 * buf);
         }
         if (ok && nt > 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * t, (nt - 1) & 1, s.status));
+            const int last = steps.index(nt - 1, t);
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * (last % NB), (last / NB + 1) & 1, s.status));
             tc_fence_after();
         }
         if (split > 1 && n > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(drain, 0, s.status));  // the other tile's too
@@ -431,9 +491,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int x = 0; x < 32; ++x) mine[(c + x) * kTile] = __uint_as_float(r[x]);
             }
         } else if (ok && rank == 0) {
-            __nv_bfloat16 *dst = out.p + b * out.batch + h * out.head + (int64_t)i * out.row;
-            if (nt > 0) store_row<HD>(dst, to, 0, s.D, sum > 0.f || sum != sum ? 1.f / sum : 0.f, live);
-            else if (live) zero_row(dst, s.D);
+            __nv_bfloat16 *const dst = out.p + b * out.batch + h * out.head + (int64_t)(i - lane) * out.row;
+            if (nt > 0) {
+                store_rows<HD>(dst, out.row, to, 0, s.D, sum > 0.f || sum != sum ? 1.f / sum : 0.f, s.Lq - (i - lane),
+                               sq + t * Z::TILE + quad * 4096);  // staged over the tile's Q: its products are done
+            } else if (live) zero_row(dst + lane * out.row, s.D);
             if (live)
                 lse[((int64_t)b * s.Hq + h) * s.Lq + i] =
                     sum == 0.f ? -INFINITY : ((m == -INFINITY ? 0.f : m * s.sl) + log2f(sum)) * kLn2;
@@ -508,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                    v_empty0 = k_empty0 + 8 * KS, q_full = v_empty0 + 8 * VS;
     const uint32_t q_ready = q_full + 8, s_full = q_full + 16, s_free = q_full + 24, p_full = q_full + 32;
     const uint32_t ds_ready = q_full + 40, done = q_full + 48;
-    float *half_d = reinterpret_cast<float *>(smem + Z::DQ_SMEM - 2 * Z::ROW);  // each half's sum of dO·O
+    float *row_D = reinterpret_cast<float *>(smem + Z::DQ_SMEM - Z::ROW);
     const uint32_t sq = smem_u32(smem), sg = sq + Z::TILE, sk = sg + Z::TILE, sv = sk + KS * Z::TILE;
 
     const int tiles = s.lq_pad / kTile, heads = s.Hq * s.B;
@@ -611,38 +673,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool live = i < s.Lq;
         const int row_hi = s.causal ? min(hi, i + s.off + 1) : hi;
         const uint32_t lanes = (uint32_t)(32 * quad) << 16;
-        // lse in units of log 2 (+inf where there is no row or it is empty: P = 0) and D = Σ dO·O, half of the row each;
-        // kept by padded rows for the dkv kernel
+        // lse in units of log 2 (+inf where there is no row or it is empty: P = 0), with D kept by padded rows for the dkv
+        // kernel
         const float l = live ? lse[(int64_t)bh * s.Lq + i] : -INFINITY, l2 = l == -INFINITY ? INFINITY : l * kLog2e;
-        const bool some = l != -INFINITY;
-        uint4 orow[HD / 16];
+        // D = Σ dO·O of 16 rows a warp, a row's 16-byte pieces in neighbouring lanes (a thread that read its own row of O
+        // took 4000 cycles)
+        constexpr int PIECES = HD / 8, ROWS = 32 / PIECES;
+        const int d_row = 16 * (warp - 2) + lane / PIECES, piece = lane % PIECES;
+        uint4 orow[16 / ROWS];
+        uint32_t some = 0;  // the rows (bits) that have a key: the others' O and dO may hold anything
 #pragma unroll
-        for (int c = 0; c < HD / 16; ++c) {
-            const int col = half * (HD / 2) + 8 * c;
-            orow[c] = some && col < s.D ? *reinterpret_cast<const uint4 *>(o.p + b * o.batch + h * o.head + (int64_t)i * o.row + col)
-                                        : make_uint4(0, 0, 0, 0);
+        for (int x = 0; x < 16 / ROWS; ++x) {
+            const int at = row0 + d_row + ROWS * x;
+            if (n > 0 && at < s.Lq && lse[(int64_t)bh * s.Lq + at] != -INFINITY) some |= 1u << x;
+            orow[x] = (some >> x & 1) && 8 * piece < s.D
+                          ? *reinterpret_cast<const uint4 *>(o.p + b * o.batch + h * o.head + (int64_t)at * o.row + 8 * piece)
+                          : make_uint4(0, 0, 0, 0);
         }
         bool ok = n > 0 && __all_sync(0xffffffffu, mbar_wait(q_full, 0, s.status));
-        float Di = 0.f;
-        if (ok && some) {
-            const int row = 32 * quad + lane;
-#pragma unroll
-            for (int c = 0; c < HD / 16; ++c) {
-                const int piece = (HD == 64 ? 4 * half : 0) + c;
-                uint4 g;
-                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(g.x), "=r"(g.y), "=r"(g.z), "=r"(g.w)
-                             : "r"(sg + (HD == 64 ? 0 : half * Z::CHUNK) + row * 128 + ((piece ^ (row & 7)) << 4)));
-                Di = dot8(orow[c], g, Di);
-            }
-        }
-        half_d[half * kTile + 32 * quad + lane] = Di;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        Di = half_d[32 * quad + lane] + half_d[kTile + 32 * quad + lane];
-        if (half == 0 && rank == split - 1) {  // (the last part is never without keys where there are any)
-            lse2[(int64_t)bh * s.lq_pad + i] = l2;
-            Dr[(int64_t)bh * s.lq_pad + i] = Di;
-        }
         if (ok) {
             if (HD == 64) {
                 chunk_to_tmem(half ? sg : sq, 32 * quad + lane, tmem + lanes + (half ? kG : kQ));
@@ -652,6 +700,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tmem_st_wait();
             warp_arrive(q_ready);
+        }
+#pragma unroll
+        for (int x = 0; x < 16 / ROWS; ++x) {
+            const int row = d_row + ROWS * x;
+            uint4 g = make_uint4(0, 0, 0, 0);
+            if (ok)
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(g.x), "=r"(g.y), "=r"(g.z), "=r"(g.w)
+                             : "r"(sg + (piece >> 3) * Z::CHUNK + row * 128 + (((piece & 7) ^ (row & 7)) << 4)));
+            float d = some >> x & 1 ? dot8(orow[x], g, 0.f) : 0.f;
+#pragma unroll
+            for (int m = 1; m < PIECES; m *= 2) d += __shfl_xor_sync(0xffffffffu, d, m);
+            if (piece == 0) row_D[row] = d;
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const float Di = row_D[32 * quad + lane];
+        if (half == 0 && rank == split - 1) {  // (the last part is never without keys where there are any)
+            lse2[(int64_t)bh * s.lq_pad + i] = l2;
+            Dr[(int64_t)bh * s.lq_pad + i] = Di;
         }
         for (int j = 0; ok && j < n; ++j) {
             ok = __all_sync(0xffffffffu, mbar_wait(s_full, j & 1, s.status));
@@ -709,9 +776,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int x = 0; x < 32; ++x) mine[(c + x) * kTile] = n > 0 ? __uint_as_float(r[x]) : 0.f;
             }
         } else if ((ok || n == 0) && rank == 0) {
-            __nv_bfloat16 *dst = dq.p + b * dq.batch + h * dq.head + (int64_t)i * dq.row;
-            if (n > 0) store_row<HD / 2>(dst, tmem + lanes + kDQ + half * (HD / 2), half * (HD / 2), s.D, s.scale, live);
-            else if (live && half == 0) zero_row(dst, s.D);
+            __nv_bfloat16 *const dst = dq.p + b * dq.batch + h * dq.head + (int64_t)(i - lane) * dq.row;
+            if (n > 0)  // (staged over Q and dO, which every warp has read)
+                store_rows<HD / 2>(dst, dq.row, tmem + lanes + kDQ + half * (HD / 2), half * (HD / 2), s.D, s.scale,
+                                   s.Lq - (i - lane), sq + (warp - 2) * 4096);
+            else if (live && half == 0) zero_row(dst + lane * dq.row, s.D);
         }
     }
     if (split > 1 && n_all > 0) {  // the parts added in the order of the keys, a share of the columns each
@@ -954,8 +1023,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (ok) {  // columns half·HD/2 .. of the thread's key
             const int c0 = half * (HD / 2);
-            __nv_bfloat16 *pk_ = dk.p + b * dk.batch + hk * dk.head + (int64_t)key * dk.row;
-            __nv_bfloat16 *pv_ = dv.p + b * dv.batch + hk * dv.head + (int64_t)key * dv.row;
+            __nv_bfloat16 *const pk_ = dk.p + b * dk.batch + hk * dk.head + (int64_t)(key - lane) * dk.row;
+            __nv_bfloat16 *const pv_ = dv.p + b * dv.batch + hk * dv.head + (int64_t)(key - lane) * dv.row;
             if (split > 1 && n > 0) {  // to the cluster: columns of 128 rows over the stages, which are done with
                 float *const mine = parts + c0 * kTile + 32 * quad + lane;
 #pragma unroll 1
@@ -969,10 +1038,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int x = 0; x < 32; ++x) mine[(m * HD + c + x) * kTile] = __uint_as_float(r[x]);
                     }
             } else if (n > 0) {
-                store_row<HD / 2>(pk_, tmem + lanes + kDK + c0, c0, s.D, s.scale, live);
-                store_row<HD / 2>(pv_, tmem + lanes + kDV + c0, c0, s.D, 1.f, live);
+                const int rows = s.Lk - (key - lane);
+                const uint32_t stage = sk + (warp - 2) * 4096;  // over K and V, which the products are done with
+                store_rows<HD / 2>(pk_, dk.row, tmem + lanes + kDK + c0, c0, s.D, s.scale, rows, stage);
+                store_rows<HD / 2>(pv_, dv.row, tmem + lanes + kDV + c0, c0, s.D, 1.f, rows, stage);
             } else if (live && rank == 0) {
-                zero_row(half ? pv_ : pk_, s.D);
+                zero_row(half ? pv_ + lane * dv.row : pk_ + lane * dk.row, s.D);
             }
         }
     }

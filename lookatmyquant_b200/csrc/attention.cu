@@ -306,6 +306,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int n0 = min(n, max(0, all0 - first)), n1 = min(n, max(0, all1 - first)), j0 = lo / kTile + first;
     const Steps steps{n0, n1};
 
+    // The loads, by the first thread: Q, then K and V through the rings in the order K0 K1 V0 K2 V1 ..., as the products
+    // want them. What finds free stages is issued before the other warps have met.
+    int k_issued = 0, v_issued = 0;
+    const auto load_next = [&](bool wait) {
+        const bool is_k = k_issued < n && k_issued <= v_issued + 1;
+        int &issued = is_k ? k_issued : v_issued;
+        const int st = issued % RING;
+        const uint32_t full = (is_k ? k_full0 : v_full0) + 8 * st;
+        if (wait && !mbar_wait((is_k ? k_empty0 : v_empty0) + 8 * st, ((issued / RING) & 1) ^ 1, s.status)) return false;
+        mbar_expect_tx(full, Z::TILE);
+        load_tile<HD>((is_k ? sk : sv) + st * Z::TILE, is_k ? &mapK : &mapV, (j0 + issued) * kTile, hk, b, full);
+        ++issued;
+        return true;
+    };
+    constexpr int EARLY = 2 * RING - 1;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2 * STAGES + 1; ++i) mbar_init(k_full0 + 8 * i, 1);
         for (int i = 0; i < NB; ++i) {
@@ -314,9 +329,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mbar_init(drain, 1);
         fence_mbar_init();
-        prefetch_tmap(&mapQ);
-        prefetch_tmap(&mapK);
-        prefetch_tmap(&mapV);
+        if (n > 0) {
+            mbar_expect_tx(q_full, 2 * Z::TILE);
+            load_tile<HD>(sq, &mapQ, 2 * qp * kTile, h, b, q_full);
+            load_tile<HD>(sq + Z::TILE, &mapQ, (2 * qp + 1) * kTile, h, b, q_full);
+            for (int i = 0; i < min(2 * n, EARLY); ++i) load_next(false);
+        }
     }
     if (warp == 1) {
         tmem_alloc(smem_u32(tmem_holder), kTmemCols);
@@ -328,23 +346,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = *tmem_holder;
 
     if (warp == 0) {
-        if (lane == 0 && n > 0) {  // ---- TMA producer: Q once, then K and V through the ring
-            mbar_expect_tx(q_full, 2 * Z::TILE);
-            load_tile<HD>(sq, &mapQ, 2 * qp * kTile, h, b, q_full);
-            load_tile<HD>(sq + Z::TILE, &mapQ, (2 * qp + 1) * kTile, h, b, q_full);
-            int k_issued = 0, v_issued = 0;
+        if (lane == 0 && n > 0) {  // ---- TMA producer
             bool ok = true;
-            for (int i = 0; i < 2 * n; ++i) {  // K0 K1 V0 K2 V1 ...: as the products want them
-                const bool is_k = k_issued < n && k_issued <= v_issued + 1 && (i == 0 || (i & 1));
-                int &issued = is_k ? k_issued : v_issued;
-                const int st = issued % RING;
-                const uint32_t full = (is_k ? k_full0 : v_full0) + 8 * st;
-                ok = mbar_wait((is_k ? k_empty0 : v_empty0) + 8 * st, ((issued / RING) & 1) ^ 1, s.status);
-                if (!ok) break;
-                mbar_expect_tx(full, Z::TILE);
-                load_tile<HD>((is_k ? sk : sv) + st * Z::TILE, is_k ? &mapK : &mapV, (j0 + issued) * kTile, hk, b, full);
-                ++issued;
-            }
+            for (int i = EARLY; ok && i < 2 * n; ++i) ok = load_next(true);
             if (!ok) {  // error path: let the copies in flight land before the CTA exits
                 wait_bounded(q_full, 0);
                 for (int i = max(0, k_issued - RING); i < k_issued; ++i) wait_bounded(k_full0 + 8 * (i % RING), (i / RING) & 1);
@@ -583,6 +587,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int n_all = key_tiles(s, row0, lo, hi), first = n_all * rank / split, n = n_all * (rank + 1) / split - first;
     const int j0 = lo / kTile + first;
 
+    // The loads, by the first thread: Q and dO, then K and V through the rings; V's stage is released by an earlier product
+    // than K's of the same key tile. What finds free stages is issued before the other warps have met.
+    int k_issued = 0, v_issued = 0;
+    const auto load = [&](int j, bool wait) {
+        const int ks = j % KS, vs = j % VS, row = (j0 + j) * kTile;
+        if (wait && !mbar_wait(k_empty0 + 8 * ks, ((j / KS) & 1) ^ 1, s.status)) return false;
+        mbar_expect_tx(k_full0 + 8 * ks, Z::TILE);
+        load_tile<HD>(sk + ks * Z::TILE, &mapK, row, hk, b, k_full0 + 8 * ks);
+        ++k_issued;
+        if (wait && !mbar_wait(v_empty0 + 8 * vs, ((j / VS) & 1) ^ 1, s.status)) return false;
+        mbar_expect_tx(v_full0 + 8 * vs, Z::TILE);
+        load_tile<HD>(sv + vs * Z::TILE, &mapV, row, hk, b, v_full0 + 8 * vs);
+        ++v_issued;
+        return true;
+    };
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2 * (KS + VS) + 1; ++i) mbar_init(k_full0 + 8 * i, 1);
         mbar_init(q_ready, 8);
@@ -592,10 +611,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(ds_ready, 8);
         mbar_init(done, 1);
         fence_mbar_init();
-        prefetch_tmap(&mapQ);
-        prefetch_tmap(&mapK);
-        prefetch_tmap(&mapV);
-        prefetch_tmap(&mapG);
+        if (n > 0) {
+            mbar_expect_tx(q_full, 2 * Z::TILE);
+            load_tile<HD>(sq, &mapQ, row0, h, b, q_full);
+            load_tile<HD>(sg, &mapG, row0, h, b, q_full);
+            for (int j = 0; j < min(n, VS); ++j) load(j, false);
+        }
     }
     if (warp == 1) {
         tmem_alloc(smem_u32(tmem_holder), kTmemCols);
@@ -608,24 +629,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 0) {
         if (lane == 0 && n > 0) {
-            mbar_expect_tx(q_full, 2 * Z::TILE);
-            load_tile<HD>(sq, &mapQ, row0, h, b, q_full);
-            load_tile<HD>(sg, &mapG, row0, h, b, q_full);
-            int k_issued = 0, v_issued = 0;
             bool ok = true;
-            for (int j = 0; j < n; ++j) {  // V's stage is released by an earlier product than K's of the same key tile
-                const int ks = j % KS, vs = j % VS, row = (j0 + j) * kTile;
-                ok = mbar_wait(k_empty0 + 8 * ks, ((j / KS) & 1) ^ 1, s.status);
-                if (!ok) break;
-                mbar_expect_tx(k_full0 + 8 * ks, Z::TILE);
-                load_tile<HD>(sk + ks * Z::TILE, &mapK, row, hk, b, k_full0 + 8 * ks);
-                ++k_issued;
-                ok = mbar_wait(v_empty0 + 8 * vs, ((j / VS) & 1) ^ 1, s.status);
-                if (!ok) break;
-                mbar_expect_tx(v_full0 + 8 * vs, Z::TILE);
-                load_tile<HD>(sv + vs * Z::TILE, &mapV, row, hk, b, v_full0 + 8 * vs);
-                ++v_issued;
-            }
+            for (int j = VS; ok && j < n; ++j) ok = load(j, true);
             if (!ok) {
                 wait_bounded(q_full, 0);
                 for (int i = max(0, k_issued - KS); i < k_issued; ++i) wait_bounded(k_full0 + 8 * (i % KS), (i / KS) & 1);
@@ -681,14 +686,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr int PIECES = HD / 8, ROWS = 32 / PIECES;
         const int d_row = 16 * (warp - 2) + lane / PIECES, piece = lane % PIECES;
         uint4 orow[16 / ROWS];
-        uint32_t some = 0;  // the rows (bits) that have a key: the others' O and dO may hold anything
+        float row_lse[16 / ROWS];
 #pragma unroll
-        for (int x = 0; x < 16 / ROWS; ++x) {
-            const int at = row0 + d_row + ROWS * x;
-            if (n > 0 && at < s.Lq && lse[(int64_t)bh * s.Lq + at] != -INFINITY) some |= 1u << x;
-            orow[x] = (some >> x & 1) && 8 * piece < s.D
-                          ? *reinterpret_cast<const uint4 *>(o.p + b * o.batch + h * o.head + (int64_t)at * o.row + 8 * piece)
-                          : make_uint4(0, 0, 0, 0);
+        for (int x = 0; x < 16 / ROWS; ++x) {  // (every load at once: rows past the end are the last one)
+            const int at = min(row0 + d_row + ROWS * x, s.Lq - 1);
+            row_lse[x] = lse[(int64_t)bh * s.Lq + at];
+            orow[x] = *reinterpret_cast<const uint4 *>(o.p + b * o.batch + h * o.head + (int64_t)at * o.row +
+                                                       (8 * piece < s.D ? 8 * piece : 0));
         }
         bool ok = n > 0 && __all_sync(0xffffffffu, mbar_wait(q_full, 0, s.status));
         if (ok) {
@@ -709,7 +713,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                              : "=r"(g.x), "=r"(g.y), "=r"(g.z), "=r"(g.w)
                              : "r"(sg + (piece >> 3) * Z::CHUNK + row * 128 + (((piece & 7) ^ (row & 7)) << 4)));
-            float d = some >> x & 1 ? dot8(orow[x], g, 0.f) : 0.f;
+            // dO is zero beyond its columns and rows; O and dO of a row without a key may hold anything
+            float d = row_lse[x] != -INFINITY && 8 * piece < s.D ? dot8(orow[x], g, 0.f) : 0.f;
 #pragma unroll
             for (int m = 1; m < PIECES; m *= 2) d += __shfl_xor_sync(0xffffffffu, d, m);
             if (piece == 0) row_D[row] = d;
@@ -844,6 +849,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int nq = key0 >= hi || key0 + kTile <= lo || first >= s.Lq ? 0 : tiles - t0;
     const int n = nq * (s.group / split);
 
+    // The loads, by the first thread: K and V, then Q and dO (with the rows' lse and D) through the rings; dO's stage is
+    // released by an earlier product than Q's of the same query tile. What finds free stages is issued before the other
+    // warps have met.
+    int q_issued = 0, g_issued = 0;
+    const auto load = [&](int j, bool wait) {
+        const int qs = j % QS, gs = j % GS, h = h0 + j / nq, row = (t0 + j % nq) * kTile;
+        const int64_t at = ((int64_t)b * s.Hq + h) * s.lq_pad + row;
+        if (wait && !mbar_wait(q_empty0 + 8 * qs, ((j / QS) & 1) ^ 1, s.status)) return false;
+        mbar_expect_tx(q_full0 + 8 * qs, Z::TILE + Z::ROW);
+        load_tile<HD>(sq + qs * Z::TILE, &mapQ, row, h, b, q_full0 + 8 * qs);
+        bulk_load(smem_u32(row_lse + qs * kTile), lse2 + at, Z::ROW, q_full0 + 8 * qs);
+        ++q_issued;
+        if (wait && !mbar_wait(g_empty0 + 8 * gs, ((j / GS) & 1) ^ 1, s.status)) return false;
+        mbar_expect_tx(g_full0 + 8 * gs, Z::TILE + Z::ROW);
+        load_tile<HD>(sg + gs * Z::TILE, &mapG, row, h, b, g_full0 + 8 * gs);
+        bulk_load(smem_u32(row_d + gs * kTile), Dr + at, Z::ROW, g_full0 + 8 * gs);
+        ++g_issued;
+        return true;
+    };
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2 * (QS + GS) + 1; ++i) mbar_init(q_full0 + 8 * i, 1);
         mbar_init(s_full, 1);
@@ -852,10 +876,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(ds_ready, 8);
         mbar_init(done, 1);
         fence_mbar_init();
-        prefetch_tmap(&mapQ);
-        prefetch_tmap(&mapK);
-        prefetch_tmap(&mapV);
-        prefetch_tmap(&mapG);
+        if (n > 0) {
+            mbar_expect_tx(kv_full, 2 * Z::TILE);
+            load_tile<HD>(sk, &mapK, key0, hk, b, kv_full);
+            load_tile<HD>(sv, &mapV, key0, hk, b, kv_full);
+            for (int j = 0; j < min(n, GS); ++j) load(j, false);
+        }
     }
     if (warp == 1) {
         tmem_alloc(smem_u32(tmem_holder), kTmemCols);
@@ -868,27 +894,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 0) {
         if (lane == 0 && n > 0) {
-            mbar_expect_tx(kv_full, 2 * Z::TILE);
-            load_tile<HD>(sk, &mapK, key0, hk, b, kv_full);
-            load_tile<HD>(sv, &mapV, key0, hk, b, kv_full);
-            int q_issued = 0, g_issued = 0;
             bool ok = true;
-            for (int j = 0; j < n; ++j) {  // dO's stage is released by an earlier product than Q's of the same query tile
-                const int qs = j % QS, gs = j % GS, h = h0 + j / nq, row = (t0 + j % nq) * kTile;
-                const int64_t at = ((int64_t)b * s.Hq + h) * s.lq_pad + row;
-                ok = mbar_wait(q_empty0 + 8 * qs, ((j / QS) & 1) ^ 1, s.status);
-                if (!ok) break;
-                mbar_expect_tx(q_full0 + 8 * qs, Z::TILE + Z::ROW);
-                load_tile<HD>(sq + qs * Z::TILE, &mapQ, row, h, b, q_full0 + 8 * qs);
-                bulk_load(smem_u32(row_lse + qs * kTile), lse2 + at, Z::ROW, q_full0 + 8 * qs);
-                ++q_issued;
-                ok = mbar_wait(g_empty0 + 8 * gs, ((j / GS) & 1) ^ 1, s.status);
-                if (!ok) break;
-                mbar_expect_tx(g_full0 + 8 * gs, Z::TILE + Z::ROW);
-                load_tile<HD>(sg + gs * Z::TILE, &mapG, row, h, b, g_full0 + 8 * gs);
-                bulk_load(smem_u32(row_d + gs * kTile), Dr + at, Z::ROW, g_full0 + 8 * gs);
-                ++g_issued;
-            }
+            for (int j = GS; ok && j < n; ++j) ok = load(j, true);
             if (!ok) {
                 wait_bounded(kv_full, 0);
                 for (int i = max(0, q_issued - QS); i < q_issued; ++i) wait_bounded(q_full0 + 8 * (i % QS), (i / QS) & 1);

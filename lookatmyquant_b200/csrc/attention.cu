@@ -587,6 +587,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int n_all = key_tiles(s, row0, lo, hi), first = n_all * rank / split, n = n_all * (rank + 1) / split - first;
     const int j0 = lo / kTile + first;
 
+    // Every elementwise thread's lse, and O for D = Σ dO·O: 16 rows a warp, a row's 16-byte pieces in neighbouring lanes (a
+    // thread that read its own row took 4000 cycles). All at once and before anything waits; rows past the end are the last.
+    constexpr int PIECES = HD / 8, ROWS = 32 / PIECES;
+    const int d_row = 16 * (warp - 2) + lane / PIECES, piece = lane % PIECES;
+    uint4 orow[16 / ROWS];
+    float o_lse[16 / ROWS], own_lse = 0.f;
+    if (warp >= 2) {
+        own_lse = lse[(int64_t)bh * s.Lq + min(row0 + 32 * (warp & 3) + lane, s.Lq - 1)];
+#pragma unroll
+        for (int x = 0; x < 16 / ROWS; ++x) {
+            const int at = min(row0 + d_row + ROWS * x, s.Lq - 1);
+            o_lse[x] = lse[(int64_t)bh * s.Lq + at];
+            orow[x] = *reinterpret_cast<const uint4 *>(o.p + b * o.batch + h * o.head + (int64_t)at * o.row +
+                                                       (8 * piece < s.D ? 8 * piece : 0));
+        }
+    }
     // The loads, by the first thread: Q and dO, then K and V through the rings; V's stage is released by an earlier product
     // than K's of the same key tile. What finds free stages is issued before the other warps have met.
     int k_issued = 0, v_issued = 0;
@@ -678,22 +694,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool live = i < s.Lq;
         const int row_hi = s.causal ? min(hi, i + s.off + 1) : hi;
         const uint32_t lanes = (uint32_t)(32 * quad) << 16;
-        // lse in units of log 2 (+inf where there is no row or it is empty: P = 0), with D kept by padded rows for the dkv
-        // kernel
-        const float l = live ? lse[(int64_t)bh * s.Lq + i] : -INFINITY, l2 = l == -INFINITY ? INFINITY : l * kLog2e;
-        // D = Σ dO·O of 16 rows a warp, a row's 16-byte pieces in neighbouring lanes (a thread that read its own row of O
-        // took 4000 cycles)
-        constexpr int PIECES = HD / 8, ROWS = 32 / PIECES;
-        const int d_row = 16 * (warp - 2) + lane / PIECES, piece = lane % PIECES;
-        uint4 orow[16 / ROWS];
-        float row_lse[16 / ROWS];
-#pragma unroll
-        for (int x = 0; x < 16 / ROWS; ++x) {  // (every load at once: rows past the end are the last one)
-            const int at = min(row0 + d_row + ROWS * x, s.Lq - 1);
-            row_lse[x] = lse[(int64_t)bh * s.Lq + at];
-            orow[x] = *reinterpret_cast<const uint4 *>(o.p + b * o.batch + h * o.head + (int64_t)at * o.row +
-                                                       (8 * piece < s.D ? 8 * piece : 0));
-        }
         bool ok = n > 0 && __all_sync(0xffffffffu, mbar_wait(q_full, 0, s.status));
         if (ok) {
             if (HD == 64) {
@@ -705,22 +705,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_st_wait();
             warp_arrive(q_ready);
         }
+        float d[16 / ROWS];
 #pragma unroll
         for (int x = 0; x < 16 / ROWS; ++x) {
             const int row = d_row + ROWS * x;
             uint4 g = make_uint4(0, 0, 0, 0);
             if (ok)
-                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(g.x), "=r"(g.y), "=r"(g.z), "=r"(g.w)
-                             : "r"(sg + (piece >> 3) * Z::CHUNK + row * 128 + (((piece & 7) ^ (row & 7)) << 4)));
+                g = *reinterpret_cast<const uint4 *>(smem + Z::TILE + (piece >> 3) * Z::CHUNK + row * 128 +
+                                                     (((piece & 7) ^ (row & 7)) << 4));
             // dO is zero beyond its columns and rows; O and dO of a row without a key may hold anything
-            float d = row_lse[x] != -INFINITY && 8 * piece < s.D ? dot8(orow[x], g, 0.f) : 0.f;
-#pragma unroll
-            for (int m = 1; m < PIECES; m *= 2) d += __shfl_xor_sync(0xffffffffu, d, m);
-            if (piece == 0) row_D[row] = d;
+            d[x] = o_lse[x] != -INFINITY && 8 * piece < s.D ? dot8(orow[x], g, 0.f) : 0.f;
         }
+#pragma unroll
+        for (int m = 1; m < PIECES; m *= 2)
+#pragma unroll
+            for (int x = 0; x < 16 / ROWS; ++x) d[x] += __shfl_xor_sync(0xffffffffu, d[x], m);
+#pragma unroll
+        for (int x = 0; x < 16 / ROWS; ++x)
+            if (piece == 0) row_D[d_row + ROWS * x] = d[x];
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        const float Di = row_D[32 * quad + lane];
+        // D, and lse in units of log 2 (+inf where there is no row or it is empty: P = 0); kept by padded rows for dkv
+        const float Di = row_D[32 * quad + lane], l2 = live && own_lse != -INFINITY ? own_lse * kLog2e : INFINITY;
         if (half == 0 && rank == split - 1) {  // (the last part is never without keys where there are any)
             lse2[(int64_t)bh * s.lq_pad + i] = l2;
             Dr[(int64_t)bh * s.lq_pad + i] = Di;

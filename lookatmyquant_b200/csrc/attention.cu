@@ -54,11 +54,27 @@ struct Rows {  // where a thread writes: element (b, h, row, 0) of a (B, H, L, D
     int64_t batch, head, row;
 };
 
+// Division of 0 <= n < 2^31 by a number of the launch: a CTA's place takes several, of 100 cycles or more each as such.
+struct Div {
+    uint32_t d, m, shift;
+    Div() = default;
+    explicit Div(uint32_t by) : d(by), shift(0) {
+        while ((1ull << shift) < by) ++shift;
+        m = (uint32_t)(((1ull << 32) * ((1ull << shift) - by)) / by + 1);
+    }
+    __device__ __forceinline__ int of(int n, int &rest) const {
+        const uint32_t q = (__umulhi((uint32_t)n, m) + (uint32_t)n) >> shift;
+        rest = n - (int)(q * d);
+        return (int)q;
+    }
+};
+
 struct Shape {
     int B, Hq, Hkv, group, D;
     int Lq, Lk, off;  // off = Lk − Lq
     int lq_pad;       // Lq rounded up to whole tiles
     int causal;
+    Div by_heads, by_kv_heads, by_q, by_kv, by_group;  // B·Hq, B·Hkv, Hq, Hkv, group
     float scale, sl;  // sl = scale·log2 e
     const int32_t *ks, *ke;
     int *status;
@@ -294,15 +310,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_full0 = q_full + 8, p_ready0 = s_full0 + 8 * NB, drain = p_ready0 + 8 * NB;
     const uint32_t sq = smem_u32(smem), sk = sq + 2 * Z::TILE, sv = sk + RING * Z::TILE;
 
-    const int pairs = s.lq_pad / kTile / 2 + (s.lq_pad / kTile & 1), heads = s.Hq * s.B;
+    const int pairs = s.lq_pad / kTile / 2 + (s.lq_pad / kTile & 1);
     // `split` CTAs (a cluster) share a pair of query tiles where there would be too few: each takes a part of the keys
-    const int unit = (int)blockIdx.x / split, rank = (int)blockIdx.x % split;
-    const int qp = pairs - 1 - unit / heads;  // the longest rows of a causal mask first
-    const int bh = unit % heads, b = bh / s.Hq, h = bh % s.Hq, hk = h / s.group;
+    const int unit = split == 1 ? (int)blockIdx.x : (int)blockIdx.x / split, rank = split == 1 ? 0 : (int)blockIdx.x % split;
+    int bh, h, in_group;
+    const int qp = pairs - 1 - s.by_heads.of(unit, bh);  // the longest rows of a causal mask first
+    const int b = s.by_q.of(bh, h), hk = s.by_group.of(h, in_group);
     int lo, hi;
     key_range(s, b, lo, hi);
     const int all0 = key_tiles(s, (2 * qp) * kTile, lo, hi), all1 = key_tiles(s, (2 * qp + 1) * kTile, lo, hi);
-    const int n_all = max(all0, all1), first = n_all * rank / split, n = n_all * (rank + 1) / split - first;
+    const int n_all = max(all0, all1), first = split == 1 ? 0 : n_all * rank / split;
+    const int n = split == 1 ? n_all : n_all * (rank + 1) / split - first;
     const int n0 = min(n, max(0, all0 - first)), n1 = min(n, max(0, all1 - first)), j0 = lo / kTile + first;
     const Steps steps{n0, n1};
 
@@ -577,14 +595,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     float *row_D = reinterpret_cast<float *>(smem + Z::DQ_SMEM - Z::ROW);
     const uint32_t sq = smem_u32(smem), sg = sq + Z::TILE, sk = sg + Z::TILE, sv = sk + KS * Z::TILE;
 
-    const int tiles = s.lq_pad / kTile, heads = s.Hq * s.B;
-    const int unit = (int)blockIdx.x / split, rank = (int)blockIdx.x % split;  // as in the forward
-    const int qt = tiles - 1 - unit / heads;
-    const int bh = unit % heads, b = bh / s.Hq, h = bh % s.Hq, hk = h / s.group;
-    const int row0 = qt * kTile;
+    // as in the forward
+    const int unit = split == 1 ? (int)blockIdx.x : (int)blockIdx.x / split, rank = split == 1 ? 0 : (int)blockIdx.x % split;
+    int bh, h, in_group;
+    const int row0 = (s.lq_pad / kTile - 1 - s.by_heads.of(unit, bh)) * kTile;
+    const int b = s.by_q.of(bh, h), hk = s.by_group.of(h, in_group);
     int lo, hi;
     key_range(s, b, lo, hi);
-    const int n_all = key_tiles(s, row0, lo, hi), first = n_all * rank / split, n = n_all * (rank + 1) / split - first;
+    const int n_all = key_tiles(s, row0, lo, hi), first = split == 1 ? 0 : n_all * rank / split;
+    const int n = split == 1 ? n_all : n_all * (rank + 1) / split - first;
     const int j0 = lo / kTile + first;
 
     // Every elementwise thread's lse, and O for D = Σ dO·O: 16 rows a warp, a row's 16-byte pieces in neighbouring lanes (a
@@ -842,24 +861,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t sk = smem_u32(smem), sv = sk + Z::TILE, sq = sv + Z::TILE, sg = sq + QS * Z::TILE;
 
     // `split` CTAs (a cluster) share a key tile where there would be too few: each takes a part of the group's query heads
-    const int heads = s.Hkv * s.B, unit = (int)blockIdx.x / split, rank = (int)blockIdx.x % split;
-    const int kt = unit / heads;  // the first keys are seen by the most queries: they come first
-    const int bh = unit % heads, b = bh / s.Hkv, hk = bh % s.Hkv, h0 = hk * s.group + rank * (s.group / split);
-    const int key0 = kt * kTile;
+    const int unit = split == 1 ? (int)blockIdx.x : (int)blockIdx.x / split, rank = split == 1 ? 0 : (int)blockIdx.x % split;
+    int bh, hk;
+    const int key0 = s.by_kv_heads.of(unit, bh) * kTile;  // the first keys are seen by the most queries: they come first
+    const int b = s.by_kv.of(bh, hk), share = split == 1 ? s.group : s.group / split, h0 = hk * s.group + rank * share;
     int lo, hi;
     key_range(s, b, lo, hi);
     const int q_lo = s.causal ? max(0, lo - s.off) : 0;  // the queries before see no key
     const int first = s.causal ? max(q_lo, key0 - s.off) : 0;
     const int t0 = first / kTile, tiles = s.lq_pad / kTile;
     const int nq = key0 >= hi || key0 + kTile <= lo || first >= s.Lq ? 0 : tiles - t0;
-    const int n = nq * (s.group / split);
+    const int n = nq * share;
 
     // The loads, by the first thread: K and V, then Q and dO (with the rows' lse and D) through the rings; dO's stage is
     // released by an earlier product than Q's of the same query tile. What finds free stages is issued before the other
     // warps have met.
-    int q_issued = 0, g_issued = 0;
+    int q_issued = 0, g_issued = 0, h = h0, row = t0 * kTile;  // (a division by nq for each tile would take longer)
     const auto load = [&](int j, bool wait) {
-        const int qs = j % QS, gs = j % GS, h = h0 + j / nq, row = (t0 + j % nq) * kTile;
+        const int qs = j % QS, gs = j % GS;
         const int64_t at = ((int64_t)b * s.Hq + h) * s.lq_pad + row;
         if (wait && !mbar_wait(q_empty0 + 8 * qs, ((j / QS) & 1) ^ 1, s.status)) return false;
         mbar_expect_tx(q_full0 + 8 * qs, Z::TILE + Z::ROW);
@@ -871,6 +890,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         load_tile<HD>(sg + gs * Z::TILE, &mapG, row, h, b, g_full0 + 8 * gs);
         bulk_load(smem_u32(row_d + gs * kTile), Dr + at, Z::ROW, g_full0 + 8 * gs);
         ++g_issued;
+        row += kTile;
+        if (row == s.lq_pad) row = t0 * kTile, ++h;
         return true;
     };
     if (threadIdx.x == 0) {
@@ -954,8 +975,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t lanes = (uint32_t)(32 * quad) << 16;
         const bool edge_keys = key0 < lo || key0 + kTile > hi;
         bool ok = true;
-        for (int j = 0; j < n; ++j) {
-            const int qs = j % QS, gs = j % GS, row0 = (t0 + j % nq) * kTile;
+        for (int j = 0, row0 = t0 * kTile; j < n; ++j, row0 = row0 + kTile == s.lq_pad ? t0 * kTile : row0 + kTile) {
+            const int qs = j % QS, gs = j % GS;
             const float4 *l4 = reinterpret_cast<const float4 *>(row_lse + qs * kTile + 64 * half);
             const float4 *d4 = reinterpret_cast<const float4 *>(row_d + gs * kTile + 64 * half);
             const bool edge = edge_keys || (s.causal && key0 + kTile - 1 > row0 + s.off);
@@ -1165,6 +1186,11 @@ int shape_of(const char *fn, const lamq_attention_args &a, int *status, Shape &s
     s.off = s.Lk - s.Lq;
     s.lq_pad = (s.Lq + kTile - 1) / kTile * kTile;
     s.causal = a.causal;
+    s.by_heads = Div((uint32_t)(s.B * s.Hq));
+    s.by_kv_heads = Div((uint32_t)(s.B * s.Hkv));
+    s.by_q = Div((uint32_t)s.Hq);
+    s.by_kv = Div((uint32_t)s.Hkv);
+    s.by_group = Div((uint32_t)s.group);
     s.scale = a.scale;
     s.sl = a.scale * kLog2e;
     s.ks = a.key_start;

@@ -418,8 +418,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int t = (warp - 2) >> 2, quad = warp & 3, nt = t ? n1 : n0;
         const int row0 = (2 * qp + t) * kTile, i = row0 + 32 * quad + lane;
         const bool live = i < s.Lq;
-        const int row_hi = s.causal ? min(hi, i + s.off + 1) : hi;
-        const int whole = s.causal ? min(hi, row0 + s.off + 1) : hi;  // a key tile from lo to here needs no mask
+        // the keys of the text, of the thread's row and of the rows that see all, from the first key tile's first key on
+        const int start = j0 * kTile, from = lo - start, to_all = hi - start;
+        const int to_row = s.causal ? min(to_all, i + s.off + 1 - start) : to_all;
+        const int whole = s.causal ? min(to_all, row0 + s.off + 1 - start) : to_all;  // key tiles between need no mask
         const uint32_t lanes = (uint32_t)(32 * quad) << 16;
         const uint32_t to = tmem + lanes + NB * kTile + t * HD;
         float m = -INFINITY, sum = 0.f;  // m: the maximum that the exponentials are taken against
@@ -434,16 +436,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int c = 0; c < 4; ++c) tmem_load32(ts + 32 * c, r[c]);
             tmem_ld_wait();
-            const int key0 = (j0 + j) * kTile;
-            if (key0 < lo || key0 + kTile > whole) {
-                const int clo = lo - key0, chi = row_hi - key0;
+            if (from > j * kTile || whole < (j + 1) * kTile) {
+                const int clo = from - j * kTile, chi = to_row - j * kTile;
 #pragma unroll
                 for (int c = 0; c < kTile; ++c)
                     if (c < clo || c >= chi) r[c >> 5][c & 31] = 0xff800000u;
-                if (key0 < lo || key0 + kTile > hi) {  // (both tiles' warps do: the same zeros)
+                if (from > j * kTile || to_all < (j + 1) * kTile) {  // (both tiles' warps do: the same zeros)
                     ok = __all_sync(0xffffffffu, mbar_wait(v_full0 + 8 * (j % RING), (j / RING) & 1, s.status));
                     if (!ok) break;
-                    zero_rows<HD>(sv + (j % RING) * Z::TILE, lo - key0, hi - key0, threadIdx.x - 64 - 128 * t, 128);
+                    zero_rows<HD>(sv + (j % RING) * Z::TILE, from - j * kTile, to_all - j * kTile, threadIdx.x - 64 - 128 * t, 128);
                 }
             }
             float top[8];  // eight chains: one of 128 comparisons would take 500 cycles of latency

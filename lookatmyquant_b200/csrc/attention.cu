@@ -103,6 +103,43 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// Pairs of fp32 operations in one instruction (each rounded as alone), and the maximum of three: the elementwise warps are
+// bound by what they issue.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+__device__ __forceinline__ float2 pair_of(const uint32_t *r) { return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])); }
+
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -451,9 +488,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int c = 0; c < 8; ++c) top[c] = __uint_as_float(r[0][c]);
 #pragma unroll
-            for (int c = 8; c < kTile; ++c) top[c & 7] = fmaxf(top[c & 7], __uint_as_float(r[c >> 5][c & 31]));
-            const float mx = fmaxf(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])),
-                                   fmaxf(fmaxf(top[4], top[5]), fmaxf(top[6], top[7])));
+            for (int c = 8; c < kTile - 8; c += 16)
+#pragma unroll
+                for (int e = c; e < c + 8; ++e)
+                    top[e & 7] = max3(top[e & 7], __uint_as_float(r[e >> 5][e & 31]), __uint_as_float(r[(e + 8) >> 5][(e + 8) & 31]));
+#pragma unroll
+            for (int c = 0; c < 8; c += 2)
+                top[c / 2] = max3(fmaxf(top[c], top[c + 1]), __uint_as_float(r[3][24 + c]), __uint_as_float(r[3][25 + c]));
+            const float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]);
             // O and the sum are rescaled only when the maximum has grown by more than 8 binary orders: until then P
             // stays below 2^8, exact enough in fp32 and bf16 alike
             const bool grow = mx > m && (m == -INFINITY || (mx - m) * s.sl > 8.f);
@@ -478,20 +520,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             const float base = m == -INFINITY ? 0.f : m * s.sl;
-            float part[4] = {0.f, 0.f, 0.f, 0.f};
+            float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 uint32_t pk[32];
 #pragma unroll
                 for (int c = 0; c < 64; c += 2) {
-                    const float p0 = ex2(fmaf(__uint_as_float(r[2 * g + (c >> 5)][c & 31]), s.sl, -base));
-                    const float p1 = ex2(fmaf(__uint_as_float(r[2 * g + (c >> 5)][(c & 31) + 1]), s.sl, -base));
-                    part[(c >> 1) & 3] += p0 + p1;
-                    pk[c >> 1] = pack_bf16(p0, p1);
+                    const float2 x = fma2(pair_of(&r[2 * g + (c >> 5)][c & 31]), make_float2(s.sl, s.sl), make_float2(-base, -base));
+                    const float2 e = make_float2(ex2(x.x), ex2(x.y));
+                    part[(c >> 1) & 1] = add2(part[(c >> 1) & 1], e);
+                    pk[c >> 1] = pack_bf16(e.x, e.y);
                 }
                 tmem_store32(ts + 32 * g, pk);
             }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            sum += (part[0].x + part[1].x) + (part[0].y + part[1].y);
             tmem_st_wait();
             warp_arrive(p_ready0 + 8 * buf);
         }
@@ -747,8 +789,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         // D, and lse in units of log 2 (+inf where there is no row or it is empty: P = 0); kept by padded rows for dkv
         const float Di = row_D[32 * quad + lane], l2 = live && own_lse != -INFINITY ? own_lse * kLog2e : INFINITY;
         if (half == 0 && rank == split - 1) {  // (the last part is never without keys where there are any)
-            lse2[(int64_t)bh * s.lq_pad + i] = l2;
-            Dr[(int64_t)bh * s.lq_pad + i] = Di;
+            lse2[(int64_t)bh * s.lq_pad + i] = -l2;  // negated, as the dkv kernel adds them
+            Dr[(int64_t)bh * s.lq_pad + i] = -Di;
         }
         for (int j = 0; ok && j < n; ++j) {
             ok = __all_sync(0xffffffffu, mbar_wait(s_full, j & 1, s.status));
@@ -763,8 +805,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool edge = key0 < lo || key0 + kTile > hi || (s.causal && key0 + kTile - 1 > row0 + s.off);
             const int clo = lo - key0 - 64 * half, chi = row_hi - key0 - 64 * half;
 #pragma unroll
-            for (int c = 0; c < 64; ++c)
-                r[c >> 5][c & 31] = __float_as_uint(ex2(fmaf(__uint_as_float(r[c >> 5][c & 31]), s.sl, -l2)));
+            for (int c = 0; c < 64; c += 2) {
+                uint32_t *const at = &r[c >> 5][c & 31];
+                const float2 x = fma2(pair_of(at), make_float2(s.sl, s.sl), make_float2(-l2, -l2));
+                at[0] = __float_as_uint(ex2(x.x)), at[1] = __float_as_uint(ex2(x.y));
+            }
             ok = __all_sync(0xffffffffu, mbar_wait(p_full, j & 1, s.status));
             if (!ok) break;
             tc_fence_after();
@@ -772,9 +817,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_load32(tmem + lanes + kP + 64 * half + 32, d[1]);
             tmem_ld_wait();
 #pragma unroll
-            for (int c = 0; c < 64; ++c) {
-                const float x = __uint_as_float(r[c >> 5][c & 31]) * (__uint_as_float(d[c >> 5][c & 31]) - Di);
-                r[c >> 5][c & 31] = __float_as_uint(x);
+            for (int c = 0; c < 64; c += 2) {
+                uint32_t *const at = &r[c >> 5][c & 31];
+                const float2 x = mul2(pair_of(at), add2(pair_of(&d[c >> 5][c & 31]), make_float2(-Di, -Di)));
+                at[0] = __float_as_uint(x.x), at[1] = __float_as_uint(x.y);
             }
             if (edge) {
 #pragma unroll
@@ -993,12 +1039,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld_wait();
 #pragma unroll
             for (int c = 0; c < 64; c += 4) {
-                const float4 l = l4[c >> 2];
-                const float ls[4] = {l.x, l.y, l.z, l.w};
+                const float4 l = l4[c >> 2];  // negated
+                const float2 ls[2] = {make_float2(l.x, l.y), make_float2(l.z, l.w)};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float p = ex2(fmaf(__uint_as_float(r[(c + e) >> 5][(c + e) & 31]), s.sl, -ls[e]));
-                    r[(c + e) >> 5][(c + e) & 31] = __float_as_uint(p);
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t *const at = &r[c >> 5][(c & 31) + 2 * e];
+                    const float2 x = fma2(pair_of(at), make_float2(s.sl, s.sl), ls[e]);
+                    at[0] = __float_as_uint(ex2(x.x)), at[1] = __float_as_uint(ex2(x.y));
                 }
             }
             if (edge) {
@@ -1029,13 +1076,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld_wait();
 #pragma unroll
             for (int c = 0; c < 64; c += 4) {
-                const float4 l = d4[c >> 2];
-                const float ds[4] = {l.x, l.y, l.z, l.w};
+                const float4 l = d4[c >> 2];  // negated
+                const float2 ds[2] = {make_float2(l.x, l.y), make_float2(l.z, l.w)};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float x = __uint_as_float(r[(c + e) >> 5][(c + e) & 31]) *
-                                    (__uint_as_float(d[(c + e) >> 5][(c + e) & 31]) - ds[e]);
-                    d[(c + e) >> 5][(c + e) & 31] = __float_as_uint(x);
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t *const at = &d[c >> 5][(c & 31) + 2 * e];
+                    const float2 x = mul2(pair_of(&r[c >> 5][(c & 31) + 2 * e]), add2(pair_of(at), ds[e]));
+                    at[0] = __float_as_uint(x.x), at[1] = __float_as_uint(x.y);
                 }
             }
             if (edge) {

@@ -26,7 +26,18 @@
 // all MMAs of a CTA and the tensor core runs them in issue order, so a product may overwrite TMEM that the product
 // issued before it reads. That thread does nothing else and waits alone: it runs hardly ahead of the tensor core, and
 // where its warp takes part (a vote after each wait, MMAs predicated by lane) a group of 24 MMAs takes 2475 cycles
-// instead of 1847. Two issuing warps were slower still (their MMAs alternate between accumulators).
+// instead of 1847. Two issuing warps were slower still (their MMAs alternate between accumulators). A wait takes it 70
+// cycles and a commit 85, in which little is queued; releases by the elementwise warps instead cost those more.
+//
+// Measured and what bounds it (causal, no padding):
+//   2 x 4096, 32/8 heads of 128: forward 276 us (990 TFLOP/s; the softmax warps, one S buffer a tile), dq 355 us (1160
+//   TFLOP/s executed) and dkv 430 us (1280 executed; shared-memory bandwidth of products that read both operands from it,
+//   and the elementwise steps between them).
+//   8 x 2048, 15/5 heads of 64: forward 129 us, dq 170, dkv 195: an MMA of 64 columns takes as long as one of 128, so half
+//   the tensor rate is lost; exponentials run at half of their rate.
+//   A CTA's start and end cost as much as 3 to 5 of its tiles. CTAs that took over further units (cluster launch control)
+//   made short rows 5 to 8 % faster (dq of 5 x 1337, 32/8 heads of 128: 174 -> 161 us) and long ones 3 to 6 % slower (2 x
+//   8192, 15/5 of 64: 501 -> 528 us), and were left out.
 #include <algorithm>
 #include <climits>
 #include <mutex>
@@ -1028,9 +1039,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float4 *d4 = reinterpret_cast<const float4 *>(row_d + gs * kTile + 64 * half);
             const bool edge = edge_keys || (s.causal && key0 + kTile - 1 > row0 + s.off);
             const int clo = !in ? 64 : s.causal ? key - s.off - row0 - 64 * half : 0;  // columns before are masked
-            ok = __all_sync(0xffffffffu, mbar_wait(s_full, j & 1, s.status));
             // the tile's statistics came with Q and dO: their barriers make them visible to this thread
-            ok = ok && __all_sync(0xffffffffu, mbar_wait(q_full0 + 8 * qs, (j / QS) & 1, s.status));
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full, j & 1, s.status) &&
+                                             mbar_wait(q_full0 + 8 * qs, (j / QS) & 1, s.status));
             if (!ok) break;
             tc_fence_after();
             uint32_t r[2][32], pk[32];
@@ -1066,8 +1077,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_st_wait();
             warp_arrive(p_ready);
 
-            ok = __all_sync(0xffffffffu, mbar_wait(p_full, j & 1, s.status));
-            ok = ok && __all_sync(0xffffffffu, mbar_wait(g_full0 + 8 * gs, (j / GS) & 1, s.status));
+            ok = __all_sync(0xffffffffu, mbar_wait(p_full, j & 1, s.status) &&
+                                             mbar_wait(g_full0 + 8 * gs, (j / GS) & 1, s.status));
             if (!ok) break;
             tc_fence_after();
             uint32_t d[2][32];

@@ -10,8 +10,10 @@
 // without its a, moves singular vectors by 2^-12 relative where singular values have already reached 1 and nothing
 // where they have not. Single products (hi·hi) are therefore enough for A in every step and for B·X in all but the last;
 // A·A and the last B·X take three (hi·hi + hi·lo + lo·hi), and so does everything after a fifth step, where the roundings
-// of saturated directions would go on adding up. In simulation (64 x 2000 .. 500 x 520; Gaussian, low-rank,
-// power-law, row-scaled updates) this leaves 2e-4 .. 1.8e-3 of relative error, against 1.65e-3 of the bf16 output's
+// of saturated directions would go on adding up, and everything where the shorter side is 128 at most: with few directions
+// single products came to 2.7e-3 (198 x 21), and those products are short (70 x 458: 154 us so, 140 with single ones). In
+// simulation (64 x 2000 .. 500 x 520; Gaussian, low-rank, power-law, row-scaled updates) this leaves 2e-4 .. 1.8e-3 of
+// relative error beside 1.65e-3 of the bf16 output's
 // rounding; three products everywhere leave 1e-5 for 2.6 times the work, single ones 4e-3. Everything is held times
 // kScale = 2^10, which keeps entries of order 1/max(m, n) clear of fp16's subnormals and the largest (singular values
 // up to 5, B up to 32) below its maximum. Accumulation is fp32 in TMEM.
@@ -120,7 +122,7 @@ __device__ __forceinline__ Phase phase_of(const Params &p, int index) {
     const int step = index / 3;
     f.kind = index % 3;
     f.last = step == p.steps - 1;
-    f.split = f.kind == kPoly || step > 4 || (f.kind == kApply && (step == 4 || f.last));
+    f.split = f.kind == kPoly || step > 4 || p.s <= BM || (f.kind == kApply && (step == 4 || f.last));
     f.M = f.kind == kApply && p.tall ? p.l : p.s;
     f.N = f.kind == kApply && !p.tall ? p.l : p.s;
     f.K = f.kind == kGram ? p.l : p.s;

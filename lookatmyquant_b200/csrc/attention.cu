@@ -31,9 +31,9 @@
 //
 // Measured and what bounds it (causal, no padding):
 //   2 x 4096, 32/8 heads of 128: forward 276 us (990 TFLOP/s; the softmax warps, one S buffer a tile), dq 355 us (1160
-//   TFLOP/s executed) and dkv 430 us (1280 executed; shared-memory bandwidth of products that read both operands from it,
+//   TFLOP/s executed) and dkv 418 us (1320 executed; shared-memory bandwidth of products that read both operands from it,
 //   and the elementwise steps between them).
-//   8 x 2048, 15/5 heads of 64: forward 129 us, dq 170, dkv 195: an MMA of 64 columns takes as long as one of 128, so half
+//   8 x 2048, 15/5 heads of 64: forward 129 us, dq 170, dkv 182: an MMA of 64 columns takes as long as one of 128, so half
 //   the tensor rate is lost; exponentials run at half of their rate.
 //   A CTA's start and end cost as much as 3 to 5 of its tiles. CTAs that took over further units (cluster launch control)
 //   made short rows 5 to 8 % faster (dq of 5 x 1337, 32/8 heads of 128: 174 -> 161 us) and long ones 3 to 6 % slower (2 x
@@ -141,6 +141,25 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
         : "=f"(d.x), "=f"(d.y)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
+}
+
+// 2^x of a pair with x <= 1 or so, in fp32 instructions alone: x = n + f with n the nearest integer (from the low bits of x
+// + 1.5·2^23), 2^f by the polynomial that meets it in the six Chebyshev points of [-1/2, 1/2] (2e-7 off with its roundings),
+// times 2^n. Below -126 it stays at 2^-126; NaN stays NaN.
+__device__ __forceinline__ float2 ex2_pair(float2 x) {
+    constexpr float kMagic = 12582912.f;
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+    const float2 t = add2(x, make_float2(kMagic, kMagic)), n = add2(t, make_float2(-kMagic, -kMagic));
+    const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+    float2 y = make_float2(0.00133908633f, 0.00133908633f);
+    y = fma2(y, f, make_float2(0.00967603177f, 0.00967603177f));
+    y = fma2(y, f, make_float2(0.0555035695f, 0.0555035695f));
+    y = fma2(y, f, make_float2(0.240221068f, 0.240221068f));
+    y = fma2(y, f, make_float2(0.693147182f, 0.693147182f));
+    y = fma2(y, f, make_float2(1.00000012f, 1.00000012f));
+    return mul2(y, make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                               __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)));
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -1056,7 +1075,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int e = 0; e < 2; ++e) {
                     uint32_t *const at = &r[c >> 5][(c & 31) + 2 * e];
                     const float2 x = fma2(pair_of(at), make_float2(s.sl, s.sl), ls[e]);
-                    at[0] = __float_as_uint(ex2(x.x)), at[1] = __float_as_uint(ex2(x.y));
+                    // a quarter of the exponentials in fp32 instructions: the 16 a cycle of the special-function unit hold the
+                    // step up (dkv of 2 x 4096, 32/8 heads of 128: 432 -> 418 us; of 2 x 8192, 15/5 of 64: 650 -> 614; a
+                    // third: 424 and 607; the dq kernel, with more to do beside, became 4 to 14 % slower)
+                    const float2 y = (c / 2 + e) % 4 == 3 ? ex2_pair(x) : make_float2(ex2(x.x), ex2(x.y));
+                    at[0] = __float_as_uint(y.x), at[1] = __float_as_uint(y.y);
                 }
             }
             if (edge) {

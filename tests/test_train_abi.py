@@ -140,3 +140,25 @@ def test_attention_args_layout_matches_the_header(lib):
         assert lib.lamq_attention_backward(args, P, 0, P, None) == _lib.LAMQ_ERR_INVALID
         assert f"({name})".encode() in lib.lamq_last_error()
     assert ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+def test_exponential_polynomial_error():
+    """The polynomial of the attention's exponentials in fp32 instructions, evaluated as the kernel does (fused multiply-adds
+    in fp32): within 3e-7 of 2^x (its six-point Chebyshev interpolation is 1.02e-7 off, each of five roundings up to 6e-8 of a
+    partial sum that the next factor, at most 1/2, shrinks)."""
+    import numpy as np
+
+    src = (HEADER.parents[1] / "lookatmyquant_b200" / "csrc" / "attention.cu").read_text()
+    body = src[src.index("float2 ex2_pair(") :]
+    body = body[: body.index("\n}\n")]
+    coefficients = [np.float32(m) for m in re.findall(r"make_float2\((0\.\d+|1\.0+\d+)f, \1f\)", body)]
+    assert len(coefficients) == 6
+    x = np.concatenate([np.linspace(-126, 1, 400_001), np.arange(-126, 2) + 0.5, np.arange(-126, 2)]).astype(np.float32)
+    n = (x + np.float32(12582912.0)) - np.float32(12582912.0)
+    f = (x - n).astype(np.float64)
+    assert np.abs(f).max() <= 0.5
+    y = np.full(f.shape, coefficients[0], np.float32)
+    for c in coefficients[1:]:
+        y = (y.astype(np.float64) * f + np.float64(c)).astype(np.float32)
+    got = y.astype(np.float64) * 2.0 ** n.astype(np.float64)
+    assert np.abs(got / 2.0 ** x.astype(np.float64) - 1).max() < 3e-7

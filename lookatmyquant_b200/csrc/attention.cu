@@ -168,7 +168,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-__device__ __forceinline__ float2 pair_of(const uint32_t *r) { return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1])); }
+__device__ __forceinline__ float2 pair_of(const uint32_t *r) {
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
@@ -436,8 +438,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = EARLY; ok && i < 2 * n; ++i) ok = load_next(true);
             if (!ok) {  // error path: let the copies in flight land before the CTA exits
                 wait_bounded(q_full, 0);
-                for (int i = max(0, k_issued - RING); i < k_issued; ++i) wait_bounded(k_full0 + 8 * (i % RING), (i / RING) & 1);
-                for (int i = max(0, v_issued - RING); i < v_issued; ++i) wait_bounded(v_full0 + 8 * (i % RING), (i / RING) & 1);
+                for (int i = max(0, k_issued - RING); i < k_issued; ++i)
+                    wait_bounded(k_full0 + 8 * (i % RING), (i / RING) & 1);
+                for (int i = max(0, v_issued - RING); i < v_issued; ++i)
+                    wait_bounded(v_full0 + 8 * (i % RING), (i / RING) & 1);
             }
         }
     } else if (warp == 1) {
@@ -449,7 +453,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const auto issue_s = [&](int u, int to) {
                 if (steps.begins(u)) ok = mbar_wait(k_full0 + 8 * k.at, k.parity, s.status);
                 if (!ok) return;
-                mma_rows_rows<HD>(tmem + to * kTile, q_desc + steps.query_tile(u) * (Z::TILE >> 4), k_desc + k.at * (Z::TILE >> 4));
+                mma_rows_rows<HD>(tmem + to * kTile, q_desc + steps.query_tile(u) * (Z::TILE >> 4),
+                                  k_desc + k.at * (Z::TILE >> 4));
                 if (steps.ends(u)) {
                     mma_commit(k_empty0 + 8 * k.at);
                     k.next<RING>();
@@ -511,7 +516,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (from > j * kTile || to_all < (j + 1) * kTile) {  // (both tiles' warps do: the same zeros)
                     ok = __all_sync(0xffffffffu, mbar_wait(v_full0 + 8 * (j % RING), (j / RING) & 1, s.status));
                     if (!ok) break;
-                    zero_rows<HD>(sv + (j % RING) * Z::TILE, from - j * kTile, to_all - j * kTile, threadIdx.x - 64 - 128 * t, 128);
+                    zero_rows<HD>(sv + (j % RING) * Z::TILE, from - j * kTile, to_all - j * kTile,
+                                  threadIdx.x - 64 - 128 * t, 128);
                 }
             }
             float top[8];  // eight chains: one of 128 comparisons would take 500 cycles of latency
@@ -521,7 +527,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 8; c < kTile - 8; c += 16)
 #pragma unroll
                 for (int e = c; e < c + 8; ++e)
-                    top[e & 7] = max3(top[e & 7], __uint_as_float(r[e >> 5][e & 31]), __uint_as_float(r[(e + 8) >> 5][(e + 8) & 31]));
+                    top[e & 7] = max3(top[e & 7], __uint_as_float(r[e >> 5][e & 31]),
+                                      __uint_as_float(r[(e + 8) >> 5][(e + 8) & 31]));
 #pragma unroll
             for (int c = 0; c < 8; c += 2)
                 top[c / 2] = max3(fmaxf(top[c], top[c + 1]), __uint_as_float(r[3][24 + c]), __uint_as_float(r[3][25 + c]));
@@ -556,7 +563,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint32_t pk[32];
 #pragma unroll
                 for (int c = 0; c < 64; c += 2) {
-                    const float2 x = fma2(pair_of(&r[2 * g + (c >> 5)][c & 31]), make_float2(s.sl, s.sl), make_float2(-base, -base));
+                    const float2 x = fma2(pair_of(&r[2 * g + (c >> 5)][c & 31]), make_float2(s.sl, s.sl),
+                                          make_float2(-base, -base));
                     const float2 e = make_float2(ex2(x.x), ex2(x.y));
                     part[(c >> 1) & 1] = add2(part[(c >> 1) & 1], e);
                     pk[c >> 1] = pack_bf16(e.x, e.y);

@@ -193,7 +193,10 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t saddr, uint32_t rank) {
     return r;
 }
 
+// Every thread of the cluster meets the others here. `.aligned` wants a warp's threads at the instruction together, and a
+// warp that comes from a branch of one lane (a producer's loop) need not be: it reconverges first.
 __device__ __forceinline__ void cluster_sync_all() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 

@@ -46,6 +46,7 @@
 #include <cuda_bf16.h>
 
 #include "../../include/lamq_b200_train.h"
+#include "attention_steps.cuh"
 #include "lamq_common.cuh"
 #include "sm100.cuh"
 
@@ -322,18 +323,6 @@ __device__ __forceinline__ void zero_row(__nv_bfloat16 *dst, int D) {
 
 // ------------------------------------------------------------------------------------------------------------ forward
 
-// The order of the forward's steps (key tile j, query tile t) where the two query tiles meet n0 and n1 key tiles: by key
-// tiles, and by query tiles where both meet one.
-struct Steps {
-    int n0, n1;
-    __device__ __forceinline__ int both() const { return min(n0, n1); }
-    __device__ __forceinline__ int count() const { return n0 + n1; }
-    __device__ __forceinline__ int index(int j, int t) const { return min(2 * j + t, both() + j); }
-    __device__ __forceinline__ int query_tile(int u) const { return u < 2 * both() ? u & 1 : (int)(n1 > n0); }
-    __device__ __forceinline__ bool begins(int u) const { return u >= 2 * both() || !(u & 1); }  // a key tile's first step
-    __device__ __forceinline__ bool ends(int u) const { return u >= 2 * both() || (u & 1); }
-};
-
 // A stage of a ring and the parity of its barrier: counted up, since a remainder costs the issuing thread time in which
 // the tensor core idles.
 struct Turn {
@@ -368,15 +357,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int STAGES = Z::FWD_STAGES, RING = STAGES / 2, NB = Z::FWD_S;
     extern __shared__ __align__(1024) uint8_t smem[];  // swizzled tiles start at multiples of 1024 bytes
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (2 + STAGES) * Z::TILE);
-    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 2 * NB + 2);
+    uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + 2 * STAGES + 2 * NB + 3);
     float *const parts = reinterpret_cast<float *>(smem + 2 * Z::TILE);
     float *const row_max = reinterpret_cast<float *>(smem + Z::FWD_SMEM - 4 * Z::ROW), *const row_sum = row_max + 2 * kTile;
     static_assert(2 * HD * kTile * 4 <= STAGES * Z::TILE, "the parts of O fit into the stages");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t k_full0 = smem_u32(bars), v_full0 = k_full0 + 8 * RING, k_empty0 = v_full0 + 8 * RING,
                    v_empty0 = k_empty0 + 8 * RING, q_full = v_empty0 + 8 * RING;
-    // a buffer's s_full completes for step u when S(u) is there, and once more when P·V of the step has read it
-    const uint32_t s_full0 = q_full + 8, p_ready0 = s_full0 + 8 * NB, drain = p_ready0 + 8 * NB;
+    // s_full: the issuing thread's barriers of the buffers and, last, of the query tile that ends first (Steps)
+    const uint32_t s_full0 = q_full + 8, p_ready0 = s_full0 + 8 * (NB + 1), drain = p_ready0 + 8 * NB;
     const uint32_t sq = smem_u32(smem), sk = sq + 2 * Z::TILE, sv = sk + RING * Z::TILE;
 
     const int pairs = s.lq_pad / kTile / 2 + (s.lq_pad / kTile & 1);
@@ -391,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int n_all = max(all0, all1), first = split == 1 ? 0 : n_all * rank / split;
     const int n = split == 1 ? n_all : n_all * (rank + 1) / split - first;
     const int n0 = min(n, max(0, all0 - first)), n1 = min(n, max(0, all1 - first)), j0 = lo / kTile + first;
-    const Steps steps{n0, n1};
+    const Steps<NB> steps{n0, n1};
 
     // The loads, by the first thread: Q, then K and V through the rings in the order K0 K1 V0 K2 V1 ..., as the products
     // want them. What finds free stages is issued before the other warps have met.
@@ -410,10 +399,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int EARLY = 2 * RING - 1;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2 * STAGES + 1; ++i) mbar_init(k_full0 + 8 * i, 1);
-        for (int i = 0; i < NB; ++i) {
-            mbar_init(s_full0 + 8 * i, 1);
-            mbar_init(p_ready0 + 8 * i, 4);
-        }
+        for (int i = 0; i < NB + 1; ++i) mbar_init(s_full0 + 8 * i, 1);
+        for (int i = 0; i < NB; ++i) mbar_init(p_ready0 + 8 * i, 4);
         mbar_init(drain, 1);
         fence_mbar_init();
         if (n > 0) {
@@ -447,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 1) {
         if (lane == 0 && n > 0) {  // ---- MMA issuer. P lies over S: P·V of a step goes before the buffer's next S
             const uint64_t q_desc = rows_desc(sq), k_desc = rows_desc(sk), v_desc = cols_desc<HD>(sv);
-            const int count = steps.count();
+            const int count = steps.count(), ends_first = steps.ends_first();
             Turn k, v, buf;
             bool ok = mbar_wait(q_full, 0, s.status);
             const auto issue_s = [&](int u, int to) {
@@ -466,22 +453,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (ok) mma_commit(s_full0 + 8 * u);
             }
             uint32_t first_of = 3;  // the query tiles (bits) whose O holds nothing yet
-            for (int u = 0; ok && u < count; ++u, buf.next<NB>()) {
-                const int t = steps.query_tile(u);
-                ok = (!steps.begins(u) || mbar_wait(v_full0 + 8 * v.at, v.parity, s.status)) &&
-                     mbar_wait(p_ready0 + 8 * buf.at, buf.parity, s.status);
-                if (!ok) break;
-                tc_fence_after();
-                mma_tmem_rows<HD>(tmem + NB * kTile + t * HD, tmem + buf.at * kTile, 32, v_desc + v.at * (Z::TILE >> 4),
-                                  !(first_of >> t & 1));
-                first_of &= ~(1u << t);
-                if (steps.ends(u)) {
-                    mma_commit(v_empty0 + 8 * v.at);
-                    v.next<RING>();
+            int u = 0;
+            const auto run_to = [&](int end) {
+                for (; ok && u < end; ++u, buf.next<NB>()) {
+                    const int t = steps.query_tile(u);
+                    ok = (!steps.begins(u) || mbar_wait(v_full0 + 8 * v.at, v.parity, s.status)) &&
+                         mbar_wait(p_ready0 + 8 * buf.at, buf.parity, s.status);
+                    if (!ok) break;
+                    tc_fence_after();
+                    mma_tmem_rows<HD>(tmem + NB * kTile + t * HD, tmem + buf.at * kTile, 32, v_desc + v.at * (Z::TILE >> 4),
+                                      !(first_of >> t & 1));
+                    first_of &= ~(1u << t);
+                    if (steps.ends(u)) {
+                        mma_commit(v_empty0 + 8 * v.at);
+                        v.next<RING>();
+                    }
+                    if (u + NB < count) issue_s(u + NB, buf.at);
+                    if (ok) mma_commit(s_full0 + 8 * buf.at);
                 }
-                if (u + NB < count) issue_s(u + NB, buf.at);
-                if (ok) mma_commit(s_full0 + 8 * buf.at);
-            }
+            };
+            run_to(ends_first + 1);
+            // (a test in each step for this one commit took 3 % more: 2 x 8192, 15/5 heads of 64: 386 us instead of 370)
+            if (ok && ends_first >= 0) mma_commit(s_full0 + 8 * NB);
+            run_to(count);
             mma_commit(drain);  // every MMA this thread issued completes before TMEM is released
             wait_bounded(drain, 0);
         }
@@ -498,10 +492,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t to = tmem + lanes + NB * kTile + t * HD;
         float m = -INFINITY, sum = 0.f;  // m: the maximum that the exponentials are taken against
         bool ok = true;
+        const auto wait_for = [&](Wait w) {
+            return __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * w.bar, w.phase & 1, s.status)) != 0;
+        };
         for (int j = 0; j < nt; ++j) {
             const int u = steps.index(j, t), buf = u % NB;
             const uint32_t ts = tmem + lanes + buf * kTile;
-            ok = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * buf, (u / NB) & 1, s.status));
+            ok = wait_for(steps.scores(u));
             if (!ok) break;
             tc_fence_after();
             uint32_t r[4][32];
@@ -541,8 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (grow) m = mx;
                 sum *= f;
                 if (j > 0) {
-                    const int before = steps.index(j - 1, t);
-                    ok = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * (before % NB), (before / NB + 1) & 1, s.status));
+                    ok = wait_for(steps.read(steps.index(j - 1, t)));
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
@@ -576,8 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             warp_arrive(p_ready0 + 8 * buf);
         }
         if (ok && nt > 0) {
-            const int last = steps.index(nt - 1, t);
-            ok = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * (last % NB), (last / NB + 1) & 1, s.status));
+            ok = wait_for(steps.last_read(steps.index(nt - 1, t)));
             tc_fence_after();
         }
         if (split > 1 && n > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(drain, 0, s.status));  // the other tile's too

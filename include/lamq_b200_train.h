@@ -30,7 +30,7 @@ int lamq_embedding_lookup(const void *table, int dtype, int64_t ldt, int64_t row
  * invalid id (which sets *status to LAMQ_ERR_INVALID) add nothing. Sums are fp32 in the order of the tokens (above 2048
  * tokens, within fixed chunks of the sorted tokens, then chunk by chunk): equal calls give equal bits. Workspace:
  * lamq_embedding_gradient_workspace_size(n, d) bytes, 16-byte aligned (0, and NULL allowed, up to 2048 tokens). *status
- * becomes LAMQ_ERR_TIMEOUT if a bounded device wait gives up.
+ * becomes LAMQ_ERR_TIMEOUT if a bounded device wait gives up: no sums are written then.
  */
 size_t lamq_embedding_gradient_workspace_size(int64_t n, int d);
 int lamq_embedding_gradient(const void *dy, int dtype, int64_t ldy, const void *ids, int ids64, int64_t n, int64_t rows,

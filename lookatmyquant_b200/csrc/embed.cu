@@ -345,6 +345,7 @@ struct SortedParams {
     int64_t chunks;
     float *head, *tail;       // a partial per chunk: of the row that began before it, of the row that goes on after it
     unsigned *barrier;        // arrivals of the sorting blocks, zero before the launch
+    unsigned *gave_up;        // not zero once a sorting block has given up, zero before the launch: no keys to go by
 };
 
 // The blocks that count on `counter` have arrived `target` times in all and see each other's writes. Bounded.
@@ -516,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     __shared__ uint32_t seen[kWarps][kMaxBins], place[kMaxBins], scan[kWarps];
     __shared__ int shared_ok;
     if ((int)blockIdx.x < s.sorters) {
-        sort_tokens(s, seen, place, scan, &shared_ok);
+        if (!sort_tokens(s, seen, place, scan, &shared_ok) && threadIdx.x == 0) *s.gave_up = 1u;
         return;
     }
     const int64_t total = s.g.rows * s.g.packs, step = (int64_t)(gridDim.x - s.sorters) * kThreads;
@@ -539,6 +540,7 @@ __global__ void __launch_bounds__(kSumThreads)
     if (col >= s.g.packs) return;
     const uint32_t dead = (uint32_t)s.g.rows;
     const uint32_t prev = lo > 0 ? keys[lo - 1] : dead, next = hi < s.g.n ? keys[hi] : dead;
+    if (*s.gave_up) return;  // without a whole sort, keys and pos may hold anything
     float acc[V];
     bool open = false;   // acc holds tokens of row `cur`
     bool first = true;   // no row has been closed in this chunk yet
@@ -595,7 +597,7 @@ __global__ void __launch_bounds__(kSumThreads)
     const int64_t lo = c * s.chunk, hi = lo + s.chunk;
     if (hi >= s.g.n) return;
     const uint32_t key = keys[hi - 1], next = keys[hi], begin = keys[lo], prev = lo > 0 ? keys[lo - 1] : (uint32_t)s.g.rows;
-    if (key >= (uint32_t)s.g.rows || next != key) return;  // nothing goes on
+    if (*s.gave_up || key >= (uint32_t)s.g.rows || next != key) return;  // no sort; nothing goes on
     if (begin == key && prev == key) return;               // it began before
     int64_t end = c + 1;  // the row's last chunk: the first whose next token is another's, 32 at a time
     for (;; end += 32) {
@@ -692,6 +694,7 @@ int run_gradient(const void *dyv, void *dEv, GradParams g, int d, void *workspac
     SortedParams p{};
     p.g = g;
     p.barrier = reinterpret_cast<unsigned *>(ws);
+    p.gave_up = p.barrier + 1;
     for (int i = 0; i < 2; ++i) {
         p.keys[i] = reinterpret_cast<uint32_t *>(ws + 256 + (2 * i) * L.keys);
         p.pos[i] = reinterpret_cast<uint32_t *>(ws + 256 + (2 * i + 1) * L.keys);
@@ -711,7 +714,7 @@ int run_gradient(const void *dyv, void *dEv, GradParams g, int d, void *workspac
     const auto kernel = gradient_sort_kernel<T, V>;
     int per_sm = 0;
     e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, 0);
-    if (e == cudaSuccess) e = cudaMemsetAsync(p.barrier, 0, sizeof(unsigned), s);
+    if (e == cudaSuccess) e = cudaMemsetAsync(p.barrier, 0, 2 * sizeof(unsigned), s);
     if (e != cudaSuccess) return cuda_failed(e);
     const int grid = g.accumulate ? p.sorters : p.sorters + sms * std::max(1, std::min(per_sm, 4) - 1);
     LAMQ_REQUIRE(grid <= sms * per_sm, "lamq_embedding_gradient: the device has too few multiprocessors");

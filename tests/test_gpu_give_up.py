@@ -1,0 +1,43 @@
+"""Bounded device waits that run out: the call ends with a status, and what depended on the wait is left alone."""
+
+import ctypes
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+HERE = Path(__file__).resolve().parent
+
+
+@pytest.fixture(scope="module")
+def harness(tmp_path_factory):
+    from lookatmyquant_b200 import build
+    out = tmp_path_factory.mktemp("give_up") / "embed_give_up.so"
+    subprocess.run([build.nvcc(), *build.ARCH, *build.NVCC_FLAGS, "-shared", str(HERE / "embed_give_up.cu"),
+                    str(build.CSRC / "api.cu"), "-o", str(out)], check=True, capture_output=True)
+    return ctypes.CDLL(str(out))
+
+
+def test_a_sort_that_gives_up_leaves_the_gradient_alone(harness):
+    """The kernels after the sort do not go by keys and positions that nobody wrote: the gradient that was to be added to
+    stays as it was. (Here they hold valid places, so that a kernel that did go by them would be seen in the result.)"""
+    n, rows, d = 3000, 100, 64
+    g = torch.Generator("cuda").manual_seed(1)
+    dy = torch.randn(n, d, device="cuda", generator=g)
+    ids = torch.randint(0, rows, (n,), device="cuda", generator=g)
+    dE = torch.randn(rows, d, device="cuda", generator=g)
+    before = dE.clone()
+    keys = (torch.arange(n, device="cuda", dtype=torch.int32) * rows // n).repeat(2)
+    pos = torch.arange(n, device="cuda", dtype=torch.int32).repeat(2)
+    counts = torch.zeros(64 * 512, dtype=torch.int32, device="cuda")
+    head, tail = torch.zeros(n, d, device="cuda"), torch.zeros(n, d, device="cuda")
+    words, status = (torch.zeros(2, dtype=torch.int32, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    p = lambda t: ctypes.c_void_p(t.data_ptr())
+    err = harness.gradient_with_a_block_missing(p(dy), p(ids), ctypes.c_int64(n), ctypes.c_int64(rows), d, p(dE), p(keys),
+                                                p(pos), p(counts), p(head), p(tail), p(words), p(status))
+    assert err == 0
+    assert status.tolist() == [4, 0] and words.tolist() == [1, 1]  # LAMQ_ERR_TIMEOUT; one arrival, given up
+    assert torch.equal(dE, before)

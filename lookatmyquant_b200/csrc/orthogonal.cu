@@ -186,6 +186,13 @@ __device__ __forceinline__ bool grid_barrier(const Params &p, unsigned target, i
     return *shared_ok != 0;
 }
 
+// A word of another CTA's shared memory.
+__device__ __forceinline__ uint32_t load_cluster(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
+}
+
 // Eight entries of G's row r from column c (zero past the end).
 __device__ __forceinline__ void load_g8(const Params &p, int z, int r, int c, float (&v)[8]) {
     const int64_t at = z * p.gbatch + (int64_t)r * p.ldg + c;
@@ -329,6 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     double *red = reinterpret_cast<double *>(bars + 2 * SLOTS + 6);
     uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(red + kThreads / 32);
     int *shared_ok = reinterpret_cast<int *>(tmem_holder + 1);
+    uint32_t *issued = tmem_holder + 2;  // slots that this CTA's loads have taken, at the end
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + SLOTS);
     const uint32_t tfull0 = smem_u32(bars + 2 * SLOTS), tempty0 = tfull0 + 16, drain = tfull0 + 32;
@@ -644,13 +652,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (go) go = grid_barrier(p, target += gridDim.x, shared_ok);
     }
-    if (warp == 0 && lane == 0 && !ok) {  // after an error, copies may still be in flight: they land before the CTA exits
-        if (PAIR) __nanosleep(200000);  // (their barrier is the even CTA's)
-        for (uint32_t i = slots > SLOTS ? slots - SLOTS : 0; !PAIR && i < slots; ++i) {
-            const unsigned long long t0 = globaltimer();
-            while (!mbar_try_wait(full0 + 8 * (i % SLOTS), (i / SLOTS) & 1) && globaltimer() - t0 < kWaitTimeoutNs) {
-            }
+    // Copies that were issued land before their CTA leaves, also where an error, of any thread, ended a phase before they were
+    // waited for.
+    const auto landed = [&](uint32_t i) {
+        const unsigned long long t0 = globaltimer();
+        while (!mbar_try_wait(full0 + 8 * (i % SLOTS), (i / SLOTS) & 1) && globaltimer() - t0 < kWaitTimeoutNs) {
         }
+    };
+    if (threadIdx.x == 0) {
+        *issued = slots;
+        for (uint32_t i = slots > SLOTS ? slots - SLOTS : 0; !PAIR && i < slots; ++i) landed(i);
     }
     if (warp == 1 && lane == 0 && rank == 0) {  // every MMA completes before TMEM is released
         if (PAIR) mma_commit_pair(drain);
@@ -662,7 +673,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (PAIR) cluster_sync_all();  // neither CTA leaves while the pair's MMAs or arrivals may still touch it
+    if (PAIR) {  // neither CTA leaves while the pair's MMAs, arrivals or copies may still touch it
+        cluster_sync_all();
+        if (rank == 0 && threadIdx.x == 0) {  // all copies are counted on this CTA's barriers, where both took part
+            const uint32_t other = load_cluster(map_to_rank(smem_u32(issued), 1)), most = other > slots ? other : slots;
+            for (uint32_t i = most > SLOTS ? most - SLOTS : 0; i < most; ++i) {
+                const uint32_t bar = full0 + 8 * (i % SLOTS);
+                if (i >= slots) mbar_expect_tx(bar, SLOT);        // the odd CTA's half alone
+                else if (i >= other) mbar_complete_tx(bar, SLOT);  // this CTA's half alone
+                landed(i);
+            }
+        }
+        cluster_sync_all();
+    }
     tc_fence_after();
     if (warp == 1) {
         if (PAIR) tmem_dealloc_pair(tmem, kTmemCols);

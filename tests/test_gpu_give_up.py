@@ -41,3 +41,24 @@ def test_a_sort_that_gives_up_leaves_the_gradient_alone(harness):
     assert err == 0
     assert status.tolist() == [4, 0] and words.tolist() == [1, 1]  # LAMQ_ERR_TIMEOUT; one arrival, given up
     assert torch.equal(dE, before)
+
+
+@pytest.mark.parametrize("m,n", [(2560, 2561), (2561, 2500), (300, 500)])
+def test_newton_schulz_ends_where_an_error_has_been_recorded(m, n):
+    """Every CTA gives up at its next wait, somewhere between the products; the call ends, and the next one is right."""
+    from lookatmyquant_b200 import _lib, orthogonal as N
+    lib = _lib.load()
+    G = torch.randn(m, n, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    want = N.newton_schulz(G)
+    ws = torch.empty(lib.lamq_newton_schulz_workspace_size(1, m, n), dtype=torch.uint8, device="cuda")
+    out, status = torch.empty_like(want), torch.full((1,), 4, dtype=torch.int32, device="cuda")
+    call = lambda: lib.lamq_newton_schulz(G.data_ptr(), 0, n, 0, 1, m, n, 5, N._coefficients(N.COEFFICIENTS, 5), 1e-7,
+                                          out.data_ptr(), ws.data_ptr(), ws.numel(), status.data_ptr(), _lib.stream_ptr())
+    for _ in range(3):
+        assert call() == _lib.LAMQ_OK
+    torch.cuda.synchronize()
+    assert status.item() == 4
+    status.zero_()
+    assert call() == _lib.LAMQ_OK
+    assert torch.equal(out, want) and status.item() == 0
+    N.check_status()

@@ -423,13 +423,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0 && n > 0) {  // ---- TMA producer
             bool ok = true;
             for (int i = EARLY; ok && i < 2 * n; ++i) ok = load_next(true);
-            if (!ok) {  // error path: let the copies in flight land before the CTA exits
-                wait_bounded(q_full, 0);
-                for (int i = max(0, k_issued - RING); i < k_issued; ++i)
-                    wait_bounded(k_full0 + 8 * (i % RING), (i / RING) & 1);
-                for (int i = max(0, v_issued - RING); i < v_issued; ++i)
-                    wait_bounded(v_full0 + 8 * (i % RING), (i / RING) & 1);
-            }
+            // the copies land before the CTA exits, also where another thread's error keeps anyone else from waiting for them
+            wait_bounded(q_full, 0);
+            for (int i = max(0, k_issued - RING); i < k_issued; ++i) wait_bounded(k_full0 + 8 * (i % RING), (i / RING) & 1);
+            for (int i = max(0, v_issued - RING); i < v_issued; ++i) wait_bounded(v_full0 + 8 * (i % RING), (i / RING) & 1);
         }
     } else if (warp == 1) {
         if (lane == 0 && n > 0) {  // ---- MMA issuer. P lies over S: P·V of a step goes before the buffer's next S
@@ -742,11 +739,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0 && n > 0) {
             bool ok = true;
             for (int j = VS; ok && j < n; ++j) ok = load(j, true);
-            if (!ok) {
-                wait_bounded(q_full, 0);
-                for (int i = max(0, k_issued - KS); i < k_issued; ++i) wait_bounded(k_full0 + 8 * (i % KS), (i / KS) & 1);
-                for (int i = max(0, v_issued - VS); i < v_issued; ++i) wait_bounded(v_full0 + 8 * (i % VS), (i / VS) & 1);
-            }
+            wait_bounded(q_full, 0);  // the copies land before the CTA exits
+            for (int i = max(0, k_issued - KS); i < k_issued; ++i) wait_bounded(k_full0 + 8 * (i % KS), (i / KS) & 1);
+            for (int i = max(0, v_issued - VS); i < v_issued; ++i) wait_bounded(v_full0 + 8 * (i % VS), (i / VS) & 1);
         }
     } else if (warp == 1) {
         if (lane == 0 && n > 0) {
@@ -1002,11 +997,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0 && n > 0) {
             bool ok = true;
             for (int j = GS; ok && j < n; ++j) ok = load(j, true);
-            if (!ok) {
-                wait_bounded(kv_full, 0);
-                for (int i = max(0, q_issued - QS); i < q_issued; ++i) wait_bounded(q_full0 + 8 * (i % QS), (i / QS) & 1);
-                for (int i = max(0, g_issued - GS); i < g_issued; ++i) wait_bounded(g_full0 + 8 * (i % GS), (i / GS) & 1);
-            }
+            wait_bounded(kv_full, 0);  // the copies land before the CTA exits
+            for (int i = max(0, q_issued - QS); i < q_issued; ++i) wait_bounded(q_full0 + 8 * (i % QS), (i / QS) & 1);
+            for (int i = max(0, g_issued - GS); i < g_issued; ++i) wait_bounded(g_full0 + 8 * (i % GS), (i / GS) & 1);
         }
     } else if (warp == 1) {
         if (lane == 0 && n > 0) {

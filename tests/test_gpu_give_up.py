@@ -62,3 +62,35 @@ def test_newton_schulz_ends_where_an_error_has_been_recorded(m, n):
     assert call() == _lib.LAMQ_OK
     assert torch.equal(out, want) and status.item() == 0
     N.check_status()
+
+
+@pytest.mark.parametrize("Lq,Lk,D", [(900, 900, 64), (900, 900, 128), (5, 2000, 128)])
+def test_attention_ends_where_an_error_has_been_recorded(Lq, Lk, D):
+    """Threads that wait long enough to look give up, wherever they are; the calls end, and the next ones are right."""
+    from lookatmyquant_b200 import _lib, attention as A
+    lib = _lib.load()
+    g = torch.Generator("cuda").manual_seed(3)
+    rand = lambda H, L: torch.randn(2, L, H, D, device="cuda", generator=g).bfloat16().transpose(1, 2)
+    q, k, v, do = rand(8, Lq), rand(2, Lk), rand(2, Lk), rand(8, Lq)
+    o, lse = A.forward(q, k, v)
+    want = (o, lse, *A.backward(do, q, k, v, o, lse))
+    got = [torch.empty_like(x) for x in want]
+    size = lib.lamq_attention_backward_workspace_size(2, 8, Lq)
+    ws, status = torch.empty(size, dtype=torch.uint8, device="cuda"), torch.full((1,), 4, dtype=torch.int32, device="cuda")
+    heads = lambda x: (x.data_ptr(), *x.stride()[:3])
+    args = _lib.ATTENTION_ARGS.pack(2, 8, 2, D, True, Lq, Lk, D**-0.5, 0, 0, 0, *heads(q), *heads(k), *heads(v), *heads(got[0]),
+                                    got[1].data_ptr(), *heads(do), *(y for x in got[2:] for y in heads(x)))
+
+    def calls():
+        assert lib.lamq_attention_forward(args, status.data_ptr(), _lib.stream_ptr()) == _lib.LAMQ_OK
+        assert lib.lamq_attention_backward(args, ws.data_ptr(), size, status.data_ptr(), _lib.stream_ptr()) == _lib.LAMQ_OK
+    for _ in range(3):
+        calls()
+    torch.cuda.synchronize()
+    assert status.item() == 4
+    status.zero_()
+    calls()
+    assert status.item() == 0
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    A.check_status()

@@ -184,9 +184,12 @@ class StatusWord:
         return word
 
     def check(self):
-        """Raises if a kernel of any call so far set a word, and clears it."""
-        for word in self.words.values():
+        """Raises if a kernel of any call so far, on whatever stream, set a word, and clears it."""
+        import torch
+        for device, word in self.words.items():
+            torch.cuda.synchronize(device)  # .item() would wait for the current stream alone
             st = int(word.item())
             if st:
                 word.zero_()
+                torch.cuda.synchronize(device)  # cleared before any stream's next kernel can set it
                 raise (ValueError if st == LAMQ_ERR_INVALID else LamqError)(f"{self.what} (status {st})")

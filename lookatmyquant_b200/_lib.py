@@ -172,21 +172,27 @@ class StatusWord:
     def __init__(self, what: str):
         self.what = what
         self.words = {}
+        self.lock = threading.Lock()
 
     def on(self, device):
+        """The device's word, made by the first call there (one word, whichever threads come first)."""
         word = self.words.get(device)
-        if word is None:
-            import torch
-            with torch.cuda.device(device):
-                word = torch.zeros(1, dtype=torch.int32, device=device)
-                torch.cuda.synchronize(device)  # zero before any stream's kernel can set it
-            self.words[device] = word
-        return word
+        return word if word is not None else self._make(device)
+
+    def _make(self, device):
+        import torch
+        with self.lock:
+            if device not in self.words:
+                with torch.cuda.device(device):
+                    word = torch.zeros(1, dtype=torch.int32, device=device)
+                    torch.cuda.synchronize(device)  # zero before any stream's kernel can set it
+                self.words[device] = word
+            return self.words[device]
 
     def check(self):
         """Raises if a kernel of any call so far, on whatever stream, set a word, and clears it."""
         import torch
-        for device, word in self.words.items():
+        for device, word in list(self.words.items()):
             torch.cuda.synchronize(device)  # .item() would wait for the current stream alone
             st = int(word.item())
             if st:

@@ -167,7 +167,8 @@ def launch_on(device):
 
 class StatusWord:
     """One device int per GPU that an operator's kernels set on an error (a status argument of the C ABI). Calls only
-    pass it on; `check` reads it, which waits for the device."""
+    pass it on; `check` reads it, which waits for the device. The first call on a device makes it, so that one cannot be
+    captured in a CUDA graph."""
 
     def __init__(self, what: str):
         self.what = what
@@ -183,6 +184,8 @@ class StatusWord:
         import torch
         with self.lock:
             if device not in self.words:
+                if torch.cuda.is_current_stream_capturing():  # memory of the graph's would be cleared by every replay
+                    raise LamqError("the first call of an operator on a device cannot be captured: make one before")
                 with torch.cuda.device(device):
                     word = torch.zeros(1, dtype=torch.int32, device=device)
                     torch.cuda.synchronize(device)  # zero before any stream's kernel can set it

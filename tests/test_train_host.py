@@ -4,6 +4,7 @@ import contextlib
 import threading
 import time
 
+import pytest
 import torch
 
 
@@ -17,6 +18,7 @@ def test_threads_share_one_status_word(monkeypatch):
         return zeros(*a, **kw)
     monkeypatch.setattr(torch, "zeros", slow_zeros)
     monkeypatch.setattr(torch.cuda, "device", contextlib.nullcontext)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: None)
     words, got = _lib.StatusWord("x"), []
     threads = [threading.Thread(target=lambda: got.append(words.on(torch.device("cuda", 0)))) for _ in range(4)]

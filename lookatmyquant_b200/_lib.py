@@ -170,8 +170,8 @@ class StatusWord:
     pass it on; `check` reads it, which waits for the device. The first call on a device makes it, so that one cannot be
     captured in a CUDA graph."""
 
-    def __init__(self, what: str):
-        self.what = what
+    def __init__(self, what: str, invalid: str | None = None):
+        self.what, self.invalid = what, invalid  # the operator; what LAMQ_ERR_INVALID says of its inputs
         self.words = {}
         self.lock = threading.Lock()
 
@@ -201,4 +201,7 @@ class StatusWord:
             if st:
                 word.zero_()
                 torch.cuda.synchronize(device)  # cleared before any stream's next kernel can set it
-                raise (ValueError if st == LAMQ_ERR_INVALID else LamqError)(f"{self.what} (status {st})")
+                if st == LAMQ_ERR_INVALID and self.invalid:
+                    raise ValueError(self.invalid)
+                raise LamqError(f"{self.what}: a kernel gave up on a device wait (status {st}): results since the last "
+                                "check may be invalid")

@@ -29,6 +29,9 @@
 namespace lamq {
 namespace {
 
+// The status word keeps the greatest code: a bad id (LAMQ_ERR_INVALID) does not hide a wait that gave up (LAMQ_ERR_TIMEOUT).
+static_assert(LAMQ_ERR_TIMEOUT > LAMQ_ERR_INVALID, "atomicMax keeps the graver error");
+
 // ---- element access: V values of T at p as fp32, V·sizeof(T) = 16 bytes where rows are 16-byte aligned, else V = 1
 
 template <typename T, int V>
@@ -115,7 +118,7 @@ __global__ void __launch_bounds__(kThreads)
     const int first = (int)(parts == 1 ? 0 : item - t * parts) * (32 * kLookupVecs) + lane;
     const int64_t id = id_at(ids, ids64, t);
     const bool valid = id >= 0 && id < rows, live = valid && id != padding;
-    if (!valid && first == 0) atomicCAS(status, 0, LAMQ_ERR_INVALID);
+    if (!valid && first == 0) atomicMax(status, LAMQ_ERR_INVALID);
     const T *src = table + (live ? id : 0) * ldt;
     T *dst = out + t * ldo;
     Pack<T, V> x[kLookupVecs];
@@ -231,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 4)
 #pragma unroll
     for (int q = 0; q < kRounds; ++q) {
         const bool in = t0 + 32 * q < p.n;
-        if (blockIdx.x == 0 && in && (my[q] < 0 || my[q] >= p.rows)) atomicCAS(p.status, 0, LAMQ_ERR_INVALID);
+        if (blockIdx.x == 0 && in && (my[q] < 0 || my[q] >= p.rows)) atomicMax(p.status, LAMQ_ERR_INVALID);
         mask[q] = __ballot_sync(0xffffffffu, in && my[q] >= r0 && my[q] < r0 + nrows && my[q] != p.padding);
         mine += __popc(mask[q]);
     }
@@ -364,7 +367,7 @@ __device__ __forceinline__ bool wait_all(unsigned *counter, unsigned target, int
             if ((it & 255u) == 0u) {
                 asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
                 if (t - t0 > kBarrierTimeoutNs) {
-                    atomicCAS(status, 0, LAMQ_ERR_TIMEOUT);
+                    atomicMax(status, LAMQ_ERR_TIMEOUT);
                     ok = 0;
                     break;
                 }
@@ -397,7 +400,7 @@ __device__ bool sort_tokens(const SortedParams &s, uint32_t (*seen)[kMaxBins], u
             const uint32_t key = key_at(s, pass, t);
             if (pass == 0 && key == (uint32_t)s.g.rows) {
                 const int64_t id = id_at(s.g.ids, s.g.ids64, t);
-                if (id < 0 || id >= s.g.rows) atomicCAS(s.g.status, 0, LAMQ_ERR_INVALID);
+                if (id < 0 || id >= s.g.rows) atomicMax(s.g.status, LAMQ_ERR_INVALID);
             }
             atomicAdd(&place[(key >> shift) & (bins - 1)], 1u);
         }

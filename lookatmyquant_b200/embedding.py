@@ -98,13 +98,14 @@ def quantize_embedding(E: torch.Tensor, spec: dict, H: torch.Tensor | None, orde
     return bits, E.numel()
 
 
-_STATUS = _lib.StatusWord("embedding ids outside the table")
+_STATUS = _lib.StatusWord("embedding", "embedding ids outside the table")
 _DTYPES = {torch.float32: _lib.LAMQ_F32, torch.bfloat16: _lib.LAMQ_BF16}
 
 
 def check_status():
-    """Raises ValueError if a lookup or gradient so far met an id outside its table (its row is taken as zero). Waits
-    for the device."""
+    """Raises ValueError if a lookup or gradient so far met an id outside its table (its row is taken as zero), and
+    LamqError if a kernel gave up on a device wait (then no sums were written; reported
+    before a bad id). Waits for the device."""
     _STATUS.check()
 
 

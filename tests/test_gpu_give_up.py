@@ -20,9 +20,10 @@ def harness(tmp_path_factory):
     return ctypes.CDLL(str(out))
 
 
-def test_a_sort_that_gives_up_leaves_the_gradient_alone(harness):
+@pytest.mark.parametrize("before_status", [0, 1])
+def test_a_sort_that_gives_up_leaves_the_gradient_alone(harness, before_status):
     """The kernels after the sort do not go by keys and positions that nobody wrote: the gradient that was to be added to
-    stays as it was. (Here they hold valid places, so that a kernel that did go by them would be seen in the result.)"""
+    stays as it was. (Here they hold valid places, so that a kernel that did go by them would be seen in the result.) The status says so, also where a bad id was met before."""
     n, rows, d = 3000, 100, 64
     g = torch.Generator("cuda").manual_seed(1)
     dy = torch.randn(n, d, device="cuda", generator=g)
@@ -34,6 +35,7 @@ def test_a_sort_that_gives_up_leaves_the_gradient_alone(harness):
     counts = torch.zeros(64 * 512, dtype=torch.int32, device="cuda")
     head, tail = torch.zeros(n, d, device="cuda"), torch.zeros(n, d, device="cuda")
     words, status = (torch.zeros(2, dtype=torch.int32, device="cuda") for _ in range(2))
+    status[0] = before_status
     torch.cuda.synchronize()
     p = lambda t: ctypes.c_void_p(t.data_ptr())
     err = harness.gradient_with_a_block_missing(p(dy), p(ids), ctypes.c_int64(n), ctypes.c_int64(rows), d, p(dE), p(keys),

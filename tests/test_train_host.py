@@ -27,3 +27,16 @@ def test_threads_share_one_status_word(monkeypatch):
     for t in threads:
         t.join()
     assert len(got) == 4 and all(w is words.on(torch.device("cuda", 0)) for w in got)
+
+
+def test_each_error_has_its_own_words(monkeypatch):
+    from lookatmyquant_b200 import _lib, embedding, orthogonal
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: None)
+    for words, code, error, text in ((embedding._STATUS, _lib.LAMQ_ERR_INVALID, ValueError, "outside the table"),
+                                     (embedding._STATUS, _lib.LAMQ_ERR_TIMEOUT, _lib.LamqError, "gave up on a device wait"),
+                                     (orthogonal._STATUS, _lib.LAMQ_ERR_TIMEOUT, _lib.LamqError, "newton_schulz.*gave up")):
+        monkeypatch.setattr(words, "words", {torch.device("cuda", 0): torch.tensor([code], dtype=torch.int32)})
+        with pytest.raises(error, match=text) as e:
+            words.check()
+        assert code != _lib.LAMQ_ERR_TIMEOUT or "outside" not in str(e.value)
+        words.check()

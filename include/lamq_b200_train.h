@@ -3,7 +3,8 @@
  * matrices runs: attention forwards and backwards, the scaled embedding lookup and its gradient, and the Newton-Schulz
  * orthogonalisation of an update. The conventions are lamq_b200.h's: plain device pointers and sizes, asynchronous on
  * the given stream, an int status, buffers and workspaces owned by the caller, nothing allocated by a call.
- * `status` arguments are a device int, 0 before the call, that a kernel sets to an error code.
+ * `status` arguments are a device int, 0 at first, that kernels raise to an error code (the greater where there are two).
+ * They do not read it: calls may share one, and an error that is still in it affects none of them.
  */
 #ifndef LAMQ_B200_TRAIN_H
 #define LAMQ_B200_TRAIN_H

@@ -47,6 +47,7 @@
 
 #include "../../include/lamq_b200_train.h"
 #include "attention_steps.cuh"
+#include "give_up.cuh"
 #include "lamq_common.cuh"
 #include "sm100.cuh"
 
@@ -390,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int &issued = is_k ? k_issued : v_issued;
         const int st = issued % RING;
         const uint32_t full = (is_k ? k_full0 : v_full0) + 8 * st;
-        if (wait && !mbar_wait((is_k ? k_empty0 : v_empty0) + 8 * st, ((issued / RING) & 1) ^ 1, s.status)) return false;
+        if (wait && !await((is_k ? k_empty0 : v_empty0) + 8 * st, ((issued / RING) & 1) ^ 1, s.status)) return false;
         mbar_expect_tx(full, Z::TILE);
         load_tile<HD>((is_k ? sk : sv) + st * Z::TILE, is_k ? &mapK : &mapV, (j0 + issued) * kTile, hk, b, full);
         ++issued;
@@ -433,9 +434,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t q_desc = rows_desc(sq), k_desc = rows_desc(sk), v_desc = cols_desc<HD>(sv);
             const int count = steps.count(), ends_first = steps.ends_first();
             Turn k, v, buf;
-            bool ok = mbar_wait(q_full, 0, s.status);
+            bool ok = await(q_full, 0, s.status);
             const auto issue_s = [&](int u, int to) {
-                if (steps.begins(u)) ok = mbar_wait(k_full0 + 8 * k.at, k.parity, s.status);
+                if (steps.begins(u)) ok = await(k_full0 + 8 * k.at, k.parity, s.status);
                 if (!ok) return;
                 mma_rows_rows<HD>(tmem + to * kTile, q_desc + steps.query_tile(u) * (Z::TILE >> 4),
                                   k_desc + k.at * (Z::TILE >> 4));
@@ -454,8 +455,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const auto run_to = [&](int end) {
                 for (; ok && u < end; ++u, buf.next<NB>()) {
                     const int t = steps.query_tile(u);
-                    ok = (!steps.begins(u) || mbar_wait(v_full0 + 8 * v.at, v.parity, s.status)) &&
-                         mbar_wait(p_ready0 + 8 * buf.at, buf.parity, s.status);
+                    ok = (!steps.begins(u) || await(v_full0 + 8 * v.at, v.parity, s.status)) &&
+                         await(p_ready0 + 8 * buf.at, buf.parity, s.status);
                     if (!ok) break;
                     tc_fence_after();
                     mma_tmem_rows<HD>(tmem + NB * kTile + t * HD, tmem + buf.at * kTile, 32, v_desc + v.at * (Z::TILE >> 4),
@@ -490,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float m = -INFINITY, sum = 0.f;  // m: the maximum that the exponentials are taken against
         bool ok = true;
         const auto wait_for = [&](Wait w) {
-            return __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * w.bar, w.phase & 1, s.status)) != 0;
+            return __all_sync(0xffffffffu, await(s_full0 + 8 * w.bar, w.phase & 1, s.status)) != 0;
         };
         for (int j = 0; j < nt; ++j) {
             const int u = steps.index(j, t), buf = u % NB;
@@ -508,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int c = 0; c < kTile; ++c)
                     if (c < clo || c >= chi) r[c >> 5][c & 31] = 0xff800000u;
                 if (from > j * kTile || to_all < (j + 1) * kTile) {  // (both tiles' warps do: the same zeros)
-                    ok = __all_sync(0xffffffffu, mbar_wait(v_full0 + 8 * (j % RING), (j / RING) & 1, s.status));
+                    ok = __all_sync(0xffffffffu, await(v_full0 + 8 * (j % RING), (j / RING) & 1, s.status));
                     if (!ok) break;
                     zero_rows<HD>(sv + (j % RING) * Z::TILE, from - j * kTile, to_all - j * kTile,
                                   threadIdx.x - 64 - 128 * t, 128);
@@ -572,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = wait_for(steps.last_read(steps.index(nt - 1, t)));
             tc_fence_after();
         }
-        if (split > 1 && n > 0) ok = ok && __all_sync(0xffffffffu, mbar_wait(drain, 0, s.status));  // the other tile's too
+        if (split > 1 && n > 0) ok = ok && __all_sync(0xffffffffu, await(drain, 0, s.status));  // the other tile's too
         if (ok && split > 1 && n_all > 0) {  // to the cluster: columns of 128 rows over the stages, which are done with
             row_max[t * kTile + 32 * quad + lane] = m;
             row_sum[t * kTile + 32 * quad + lane] = sum;
@@ -700,11 +701,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     int k_issued = 0, v_issued = 0;
     const auto load = [&](int j, bool wait) {
         const int ks = j % KS, vs = j % VS, row = (j0 + j) * kTile;
-        if (wait && !mbar_wait(k_empty0 + 8 * ks, ((j / KS) & 1) ^ 1, s.status)) return false;
+        if (wait && !await(k_empty0 + 8 * ks, ((j / KS) & 1) ^ 1, s.status)) return false;
         mbar_expect_tx(k_full0 + 8 * ks, Z::TILE);
         load_tile<HD>(sk + ks * Z::TILE, &mapK, row, hk, b, k_full0 + 8 * ks);
         ++k_issued;
-        if (wait && !mbar_wait(v_empty0 + 8 * vs, ((j / VS) & 1) ^ 1, s.status)) return false;
+        if (wait && !await(v_empty0 + 8 * vs, ((j / VS) & 1) ^ 1, s.status)) return false;
         mbar_expect_tx(v_full0 + 8 * vs, Z::TILE);
         load_tile<HD>(sv + vs * Z::TILE, &mapV, row, hk, b, v_full0 + 8 * vs);
         ++v_issued;
@@ -746,23 +747,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 1) {
         if (lane == 0 && n > 0) {
             const uint64_t k_desc = rows_desc(sk), v_desc = rows_desc(sv), kc_desc = cols_desc<HD>(sk);
-            bool ok = mbar_wait(q_ready, 0, s.status);
+            bool ok = await(q_ready, 0, s.status);
             // in issue order: S(0) dP(0) | S(j + 1) | dQ(j) dP(j + 1) | ...: while the warps form P(j), S(j + 1) runs; while
             // they go on to P(j + 1), dQ(j) and, over the dS(j) that it read, dP(j + 1) run
             for (int j = -1; ok && j < n; ++j) {
                 const int kn = (j + 1) % KS, vn = (j + 1) % VS;
                 if (j + 1 < n) {
-                    ok = mbar_wait(k_full0 + 8 * kn, ((j + 1) / KS) & 1, s.status) &&
-                         (j < 0 || mbar_wait(s_free, j & 1, s.status));
+                    ok = await(k_full0 + 8 * kn, ((j + 1) / KS) & 1, s.status) &&
+                         (j < 0 || await(s_free, j & 1, s.status));
                     if (!ok) break;
                     tc_fence_after();
                     mma_tmem_rows_t<HD>(tmem + kS, tmem + kQ, k_desc + kn * (Z::TILE >> 4));
                     mma_commit(s_full);
-                    ok = mbar_wait(v_full0 + 8 * vn, ((j + 1) / VS) & 1, s.status);
+                    ok = await(v_full0 + 8 * vn, ((j + 1) / VS) & 1, s.status);
                     if (!ok) break;
                 }
                 if (j >= 0) {
-                    ok = mbar_wait(ds_ready, j & 1, s.status);
+                    ok = await(ds_ready, j & 1, s.status);
                     if (!ok) break;
                     tc_fence_after();
                     mma_tmem_rows<HD>(tmem + kDQ, tmem + kP, 64, kc_desc + (j % KS) * (Z::TILE >> 4), j > 0);
@@ -784,7 +785,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool live = i < s.Lq;
         const int row_hi = s.causal ? min(hi, i + s.off + 1) : hi;
         const uint32_t lanes = (uint32_t)(32 * quad) << 16;
-        bool ok = n > 0 && __all_sync(0xffffffffu, mbar_wait(q_full, 0, s.status));
+        bool ok = n > 0 && __all_sync(0xffffffffu, await(q_full, 0, s.status));
         if (ok) {
             if (HD == 64) {
                 chunk_to_tmem(half ? sg : sq, 32 * quad + lane, tmem + lanes + (half ? kG : kQ));
@@ -821,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             Dr[(int64_t)bh * s.lq_pad + i] = -Di;
         }
         for (int j = 0; ok && j < n; ++j) {
-            ok = __all_sync(0xffffffffu, mbar_wait(s_full, j & 1, s.status));
+            ok = __all_sync(0xffffffffu, await(s_full, j & 1, s.status));
             if (!ok) break;
             tc_fence_after();
             uint32_t r[2][32], d[2][32];
@@ -838,7 +839,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float2 x = fma2(pair_of(at), make_float2(s.sl, s.sl), make_float2(-l2, -l2));
                 at[0] = __float_as_uint(ex2(x.x)), at[1] = __float_as_uint(ex2(x.y));
             }
-            ok = __all_sync(0xffffffffu, mbar_wait(p_full, j & 1, s.status));
+            ok = __all_sync(0xffffffffu, await(p_full, j & 1, s.status));
             if (!ok) break;
             tc_fence_after();
             tmem_load32(tmem + lanes + kP + 64 * half, d[0]);
@@ -866,7 +867,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             warp_arrive(ds_ready);
         }
         if (ok) {
-            ok = __all_sync(0xffffffffu, mbar_wait(done, 0, s.status));
+            ok = __all_sync(0xffffffffu, await(done, 0, s.status));
             tc_fence_after();
         }
         if (split > 1 && n_all > 0) {  // to the cluster: columns of 128 rows over the stages, which are done with
@@ -955,12 +956,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const auto load = [&](int j, bool wait) {
         const int qs = j % QS, gs = j % GS;
         const int64_t at = ((int64_t)b * s.Hq + h) * s.lq_pad + row;
-        if (wait && !mbar_wait(q_empty0 + 8 * qs, ((j / QS) & 1) ^ 1, s.status)) return false;
+        if (wait && !await(q_empty0 + 8 * qs, ((j / QS) & 1) ^ 1, s.status)) return false;
         mbar_expect_tx(q_full0 + 8 * qs, Z::TILE + Z::ROW);
         load_tile<HD>(sq + qs * Z::TILE, &mapQ, row, h, b, q_full0 + 8 * qs);
         bulk_load(smem_u32(row_lse + qs * kTile), lse2 + at, Z::ROW, q_full0 + 8 * qs);
         ++q_issued;
-        if (wait && !mbar_wait(g_empty0 + 8 * gs, ((j / GS) & 1) ^ 1, s.status)) return false;
+        if (wait && !await(g_empty0 + 8 * gs, ((j / GS) & 1) ^ 1, s.status)) return false;
         mbar_expect_tx(g_full0 + 8 * gs, Z::TILE + Z::ROW);
         load_tile<HD>(sg + gs * Z::TILE, &mapG, row, h, b, g_full0 + 8 * gs);
         bulk_load(smem_u32(row_d + gs * kTile), Dr + at, Z::ROW, g_full0 + 8 * gs);
@@ -1005,14 +1006,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0 && n > 0) {
             const uint64_t k_desc = rows_desc(sk), v_desc = rows_desc(sv), q_desc = rows_desc(sq), g_desc = rows_desc(sg),
                            qc_desc = cols_desc<HD>(sq), gc_desc = cols_desc<HD>(sg);
-            bool ok = mbar_wait(kv_full, 0, s.status);
+            bool ok = await(kv_full, 0, s.status);
             // in issue order: S(0) dP(0) | dV(j) S(j + 1) | dK(j) dP(j + 1) | ...: the warps form P(j) while dK(j − 1)
             // and dP(j) run, and dS(j) while dV(j) and S(j + 1) run
             for (int j = -1; ok && j < n; ++j) {
                 const int qs = j % QS, gs = j % GS, qn = (j + 1) % QS, gn = (j + 1) % GS;
-                if (j + 1 < n) ok = mbar_wait(q_full0 + 8 * qn, ((j + 1) / QS) & 1, s.status);
+                if (j + 1 < n) ok = await(q_full0 + 8 * qn, ((j + 1) / QS) & 1, s.status);
                 if (j >= 0) {
-                    ok = ok && mbar_wait(p_ready, j & 1, s.status);
+                    ok = ok && await(p_ready, j & 1, s.status);
                     if (!ok) break;
                     tc_fence_after();
                     mma_tmem_rows<HD>(tmem + kDV, tmem + kS, 64, gc_desc + gs * (Z::TILE >> 4), j > 0);
@@ -1021,10 +1022,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!ok) break;
                     mma_rows_rows<HD>(tmem + kS, k_desc, q_desc + qn * (Z::TILE >> 4));
                     mma_commit(s_full);
-                    ok = mbar_wait(g_full0 + 8 * gn, ((j + 1) / GS) & 1, s.status);
+                    ok = await(g_full0 + 8 * gn, ((j + 1) / GS) & 1, s.status);
                 }
                 if (j >= 0) {
-                    ok = ok && mbar_wait(ds_ready, j & 1, s.status);
+                    ok = ok && await(ds_ready, j & 1, s.status);
                     if (!ok) break;
                     tc_fence_after();
                     mma_commit(g_empty0 + 8 * gs);  // D(j) was read before ds_ready, dO(j) by dV(j)
@@ -1055,8 +1056,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool edge = edge_keys || (s.causal && key0 + kTile - 1 > row0 + s.off);
             const int clo = !in ? 64 : s.causal ? key - s.off - row0 - 64 * half : 0;  // columns before are masked
             // the tile's statistics came with Q and dO: their barriers make them visible to this thread
-            ok = __all_sync(0xffffffffu, mbar_wait(s_full, j & 1, s.status) &&
-                                             mbar_wait(q_full0 + 8 * qs, (j / QS) & 1, s.status));
+            ok = __all_sync(0xffffffffu, await(s_full, j & 1, s.status) &&
+                                             await(q_full0 + 8 * qs, (j / QS) & 1, s.status));
             if (!ok) break;
             tc_fence_after();
             uint32_t r[2][32], pk[32];
@@ -1087,7 +1088,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 0; c < 64; c += 2)
                 pk[c >> 1] = pack_bf16(__uint_as_float(r[c >> 5][c & 31]), __uint_as_float(r[c >> 5][(c & 31) + 1]));
             if (row0 < q_lo) {  // dV sums over dO's rows, dK over Q's: those of queries without a key
-                ok = __all_sync(0xffffffffu, mbar_wait(g_full0 + 8 * gs, (j / GS) & 1, s.status));
+                ok = __all_sync(0xffffffffu, await(g_full0 + 8 * gs, (j / GS) & 1, s.status));
                 if (!ok) break;
                 zero_rows<HD>(sg + gs * Z::TILE, q_lo - row0, kTile, threadIdx.x - 64, 256);
                 zero_rows<HD>(sq + qs * Z::TILE, q_lo - row0, kTile, threadIdx.x - 64, 256);
@@ -1096,8 +1097,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_st_wait();
             warp_arrive(p_ready);
 
-            ok = __all_sync(0xffffffffu, mbar_wait(p_full, j & 1, s.status) &&
-                                             mbar_wait(g_full0 + 8 * gs, (j / GS) & 1, s.status));
+            ok = __all_sync(0xffffffffu, await(p_full, j & 1, s.status) &&
+                                             await(g_full0 + 8 * gs, (j / GS) & 1, s.status));
             if (!ok) break;
             tc_fence_after();
             uint32_t d[2][32];
@@ -1129,7 +1130,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const bool live = key < s.Lk;
         if (ok && n > 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait(done, 0, s.status));
+            ok = __all_sync(0xffffffffu, await(done, 0, s.status));
             tc_fence_after();
         }
         if (ok) {  // columns half·HD/2 .. of the thread's key

@@ -35,6 +35,7 @@
 #include <cuda_fp16.h>
 
 #include "../../include/lamq_b200_train.h"
+#include "give_up.cuh"
 #include "lamq_common.cuh"
 #include "sm100.cuh"
 
@@ -157,8 +158,8 @@ __device__ __forceinline__ void tile_of(const Params &p, const Phase &f, int u, 
     ti = t;
 }
 
-// Every CTA has finished the phase and what it wrote is visible to all, to TMA too. Bounded: false when it gives up or
-// an error has been recorded.
+// Every CTA has finished the phase and what it wrote is visible to all, to TMA too. Bounded: false when it or
+// another wait of the launch gives up.
 __device__ __forceinline__ bool grid_barrier(const Params &p, unsigned target, int *shared_ok) {
     asm volatile("fence.proxy.async.global;" ::: "memory");  // this thread's writes before other SMs' TMA reads
     __syncthreads();
@@ -170,10 +171,10 @@ __device__ __forceinline__ bool grid_barrier(const Params &p, unsigned target, i
             unsigned v;
             asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p.barrier) : "memory");
             if (v >= target) break;
-            if ((it & 255u) == 0u) {
-                if (*reinterpret_cast<volatile int *>(p.status) != 0) ok = 0;
-                else if (globaltimer() - t0 > kWaitTimeoutNs) {
-                    atomicCAS(p.status, 0, LAMQ_ERR_TIMEOUT);
+            if (it % LAMQ_GIVE_UP_POLLS == 0u) {
+                if (launch_gave_up()) ok = 0;
+                else if (globaltimer() - t0 > LAMQ_GIVE_UP_NS) {
+                    give_up(p.status);
                     ok = 0;
                 }
                 if (!ok) break;
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int kb = k0; ok && kb < k1; ++kb)
                         for (int q = 0; q < parts; ++q, ++slots) {
                             const uint32_t st = slots % SLOTS;
-                            ok = mbar_wait(empty0 + 8 * st, ((slots / SLOTS) & 1) ^ 1, p.status);
+                            ok = await(empty0 + 8 * st, ((slots / SLOTS) & 1) ^ 1, p.status);
                             if (!ok) break;
                             const uint32_t sa = ring + st * SLOT, sb = sa + A_BYTES, bar = full0 + 8 * st;
                             const int k = kb * BK, ra = ti * Z::ROWS + 128 * rank, rb = tj * BN + 128 * rank;
@@ -471,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t a_lbo = f.a_mn ? BOX : 16, b_lbo = f.b_mn ? BOX : 16;
                 for (int u = worker; ok && u < units; u += workers, ++accs) {
                     const int acc = accs & 1;
-                    ok = mbar_wait(tempty0 + 8 * acc, ((accs >> 1) & 1) ^ 1, p.status);
+                    ok = await(tempty0 + 8 * acc, ((accs >> 1) & 1) ^ 1, p.status);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t d = tmem + acc * BN;
@@ -481,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         uint64_t da[2], db[2];
                         for (int q = 0; q < parts; ++q) {
                             const uint32_t st = (slots + q) % SLOTS;
-                            ok = ok && mbar_wait(full0 + 8 * st, ((slots + q) / SLOTS) & 1, p.status);
+                            ok = ok && await(full0 + 8 * st, ((slots + q) / SLOTS) & 1, p.status);
                             da[q] = smem_desc_sw128(ring + st * SLOT, a_lbo, 1024);
                             db[q] = smem_desc_sw128(ring + st * SLOT + A_BYTES, b_lbo, 1024);
                         }
@@ -536,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     load_block(old[0] + at0, ld, rows, early_h);
                     load_block(old[1] + at0, ld, rows, early_l);
                 }
-                ok = __all_sync(0xffffffffu, mbar_wait(tfull0 + 8 * acc, (accs >> 1) & 1, p.status));
+                ok = __all_sync(0xffffffffu, await(tfull0 + 8 * acc, (accs >> 1) & 1, p.status));
                 if (!ok) break;
                 tc_fence_after();
                 // (j, i) lies in no computed tile (EPI columns share a row tile, a warp's rows a column tile)

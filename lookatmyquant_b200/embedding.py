@@ -147,7 +147,7 @@ def _padding(padding_idx: int | None, rows: int) -> int:
 
 def lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None) -> torch.Tensor:
     """scale · table[ids] (ids of any shape; table V x d fp32 or bf16; the result in the table's type, the product in
-    fp32). Tokens with id `padding_idx` get zero rows. An id outside the table gets a zero row and is reported by
+    fp32). Tokens with id `padding_idx` get zero rows, whatever the table holds there. An id outside the table gets a zero row and is reported by
     `check_status()`."""
     if table.ndim != 2:
         raise ValueError("the table must be a matrix")
@@ -200,9 +200,10 @@ def lookup_gradient(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: flo
 class _ScaledEmbedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, ids, scale, padding_idx):
+        _padding(padding_idx, table.shape[0])
         ctx.save_for_backward(ids)
         ctx.rows, ctx.scale, ctx.padding_idx = table.shape[0], scale, padding_idx
-        return lookup(table, ids, scale, padding_idx)
+        return lookup(table, ids, scale)  # the padding token's row as it is stored; its gradient is what stays zero
 
     @staticmethod
     def backward(ctx, grad):
@@ -211,5 +212,6 @@ class _ScaledEmbedding(torch.autograd.Function):
 
 
 def scaled_embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None):
-    """`lookup` under autograd: the table's gradient is `lookup_gradient`."""
+    """scale · table[ids] under autograd, as torch's embedding: tokens with id `padding_idx` get the stored row (not
+    `lookup`'s zeros) and add nothing to the table's gradient, which is `lookup_gradient`."""
     return _ScaledEmbedding.apply(table, ids, float(scale), padding_idx)

@@ -138,11 +138,12 @@ def _ids(ids: torch.Tensor, device) -> torch.Tensor:
 
 
 def _padding(padding_idx: int | None, rows: int) -> int:
+    """The row, or -1 for none; negative indices count from the table's end, as in torch."""
     if padding_idx is None:
         return -1
-    if not 0 <= padding_idx < rows:
+    if not -rows <= padding_idx < rows:
         raise ValueError(f"padding_idx {padding_idx} outside the table's {rows} rows")
-    return padding_idx
+    return padding_idx % rows
 
 
 def lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None) -> torch.Tensor:

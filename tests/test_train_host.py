@@ -40,3 +40,11 @@ def test_each_error_has_its_own_words(monkeypatch):
             words.check()
         assert code != _lib.LAMQ_ERR_TIMEOUT or "outside" not in str(e.value)
         words.check()
+
+
+def test_negative_padding_indices_count_from_the_end():
+    from lookatmyquant_b200 import embedding
+    assert [embedding._padding(p, 40) for p in (None, 0, 39, -1, -40)] == [-1, 0, 39, 39, 0]
+    for p, rows in ((40, 40), (-41, 40), (0, 0), (-1, 0)):
+        with pytest.raises(ValueError):
+            embedding._padding(p, rows)

@@ -127,6 +127,7 @@ class _Attention(torch.autograd.Function):
         return o
 
     @staticmethod
+    @torch.autograd.function.once_differentiable  # the kernels leave no graph behind: a second derivative is an error
     def backward(ctx, do):
         q, k, v, o, lse, start, end = ctx.saved_tensors
         return (*backward(do, q, k, v, o, lse, ctx.scale, ctx.causal, start, end), None, None, None, None)
@@ -134,7 +135,7 @@ class _Attention(torch.autograd.Function):
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None, causal: bool = True,
               key_start: torch.Tensor | None = None, key_end: torch.Tensor | None = None) -> torch.Tensor:
-    """`forward`'s output under autograd: its gradients are `backward`'s."""
+    """`forward`'s output under autograd: its gradients are `backward`'s (once: differentiating them raises)."""
     return _Attention.apply(q, k, v, scale, causal, key_start, key_end)
 
 

@@ -48,3 +48,21 @@ def test_negative_padding_indices_count_from_the_end():
     for p, rows in ((40, 40), (-41, 40), (0, 0), (-1, 0)):
         with pytest.raises(ValueError):
             embedding._padding(p, rows)
+
+
+def stand_ins_for_attention(monkeypatch):
+    from lookatmyquant_b200 import attention as A
+    monkeypatch.setattr(A, "forward", lambda q, k, v, *a: (q * k * v, q.detach().sum(-1)))
+    monkeypatch.setattr(A, "backward", lambda do, q, k, v, *a: (do * k * v, do * q * v, do * q * k))
+    return A
+
+
+def test_second_derivatives_of_attention_raise(monkeypatch):
+    """Gradients come from kernels that autograd does not see; what is differentiated through them must not take them for
+    constants."""
+    A = stand_ins_for_attention(monkeypatch)
+    q, k, v = (torch.randn(1, 2, 3, 8).requires_grad_(True) for _ in range(3))
+    first = torch.autograd.grad(A.attention(q, k, v).sum(), (q, k, v), create_graph=True)
+    assert torch.equal(first[0], k * v)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        torch.autograd.grad(first[0].square().sum() + q.sum(), q)

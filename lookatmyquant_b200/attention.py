@@ -127,10 +127,25 @@ class _Attention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable  # the kernels leave no graph behind: a second derivative is an error
     def backward(ctx, do):
         q, k, v, o, lse, start, end = ctx.saved_tensors
-        return (*backward(do, q, k, v, o, lse, ctx.scale, ctx.causal, start, end), None, None, None, None)
+        grads = backward(do, q, k, v, o, lse, ctx.scale, ctx.causal, start, end)
+        if torch.is_grad_enabled():  # create_graph
+            grads = _Once.apply(do, q, k, v, *grads)
+        return (*grads, None, None, None, None)
+
+
+class _Once(torch.autograd.Function):
+    """The gradients, which come from kernels that leave no graph behind, made to depend on what they were computed from:
+    differentiating them raises. (torch's once_differentiable lets them pass for constants where `do` is one.)"""
+
+    @staticmethod
+    def forward(ctx, do, q, k, v, *grads):
+        return tuple(g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the lamq attention has no second derivatives")
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None, causal: bool = True,

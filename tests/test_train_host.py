@@ -64,5 +64,11 @@ def test_second_derivatives_of_attention_raise(monkeypatch):
     q, k, v = (torch.randn(1, 2, 3, 8).requires_grad_(True) for _ in range(3))
     first = torch.autograd.grad(A.attention(q, k, v).sum(), (q, k, v), create_graph=True)
     assert torch.equal(first[0], k * v)
-    with pytest.raises(RuntimeError, match="once_differentiable"):
+    with pytest.raises(RuntimeError, match="no second derivatives"):
         torch.autograd.grad(first[0].square().sum() + q.sum(), q)
+    c = torch.randn(1, 2, 3, 8).requires_grad_(True)
+    first = torch.autograd.grad((A.attention(q, k, v) * c).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivatives"):
+        torch.autograd.grad(first[0].sum(), c)
+    A.attention(q, k, v).sum().backward()  # a first derivative alone is none of its business
+    assert torch.equal(q.grad, k * v) and not q.grad.requires_grad

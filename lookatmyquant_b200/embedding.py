@@ -200,19 +200,35 @@ def lookup_gradient(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: flo
 
 class _ScaledEmbedding(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, table, ids, scale, padding_idx):
+    def forward(ctx, table, ids, scale, padding_idx, zeros):
         _padding(padding_idx, table.shape[0])
         ctx.save_for_backward(ids)
         ctx.rows, ctx.scale, ctx.padding_idx = table.shape[0], scale, padding_idx
-        return lookup(table, ids, scale)  # the padding token's row as it is stored; its gradient is what stays zero
+        # without `zeros` the padding token's row as it is stored; its gradient stays zero in both
+        return lookup(table, ids, scale, padding_idx if zeros else None)
 
     @staticmethod
     def backward(ctx, grad):
         (ids,) = ctx.saved_tensors
-        return lookup_gradient(grad, ids, ctx.rows, ctx.scale, ctx.padding_idx), None, None, None
+        return _ScaledGradient.apply(grad, ids, ctx.rows, ctx.scale, ctx.padding_idx), None, None, None, None
+
+
+class _ScaledGradient(torch.autograd.Function):
+    """`lookup_gradient`, linear in its rows: its own gradient is a lookup, with zeros for the tokens that add nothing."""
+
+    @staticmethod
+    def forward(ctx, grad, ids, rows, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.scale, ctx.padding_idx = scale, padding_idx
+        return lookup_gradient(grad, ids, rows, scale, padding_idx)
+
+    @staticmethod
+    def backward(ctx, grad):
+        (ids,) = ctx.saved_tensors
+        return _ScaledEmbedding.apply(grad, ids, ctx.scale, ctx.padding_idx, True), None, None, None, None
 
 
 def scaled_embedding(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None):
     """scale · table[ids] under autograd, as torch's embedding: tokens with id `padding_idx` get the stored row (not
     `lookup`'s zeros) and add nothing to the table's gradient, which is `lookup_gradient`."""
-    return _ScaledEmbedding.apply(table, ids, float(scale), padding_idx)
+    return _ScaledEmbedding.apply(table, ids, float(scale), padding_idx, False)

@@ -28,3 +28,25 @@ def test_padding_is_torchs(padding):
     with pytest.raises(ValueError):
         E.scaled_embedding(mine, ids, 4.0, -41)
     E.check_status()
+
+
+@pytest.mark.parametrize("padding", [None, 3])
+def test_second_derivatives_are_torchs(padding):
+    """A penalty on the first gradients, differentiated again (and a third time through the lookup of the second), against
+    torch's embedding in 64 bits: every value passes a dozen fp32 operations on numbers of like magnitude."""
+    from lookatmyquant_b200 import embedding as E
+    g = torch.Generator("cuda").manual_seed(2)
+    t = torch.randn(12, 8, device="cuda", generator=g)
+    ids = torch.randint(0, 12, (40,), device="cuda", generator=g)
+    got = {}
+    for name, table in (("mine", t.clone()), ("torch", t.double())):
+        table.requires_grad_(True)
+        look = (lambda: E.scaled_embedding(table, ids, 0.5, padding)) if name == "mine" else (
+            lambda: torch.nn.functional.embedding(ids, table, padding_idx=padding) * 0.5)
+        first, = torch.autograd.grad(look().pow(4).sum(), table, create_graph=True)
+        second, = torch.autograd.grad(first.square().sum() + look().square().sum(), table, create_graph=True)
+        third, = torch.autograd.grad(second.square().sum(), table)
+        got[name] = first, second, third
+    for a, b in zip(got["mine"], got["torch"]):
+        assert float((a.detach().double() - b.detach()).norm()) <= 1e-4 * float(b.detach().norm())
+        assert padding is None or float(a[padding].abs().sum()) == 0

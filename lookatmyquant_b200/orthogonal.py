@@ -82,6 +82,15 @@ class Muon(torch.optim.Optimizer):
             if any(p.ndim < 2 for p in group["params"]):
                 raise ValueError("Muon updates matrices: leave vectors to another optimiser")
 
+    def load_state_dict(self, state_dict):
+        """As every optimiser's, with the momentum kept in fp32 (torch casts state to the parameters' type)."""
+        super().load_state_dict(state_dict)
+        saved = (key for group in state_dict["param_groups"] for key in group["params"])
+        for key, p in zip(saved, (p for group in self.param_groups for p in group["params"])):
+            momentum = state_dict["state"].get(key, {}).get("momentum")
+            if momentum is not None:
+                self.state[p]["momentum"] = momentum.detach().to(p.device, torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None

@@ -72,3 +72,43 @@ def test_second_derivatives_of_attention_raise(monkeypatch):
         torch.autograd.grad(first[0].sum(), c)
     A.attention(q, k, v).sum().backward()  # a first derivative alone is none of its business
     assert torch.equal(q.grad, k * v) and not q.grad.requires_grad
+
+
+def muon_run(monkeypatch, dtype, reload):
+    """Six Muon steps on two matrices, through a state dict after three of them: parameters and momenta."""
+    from lookatmyquant_b200 import orthogonal as N
+    monkeypatch.setattr(N, "newton_schulz", lambda G, steps, coefficients: (G / G.norm()).bfloat16())
+    g = torch.Generator().manual_seed(1)
+    params = [torch.nn.Parameter(torch.randn(*s, generator=g).to(dtype)) for s in ((8, 5), (3, 7))]
+    opt = N.Muon(params, lr=0.1, weight_decay=0.01)
+    for step in range(6):
+        if step == 3 and reload:
+            state = opt.state_dict()
+            params = [torch.nn.Parameter(p.detach().clone()) for p in params]
+            opt = N.Muon(params, lr=0.5)
+            opt.load_state_dict(state)
+        for p in params:
+            p.grad = torch.randn(p.shape, generator=g).to(dtype)
+        opt.step()
+    return [p.detach() for p in params] + [opt.state[p]["momentum"] for p in params]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_muon_goes_on_from_a_state_dict_as_if_nothing_had_been(monkeypatch, dtype):
+    want, got = muon_run(monkeypatch, dtype, False), muon_run(monkeypatch, dtype, True)
+    for a, b in zip(got, want):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+    assert got[2].dtype == got[3].dtype == torch.float32
+
+
+def test_muon_shares_no_buffer_with_the_state_dict_it_loaded(monkeypatch):
+    from lookatmyquant_b200 import orthogonal as N
+    monkeypatch.setattr(N, "newton_schulz", lambda G, steps, coefficients: G.bfloat16())
+    p = torch.nn.Parameter(torch.ones(2, 2))
+    first, second = N.Muon([p]), N.Muon([p])
+    p.grad = torch.ones(2, 2)
+    first.step()
+    second.load_state_dict(first.state_dict())
+    second.step()
+    assert torch.equal(first.state[p]["momentum"], torch.ones(2, 2))
+    assert torch.equal(second.state[p]["momentum"], torch.full((2, 2), 1.95))

@@ -106,8 +106,10 @@ class Muon(torch.optim.Optimizer):
             for params in shapes.values():
                 us = []
                 for p in params:
-                    b = self.state[p].setdefault("momentum", torch.zeros_like(p, dtype=torch.float32))
-                    g = p.grad.float()
+                    state = self.state[p]
+                    if "momentum" not in state:
+                        state["momentum"] = torch.zeros_like(p, dtype=torch.float32)
+                    b, g = state["momentum"], p.grad.float()
                     b.mul_(mu).add_(g)
                     us.append(torch.add(g, b, alpha=mu) if group["nesterov"] else b)
                 O = newton_schulz(us[0] if len(us) == 1 else torch.stack(us), group["steps"], group["coefficients"])

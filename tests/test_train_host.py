@@ -112,3 +112,17 @@ def test_muon_shares_no_buffer_with_the_state_dict_it_loaded(monkeypatch):
     second.step()
     assert torch.equal(first.state[p]["momentum"], torch.ones(2, 2))
     assert torch.equal(second.state[p]["momentum"], torch.full((2, 2), 1.95))
+
+
+def test_muon_makes_a_momentum_once(monkeypatch):
+    from lookatmyquant_b200 import orthogonal as N
+    monkeypatch.setattr(N, "newton_schulz", lambda G, steps, coefficients: G.bfloat16())
+    made, zeros_like = [], torch.zeros_like
+    monkeypatch.setattr(torch, "zeros_like", lambda *a, **kw: made.append(1) or zeros_like(*a, **kw))
+    params = [torch.nn.Parameter(torch.ones(2, 3)) for _ in range(3)]
+    opt = N.Muon(params)
+    for _ in range(4):
+        for p in params:
+            p.grad = torch.ones(2, 3)
+        opt.step()
+    assert len(made) == 3

@@ -40,7 +40,8 @@ def _heads(x: torch.Tensor, what: str):
         n, m, k, d = x.shape  # the stride of an axis of one entry does not matter
         if d and ((one != 1 and d > 1) or p & 15 or (n > 1 and (b & 7 or b <= 0)) or (m > 1 and (h & 7 or h <= 0)) or
                   (k > 1 and (r & 7 or r <= 0))):
-            x = x.contiguous()
+            y = x.contiguous()
+            x = y if y.data_ptr() & 15 == 0 else y.clone()  # a contiguous tensor may start between two 16-byte pieces
             b, h, r, one = x.stride()
             p = x.data_ptr()
     return x, (p, b, h, r)

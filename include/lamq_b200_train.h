@@ -53,7 +53,8 @@ typedef struct lamq_heads {
  * from 0, to kv_len) and, with causal != 0, j <= i + kv_len − q_len (the last query sees the last key). head_dim is a
  * multiple of 8 up to 128; lengths are arbitrary, zero included. q, k, v: read. o and lse (batch x heads x q_len fp32,
  * contiguous): written by the forward, read by the backward. d_o is read and dq, dk, dv are written by the backward
- * only. Outputs are written whole and overlap no input. 328 bytes, no padding (`reserved` is ignored).
+ * only. Outputs are written whole (with no query heads at all nothing is: the call is a no-op) and overlap no input.
+ * 328 bytes, no padding (`reserved` is ignored).
  */
 typedef struct lamq_attention_args {
     int64_t batch;

@@ -27,3 +27,13 @@ def test_attention_takes_contiguous_tensors_that_start_anywhere():
     o, lse = A.forward(q, k, v)
     for a, b in zip((o, lse, *A.backward(do, q, k, v, moved(o.contiguous()), lse)), want):
         assert torch.equal(a, b)
+
+
+def test_keys_without_query_heads_get_zero_gradients():
+    from lookatmyquant_b200 import attention as A
+    q, k = torch.zeros(1, 0, 5, 64, device="cuda").bfloat16(), torch.randn(1, 2, 9, 64, device="cuda").bfloat16()
+    for _ in range(3):
+        torch.full((1 << 16,), math.nan, device="cuda")  # what the allocator hands out next holds no zeros
+        dq, dk, dv = A.backward(q, q, k, k, *A.forward(q, k, k))
+        assert dq.shape == q.shape and dk.shape == dv.shape == k.shape
+        assert float(dk.abs().sum()) == float(dv.abs().sum()) == 0

@@ -175,7 +175,7 @@ def lookup_gradient(grad: torch.Tensor, ids: torch.Tensor, rows: int, scale: flo
     if rows < 0:
         raise ValueError("rows must not be negative")
     d = grad.shape[-1]
-    grad, ld, code = _matrix(grad if grad.ndim == 2 else grad.reshape(-1, d), "the gradient")
+    grad, ld, code = _matrix(grad if grad.ndim == 2 else grad.reshape(ids.numel(), d), "the gradient")
     dev = grad.device
     ids = _ids(ids, dev)
     accumulate = out is not None

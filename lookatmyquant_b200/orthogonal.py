@@ -10,6 +10,7 @@ polynomial iterated in the matrix, products only. All iterations run in one kern
 from __future__ import annotations
 
 import functools
+import math
 import struct
 
 import torch
@@ -50,7 +51,7 @@ def newton_schulz(G: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS, ep
     coef = _coefficients(coefficients, steps) if steps > 0 else b""
     m, n = G.shape[-2:]
     dev = G.device
-    X = G if G.ndim <= 3 else G.reshape(-1, m, n)
+    X = G if G.ndim <= 3 else G.reshape(math.prod(G.shape[:-2]), m, n)
     batch = X.shape[0] if X.ndim == 3 else 1
     if X.numel() and (X.stride(-1) != 1 or (m > 1 and X.stride(-2) < n) or
                       (batch > 1 and X.stride(0) < (m - 1) * X.stride(-2) + n)):

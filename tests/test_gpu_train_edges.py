@@ -37,3 +37,14 @@ def test_keys_without_query_heads_get_zero_gradients():
         dq, dk, dv = A.backward(q, q, k, k, *A.forward(q, k, k))
         assert dq.shape == q.shape and dk.shape == dv.shape == k.shape
         assert float(dk.abs().sum()) == float(dv.abs().sum()) == 0
+
+
+def test_empty_shapes_of_any_rank():
+    """Shapes with an axis of none come back as they are: no axis's length is to be guessed from no elements."""
+    from lookatmyquant_b200 import embedding as E, orthogonal as N
+    for shape in ((2, 3, 0, 4), (2, 3, 4, 0), (2, 0, 3, 4), (0, 2, 0, 0)):
+        assert N.newton_schulz(torch.zeros(shape, device="cuda")).shape == shape
+    ids = torch.zeros(2, 3, dtype=torch.long, device="cuda")
+    assert E.lookup(torch.zeros(5, 0, device="cuda"), ids).shape == (2, 3, 0)
+    assert E.lookup_gradient(torch.zeros(2, 3, 0, device="cuda"), ids, 5).shape == (5, 0)
+    assert E.lookup_gradient(torch.zeros(2, 0, 4, device="cuda"), ids[:, :0], 5).shape == (5, 4)

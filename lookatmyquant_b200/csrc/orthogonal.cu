@@ -397,14 +397,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         double acc = 0.0;
         for (int i = threadIdx.x; i < p.parts; i += kThreads)
             acc += *reinterpret_cast<volatile double *>(p.partial + (int64_t)z * p.parts + i);
-        const float inv = (float)((double)kScale / (sqrt(block_sum(acc, red)) + (double)p.eps));
+        const double norm = sqrt(block_sum(acc, red)) + (double)p.eps;
+        // in two factors where a tiny matrix's one is past fp32; a zero matrix without an eps stays zero
+        const double factor = norm == 0.0 ? 0.0 : (double)kScale / norm;
+        const float lift = factor > 1e38 ? 0x1p64f : 1.f, inv = (float)(factor / (double)lift);
         const uint32_t g1 = (uint32_t)((uint64_t)groups * (part + 1) / p.parts);
         for (uint32_t g = (uint32_t)((uint64_t)groups * part / p.parts) + threadIdx.x; g < g1; g += kThreads) {
             const uint32_t r = g / row_groups, c = (g - r * row_groups) * 8;
             float v[8];
             load_g8(p, z, (int)r, (int)c, v);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= inv;
+            for (int e = 0; e < 8; ++e) v[e] = v[e] * lift * inv;
             const int64_t at = ((int64_t)z * p.m + r) * p.ldx + c;
             split8(v, *reinterpret_cast<uint4 *>(p.x[0][0] + at), *reinterpret_cast<uint4 *>(p.x[0][1] + at));
         }

@@ -48,3 +48,17 @@ def test_empty_shapes_of_any_rank():
     assert E.lookup(torch.zeros(5, 0, device="cuda"), ids).shape == (2, 3, 0)
     assert E.lookup_gradient(torch.zeros(2, 3, 0, device="cuda"), ids, 5).shape == (5, 0)
     assert E.lookup_gradient(torch.zeros(2, 0, 4, device="cuda"), ids[:, :0], 5).shape == (5, 4)
+
+
+def test_newton_schulz_of_matrices_at_the_end_of_fp32():
+    """Without an eps: a zero matrix gives zeros, and a matrix is its own multiple's (a power of two takes no bits) down to
+    where fp32 ends. Norms of about 7e-2 · 2^-k."""
+    from lookatmyquant_b200 import orthogonal as N
+    G = (torch.randn(60, 90, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) * 1e-3)
+    G = G.bfloat16().float()  # 8 bits, so that they survive as subnormals
+    G = torch.where(G.abs() < 2.0**-16, 0.0, G)
+    want = N.newton_schulz(G, eps=0.0)
+    for k in (60, 100, 115, 125):
+        assert torch.equal(N.newton_schulz(G * 2.0**-k, eps=0.0), want), k
+    assert float(N.newton_schulz(torch.zeros(40, 60, device="cuda"), eps=0.0).abs().sum()) == 0
+    N.check_status()

@@ -14,7 +14,10 @@
 // single products came to 2.7e-3 (198 x 21), and those products are short (70 x 458: 154 us so, 140 with single ones). In
 // simulation (64 x 2000 .. 500 x 520; Gaussian, low-rank, power-law, row-scaled updates) this leaves 2e-4 .. 1.8e-3 of
 // relative error beside 1.65e-3 of the bf16 output's
-// rounding; three products everywhere leave 1e-5 for 2.6 times the work, single ones 4e-3. Everything is held times
+// rounding; three products everywhere leave 1e-5 for 2.6 times the work, single ones 4e-3. That is for steps that multiply a
+// rounding by 4 (Muon's, the largest derivative of the step's polynomial) to 8. Steeper schedules take three products
+// everywhere: for one that begins with (8.287, -23.596, 17.3), a derivative of 24, the model gives 2.1e-3 to 5.2e-3 otherwise
+// (150 x 2000 the worst). Everything is held times
 // kScale = 2^10, which keeps entries of order 1/max(m, n) clear of fp16's subnormals and the largest (singular values
 // up to 5, B up to 32) below its maximum. Accumulation is fp32 in TMEM.
 //
@@ -65,6 +68,7 @@ constexpr int kThreads = 320;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kScale = 1024.f;
 constexpr int kMaxSteps = 16;
+constexpr double kSteep = 9.0;                   // the derivative of a step's polynomial from which single products are too few
 constexpr int kParts = 296;                      // parts of a batch in the sum of squares, at most
 constexpr int kSplitUnits = 148;                 // pieces of A's products over all of K, at most
 
@@ -91,6 +95,7 @@ struct Params {
     float eps;
     int steps;
     float coef[kMaxSteps][3];
+    int exact;            // three products everywhere
     unsigned *barrier;    // zero before the launch
     int *status;
 };
@@ -123,7 +128,7 @@ __device__ __forceinline__ Phase phase_of(const Params &p, int index) {
     const int step = index / 3;
     f.kind = index % 3;
     f.last = step == p.steps - 1;
-    f.split = f.kind == kPoly || step > 4 || p.s <= BM || (f.kind == kApply && (step == 4 || f.last));
+    f.split = f.kind == kPoly || step > 4 || p.s <= BM || p.exact || (f.kind == kApply && (step == 4 || f.last));
     f.M = f.kind == kApply && p.tall ? p.l : p.s;
     f.N = f.kind == kApply && !p.tall ? p.l : p.s;
     f.K = f.kind == kGram ? p.l : p.s;
@@ -839,7 +844,7 @@ extern "C" int lamq_newton_schulz(const void *G, int dtype, int64_t ldg, int64_t
                  workspace_bytes);
     Params p{};
     // singular values start within [0, 1]: the polynomials must keep them, and B, within what fp16 holds
-    double top = 1.0;
+    double top = 1.0, steepest = 0.0;
     for (int k = 0; k < steps; ++k) {
         double next = 0.0, big = 0.0;
         for (int e = 0; e < 3; ++e) p.coef[k][e] = coefficients[3 * k + e];
@@ -847,6 +852,8 @@ extern "C" int lamq_newton_schulz(const void *G, int dtype, int64_t ldg, int64_t
             const double x = top * i / 1024, q = p.coef[k][0] + x * x * (p.coef[k][1] + x * x * p.coef[k][2]);
             big = std::max(big, q < 0 ? -q : q);
             next = std::max(next, (q < 0 ? -q : q) * x);
+            const double slope = p.coef[k][0] + x * x * (3.0 * p.coef[k][1] + x * x * 5.0 * p.coef[k][2]);
+            steepest = std::max(steepest, slope < 0 ? -slope : slope);
         }
         LAMQ_REQUIRE(p.coef[k][0] + p.coef[k][1] + p.coef[k][2] == p.coef[k][0] + p.coef[k][1] + p.coef[k][2] &&
                          big <= 32.0 && next <= 5.0,
@@ -854,6 +861,7 @@ extern "C" int lamq_newton_schulz(const void *G, int dtype, int64_t ldg, int64_t
                      "polynomial of A up to 32)", k);
         top = std::max(1.0, next);
     }
+    p.exact = steepest > kSteep;
     cudaStream_t s = (cudaStream_t)stream;
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);

@@ -62,3 +62,31 @@ def test_newton_schulz_of_matrices_at_the_end_of_fp32():
         assert torch.equal(N.newton_schulz(G * 2.0**-k, eps=0.0), want), k
     assert float(N.newton_schulz(torch.zeros(40, 60, device="cuda"), eps=0.0).abs().sum()) == 0
     N.check_status()
+
+
+POLAR = [(8.28721201814563, -23.595886519098837, 17.300387312530933),
+         (4.107059111542203, -2.9478499167379106, 0.5448431082926601),
+         (3.9486908534822946, -2.908902115962949, 0.5518191394370137),
+         (3.3184196573706015, -2.488488024314874, 0.51004894012372),
+         (2.300652019954817, -1.6689039845747493, 0.4188073119525673)]
+
+
+@pytest.mark.parametrize("scale", [1.0, 1.01])
+@pytest.mark.parametrize("m,n,rank,noise", [(320, 960, 4, 1.0), (150, 2000, 2, 3.0), (2000, 150, 2, 3.0), (256, 512, 256, 1.0)])
+def test_steep_schedules_are_as_exact_as_muons(m, n, rank, noise, scale):
+    """A published schedule whose first step multiplies a small rounding by 24, within the tolerance of Muon's coefficients:
+    the bf16 output's rounding (at most 2^-8 of each entry, uniform) and ten roundings of 2^-11."""
+    from lookatmyquant_b200 import orthogonal as N
+    g = torch.Generator("cuda").manual_seed(m + n)
+    G = 1e-3 * (torch.randn(m, rank, device="cuda", generator=g) @ torch.randn(rank, n, device="cuda", generator=g)
+                + noise * torch.randn(m, n, device="cuda", generator=g))
+    abc = [(a / scale, b / scale**3, c / scale**5) for a, b, c in POLAR]
+    X = G.double() / (G.double().norm() + 1e-7)
+    X = X.T if m > n else X
+    for a, b, c in abc:
+        A = X @ X.T
+        X = a * X + (b * A + c * A @ A) @ X
+    X = X.T if m > n else X
+    got = N.newton_schulz(G, coefficients=abc)
+    assert float((got.double() - X).norm()) <= math.hypot(2.0**-8, 10 * 2.0**-11) / math.sqrt(3) * float(X.norm())
+    N.check_status()

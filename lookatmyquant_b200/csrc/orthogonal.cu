@@ -762,8 +762,14 @@ Plan plan_of(int batch, int m, int n) {
     const int s = std::min(m, n), l = std::max(m, n);
     // The wide tiles have the better ratio of products to operand bytes (single CTAs of 128 x 256 waited for L2: 9728 x
     // 2560 took 1.57 ms), the narrow ones half of the latency (narrower still would not: an MMA of 64 columns takes as
-    // long as one of 128). Wide ones as soon as the larger phase (B·X) gives every pair of SMs a tile.
-    L.wide = batch * tiles_of(l, 256) * tiles_of(s, 256) >= kSplitUnits / 2;
+    // long as one of 128) and their sums for A can be cut. Wide ones where the larger phase (B·X) gives every pair of SMs a
+    // tile, A has 15 of them or more, each of which sums over all of K on one pair, and s fills more than half of one.
+    // Measured, us (narrow, wide): 2560 x 2560 1245, 695; 4 x 960 x 2560 681, 518; 1280 x 9728 915, 796; 80 x 130 x 200 286,
+    // 245; and where A has few tiles 960 x 9728 621, 715; 512 x 9728 294, 579; 2 x 16 x 9728 159, 770; 64 x 131072 357, 8849;
+    // or s is mostly padding 300 x 20 x 24 185, 239. (Near the rule's edges it is up to 8 % off: 2 x 960 x 2560 409, 428; 16 x
+    // 320 x 960 243, 262; and 1600 x 1600, with 49 tiles in B·X, 582, 417.)
+    const int64_t st = tiles_of(s, 256);
+    L.wide = batch * tiles_of(l, 256) * st >= kSplitUnits / 2 && batch * st * (st + 1) / 2 >= 15 && s > BM;
     L.parts = (int)std::max<int64_t>(1, std::min<int64_t>(kParts / batch, (int64_t)m * up64(n) / 16384));
     // A is s x s over K = l: of a skinny matrix few tiles, each a long sum. Cut K, in parts of four steps or more, where
     // SMs would be idle (16 x 9728: 152 steps of some 700 cycles on one SM otherwise)

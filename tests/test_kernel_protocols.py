@@ -93,3 +93,19 @@ def test_no_wait_of_the_attention_forward_can_miss_its_phase(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-O1", f"-I{CSRC}", "-x", "c++", str(src), "-o", str(exe)], check=True)
     bad, by_buffer = map(int, subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split())
     assert bad == 0 and by_buffer > 0
+
+
+def test_skinny_updates_keep_the_cut_of_their_long_sums():
+    """A = X·Xᵀ of a skinny matrix is a few tiles of long sums: they are cut into pieces over the idle SMs, whose fp32 sums the
+    workspace holds, for a batch of two and for the longest as for one."""
+    from lookatmyquant_b200 import _lib
+    from lookatmyquant_b200.build import LIB, build
+    if not LIB.exists():
+        build()
+    size, tile = _lib.load().lamq_newton_schulz_workspace_size, 128 * 128 * 4
+    up = lambda v, to: -(-v // to) * to
+    plain = lambda b, m, n: 4 * up(b * m * up(n, 64) * 2, 256) + 4 * up(b * min(m, n) * up(min(m, n), 64) * 2, 256)
+    for b, m, n, tiles in ((1, 16, 9728, 1), (2, 16, 9728, 2), (1, 64, 131072, 1), (1, 512, 9728, 16), (2, 9728, 256, 8)):
+        assert size(b, m, n) >= plain(b, m, n) + tiles * tile * min(148 // tiles, up(max(m, n), 64) // 64 // 4), (b, m, n)
+    for b, m, n in ((1, 2560, 9728), (4, 960, 2560), (1, 2560, 2560)):  # enough tiles: whole sums
+        assert size(b, m, n) < plain(b, m, n) + tile

@@ -139,6 +139,9 @@ __global__ void __launch_bounds__(kThreads)
 
 // ---- gradient, few tokens
 
+// Tokens up to which the gradient is one launch: what its lists in shared memory hold. Measured at 2048 of them, us (so,
+// sorted): 49152 x 960 fp32 46.5, 55.8, bf16 33.5, 43.8; 8000 x 1024 fp32 17, 36; 131072 x 64 13, 41. Where the zeros are most
+// of the work the sorted path's writers do better: 131072 x 2560 bf16 160, 136, and 147, 129 at 64 tokens.
 constexpr int kDirectTokens = 2048;
 constexpr int kDirectRows = 2048;   // rows a block can own
 constexpr int kDirectCols = 32;     // packs of columns a block can own

@@ -9,7 +9,8 @@ makes it an attention implementation of Hugging Face models ("lamq").
 Tensors are (batch, heads, length, head_dim) bf16 views with contiguous head_dim (a projection's (batch, length, heads,
 head_dim) output transposed is read in place); outputs come in that memory order too. Heads may be shared: query head h
 reads key head h // (heads // kv_heads). Query i of text b sees keys key_start[b] <= j < key_end[b] and, when causal,
-j <= i + kv_len - q_len. A query that sees no key gives a zero output, lse -inf and no gradient.
+j <= i + kv_len - q_len. A query that sees no key gives a zero output, lse -inf and no gradient. head_dim is a multiple of
+8 up to 128, the scale positive and finite; anything else raises ValueError.
 """
 
 from __future__ import annotations

@@ -40,8 +40,12 @@ def _coefficients(coefficients: tuple, steps: int) -> bytes:
 
 def newton_schulz(G: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7) -> torch.Tensor:
     """G (..., m, n; fp32 or bf16) orthogonalised: X = G / (|G|_F + eps), then `steps` times X <- (aI + bA + cA²)X with
-    A = X·Xᵀ (on the smaller side). `coefficients` is one (a, b, c) or a sequence of one per step. bf16, G's shape; the
-    matrices of a batch go together in one launch."""
+    A = X·Xᵀ (on the smaller side). `coefficients` is one (a, b, c) or a sequence of one per step; 1 to 16 steps. bf16, G's
+    shape; the matrices of a batch go together in one launch.
+
+    X and the polynomials are held in fp16 pairs, so coefficients raise ValueError where they can take a singular value of
+    [0, 1] above 5, or |a + b·s² + c·s⁴| above 32, in any step. Steps steeper than 9 anywhere (Muon's: 4) take 2.6 times the
+    products, for the same error."""
     if G.dtype not in _DTYPES or not G.is_cuda:
         raise TypeError("the update must be a float32 or bfloat16 CUDA tensor")
     if G.ndim < 2:

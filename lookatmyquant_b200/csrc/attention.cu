@@ -30,10 +30,10 @@
 // cycles and a commit 85, in which little is queued; releases by the elementwise warps instead cost those more.
 //
 // Measured and what bounds it (causal, no padding):
-//   2 x 4096, 32/8 heads of 128: forward 276 us (990 TFLOP/s; the softmax warps, one S buffer a tile), dq 355 us (1160
+//   2 x 4096, 32/8 heads of 128: forward 278 us (983 TFLOP/s; the softmax warps, one S buffer a tile), dq 355 us (1160
 //   TFLOP/s executed) and dkv 418 us (1320 executed; shared-memory bandwidth of products that read both operands from it,
 //   and the elementwise steps between them).
-//   8 x 2048, 15/5 heads of 64: forward 129 us, dq 170, dkv 182: an MMA of 64 columns takes as long as one of 128, so half
+//   8 x 2048, 15/5 heads of 64: forward 131 us, dq 170, dkv 182: an MMA of 64 columns takes as long as one of 128, so half
 //   the tensor rate is lost; exponentials run at half of their rate.
 //   A CTA's start and end cost as much as 3 to 5 of its tiles. CTAs that took over further units (cluster launch control)
 //   made short rows 5 to 8 % faster (dq of 5 x 1337, 32/8 heads of 128: 174 -> 161 us) and long ones 3 to 6 % slower (2 x

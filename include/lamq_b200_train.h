@@ -96,8 +96,8 @@ int lamq_attention_backward(const lamq_attention_args *args, void *workspace, si
  * X, A and B are held in 22 bits, products take fp16 operands where their rounding cannot grow, fp16 pairs elsewhere,
  * with fp32 accumulation: the relative error is about the bf16 output's rounding (2^-9) again. (Coefficients whose steps are
  * steeper than 9 anywhere take pairs everywhere, 2.6 times the work.) Coefficients that take singular values of [0, 1]
- * above 5, or the polynomial of A above 32, are rejected. A zero matrix gives zeros; a matrix with a NaN or an infinity gives NaN. Workspace:
- * lamq_newton_schulz_workspace_size(batch, m, n) bytes, 16-byte aligned. One cooperative kernel; *status becomes
+ * above 5, or the polynomial of A above 32, are rejected. A zero matrix gives zeros; a matrix with a NaN or an infinity
+ * gives NaN. Workspace: lamq_newton_schulz_workspace_size(batch, m, n) bytes, 16-byte aligned. One cooperative kernel; *status becomes
  * LAMQ_ERR_TIMEOUT if a bounded device wait gives up. Equal calls give equal bits.
  */
 size_t lamq_newton_schulz_workspace_size(int batch, int m, int n);

@@ -148,8 +148,8 @@ def _padding(padding_idx: int | None, rows: int) -> int:
 
 def lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None) -> torch.Tensor:
     """scale · table[ids] (ids of any shape; table V x d fp32 or bf16; the result in the table's type, the product in
-    fp32). Tokens with id `padding_idx` get zero rows, whatever the table holds there. An id outside the table gets a zero row and is reported by
-    `check_status()`."""
+    fp32). Tokens with id `padding_idx` get zero rows, whatever the table holds there. An id outside the table gets a zero
+    row and is reported by `check_status()`."""
     if table.ndim != 2:
         raise ValueError("the table must be a matrix")
     table, ld, code = _matrix(table, "the table")

@@ -45,7 +45,8 @@ def hasty(tmp_path_factory):
 @pytest.mark.parametrize("before_status", [0, 1])
 def test_a_sort_that_gives_up_leaves_the_gradient_alone(harness, before_status):
     """The kernels after the sort do not go by keys and positions that nobody wrote: the gradient that was to be added to
-    stays as it was. (Here they hold valid places, so that a kernel that did go by them would be seen in the result.) The status says so, also where a bad id was met before."""
+    stays as it was. (Here they hold valid places, so that a kernel that did go by them would be seen in the result.) The
+    status says so, also where a bad id was met before."""
     n, rows, d = 3000, 100, 64
     g = torch.Generator("cuda").manual_seed(1)
     dy = torch.randn(n, d, device="cuda", generator=g)

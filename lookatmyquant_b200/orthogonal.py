@@ -119,7 +119,7 @@ class Muon(torch.optim.Optimizer):
                     us.append(torch.add(g, b, alpha=mu) if group["nesterov"] else b)
                 O = newton_schulz(us[0] if len(us) == 1 else torch.stack(us), group["steps"], group["coefficients"])
                 m, n = params[0].shape[-2:]
-                rate = -group["lr"] * max(1.0, m / n) ** 0.5
+                rate = -group["lr"] * max(1.0, m / max(n, 1)) ** 0.5
                 for p, o in zip(params, (O,) if len(us) == 1 else O.unbind(0)):
                     if group["weight_decay"]:
                         p.mul_(1.0 - group["lr"] * group["weight_decay"])

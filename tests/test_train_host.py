@@ -126,3 +126,14 @@ def test_muon_makes_a_momentum_once(monkeypatch):
             p.grad = torch.ones(2, 3)
         opt.step()
     assert len(made) == 3
+
+
+def test_muon_steps_over_empty_matrices(monkeypatch):
+    from lookatmyquant_b200 import orthogonal as N
+    monkeypatch.setattr(N, "newton_schulz", lambda G, steps, coefficients: G.bfloat16())
+    params = [torch.nn.Parameter(torch.ones(*s)) for s in ((3, 0), (0, 3), (2, 2))]
+    opt = N.Muon(params, lr=0.5, nesterov=False)
+    for p in params:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    assert [p.shape for p in params] == [(3, 0), (0, 3), (2, 2)] and torch.equal(params[2], torch.full((2, 2), 0.5))

@@ -1,4 +1,4 @@
-"""ctypes bindings to liblamq_b200.so (the C ABI declared in include/lamq_b200.h and include/lamq_b200_train.h).
+"""ctypes bindings to liblamq_b200.so (the C ABI declared in include/lamq_b200*.h).
 
 The library is the product's only compute path: if it is missing or cannot load, every entry point raises — there is
 no CPU or PyTorch fallback. `torch` tensors are passed as raw device pointers on the current CUDA stream.
@@ -22,7 +22,7 @@ LAMQ_F32, LAMQ_BF16, LAMQ_F64 = 0, 1, 2
 _c = ctypes
 _P, _I64, _I32, _SZ, _D = _c.c_void_p, _c.c_int64, _c.c_int, _c.c_size_t, _c.c_double
 
-# name -> (restype, argtypes): every symbol include/lamq_b200.h and include/lamq_b200_train.h declare
+# name -> (restype, argtypes): every symbol include/lamq_b200.h, lamq_b200_train.h and lamq_b200_step.h declare
 SIGNATURES = {
     "lamq_abi_version": (_I32, []),
     "lamq_kernel_launches": (_c.c_uint64, []),
@@ -77,11 +77,22 @@ SIGNATURES = {
     "lamq_attention_backward": (_I32, [_P, _P, _SZ, _P, _P]),
     "lamq_newton_schulz_workspace_size": (_SZ, [_I32, _I32, _I32]),
     "lamq_newton_schulz": (_I32, [_P, _I32, _I64, _I64, _I32, _I32, _I32, _I32, _P, _c.c_float, _P, _P, _SZ, _P, _P]),
+    "lamq_norm_forward": (_I32, [_P, _P]),
+    "lamq_norm_backward_workspace_size": (_SZ, [_P]),
+    "lamq_norm_backward": (_I32, [_P, _P, _SZ, _P]),
+    "lamq_gradient_workspace_size": (_SZ, [_I64]),
+    "lamq_gradient_norm": (_I32, [_P, _I64, _P, _P, _SZ, _P]),
+    "lamq_gradient_clip": (_I32, [_P, _I64, _D, _D, _P, _P, _SZ, _P]),
 }
 
 # lamq_attention_args (328 bytes): batch; heads, kv_heads, head_dim, causal; q_len, kv_len; scale, reserved; key_start,
 # key_end; q, k, v, o; lse; d_o, dq, dk, dv (a lamq_heads is a pointer and three strides)
 ATTENTION_ARGS = struct.Struct("=q4i2qfi2Q16qQ16q")
+
+# lamq_norm_args (264 bytes): rows, gate_span; d, residual_dtype, branch_dtype, weight_dtype, post_dtype, gate_dtype; scale,
+# eps, offset, reserved; residual, branch; weight, post, gate; h, y; dh, dy; d_residual, d_branch, d_weight, d_post, d_gate (a
+# lamq_rows is a pointer, an inner count and two strides)
+NORM_ARGS = struct.Struct("=2q6i3fi8q5Q8q5Q")
 
 
 class ProductGroup(_c.Structure):

@@ -1,0 +1,286 @@
+// What the norms' forward and backward kernels share: rows held in registers by teams of threads, their sums, and how a
+// call's sizes choose a kernel.
+//
+// A team of `team` threads owns a row at a time: thread t holds the packs t, t + team, ... of V elements, P of them at
+// most, so every row is read once and its sums need one exchange. Teams of 32 threads or less live in a warp (a power of
+// two of lanes); larger ones are whole warps that meet at a named barrier of their own, so a block's teams never wait for
+// one another.
+#pragma once
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstdint>
+
+#include <cuda_bf16.h>
+
+#include "../../include/lamq_b200_step.h"
+#include "lamq_common.cuh"
+
+namespace lamq {
+
+// The checks of a call's arguments (norm.cu): LAMQ_OK, or LAMQ_ERR_INVALID with the reason set.
+int norm_args_status(const lamq_norm_args *a, bool backward);
+
+namespace {
+
+constexpr int kNormThreads = 512;   // most threads of a block
+constexpr int kNormMaxD = 16384;    // widest row
+constexpr int kNormSums = 2;        // sums exchanged at once
+constexpr int kSMs = 148;
+
+// ---- loads
+//
+// As volatile assembly: the compiler runs none of them where the source does not. (Plain __ldg loads behind a condition were
+// executed ahead of it: kernels that tested a pointer for NULL before they read it faulted.) Absent tensors have a pointer
+// that may be read, too (the host's `present`).
+
+__device__ __forceinline__ uint4 load16(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+__device__ __forceinline__ float load_one(const float *p) {
+    float v;
+    asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
+
+__device__ __forceinline__ float load_one(const __nv_bfloat16 *p) {
+    uint16_t v;
+    asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(v) : "l"(p));
+    return __uint_as_float((uint32_t)v << 16);
+}
+
+// ---- V elements of T: 16 bytes (bf16) or 32 (fp32) where V is 8, one element where rows may begin anywhere
+
+template <typename T, int V>
+struct Raw;
+
+template <>
+struct Raw<float, 8> {
+    uint4 a, b;
+    __device__ __forceinline__ void load(const float *p) { a = load16(p), b = load16(p + 4); }
+    __device__ __forceinline__ void zero() { a = b = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void get(float (&f)[8]) const {
+        f[0] = __uint_as_float(a.x), f[1] = __uint_as_float(a.y), f[2] = __uint_as_float(a.z), f[3] = __uint_as_float(a.w);
+        f[4] = __uint_as_float(b.x), f[5] = __uint_as_float(b.y), f[6] = __uint_as_float(b.z), f[7] = __uint_as_float(b.w);
+    }
+    __device__ __forceinline__ static void store(float *p, const float (&f)[8]) {
+        reinterpret_cast<float4 *>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+        reinterpret_cast<float4 *>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+};
+
+template <>
+struct Raw<__nv_bfloat16, 8> {
+    uint4 v;
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { v = load16(p); }
+    __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void get(float (&f)[8]) const {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    __device__ __forceinline__ static void store(__nv_bfloat16 *p, const float (&f)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&b);
+        }
+        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+template <typename T>
+struct Raw<T, 1> {
+    float v;
+    __device__ __forceinline__ void load(const T *p) { v = load_one(p); }
+    __device__ __forceinline__ void zero() { v = 0.f; }
+    __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = v; }
+    __device__ __forceinline__ static void store(float *p, const float (&f)[1]) { *p = f[0]; }
+    __device__ __forceinline__ static void store(__nv_bfloat16 *p, const float (&f)[1]) { *p = __float2bfloat16_rn(f[0]); }
+};
+
+// V elements at index i of an array whose type is known when the call is made: weights, gates and their gradients.
+template <int V>
+__device__ __forceinline__ void load_typed(const void *base, int dtype, int64_t i, float (&f)[V]) {
+    if (dtype == LAMQ_F32) {
+        Raw<float, V> x;
+        x.load(reinterpret_cast<const float *>(base) + i);
+        x.get(f);
+    } else {
+        Raw<__nv_bfloat16, V> x;
+        x.load(reinterpret_cast<const __nv_bfloat16 *>(base) + i);
+        x.get(f);
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void store_typed(void *base, int dtype, int64_t i, const float (&f)[V]) {
+    if (dtype == LAMQ_F32)
+        Raw<float, V>::store(reinterpret_cast<float *>(base) + i, f);
+    else
+        Raw<__nv_bfloat16, V>::store(reinterpret_cast<__nv_bfloat16 *>(base) + i, f);
+}
+
+template <typename T>
+__device__ __forceinline__ const T *row_at(const lamq_rows &r, int i) {
+    const int inner = (int)r.inner;  // the host keeps it within an int
+    const int o = i / inner;
+    return reinterpret_cast<const T *>(r.data) + o * r.outer + (i - o * inner) * r.row;
+}
+
+// ---- teams
+
+struct Team {
+    int size, t, slot;  // threads of a team; this one's place; the team's place in the block
+    int turn;           // which half of the scratch the next exchange uses
+    float *scratch;     // 2 x (kNormThreads / 32) x kNormSums
+
+    __device__ Team(int size_, float *scratch_)
+        : size(size_), t(threadIdx.x % size_), slot(threadIdx.x / size_), turn(0), scratch(scratch_) {}
+
+    // The sums over the team, in every thread of it and in a fixed order. All threads of the team call it (and all of the
+    // warp, where teams are parts of one). Two halves of the scratch in turn: a team's thread comes to an exchange only
+    // when the whole team has read the one before the last.
+    template <int K>
+    __device__ __forceinline__ void sum(float (&v)[K]) {
+        static_assert(K <= kNormSums, "the scratch holds kNormSums sums a warp");
+        for (int o = min(size, 32) >> 1; o > 0; o >>= 1)
+#pragma unroll
+            for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+        if (size <= 32) return;
+        float *const half = scratch + turn * (kNormThreads / 32 * kNormSums);
+        turn ^= 1;
+        const int first = slot * (size >> 5), warps = size >> 5;
+        if ((t & 31) == 0)
+#pragma unroll
+            for (int k = 0; k < K; ++k) half[(first + (t >> 5)) * kNormSums + k] = v[k];
+        asm volatile("bar.sync %0, %1;" ::"r"(slot + 1), "r"(size) : "memory");
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = 0.f;
+        for (int w = 0; w < warps; ++w)
+#pragma unroll
+            for (int k = 0; k < K; ++k) v[k] += half[(first + w) * kNormSums + k];
+    }
+};
+
+// v^-1/2 for a normal v: the hardware's approximation (2 units in the last place) and a Newton step. An infinite v gives 0.
+__device__ __forceinline__ float reciprocal_root(float v) {
+    const float r = rsqrtf(v);
+    const float e = fmaf(-v * r, r, 1.f);
+    return isinf(v) ? 0.f : fmaf(0.5f * r, e, r);
+}
+
+constexpr float kShrink = 0x1p-80f;  // brings fp32's largest numbers where 16384 of their squares have a sum
+
+// The factor (mean(x²) + eps)^-1/2 of a row, from the sum of squares, for x as it stands after the call: where the sum
+// overflowed, x is multiplied by kShrink and summed again (eps is then far below the mean's last bit). `shrunk` is
+// kShrink or 1: the factor of x as it was is the result times `shrunk`.
+template <int P, int V>
+__device__ __forceinline__ float unit_factor(Team &team, float (&x)[P][V], float ss, float inv_d, float eps, float &shrunk) {
+    shrunk = 1.f;
+    const bool over = isinf(ss);
+    if (team.size < 32 ? __any_sync(0xffffffffu, over) : over) {
+        if (over) shrunk = kShrink;
+        float again[1] = {0.f};
+#pragma unroll
+        for (int q = 0; q < P; ++q)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                x[q][e] *= shrunk;
+                again[0] = fmaf(x[q][e], x[q][e], again[0]);
+            }
+        team.sum(again);
+        ss = again[0];
+        if (over) eps = 0.f;
+    }
+    return reciprocal_root(fmaf(ss, inv_d, eps));
+}
+
+// ---- the host's side
+
+// How many threads share a row, and P: what they hold of it each (kWide: nothing, norm_wide.cuh).
+constexpr int kWide = 1 << 20;
+constexpr int kNormFull = 16;  // elements a thread of the backward kernel with post norms and gates: more would spill
+struct NormShape {
+    int V, P, team, packs;
+};
+
+// Which tensors a call has, and in the place of the others an output's memory of the same shape and no smaller a type: what
+// a kernel gets may be read whether or not it is there.
+enum { kHasWeight = 1, kHasPost = 2, kHasGate = 4, kHasDh = 8, kHasDy = 16, kHasBranch = 32 };
+
+struct Present {
+    int has;
+    lamq_rows branch, dh, dy;
+    const void *weight, *post, *gate;
+    int weight_dtype, post_dtype, gate_dtype, gate_span;
+};
+
+inline Present present(const lamq_norm_args &a, bool backward) {
+    const void *const out = backward ? a.d_residual : a.branch.data ? a.h : a.y;
+    const lamq_rows rows{const_cast<void *>(out), INT_MAX, a.d, 0};
+    Present p;
+    p.has = (a.weight ? kHasWeight : 0) | (a.post ? kHasPost : 0) | (a.gate ? kHasGate : 0) |
+            (a.branch.data ? kHasBranch : 0) | (backward && a.dh.data ? kHasDh : 0) | (backward && a.dy.data ? kHasDy : 0);
+    p.branch = a.branch.data ? a.branch : rows;
+    p.dh = p.has & kHasDh ? a.dh : rows;
+    p.dy = p.has & kHasDy ? a.dy : rows;
+    p.weight = a.weight ? a.weight : out, p.weight_dtype = a.weight ? a.weight_dtype : a.residual_dtype;
+    p.post = a.post ? a.post : out, p.post_dtype = a.post ? a.post_dtype : a.residual_dtype;
+    p.gate = a.gate ? a.gate : out, p.gate_dtype = a.gate ? a.gate_dtype : a.residual_dtype;
+    p.gate_span = a.gate ? (int)a.gate_span : 1;
+    return p;
+}
+
+inline bool aligned_rows(const lamq_rows &r) {
+    return !r.data || ((reinterpret_cast<uintptr_t>(r.data) & 15) == 0 && r.row % 8 == 0 && r.outer % 8 == 0);
+}
+
+// Vectors where every row and every array begins on 16 bytes, elements elsewhere. Up to 32 packs a team is a power of two
+// of lanes; wider rows take the fewest packs a thread that 512 threads can hold. (Elements: eight a thread, so that a
+// thread has as many bytes under way as it can.)
+inline NormShape norm_shape(const lamq_norm_args &a, bool backward) {
+    const void *arrays[] = {a.weight, a.post, a.gate, a.h, a.y, a.d_residual, a.d_branch, a.d_weight, a.d_post, a.d_gate};
+    bool vec = a.d % 8 == 0 && aligned_rows(a.residual) && aligned_rows(a.branch);
+    if (backward) vec = vec && aligned_rows(a.dh) && aligned_rows(a.dy);
+    for (const void *p : arrays) vec = vec && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+    NormShape s;
+    s.V = vec ? 8 : 1;
+    s.packs = a.d / s.V;
+    if (s.packs <= 32) {
+        s.P = 1;
+        s.team = 1;
+        while (s.team < s.packs) s.team *= 2;
+    } else {
+        if (vec)
+            s.P = s.packs <= 512 ? 1 : s.packs <= 1024 ? 2 : 4;
+        else
+            s.P = s.packs <= 4096 ? 8 : kWide;
+        if (backward && (a.post || a.gate) && s.P != kWide && s.P * s.V > kNormFull) s.V = 1, s.P = kWide, s.packs = a.d;
+        s.team = s.P == kWide ? kNormThreads : ((s.packs + s.P - 1) / s.P + 31) / 32 * 32;
+    }
+    return s;
+}
+
+// Teams whose threads hold more than this of a row have a block to themselves: the memory in which a block adds its teams'
+// sums holds no more.
+constexpr int kNormShared = 8;
+
+// Teams of a block: blocks of about `threads` threads, fewer where there are few rows, whole warps always.
+inline int norm_slots(const NormShape &s, int64_t rows, int threads) {
+    if (s.P > kNormShared / s.V) return 1;
+    const int least = std::max(1, 32 / s.team), most = std::max(least, threads / s.team);
+    const int64_t wanted = (rows + 2 * kSMs - 1) / (2 * kSMs);
+    return (int)std::min<int64_t>(most, std::max<int64_t>(least, (wanted + least - 1) / least * least));
+}
+
+}  // namespace
+}  // namespace lamq

@@ -18,40 +18,80 @@ struct ForwardParams {
     int rows, d;
     float scale, eps, offset, inv_d;
     int team, slots, packs;
+    RingParams ring;
 };
 
-// kBranch: a join; else the norm alone (of `residual`).
-template <typename R, typename B, int V, int P, bool kBranch>
-__global__ void __launch_bounds__(kNormThreads, 1) norm_forward_kernel(const __grid_constant__ ForwardParams p) {
-    __shared__ float scratch[2 * (kNormThreads / 32) * kNormSums];
+// The weights' and gates' packs of a thread that holds few of them stay in its registers.
+template <typename R, typename B, int V, int P, int kMode>
+__global__ void __launch_bounds__(kNormThreads, P * V <= 8 ? 2 : 1) norm_forward_kernel(const __grid_constant__ ForwardParams p) {
+    extern __shared__ uint4 stages[];
+    __shared__ alignas(16) float scratch[Team::kScratch];
+    constexpr bool kBranch = kMode != kNormAlone, kFull = kMode == kJoinFull, kHold = P * V <= kNormShared;
     Team team(p.team, scratch);
-    // Teams of a warp take steps together: the loop ends when the first of them has no row.
-    const int ahead = p.team < 32 ? team.slot % (32 / p.team) : 0;
-    for (int row0 = blockIdx.x * p.slots + team.slot - ahead; row0 < p.rows; row0 += gridDim.x * p.slots) {
-        const int row = row0 + ahead;
-        const bool live = row < p.rows;
-        const int at = live ? row : 0;
-        const R *const src = row_at<R>(p.residual, at);
-        float x[P][V];
-        Raw<R, V> r[P];
+    const Ring<V, P> ring(stages, p.ring, team, p.packs);
+    const bool post = kFull && (p.in.has & kHasPost), gate = kFull && (p.in.has & kHasGate), pre = p.in.has & kHasWeight;
+    const bool gates = gate && p.in.gate_span == 1;  // a gate row for each row
+    const auto weight = [&](const void *from, int dtype, int pack, float (&w)[V]) {
+        load_typed<V>(from, dtype, pack * V, w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[e] += p.offset;
+    };
+    float w_held[kHold ? P : 1][V], u_held[kHold && kFull ? P : 1][V], gate_held[kHold && kFull ? P : 1][V];
+    int gate_row = -1;
+    if constexpr (kHold)
 #pragma unroll
         for (int q = 0; q < P; ++q) {
             const int pack = team.t + q * p.team;
-            r[q].zero();
-            if (live && pack < p.packs) r[q].load(src + pack * V);
+            if (pack >= p.packs) break;
+            if (pre) weight(p.in.weight, p.in.weight_dtype, pack, w_held[q]);
+            if constexpr (kFull)
+                if (post) weight(p.in.post, p.in.post_dtype, pack, u_held[q]);
         }
+    const auto gate_at = [&](int row) {
+        return reinterpret_cast<const unsigned char *>(p.in.gate) +
+               (int64_t)(row / p.in.gate_span) * p.d * (p.in.gate_dtype == LAMQ_F32 ? 4 : 2);
+    };
+    const int step = gridDim.x * p.slots, first = blockIdx.x * p.slots + team.slot;
+    const auto fetch = [&](int row, int stage) {
+        if (row < p.rows) {
+            ring.fetch(stage, kTensorH, row_at<R>(p.residual, row));
+            if (kBranch) ring.fetch(stage, kTensorBranch, row_at<B>(p.in.branch, row));
+            if (gates) ring.fetch_typed(stage, kTensorGate, gate_at(row), p.in.gate_dtype);
+        }
+        ring.commit();
+    };
+    int stage = 0, to = 0, ahead = first;
+    for (int i = 1; i < p.ring.stages; ++i, ahead += step, to = ring.after(to)) fetch(ahead, to);
+    // Teams of a warp take steps together: the loop ends when the first of them has no row.
+    const int lead = p.team < 32 ? team.slot % (32 / p.team) : 0;
+    for (int row = first; row - lead < p.rows; row += step, ahead += step, stage = ring.after(stage), to = ring.after(to)) {
+        if (p.ring.stages == 1) {
+            fetch(row, 0);
+            ring.wait();
+        } else {
+            if (V == 1) {
+                ring.wait();
+                fetch(ahead, to);
+            } else {
+                fetch(ahead, to);
+                ring.wait();
+            }
+        }
+        const bool live = row < p.rows;
+        const int at = live ? row : 0;
+        float x[P][V];
+        const R *const src = row_at<R>(p.residual, at);
         if constexpr (kBranch) {
             const B *const add = row_at<B>(p.in.branch, at);
-            Raw<B, V> b[P];
 #pragma unroll
             for (int q = 0; q < P; ++q) {
-                const int pack = team.t + q * p.team;
-                b[q].zero();
-                if (live && pack < p.packs) b[q].load(add + pack * V);
-            }
 #pragma unroll
-            for (int q = 0; q < P; ++q) b[q].get(x[q]);
-            if (p.in.has & kHasPost) {
+                for (int e = 0; e < V; ++e) x[q][e] = 0.f;
+                if (live && team.t + q * p.team < p.packs) ring.read(stage, kTensorBranch, add, q, x[q]);
+            }
+        }
+        if constexpr (kFull) {
+            if (post) {
                 float ss[1] = {0.f}, shrunk;
 #pragma unroll
                 for (int q = 0; q < P; ++q)
@@ -64,38 +104,44 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_forward_kernel(const __g
                     const int pack = team.t + q * p.team;
                     if (pack >= p.packs) break;
                     float u[V];
-                    load_typed<V>(p.in.post, p.in.post_dtype, pack * V, u);
+                    if (!kHold) weight(p.in.post, p.in.post_dtype, pack, u);
 #pragma unroll
-                    for (int e = 0; e < V; ++e) x[q][e] *= f * (p.offset + u[e]);
+                    for (int e = 0; e < V; ++e) x[q][e] *= f * (kHold ? u_held[kHold ? q : 0][e] : u[e]);
                 }
             }
-            if (p.in.has & kHasGate) {
-                const int64_t g = (int64_t)(at / p.in.gate_span) * p.d;
+            if (gate) {
+                const int g = at / p.in.gate_span;
+                const unsigned char *const from = gate_at(at);
 #pragma unroll
                 for (int q = 0; q < P; ++q) {
                     const int pack = team.t + q * p.team;
-                    if (pack >= p.packs) break;
+                    if (pack >= p.packs || !live) break;
                     float u[V];
-                    load_typed<V>(p.in.gate, p.in.gate_dtype, g + pack * V, u);
+                    if (gates)
+                        ring.read_typed(stage, kTensorGate, from, p.in.gate_dtype, q, u);
+                    else if (!kHold)
+                        load_typed<V>(from, p.in.gate_dtype, pack * V, u);
+                    else if (g != gate_row)
+                        load_typed<V>(from, p.in.gate_dtype, pack * V, gate_held[kHold ? q : 0]);
 #pragma unroll
-                    for (int e = 0; e < V; ++e) x[q][e] *= u[e];
+                    for (int e = 0; e < V; ++e) x[q][e] *= kHold && !gates ? gate_held[kHold ? q : 0][e] : u[e];
                 }
+                if (live) gate_row = g;
             }
-            R *const out = reinterpret_cast<R *>(p.h) + (int64_t)at * p.d;
-#pragma unroll
-            for (int q = 0; q < P; ++q) {
-                const int pack = team.t + q * p.team;
-                float add_to[V];
-                r[q].get(add_to);
-#pragma unroll
-                for (int e = 0; e < V; ++e) x[q][e] = fmaf(p.scale, x[q][e], add_to[e]);
-                if (live && pack < p.packs) Raw<R, V>::store(out + pack * V, x[q]);
-            }
-        } else {
-#pragma unroll
-            for (int q = 0; q < P; ++q) r[q].get(x[q]);
         }
-        if (p.in.has & kHasWeight) {
+        R *const out = reinterpret_cast<R *>(p.h) + (int64_t)at * p.d;
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+            const int pack = team.t + q * p.team;
+            float r[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) r[e] = 0.f;
+            if (live && pack < p.packs) ring.read(stage, kTensorH, src, q, r);
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[q][e] = kBranch ? fmaf(p.scale, x[q][e], r[e]) : r[e];
+            if (kBranch && live && pack < p.packs) Raw<R, V>::store(out + pack * V, x[q]);
+        }
+        if (pre) {
             float ss[1] = {0.f}, shrunk;
 #pragma unroll
             for (int q = 0; q < P; ++q)
@@ -103,16 +149,16 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_forward_kernel(const __g
                 for (int e = 0; e < V; ++e) ss[0] = fmaf(x[q][e], x[q][e], ss[0]);
             team.sum(ss);
             const float f = unit_factor(team, x, ss[0], p.inv_d, p.eps, shrunk);
-            B *const out = reinterpret_cast<B *>(p.y) + (int64_t)at * p.d;
+            B *const normed = reinterpret_cast<B *>(p.y) + (int64_t)at * p.d;
 #pragma unroll
             for (int q = 0; q < P; ++q) {
                 const int pack = team.t + q * p.team;
                 if (pack >= p.packs) break;
                 float w[V];
-                load_typed<V>(p.in.weight, p.in.weight_dtype, pack * V, w);
+                if (!kHold) weight(p.in.weight, p.in.weight_dtype, pack, w);
 #pragma unroll
-                for (int e = 0; e < V; ++e) w[e] = x[q][e] * f * (p.offset + w[e]);
-                if (live) Raw<B, V>::store(out + pack * V, w);
+                for (int e = 0; e < V; ++e) w[e] = x[q][e] * f * (kHold ? w_held[kHold ? q : 0][e] : w[e]);
+                if (live) Raw<B, V>::store(normed + pack * V, w);
             }
         }
     }
@@ -120,7 +166,7 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_forward_kernel(const __g
 
 template <typename R, typename B, bool kBranch>
 __global__ void __launch_bounds__(kWideThreads, 1) norm_forward_wide_kernel(const __grid_constant__ ForwardParams p) {
-    __shared__ float scratch[2 * (kNormThreads / 32) * kNormSums];
+    __shared__ alignas(16) float scratch[Team::kScratch];
     Team team(kWideThreads, scratch);
     for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const R *const src = row_at<R>(p.residual, row);
@@ -164,24 +210,32 @@ void launch_wide(const ForwardParams &p, int grid, bool branch, cudaStream_t str
         norm_forward_wide_kernel<R, B, false><<<grid, kWideThreads, 0, stream>>>(p);
 }
 
+template <typename R, typename B, int V, int P, int kMode>
+int launch_forward(const ForwardParams &p, int grid, int shared, cudaStream_t stream) {
+    const auto kernel = norm_forward_kernel<R, B, V, P, kMode>;
+    if (const int st = allow_shared(reinterpret_cast<const void *>(kernel), shared)) return st;
+    kernel<<<grid, p.team * p.slots, shared, stream>>>(p);
+    return LAMQ_OK;
+}
+
 template <typename R, typename B, int V, int P>
-void launch_forward(const ForwardParams &p, int grid, bool branch, cudaStream_t stream) {
-    if (branch)
-        norm_forward_kernel<R, B, V, P, true><<<grid, p.team * p.slots, 0, stream>>>(p);
-    else if constexpr (std::is_same_v<R, B>)
-        norm_forward_kernel<R, B, V, P, false><<<grid, p.team * p.slots, 0, stream>>>(p);
+int launch_forward(const ForwardParams &p, int grid, int mode, int shared, cudaStream_t stream) {
+    if (mode == kJoinFull) return launch_forward<R, B, V, P, kJoinFull>(p, grid, shared, stream);
+    if (mode == kJoinPlain) return launch_forward<R, B, V, P, kJoinPlain>(p, grid, shared, stream);
+    if constexpr (std::is_same_v<R, B>) return launch_forward<R, B, V, P, kNormAlone>(p, grid, shared, stream);
+    return LAMQ_ERR_INVALID;  // the checks refuse a norm of two types
 }
 
 template <typename R, typename B>
-void launch_forward(const NormShape &s, const ForwardParams &p, int grid, bool branch, cudaStream_t stream) {
+int launch_forward(const NormShape &s, const ForwardParams &p, int grid, int mode, int shared, cudaStream_t stream) {
     if (s.V == 8)
-        s.P == 1   ? launch_forward<R, B, 8, 1>(p, grid, branch, stream)
-        : s.P == 2 ? launch_forward<R, B, 8, 2>(p, grid, branch, stream)
-                   : launch_forward<R, B, 8, 4>(p, grid, branch, stream);
-    else
-        s.P == 1   ? launch_forward<R, B, 1, 1>(p, grid, branch, stream)
-        : s.P == 8 ? launch_forward<R, B, 1, 8>(p, grid, branch, stream)
-                   : launch_wide<R, B>(p, grid, branch, stream);
+        return s.P == 1   ? launch_forward<R, B, 8, 1>(p, grid, mode, shared, stream)
+               : s.P == 2 ? launch_forward<R, B, 8, 2>(p, grid, mode, shared, stream)
+                          : launch_forward<R, B, 8, 4>(p, grid, mode, shared, stream);
+    if (s.P == 1) return launch_forward<R, B, 1, 1>(p, grid, mode, shared, stream);
+    if (s.P == 8) return launch_forward<R, B, 1, 8>(p, grid, mode, shared, stream);
+    launch_wide<R, B>(p, grid, mode != kNormAlone, stream);
+    return LAMQ_OK;
 }
 
 }  // namespace
@@ -227,23 +281,23 @@ using namespace lamq;
 extern "C" int lamq_norm_forward(const lamq_norm_args *a, lamq_stream_t stream) {
     if (const int st = norm_args_status(a, false)) return st;
     if (a->rows == 0 || a->d == 0) return LAMQ_OK;
-    const bool join = a->branch.data != nullptr;
-    const NormShape s = norm_shape(*a, false);
+    const NormLayout l = norm_layout(*a, false, false, false);
+    const NormShape &s = l.shape;
+    const int mode = l.mode, shared = l.shared;
     ForwardParams p;
     p.residual = a->residual, p.in = present(*a, false);
     p.h = a->h, p.y = a->y;
     p.rows = (int)a->rows, p.d = a->d;
     p.scale = a->scale, p.eps = a->eps, p.offset = a->offset, p.inv_d = 1.f / (float)a->d;
-    p.team = s.team, p.slots = norm_slots(s, a->rows, 256), p.packs = s.packs;
-    const int64_t blocks = (a->rows + p.slots - 1) / p.slots;
-    const int grid = (int)std::min<int64_t>(blocks, kSMs * (2048 / (p.team * p.slots)));
+    p.team = s.team, p.slots = l.slots, p.packs = s.packs;
+    p.ring = l.ring;
+    const int grid = (int)std::min<int64_t>((a->rows + p.slots - 1) / p.slots, kSMs * l.blocks);
     const cudaStream_t st = (cudaStream_t)stream;
-    if (a->residual_dtype == LAMQ_BF16)
-        launch_forward<__nv_bfloat16, __nv_bfloat16>(s, p, grid, join, st);
-    else if (a->branch_dtype == LAMQ_BF16)
-        launch_forward<float, __nv_bfloat16>(s, p, grid, join, st);
-    else
-        launch_forward<float, float>(s, p, grid, join, st);
+    const int launched = a->residual_dtype == LAMQ_BF16
+                             ? launch_forward<__nv_bfloat16, __nv_bfloat16>(s, p, grid, mode, shared, st)
+                         : a->branch_dtype == LAMQ_BF16 ? launch_forward<float, __nv_bfloat16>(s, p, grid, mode, shared, st)
+                                                        : launch_forward<float, float>(s, p, grid, mode, shared, st);
+    if (launched) return launched;
     LAMQ_CHECK_LAUNCH("lamq_norm_forward");
     return LAMQ_OK;
 }

@@ -26,7 +26,7 @@ namespace {
 
 constexpr int kNormThreads = 512;   // most threads of a block
 constexpr int kNormMaxD = 16384;    // widest row
-constexpr int kNormSums = 2;        // sums exchanged at once
+constexpr int kNormSums = 3;        // sums exchanged at once
 constexpr int kSMs = 148;
 
 // ---- loads
@@ -53,6 +53,9 @@ __device__ __forceinline__ float load_one(const __nv_bfloat16 *p) {
     return __uint_as_float((uint32_t)v << 16);
 }
 
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+
 // ---- V elements of T: 16 bytes (bf16) or 32 (fp32) where V is 8, one element where rows may begin anywhere
 
 template <typename T, int V>
@@ -60,12 +63,16 @@ struct Raw;
 
 template <>
 struct Raw<float, 8> {
-    uint4 a, b;
-    __device__ __forceinline__ void load(const float *p) { a = load16(p), b = load16(p + 4); }
-    __device__ __forceinline__ void zero() { a = b = make_uint4(0, 0, 0, 0); }
-    __device__ __forceinline__ void get(float (&f)[8]) const {
-        f[0] = __uint_as_float(a.x), f[1] = __uint_as_float(a.y), f[2] = __uint_as_float(a.z), f[3] = __uint_as_float(a.w);
-        f[4] = __uint_as_float(b.x), f[5] = __uint_as_float(b.y), f[6] = __uint_as_float(b.z), f[7] = __uint_as_float(b.w);
+    __device__ __forceinline__ static void unpack(const uint4 (&v)[2], float (&f)[8]) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            f[4 * i] = __uint_as_float(v[i].x), f[4 * i + 1] = __uint_as_float(v[i].y);
+            f[4 * i + 2] = __uint_as_float(v[i].z), f[4 * i + 3] = __uint_as_float(v[i].w);
+        }
+    }
+    __device__ __forceinline__ static void load(const float *p, float (&f)[8]) {
+        const uint4 v[2] = {load16(p), load16(p + 4)};
+        unpack(v, f);
     }
     __device__ __forceinline__ static void store(float *p, const float (&f)[8]) {
         reinterpret_cast<float4 *>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
@@ -75,16 +82,17 @@ struct Raw<float, 8> {
 
 template <>
 struct Raw<__nv_bfloat16, 8> {
-    uint4 v;
-    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { v = load16(p); }
-    __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
-    __device__ __forceinline__ void get(float (&f)[8]) const {
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    __device__ __forceinline__ static void unpack(const uint4 (&v)[1], float (&f)[8]) {
+        const uint32_t w[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             f[2 * i] = __uint_as_float(w[i] << 16);
             f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
         }
+    }
+    __device__ __forceinline__ static void load(const __nv_bfloat16 *p, float (&f)[8]) {
+        const uint4 v[1] = {load16(p)};
+        unpack(v, f);
     }
     __device__ __forceinline__ static void store(__nv_bfloat16 *p, const float (&f)[8]) {
         uint32_t w[4];
@@ -99,10 +107,7 @@ struct Raw<__nv_bfloat16, 8> {
 
 template <typename T>
 struct Raw<T, 1> {
-    float v;
-    __device__ __forceinline__ void load(const T *p) { v = load_one(p); }
-    __device__ __forceinline__ void zero() { v = 0.f; }
-    __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = v; }
+    __device__ __forceinline__ static void load(const T *p, float (&f)[1]) { f[0] = load_one(p); }
     __device__ __forceinline__ static void store(float *p, const float (&f)[1]) { *p = f[0]; }
     __device__ __forceinline__ static void store(__nv_bfloat16 *p, const float (&f)[1]) { *p = __float2bfloat16_rn(f[0]); }
 };
@@ -110,15 +115,10 @@ struct Raw<T, 1> {
 // V elements at index i of an array whose type is known when the call is made: weights, gates and their gradients.
 template <int V>
 __device__ __forceinline__ void load_typed(const void *base, int dtype, int64_t i, float (&f)[V]) {
-    if (dtype == LAMQ_F32) {
-        Raw<float, V> x;
-        x.load(reinterpret_cast<const float *>(base) + i);
-        x.get(f);
-    } else {
-        Raw<__nv_bfloat16, V> x;
-        x.load(reinterpret_cast<const __nv_bfloat16 *>(base) + i);
-        x.get(f);
-    }
+    if (dtype == LAMQ_F32)
+        Raw<float, V>::load(reinterpret_cast<const float *>(base) + i, f);
+    else
+        Raw<__nv_bfloat16, V>::load(reinterpret_cast<const __nv_bfloat16 *>(base) + i, f);
 }
 
 template <int V>
@@ -138,36 +138,164 @@ __device__ __forceinline__ const T *row_at(const lamq_rows &r, int i) {
 
 // ---- teams
 
+constexpr int kNormWarps = kNormThreads / 32;
+
 struct Team {
     int size, t, slot;  // threads of a team; this one's place; the team's place in the block
     int turn;           // which half of the scratch the next exchange uses
-    float *scratch;     // 2 x (kNormThreads / 32) x kNormSums
+    float *scratch;     // kScratch floats, 16-byte aligned
+
+    // Teams of more than a warp are at most half as many as the block's warps; each has kNormWarps floats for a sum.
+    static constexpr int kSlots = kNormWarps / 2, kHalf = kSlots * kNormSums * kNormWarps, kScratch = 2 * kHalf;
 
     __device__ Team(int size_, float *scratch_)
-        : size(size_), t(threadIdx.x % size_), slot(threadIdx.x / size_), turn(0), scratch(scratch_) {}
+        : size(size_), t(threadIdx.x % size_), slot(threadIdx.x / size_), turn(0), scratch(scratch_) {
+        if (size > 32) {  // the places of the warps that there are not add zeros
+            for (int i = threadIdx.x; i < kScratch; i += blockDim.x) scratch[i] = 0.f;
+            __syncthreads();
+        }
+    }
+
+    __device__ __forceinline__ void barrier() const {
+        if (size <= 32)
+            __syncwarp();
+        else
+            asm volatile("bar.sync %0, %1;" ::"r"(slot + 1), "r"(size) : "memory");
+    }
 
     // The sums over the team, in every thread of it and in a fixed order. All threads of the team call it (and all of the
     // warp, where teams are parts of one). Two halves of the scratch in turn: a team's thread comes to an exchange only
     // when the whole team has read the one before the last.
     template <int K>
     __device__ __forceinline__ void sum(float (&v)[K]) {
-        static_assert(K <= kNormSums, "the scratch holds kNormSums sums a warp");
-        for (int o = min(size, 32) >> 1; o > 0; o >>= 1)
+        static_assert(K <= kNormSums, "the scratch holds kNormSums sums a team");
+        if (size >= 32) {
 #pragma unroll
-            for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+            for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+        } else {
+            for (int o = size >> 1; o > 0; o >>= 1)
+#pragma unroll
+                for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+        }
         if (size <= 32) return;
-        float *const half = scratch + turn * (kNormThreads / 32 * kNormSums);
+        float *const half = scratch + turn * kHalf + slot * (kNormSums * kNormWarps);
         turn ^= 1;
-        const int first = slot * (size >> 5), warps = size >> 5;
         if ((t & 31) == 0)
 #pragma unroll
-            for (int k = 0; k < K; ++k) half[(first + (t >> 5)) * kNormSums + k] = v[k];
-        asm volatile("bar.sync %0, %1;" ::"r"(slot + 1), "r"(size) : "memory");
+            for (int k = 0; k < K; ++k) half[k * kNormWarps + (t >> 5)] = v[k];
+        barrier();
 #pragma unroll
-        for (int k = 0; k < K; ++k) v[k] = 0.f;
-        for (int w = 0; w < warps; ++w)
+        for (int k = 0; k < K; ++k) {
+            const float4 *const f = reinterpret_cast<const float4 *>(half + k * kNormWarps);
+            const float4 a = f[0];
+            v[k] = (a.x + a.y) + (a.z + a.w);
+            for (int w = 4; w < size >> 5; w += 4) {
+                const float4 b = f[w / 4];
+                v[k] += (b.x + b.y) + (b.z + b.w);
+            }
+        }
+    }
+};
+
+// ---- rows on their way
+//
+// A team's next rows are fetched into shared memory while it works on one: `stages` of them, a stage holding every tensor that
+// the call reads row by row. Vectors: a thread fetches its own packs and only it reads them. Elements: the team fetches the
+// 16-byte pieces that hold the row (whatever lies beside it in the first and the last of them comes along and is not used), and
+// meets before it reads them.
+
+enum { kTensorH, kTensorDy, kTensorDh, kTensorBranch, kTensorGate, kTensors };
+
+struct RingParams {
+    int stages, stage_bytes;          // of a block
+    int at[kTensors], image[kTensors];  // where a tensor's part of a stage begins; elements: bytes of a team's row
+};
+
+template <int V, int P>
+struct Ring {
+    unsigned char *base;
+    const RingParams &p;
+    const Team &team;
+    int packs;
+
+    __device__ Ring(void *shared, const RingParams &p_, const Team &team_, int packs_)
+        : base(reinterpret_cast<unsigned char *>(shared)), p(p_), team(team_), packs(packs_) {}
+
+    __device__ __forceinline__ static void copy16(void *to, const void *from) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+                     : "memory");
+    }
+    __device__ __forceinline__ static void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+    // The oldest row on its way has arrived, for all threads that read it. Vectors: called when the row that fills the stages is
+    // on its way, too; elements: before, since this is also where the team is through with the stage that it goes to.
+    __device__ __forceinline__ void wait() const {
+        switch (p.stages - (V == 1 ? 1 : 0)) {
+            case 1: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+            case 2: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+            case 3: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+            default: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
+        }
+        if (V == 1) team.barrier();
+    }
+
+    __device__ __forceinline__ unsigned char *part(int stage, int tensor) const {
+        return base + stage * p.stage_bytes + p.at[tensor] + (V == 1 ? team.slot * p.image[tensor] : 0);
+    }
+    __device__ __forceinline__ int after(int stage) const { return stage + 1 == p.stages ? 0 : stage + 1; }
+
+    // Starts the copies of a tensor's row.
+    template <typename T>
+    __device__ __forceinline__ void fetch(int stage, int tensor, const T *row) const {
+        unsigned char *const to = part(stage, tensor);
+        if constexpr (V == 8) {
+            constexpr int kPieces = sizeof(T) / 2;
 #pragma unroll
-            for (int k = 0; k < K; ++k) v[k] += half[(first + w) * kNormSums + k];
+            for (int q = 0; q < P; ++q) {
+                const int pack = team.t + q * team.size;
+                if (pack >= packs) break;
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i)
+                    copy16(to + ((q * kPieces + i) * blockDim.x + threadIdx.x) * 16, row + pack * 8 + i * (8 / kPieces));
+            }
+        } else {
+            const int shift = (int)(reinterpret_cast<uintptr_t>(row) & 15);
+            const unsigned char *const from = reinterpret_cast<const unsigned char *>(row) - shift;
+            const int pieces = (shift + packs * (int)sizeof(T) + 15) >> 4;
+            for (int i = team.t; i < pieces; i += team.size) copy16(to + i * 16, from + i * 16);
+        }
+    }
+
+    // This thread's pack q of the row in a stage.
+    template <typename T>
+    __device__ __forceinline__ void read(int stage, int tensor, const T *row, int q, float (&f)[V]) const {
+        const unsigned char *const from = part(stage, tensor);
+        if constexpr (V == 8) {
+            constexpr int kPieces = sizeof(T) / 2;
+            uint4 v[kPieces];
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+                v[i] = *reinterpret_cast<const uint4 *>(from + ((q * kPieces + i) * blockDim.x + threadIdx.x) * 16);
+            Raw<T, 8>::unpack(v, f);
+        } else {
+            const int shift = (int)(reinterpret_cast<uintptr_t>(row) & 15);
+            f[0] = to_float(*reinterpret_cast<const T *>(from + shift + (team.t + q * team.size) * (int)sizeof(T)));
+        }
+    }
+
+    __device__ __forceinline__ void fetch_typed(int stage, int tensor, const void *row, int dtype) const {
+        if (dtype == LAMQ_F32)
+            fetch(stage, tensor, reinterpret_cast<const float *>(row));
+        else
+            fetch(stage, tensor, reinterpret_cast<const __nv_bfloat16 *>(row));
+    }
+    __device__ __forceinline__ void read_typed(int stage, int tensor, const void *row, int dtype, int q, float (&f)[V]) const {
+        if (dtype == LAMQ_F32)
+            read(stage, tensor, reinterpret_cast<const float *>(row), q, f);
+        else
+            read(stage, tensor, reinterpret_cast<const __nv_bfloat16 *>(row), q, f);
     }
 };
 
@@ -205,6 +333,10 @@ __device__ __forceinline__ float unit_factor(Team &team, float (&x)[P][V], float
 }
 
 // ---- the host's side
+
+enum { kNormAlone, kJoinPlain, kJoinFull };  // the norm alone; a join without post and gate; any join
+
+inline int element_size(int dtype) { return dtype == LAMQ_F32 ? 4 : 2; }
 
 // How many threads share a row, and P: what they hold of it each (kWide: nothing, norm_wide.cuh).
 constexpr int kWide = 1 << 20;
@@ -280,6 +412,67 @@ inline int norm_slots(const NormShape &s, int64_t rows, int threads) {
     const int least = std::max(1, 32 / s.team), most = std::max(least, threads / s.team);
     const int64_t wanted = (rows + 2 * kSMs - 1) / (2 * kSMs);
     return (int)std::min<int64_t>(most, std::max<int64_t>(least, (wanted + least - 1) / least * least));
+}
+
+// Lets a kernel have `dynamic` bytes of shared memory beside its own. LAMQ_OK, or an error that is set.
+inline int allow_shared(const void *kernel, int dynamic) {
+    if (dynamic + Team::kScratch * (int)sizeof(float) + 32 * 1024 <= 48 * 1024) return LAMQ_OK;  // with any static array
+    const cudaError_t e = smem_limit_max_once(kernel);
+    if (e == cudaSuccess) return LAMQ_OK;
+    set_error("shared memory: %s", cudaGetErrorString(e));
+    return LAMQ_ERR_CUDA;
+}
+
+// What a call runs: its shape, its blocks and their shared memory.
+struct NormLayout {
+    NormShape shape;
+    int mode, slots, blocks;  // blocks: of an SM
+    bool few;                 // a thread holds few elements (kNormShared)
+    RingParams ring;
+    int sums_bytes, shared;   // of the dynamic shared memory: the sums that registers do not hold, and all of it
+};
+
+constexpr int kSmemSM = 220 * 1024;  // of 228 KB; each block takes 1 KB for itself
+
+// `gate_sums`: the gradient of the gate is wanted; `sums`: that of any parameter. Blocks are as many as their registers allow
+// (64 for a thread that holds few elements of few tensors, else 128), or as have room for two stages each, and stages fill
+// the room, four at most. What has no room, or two stages of rows that begin anywhere, is left to the wide kernels.
+inline NormLayout norm_layout(const lamq_norm_args &a, bool backward, bool sums, bool gate_sums) {
+    NormLayout l{};
+    const bool join = a.branch.data, gates = a.gate && a.gate_span == 1;
+    l.mode = !join ? kNormAlone : a.post || a.gate ? kJoinFull : kJoinPlain;
+    l.shape = norm_shape(a, backward);
+    NormShape &s = l.shape;
+    const int r = element_size(a.residual_dtype), b = element_size(a.branch_dtype);
+    int size[kTensors] = {r, 0, 0, join ? b : 0, gates ? element_size(a.gate_dtype) : 0};
+    if (backward) {
+        size[kTensorH] = a.dy.data ? r : 0, size[kTensorDy] = a.dy.data ? b : 0, size[kTensorDh] = a.dh.data ? r : 0;
+        size[kTensorBranch] = a.post || gate_sums ? b : 0;
+    }
+    if (s.P != kWide) {
+        l.few = s.P * s.V <= kNormShared;
+        l.slots = norm_slots(s, a.rows, backward ? kNormThreads : 256);
+        const int threads = s.team * l.slots;
+        RingParams &g = l.ring;
+        for (int k = 0; k < kTensors; ++k) {
+            g.at[k] = g.stage_bytes;
+            g.image[k] = (a.d * size[k] + 15) / 16 * 16 + 16;
+            g.stage_bytes += size[k] == 0 ? 0 : s.V == 8 ? s.P * 8 * size[k] * threads : g.image[k] * l.slots;
+        }
+        l.sums_bytes = sums && !l.few ? (l.mode == kJoinFull ? 3 : 1) * s.P * s.V * threads * (int)sizeof(float) : 0;
+        const int own = Team::kScratch * (int)sizeof(float) + 1024 + l.sums_bytes +
+                        (backward && sums && l.few ? kNormThreads * kNormShared * (int)sizeof(float) : 0);
+        l.blocks = std::max(1, (!l.few || (backward && l.mode == kJoinFull) ? 512 : 1024) / threads);
+        for (;; --l.blocks) {
+            g.stages = std::min(4, (kSmemSM / l.blocks - own) / std::max(1, g.stage_bytes));
+            if (g.stages >= 2 || l.blocks == 1) break;
+        }
+        l.shared = g.stages * g.stage_bytes + l.sums_bytes;
+        if (g.stages >= (s.V == 1 ? 2 : 1)) return l;
+    }
+    s.V = 1, s.P = kWide, s.team = kNormThreads, s.packs = a.d;
+    l.slots = 1, l.blocks = 2, l.few = false, l.shared = 0;
+    return l;
 }
 
 }  // namespace

@@ -6,19 +6,18 @@ namespace {
 
 // How the rows are dealt out, and what a call's workspace holds: partial rows of d_weight, d_post and d_gate.
 struct Plan {
-    NormShape shape;
-    int slots, per, grid, gate_mode, columns;
+    NormLayout layout;
+    int per, grid, gate_mode, columns;
     int64_t g_rows;
     size_t w_at, u_at, g_at, bytes;
 };
 
 Plan plan_of(const lamq_norm_args &a) {
     Plan q{};
-    q.shape = norm_shape(a, true);
-    const bool full = a.post || a.gate;
-    q.slots = norm_slots(q.shape, a.rows, kNormThreads);
-    const int threads = q.slots * q.shape.team;
-    const int64_t most = (int64_t)kSMs * std::max(1, (full ? 512 : 1024) / threads) * q.slots;  // workers
+    q.layout = norm_layout(a, true, a.d_weight || a.d_post || a.d_gate, a.d_gate);
+    const NormShape &shape = q.layout.shape;
+    const int slots = q.layout.slots;
+    const int64_t most = (int64_t)kSMs * q.layout.blocks * slots;  // workers
     int64_t per = std::max<int64_t>(1, (a.rows + most - 1) / most);
     q.gate_mode = kGateNone;
     if (a.d_gate) {
@@ -26,7 +25,7 @@ Plan plan_of(const lamq_norm_args &a) {
             q.gate_mode = kGateOne;
         } else if (a.gate_span == 1) {
             q.gate_mode = kGateInside;
-        } else if (a.gate_span <= per && q.shape.P != kWide) {  // a wide row's sums have no place but the partial rows
+        } else if (a.gate_span <= per && shape.P != kWide) {  // a wide row's sums have no place but the partial rows
             q.gate_mode = kGateInside;
             per = (per + a.gate_span - 1) / a.gate_span * a.gate_span;
         } else {
@@ -35,10 +34,10 @@ Plan plan_of(const lamq_norm_args &a) {
     }
     q.per = (int)per;
     const int64_t workers = (a.rows + per - 1) / per;
-    q.grid = (int)((workers + q.slots - 1) / q.slots);
+    q.grid = (int)((workers + slots - 1) / slots);
     q.columns = (a.d + 7) / 8 * 8;
     q.g_rows = q.gate_mode == kGateOne ? q.grid
-               : q.gate_mode == kGateAcross ? (int64_t)q.grid * q.slots + a.rows / a.gate_span : 0;
+               : q.gate_mode == kGateAcross ? (int64_t)q.grid * slots + a.rows / a.gate_span : 0;
     const size_t row = (size_t)q.columns * sizeof(float);
     q.w_at = 0;
     q.u_at = q.w_at + (a.d_weight ? (size_t)q.grid * row : 0);
@@ -110,10 +109,12 @@ extern "C" size_t lamq_norm_backward_workspace_size(const lamq_norm_args *a) {
 extern "C" int lamq_norm_backward(const lamq_norm_args *a, void *workspace, size_t workspace_bytes, lamq_stream_t stream) {
     if (const int st = norm_args_status(a, true)) return st;
     if (a->rows == 0 || a->d == 0) return LAMQ_OK;
-    const bool join = a->branch.data != nullptr;
     const Plan q = plan_of(*a);
     LAMQ_REQUIRE(workspace_bytes >= q.bytes, "a workspace of %zu bytes is needed", q.bytes);
     LAMQ_REQUIRE(q.bytes == 0 || workspace, "null pointer (workspace)");
+    const NormLayout &l = q.layout;
+    const int mode = l.mode;
+    const bool sums = a->d_weight || a->d_post || a->d_gate;
     BackwardParams p;
     p.h = a->residual, p.in = present(*a, true);
     p.d_residual = a->d_residual, p.d_branch = a->d_branch, p.d_gate = a->d_gate;
@@ -123,28 +124,29 @@ extern "C" int lamq_norm_backward(const lamq_norm_args *a, void *workspace, size
     p.g_part = q.g_rows ? reinterpret_cast<float *>(ws + q.g_at) : nullptr;
     p.rows = (int)a->rows, p.d = a->d;
     p.scale = a->scale, p.eps = a->eps, p.offset = a->offset, p.inv_d = 1.f / (float)a->d;
-    p.team = q.shape.team, p.slots = q.slots, p.packs = q.shape.packs, p.columns = q.columns;
+    p.team = l.shape.team, p.slots = l.slots, p.packs = l.shape.packs, p.columns = q.columns;
     p.per = q.per, p.gate_mode = q.gate_mode;
-    const int mode = !join ? kNormAlone : a->post || a->gate ? kJoinFull : kJoinPlain;
-    const bool sums = a->d_weight || a->d_post || a->d_gate;
     const cudaStream_t st = (cudaStream_t)stream;
-    const int launched = q.shape.V == 1     ? launch_backward_elements(q.shape.P, *a, &p, q.grid, mode, sums, st)
-                         : q.shape.P == 1 ? launch_backward<8, 1>(*a, p, q.grid, mode, sums, st)
-                         : q.shape.P == 2 ? launch_backward<8, 2>(*a, p, q.grid, mode, sums, st)
-                                          : launch_backward<8, 4>(*a, p, q.grid, mode, sums, st);
+    p.ring = l.ring;
+    p.sums_at = l.shared - l.sums_bytes;
+    const int shared = l.shared;
+    const int launched = l.shape.V == 1   ? launch_backward_elements(l.shape.P, *a, &p, q.grid, mode, sums, shared, st)
+                         : l.shape.P == 1 ? launch_backward<8, 1>(*a, p, q.grid, mode, sums, shared, st)
+                         : l.shape.P == 2 ? launch_backward<8, 2>(*a, p, q.grid, mode, sums, shared, st)
+                                          : launch_backward<8, 4>(*a, p, q.grid, mode, sums, shared, st);
     if (launched) return launched;
     LAMQ_CHECK_LAUNCH("lamq_norm_backward");
     if (!q.bytes) return LAMQ_OK;
     const bool gates = q.gate_mode == kGateOne || q.gate_mode == kGateAcross;
-    ReduceParams r;
-    r.w_part = p.w_part, r.u_part = p.u_part, r.g_part = p.g_part;
-    r.d_weight = a->d_weight, r.d_post = a->d_post, r.d_gate = gates ? a->d_gate : nullptr;
-    r.weight_dtype = a->weight_dtype, r.post_dtype = a->post_dtype, r.gate_dtype = a->gate_dtype;
-    r.d = a->d, r.columns = q.columns, r.grid = q.grid;
-    r.gate_one = q.gate_mode == kGateOne, r.gate_span = p.in.gate_span, r.per = q.per, r.rows = p.rows;
+    ReduceParams sum;
+    sum.w_part = p.w_part, sum.u_part = p.u_part, sum.g_part = p.g_part;
+    sum.d_weight = a->d_weight, sum.d_post = a->d_post, sum.d_gate = gates ? a->d_gate : nullptr;
+    sum.weight_dtype = a->weight_dtype, sum.post_dtype = a->post_dtype, sum.gate_dtype = a->gate_dtype;
+    sum.d = a->d, sum.columns = q.columns, sum.grid = q.grid;
+    sum.gate_one = q.gate_mode == kGateOne, sum.gate_span = p.in.gate_span, sum.per = q.per, sum.rows = p.rows;
     const int64_t jobs = (a->d_weight ? 1 : 0) + (a->d_post ? 1 : 0) +
                          (q.gate_mode == kGateOne ? 1 : q.gate_mode == kGateAcross ? a->rows / a->gate_span : 0);
-    norm_reduce_kernel<<<(unsigned)(jobs * ((a->d + 31) / 32)), kReduceWarps * 32, 0, st>>>(r);
+    norm_reduce_kernel<<<(unsigned)(jobs * ((a->d + 31) / 32)), kReduceWarps * 32, 0, st>>>(sum);
     LAMQ_CHECK_LAUNCH("lamq_norm_backward (sums)");
     return LAMQ_OK;
 }

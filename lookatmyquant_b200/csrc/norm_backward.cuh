@@ -25,12 +25,14 @@ struct BackwardParams {
     int team, slots, packs, columns;  // columns: of a partial row
     int per;        // rows of a worker
     int gate_mode;  // kGate*: where the sums of d_gate go
+    int sums_at;    // of the dynamic shared memory: where the sums that registers do not hold begin
+    RingParams ring;
 };
 
 // d_gate is not wanted; one gate row for all rows (summed like a weight's gradient); its rows are whole inside a worker's
 // range (written at once); its rows span workers (a partial for each worker and gate row that meet).
 enum { kGateNone, kGateOne, kGateInside, kGateAcross };
-enum { kNormAlone, kJoinPlain, kJoinFull };  // the norm alone; a join without post and gate; any join
+
 
 // What a thread has summed of its columns: in registers where these are few, else in shared memory that no other thread
 // touches (three sums of 16384 columns take 196608 bytes).
@@ -100,76 +102,125 @@ __device__ __forceinline__ void write_partial(const BackwardParams &p, const Tea
     }
 }
 
+// Threads that hold few packs keep the weights and gates of their columns in registers.
 template <typename R, typename B, int V, int P, int kMode, bool kSums>
-__global__ void __launch_bounds__(kNormThreads, 1) norm_backward_kernel(const __grid_constant__ BackwardParams p) {
-    __shared__ float scratch[2 * (kNormThreads / 32) * kNormSums];
+__global__ void __launch_bounds__(kNormThreads, kMode != kJoinFull && P * V <= kNormShared ? 2 : 1)
+    norm_backward_kernel(const __grid_constant__ BackwardParams p) {
+    extern __shared__ uint4 stages[];
+    __shared__ alignas(16) float scratch[Team::kScratch];
     __shared__ float shared[kSums && P * V <= kNormShared ? kNormThreads * P * V : 1];
-    extern __shared__ float columns[];  // of the sums that registers do not hold (backward_shared)
+    constexpr bool kFull = kMode == kJoinFull, kJoin = kMode != kNormAlone, kHold = P * V <= kNormShared;
     Team team(p.team, scratch);
-    constexpr bool kEarly = P * V <= 16;
-    constexpr int kStep = kSums && P * V > kNormShared ? P * V : 0;
-    Columns<P, V, !kStep> dw(columns), du(columns + (kMode == kJoinFull ? 1 : 0) * kStep * p.team),
-        dg(columns + (kMode == kJoinFull ? 2 : 0) * kStep * p.team);
+    const Ring<V, P> ring(stages, p.ring, team, p.packs);
+    float *const columns = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(stages) + p.sums_at);
+    constexpr int kStep = kSums && !kHold ? P * V : 0;
+    Columns<P, V, !kStep> dw(columns), du(columns + (kFull ? 1 : 0) * kStep * p.team), dg(columns + (kFull ? 2 : 0) * kStep * p.team);
+
+    const bool has_dy = p.in.has & kHasDy, has_dh = kJoin && (p.in.has & kHasDh), post = kFull && (p.in.has & kHasPost),
+               gate = kFull && (p.in.has & kHasGate), gates = gate && p.in.gate_span == 1,
+               gate_sums = kSums && kFull && p.gate_mode != kGateNone, branch = post || gate_sums;
+    const auto weight = [&](const void *from, int dtype, int pack, float (&w)[V]) {
+        load_typed<V>(from, dtype, pack * V, w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[e] += p.offset;
+    };
+    float w_held[kHold ? P : 1][V], u_held[kHold && kFull ? P : 1][V], gate_held[kHold && kFull ? P : 1][V];
+    int gate_of = -1;  // the gate row that is held
+    if constexpr (kHold)
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+            const int pack = team.t + q * p.team;
+            if (pack >= p.packs) break;
+            if (has_dy) weight(p.in.weight, p.in.weight_dtype, pack, w_held[q]);
+            if constexpr (kFull)
+                if (post) weight(p.in.post, p.in.post_dtype, pack, u_held[q]);
+        }
+    // a pack's weights: held, or loaded into `w`
+    const auto w_of = [&](int q, int pack, float (&w)[V]) {
+        if constexpr (kHold)
+#pragma unroll
+            for (int e = 0; e < V; ++e) w[e] = w_held[q][e];
+        else
+            weight(p.in.weight, p.in.weight_dtype, pack, w);
+    };
+    const auto u_of = [&](int q, int pack, float (&u)[V]) {
+        if constexpr (kHold && kFull)
+#pragma unroll
+            for (int e = 0; e < V; ++e) u[e] = u_held[q][e];
+        else
+            weight(p.in.post, p.in.post_dtype, pack, u);
+    };
+    const auto gate_at = [&](int row) {
+        return reinterpret_cast<const unsigned char *>(p.in.gate) +
+               (int64_t)(row / p.in.gate_span) * p.d * (p.in.gate_dtype == LAMQ_F32 ? 4 : 2);
+    };
+
     const int worker = blockIdx.x * p.slots + team.slot;
-    const bool ranges = kMode == kJoinFull && p.gate_mode >= kGateInside;  // each team its own range of rows
+    const bool ranges = kFull && p.gate_mode >= kGateInside;  // each team its own range of rows
     const int first = ranges ? worker * p.per : blockIdx.x * p.slots * p.per + team.slot, step = ranges ? 1 : p.slots;
-    for (int k = 0; k < p.per; ++k) {
+    const auto fetch = [&](int k, int stage) {
+        const int row = first + k * step;
+        if (k < p.per && row < p.rows) {
+            if (has_dy) {
+                ring.fetch(stage, kTensorH, row_at<R>(p.h, row));
+                ring.fetch(stage, kTensorDy, row_at<B>(p.in.dy, row));
+            }
+            if (has_dh) ring.fetch(stage, kTensorDh, row_at<R>(p.in.dh, row));
+            if (branch) ring.fetch(stage, kTensorBranch, row_at<B>(p.in.branch, row));
+            if (gates) ring.fetch_typed(stage, kTensorGate, gate_at(row), p.in.gate_dtype);
+        }
+        ring.commit();
+    };
+    int stage = 0, to = 0;
+    for (int i = 1; i < p.ring.stages; ++i, to = ring.after(to)) fetch(i - 1, to);
+    for (int k = 0; k < p.per; ++k, stage = ring.after(stage), to = ring.after(to)) {
         const int row = first + k * step;
         const bool live = row < p.rows;
         if (p.team < 32 ? !__any_sync(0xffffffffu, live) : !live) break;
+        if (p.ring.stages == 1) {
+            fetch(k, 0);
+            ring.wait();
+        } else if (V == 1) {  // all have read the stage that is filled next
+            ring.wait();
+            fetch(k + p.ring.stages - 1, to);
+        } else {
+            fetch(k + p.ring.stages - 1, to);
+            ring.wait();
+        }
         const int at = live ? row : 0;
-        const R *const dh = row_at<R>(p.in.dh, at);
-        const bool has_dh = kMode != kNormAlone && (p.in.has & kHasDh);
-        Raw<R, V> early[kEarly ? P : 1];
-        if (kEarly && has_dh)
+        float g[P][V], b[kFull ? P : 1][V];  // dy, then the gradient at h, then at the branch; the branch
+        float s[kFull ? 3 : 2] = {};         // Σ h², Σ t h, Σ b²
+        float x[P][V];
+        const R *const h_row = row_at<R>(p.h, at), *const dh_row = row_at<R>(p.in.dh, at);
+        const B *const dy_row = row_at<B>(p.in.dy, at), *const b_row = row_at<B>(p.in.branch, at);
 #pragma unroll
-            for (int q = 0; q < P; ++q) {
-                const int pack = team.t + q * p.team;
-                early[q].zero();
-                if (live && pack < p.packs) early[q].load(dh + pack * V);
-            }
-        // dh, a pack at a time: loaded before the row's sums, or where registers are short behind them
-        const auto add_dh = [&](int q, int pack, float (&f)[V]) {
-            if (!has_dh) return;
-            float x[V];
-            if (kEarly) {
-                early[kEarly ? q : 0].get(x);
-            } else {
-                Raw<R, V> late;
-                late.zero();
-                if (live) late.load(dh + pack * V);
-                late.get(x);
-            }
+        for (int q = 0; q < P; ++q) {
+            const int pack = team.t + q * p.team;
+            const bool in = live && pack < p.packs;
 #pragma unroll
-            for (int e = 0; e < V; ++e) f[e] += x[e];
-        };
-        float g[P][V];  // dy, then the gradient at h, then at the branch
-        if (p.in.has & kHasDy) {
-            float x[P][V], s[2] = {0.f, 0.f}, shrunk;
-            const R *const src = row_at<R>(p.h, at);
-            const B *const grad = row_at<B>(p.in.dy, at);
-#pragma unroll
-            for (int q = 0; q < P; ++q) {
-                const int pack = team.t + q * p.team;
-                Raw<R, V> a;
-                Raw<B, V> b;
-                a.zero(), b.zero();
-                if (live && pack < p.packs) a.load(src + pack * V), b.load(grad + pack * V);
-                a.get(x[q]), b.get(g[q]);
-            }
-#pragma unroll
-            for (int q = 0; q < P; ++q) {
-                const int pack = team.t + q * p.team;
-                if (pack >= p.packs) break;
+            for (int e = 0; e < V; ++e) x[q][e] = g[q][e] = 0.f;
+            if (has_dy && in) {
                 float w[V];
-                load_typed<V>(p.in.weight, p.in.weight_dtype, pack * V, w);
+                ring.read(stage, kTensorH, h_row, q, x[q]);
+                ring.read(stage, kTensorDy, dy_row, q, g[q]);
+                w_of(q, pack, w);
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     s[0] = fmaf(x[q][e], x[q][e], s[0]);
-                    s[1] = fmaf(g[q][e] * (p.offset + w[e]), x[q][e], s[1]);
+                    s[1] = fmaf(g[q][e] * w[e], x[q][e], s[1]);
                 }
             }
-            team.sum(s);
+            if constexpr (kFull) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) b[q][e] = 0.f;
+                if (branch && in) ring.read(stage, kTensorBranch, b_row, q, b[q]);
+#pragma unroll
+                for (int e = 0; e < V; ++e) s[2] = fmaf(b[q][e], b[q][e], s[2]);
+            }
+        }
+        if (has_dy || post) team.sum(s);
+        if (has_dy) {
+            float shrunk;
             const float f = unit_factor(team, x, s[0], p.inv_d, p.eps, shrunk);
             if (p.team < 32 ? __any_sync(0xffffffffu, shrunk != 1.f) : shrunk != 1.f) {
                 float again[1] = {0.f};  // x changed, and the sum may have overflowed
@@ -178,9 +229,9 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_backward_kernel(const __
                     const int pack = team.t + q * p.team;
                     if (pack >= p.packs) break;
                     float w[V];
-                    load_typed<V>(p.in.weight, p.in.weight_dtype, pack * V, w);
+                    w_of(q, pack, w);
 #pragma unroll
-                    for (int e = 0; e < V; ++e) again[0] = fmaf(g[q][e] * (p.offset + w[e]), x[q][e], again[0]);
+                    for (int e = 0; e < V; ++e) again[0] = fmaf(g[q][e] * w[e], x[q][e], again[0]);
                 }
                 team.sum(again);
                 s[1] = again[0];
@@ -192,83 +243,68 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_backward_kernel(const __
                 const int pack = team.t + q * p.team;
                 if (pack >= p.packs) break;
                 float w[V];
-                load_typed<V>(p.in.weight, p.in.weight_dtype, pack * V, w);
+                w_of(q, pack, w);
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     const float unit = x[q][e] * f;
                     if (kSums) dw.add(q, e, g[q][e], unit);
-                    g[q][e] = r * fmaf(-unit, c, g[q][e] * (p.offset + w[e]));
+                    g[q][e] = r * fmaf(-unit, c, g[q][e] * w[e]);
                 }
-                add_dh(q, pack, g[q]);
-            }
-        } else {
-#pragma unroll
-            for (int q = 0; q < P; ++q) {
-                const int pack = team.t + q * p.team;
-#pragma unroll
-                for (int e = 0; e < V; ++e) g[q][e] = 0.f;
-                if (pack < p.packs) add_dh(q, pack, g[q]);
             }
         }
-        {
-            R *const out = reinterpret_cast<R *>(p.d_residual) + (int64_t)at * p.d;
+        R *const out = reinterpret_cast<R *>(p.d_residual) + (int64_t)at * p.d;
 #pragma unroll
-            for (int q = 0; q < P; ++q) {
-                const int pack = team.t + q * p.team;
-                if (live && pack < p.packs) Raw<R, V>::store(out + pack * V, g[q]);
+        for (int q = 0; q < P; ++q) {
+            const int pack = team.t + q * p.team;
+            if (pack >= p.packs || !live) break;
+            if (has_dh) {
+                float x[V];
+                ring.read(stage, kTensorDh, dh_row, q, x);
+#pragma unroll
+                for (int e = 0; e < V; ++e) g[q][e] += x[e];
             }
+            Raw<R, V>::store(out + pack * V, g[q]);
         }
-        if (kMode == kNormAlone) continue;
+        if (!kJoin) continue;
 #pragma unroll
         for (int q = 0; q < P; ++q)
 #pragma unroll
             for (int e = 0; e < V; ++e) g[q][e] *= p.scale;
-        if (kMode == kJoinFull) {
-            float x[P][V], f = 1.f, shrunk = 1.f;  // the branch
-            if ((p.in.has & kHasPost) || p.gate_mode != kGateNone) {
-                const B *const src = row_at<B>(p.in.branch, at);
-#pragma unroll
-                for (int q = 0; q < P; ++q) {
-                    const int pack = team.t + q * p.team;
-                    Raw<B, V> a;
-                    a.zero();
-                    if (live && pack < p.packs) a.load(src + pack * V);
-                    a.get(x[q]);
-                }
-            }
-            if (p.in.has & kHasPost) {
-                float ss[1] = {0.f};
+        if constexpr (kFull) {
+            float f = 1.f, shrunk = 1.f;
+            if (post) {
+                f = unit_factor(team, b, s[2], p.inv_d, p.eps, shrunk);
 #pragma unroll
                 for (int q = 0; q < P; ++q)
 #pragma unroll
-                    for (int e = 0; e < V; ++e) ss[0] = fmaf(x[q][e], x[q][e], ss[0]);
-                team.sum(ss);
-                f = unit_factor(team, x, ss[0], p.inv_d, p.eps, shrunk);
-#pragma unroll
-                for (int q = 0; q < P; ++q)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) x[q][e] *= f;
+                    for (int e = 0; e < V; ++e) b[q][e] *= f;
             }
-            if (p.in.has & kHasGate) {
-                const int64_t gate_row = at / p.in.gate_span;
+            if (gate) {
+                const int gate_row = at / p.in.gate_span;
+                const unsigned char *const from = gate_at(at);
 #pragma unroll
                 for (int q = 0; q < P; ++q) {
                     const int pack = team.t + q * p.team;
-                    if (pack >= p.packs) break;
-                    float u[V], v[V];
-                    load_typed<V>(p.in.gate, p.in.gate_dtype, gate_row * p.d + pack * V, u);
-                    if (kSums && p.gate_mode != kGateNone) {
-                        if (p.in.has & kHasPost) load_typed<V>(p.in.post, p.in.post_dtype, pack * V, v);
+                    if (pack >= p.packs || !live) break;
+                    float v[V];
+                    if (gates)
+                        ring.read_typed(stage, kTensorGate, from, p.in.gate_dtype, q, v);
+                    else if (!kHold)
+                        load_typed<V>(from, p.in.gate_dtype, pack * V, v);
+                    else if (gate_row != gate_of)
+                        load_typed<V>(from, p.in.gate_dtype, pack * V, gate_held[kHold ? q : 0]);
+                    if (gate_sums) {
+                        float u[V];
+                        if (post) u_of(q, pack, u);
 #pragma unroll
-                        for (int e = 0; e < V; ++e) {
-                            const float b = p.in.has & kHasPost ? x[q][e] * (p.offset + v[e]) : x[q][e];
-                            dg.add(q, e, g[q][e], live ? b : 0.f);
-                        }
+                        for (int e = 0; e < V; ++e) dg.add(q, e, g[q][e], post ? b[q][e] * u[e] : b[q][e]);
                     }
 #pragma unroll
-                    for (int e = 0; e < V; ++e) g[q][e] *= u[e];
+                    for (int e = 0; e < V; ++e) g[q][e] *= kHold && !gates ? gate_held[kHold ? q : 0][e] : v[e];
                 }
-                if (kSums && p.gate_mode >= kGateInside && live && (k + 1 == p.per || (at + 1) % p.in.gate_span == 0 || at + 1 == p.rows)) {
+                if (live) gate_of = gate_row;
+                if (gate_sums && p.gate_mode >= kGateInside && live &&
+                    (k + 1 == p.per || (at + 1) % p.in.gate_span == 0 || at + 1 == p.rows)) {
 #pragma unroll
                     for (int q = 0; q < P; ++q) {
                         const int pack = team.t + q * p.team;
@@ -276,34 +312,34 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_backward_kernel(const __
                         float sum[V];
                         dg.get(q, sum);
                         if (p.gate_mode == kGateInside)
-                            store_typed<V>(p.d_gate, p.in.gate_dtype, gate_row * p.d + pack * V, sum);
+                            store_typed<V>(p.d_gate, p.in.gate_dtype, (int64_t)gate_row * p.d + pack * V, sum);
                         else  // a worker and a gate row, both growing row by row: their sum names the pair
-                            Raw<float, V>::store(p.g_part + (worker + gate_row) * p.columns + pack * V, sum);
+                            Raw<float, V>::store(p.g_part + (int64_t)(worker + gate_row) * p.columns + pack * V, sum);
                     }
                     dg.clear();
                 }
             }
-            if (p.in.has & kHasPost) {
-                float s[1] = {0.f};
+            if (post) {
+                float t[1] = {0.f};
 #pragma unroll
                 for (int q = 0; q < P; ++q) {
                     const int pack = team.t + q * p.team;
                     if (pack >= p.packs) break;
                     float u[V];
-                    load_typed<V>(p.in.post, p.in.post_dtype, pack * V, u);
+                    u_of(q, pack, u);
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
-                        if (kSums) du.add(q, e, g[q][e], x[q][e]);
-                        g[q][e] *= p.offset + u[e];
-                        s[0] = fmaf(g[q][e], x[q][e], s[0]);
+                        if (kSums) du.add(q, e, g[q][e], b[q][e]);
+                        g[q][e] *= u[e];
+                        t[0] = fmaf(g[q][e], b[q][e], t[0]);
                     }
                 }
-                team.sum(s);
-                const float r = f * shrunk, c = s[0] * p.inv_d;
+                team.sum(t);
+                const float r = f * shrunk, c = t[0] * p.inv_d;
 #pragma unroll
                 for (int q = 0; q < P; ++q)
 #pragma unroll
-                    for (int e = 0; e < V; ++e) g[q][e] = r * fmaf(-x[q][e], c, g[q][e]);
+                    for (int e = 0; e < V; ++e) g[q][e] = r * fmaf(-b[q][e], c, g[q][e]);
             }
         }
         if (p.d_branch) {
@@ -317,60 +353,48 @@ __global__ void __launch_bounds__(kNormThreads, 1) norm_backward_kernel(const __
     }
     if constexpr (kSums) {
         if (p.w_part) write_partial(p, team, dw, p.w_part, shared);
-        if (kMode == kJoinFull && p.u_part) write_partial(p, team, du, p.u_part, shared);
-        if (kMode == kJoinFull && p.gate_mode == kGateOne) write_partial(p, team, dg, p.g_part, shared);
+        if (kFull && p.u_part) write_partial(p, team, du, p.u_part, shared);
+        if (kFull && p.gate_mode == kGateOne) write_partial(p, team, dg, p.g_part, shared);
     }
-}
-
-// Dynamic shared memory of a block.
-template <int V, int P>
-int backward_shared(int mode, bool sums, int team) {
-    return sums && P * V > kNormShared ? (mode == kJoinFull ? 3 : 1) * P * V * team * (int)sizeof(float) : 0;
 }
 
 template <typename R, typename B, int V, int P, int kMode, bool kSums>
-int launch_backward(const BackwardParams &p, int grid, cudaStream_t stream) {
+int launch_backward(const BackwardParams &p, int grid, int shared, cudaStream_t stream) {
     const auto kernel = norm_backward_kernel<R, B, V, P, kMode, kSums>;
-    const int shared = backward_shared<V, P>(kMode, kSums, p.team);
-    if (shared) {
-        const cudaError_t e = smem_limit_max_once(reinterpret_cast<const void *>(kernel));
-        if (e != cudaSuccess) {
-            set_error("lamq_norm_backward: %s", cudaGetErrorString(e));
-            return LAMQ_ERR_CUDA;
-        }
-    }
+    if (const int st = allow_shared(reinterpret_cast<const void *>(kernel), shared)) return st;
     kernel<<<grid, p.team * p.slots, shared, stream>>>(p);
     return LAMQ_OK;
 }
 
 template <typename R, typename B, int V, int P>
-int launch_backward(const BackwardParams &p, int grid, int mode, bool sums, cudaStream_t stream) {
+int launch_backward(const BackwardParams &p, int grid, int mode, bool sums, int shared, cudaStream_t stream) {
     if constexpr (P * V <= kNormFull)
         if (mode == kJoinFull)
-            return sums ? launch_backward<R, B, V, P, kJoinFull, true>(p, grid, stream)
-                        : launch_backward<R, B, V, P, kJoinFull, false>(p, grid, stream);
+            return sums ? launch_backward<R, B, V, P, kJoinFull, true>(p, grid, shared, stream)
+                        : launch_backward<R, B, V, P, kJoinFull, false>(p, grid, shared, stream);
     if (mode == kJoinPlain)
-        return sums ? launch_backward<R, B, V, P, kJoinPlain, true>(p, grid, stream)
-                    : launch_backward<R, B, V, P, kJoinPlain, false>(p, grid, stream);
+        return sums ? launch_backward<R, B, V, P, kJoinPlain, true>(p, grid, shared, stream)
+                    : launch_backward<R, B, V, P, kJoinPlain, false>(p, grid, shared, stream);
     if constexpr (std::is_same_v<R, B>)
-        return sums ? launch_backward<R, B, V, P, kNormAlone, true>(p, grid, stream)
-                    : launch_backward<R, B, V, P, kNormAlone, false>(p, grid, stream);
+        return sums ? launch_backward<R, B, V, P, kNormAlone, true>(p, grid, shared, stream)
+                    : launch_backward<R, B, V, P, kNormAlone, false>(p, grid, shared, stream);
     return LAMQ_ERR_INVALID;  // no such call: the checks refuse a norm of two types, the shape a wider full join
 }
 
 // By the call's types.
 template <int V, int P>
-int launch_backward(const lamq_norm_args &a, const BackwardParams &p, int grid, int mode, bool sums, cudaStream_t stream) {
+int launch_backward(const lamq_norm_args &a, const BackwardParams &p, int grid, int mode, bool sums, int shared,
+                    cudaStream_t stream) {
     if (a.residual_dtype == LAMQ_BF16)
-        return launch_backward<__nv_bfloat16, __nv_bfloat16, V, P>(p, grid, mode, sums, stream);
-    if (a.branch_dtype == LAMQ_BF16) return launch_backward<float, __nv_bfloat16, V, P>(p, grid, mode, sums, stream);
-    return launch_backward<float, float, V, P>(p, grid, mode, sums, stream);
+        return launch_backward<__nv_bfloat16, __nv_bfloat16, V, P>(p, grid, mode, sums, shared, stream);
+    if (a.branch_dtype == LAMQ_BF16) return launch_backward<float, __nv_bfloat16, V, P>(p, grid, mode, sums, shared, stream);
+    return launch_backward<float, float, V, P>(p, grid, mode, sums, shared, stream);
 }
 
 }  // namespace
 
 // The kernels for rows that may begin anywhere (norm_backward_elements.cu). `params`: a BackwardParams.
-int launch_backward_elements(int P, const lamq_norm_args &a, const void *params, int grid, int mode, bool sums,
+int launch_backward_elements(int P, const lamq_norm_args &a, const void *params, int grid, int mode, bool sums, int shared,
                              cudaStream_t stream);
 
 }  // namespace lamq

@@ -7,7 +7,7 @@ namespace {
 
 template <typename R, typename B>
 __global__ void __launch_bounds__(kWideThreads, 1) norm_backward_wide_kernel(const __grid_constant__ BackwardParams p, int mode) {
-    __shared__ float scratch[2 * (kNormThreads / 32) * kNormSums];
+    __shared__ alignas(16) float scratch[Team::kScratch];
     Team team(kWideThreads, scratch);
     const int64_t block_row = (int64_t)blockIdx.x * p.columns;
     const bool full = mode == kJoinFull;
@@ -85,11 +85,11 @@ int launch_wide(const lamq_norm_args &a, const BackwardParams &p, int grid, int 
 
 }  // namespace
 
-int launch_backward_elements(int P, const lamq_norm_args &a, const void *params, int grid, int mode, bool sums,
+int launch_backward_elements(int P, const lamq_norm_args &a, const void *params, int grid, int mode, bool sums, int shared,
                              cudaStream_t stream) {
     const BackwardParams &p = *reinterpret_cast<const BackwardParams *>(params);
-    return P == 1   ? launch_backward<1, 1>(a, p, grid, mode, sums, stream)
-           : P == 8 ? launch_backward<1, 8>(a, p, grid, mode, sums, stream)
+    return P == 1   ? launch_backward<1, 1>(a, p, grid, mode, sums, shared, stream)
+           : P == 8 ? launch_backward<1, 8>(a, p, grid, mode, sums, shared, stream)
                     : launch_wide(a, p, grid, mode, stream);
 }
 

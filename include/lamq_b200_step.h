@@ -52,7 +52,7 @@ typedef struct lamq_norm_args {
 int lamq_norm_forward(const lamq_norm_args *args, lamq_stream_t stream);
 
 /*
- * The gradients, from dh and dy (data NULL: zero) and from `residual`, which here holds the forward's h (the norm alone:
+ * The gradients, from dh and dy (data NULL: zero; the norm alone has a dy) and from `residual`, which here holds the forward's h (the norm alone:
  * its input), the statistics being computed again. d_residual is always written; d_branch (NULL: not wanted, as where it
  * equals d_residual), d_weight, d_post and d_gate where they are not NULL. The gradient of a weight or of a shared gate is
  * summed in fp32 in a fixed order: equal calls give equal bits. Workspace: lamq_norm_backward_workspace_size(args) bytes,

@@ -12,7 +12,6 @@ namespace lamq {
 namespace {
 
 struct ForwardParams {
-    lamq_rows residual;
     Present in;
     void *h, *y;
     int rows, d;
@@ -21,146 +20,135 @@ struct ForwardParams {
     RingParams ring;
 };
 
-// The weights' and gates' packs of a thread that holds few of them stay in its registers.
+// Threads that hold few elements keep the weights and the gate of their columns in registers.
 template <typename R, typename B, int V, int P, int kMode>
 __global__ void __launch_bounds__(kNormThreads, P * V <= 8 ? 2 : 1) norm_forward_kernel(const __grid_constant__ ForwardParams p) {
     extern __shared__ uint4 stages[];
     __shared__ alignas(16) float scratch[Team::kScratch];
     constexpr bool kBranch = kMode != kNormAlone, kFull = kMode == kJoinFull, kHold = P * V <= kNormShared;
+    using Row = Vec<P * V>;
     Team team(p.team, scratch);
     const Ring<V, P> ring(stages, p.ring, team, p.packs);
     const bool post = kFull && (p.in.has & kHasPost), gate = kFull && (p.in.has & kHasGate), pre = p.in.has & kHasWeight;
     const bool gates = gate && p.in.gate_span == 1;  // a gate row for each row
-    const auto weight = [&](const void *from, int dtype, int pack, float (&w)[V]) {
-        load_typed<V>(from, dtype, pack * V, w);
-#pragma unroll
-        for (int e = 0; e < V; ++e) w[e] += p.offset;
-    };
-    float w_held[kHold ? P : 1][V], u_held[kHold && kFull ? P : 1][V], gate_held[kHold && kFull ? P : 1][V];
-    int gate_row = -1;
-    if constexpr (kHold)
+    const auto each = [&](auto f) {  // this thread's packs
 #pragma unroll
         for (int q = 0; q < P; ++q) {
             const int pack = team.t + q * p.team;
-            if (pack >= p.packs) break;
-            if (pre) weight(p.in.weight, p.in.weight_dtype, pack, w_held[q]);
-            if constexpr (kFull)
-                if (post) weight(p.in.post, p.in.post_dtype, pack, u_held[q]);
+            if (pack < p.packs) f(q, pack);
         }
+    };
+    const auto load = [&](const void *from, int dtype, float add, Row &w) {  // a weight, or a row of the gate
+        w.clear();
+        each([&](int q, int pack) {
+            float f[V];
+            load_typed<V>(from, dtype, pack * V, f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] += add;
+            w.set(q * V, f);
+        });
+    };
     const auto gate_at = [&](int row) {
         return reinterpret_cast<const unsigned char *>(p.in.gate) +
-               (int64_t)(row / p.in.gate_span) * p.d * (p.in.gate_dtype == LAMQ_F32 ? 4 : 2);
+               (int64_t)p.in.by_span.of(row) * p.d * (p.in.gate_dtype == LAMQ_F32 ? 4 : 2);
     };
+    Row w, u, held;
+    int gate_row = -1;  // the gate row that is held
+    if (kHold) {
+        if (pre) load(p.in.weight, p.in.weight_dtype, p.offset, w);
+        if (kFull && post) load(p.in.post, p.in.post_dtype, p.offset, u);
+    }
     const int step = gridDim.x * p.slots, first = blockIdx.x * p.slots + team.slot;
     const auto fetch = [&](int row, int stage) {
-        if (row < p.rows) {
-            ring.fetch(stage, kTensorH, row_at<R>(p.residual, row));
-            if (kBranch) ring.fetch(stage, kTensorBranch, row_at<B>(p.in.branch, row));
-            if (gates) ring.fetch_typed(stage, kTensorGate, gate_at(row), p.in.gate_dtype);
+        if (row < p.rows || p.team < 32) {  // a team that has no row beside others of its warp that do: zeros
+            const int at = row < p.rows ? row : 0, bytes = row < p.rows ? 16 : 0;
+            ring.fetch(stage, kTensorH, row_at<R>(p.in.h, at), bytes);
+            if (kBranch) ring.fetch(stage, kTensorBranch, row_at<B>(p.in.branch, at), bytes);
+            if (gates) ring.fetch_typed(stage, kTensorGate, gate_at(at), p.in.gate_dtype, bytes);
         }
         ring.commit();
+    };
+    const auto read = [&](int stage, int tensor, const auto *row, Row &x) {
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+            float f[V];
+            ring.read(stage, tensor, row, q, f);
+            x.set(q * V, f);
+        }
     };
     int stage = 0, to = 0, ahead = first;
     for (int i = 1; i < p.ring.stages; ++i, ahead += step, to = ring.after(to)) fetch(ahead, to);
     // Teams of a warp take steps together: the loop ends when the first of them has no row.
     const int lead = p.team < 32 ? team.slot % (32 / p.team) : 0;
-    for (int row = first; row - lead < p.rows; row += step, ahead += step, stage = ring.after(stage), to = ring.after(to)) {
-        if (p.ring.stages == 1) {
-            fetch(row, 0);
+    for (int row = first; row - lead < p.rows; row += step, ahead += step) {
+        if (V == 1 && p.ring.stages > 1) {  // all have read the stage that is filled next
             ring.wait();
+            fetch(ahead, to);
         } else {
-            if (V == 1) {
-                ring.wait();
-                fetch(ahead, to);
-            } else {
-                fetch(ahead, to);
-                ring.wait();
-            }
+            fetch(ahead, to);
+            ring.wait();
         }
         const bool live = row < p.rows;
         const int at = live ? row : 0;
-        float x[P][V];
-        const R *const src = row_at<R>(p.residual, at);
-        if constexpr (kBranch) {
-            const B *const add = row_at<B>(p.in.branch, at);
-#pragma unroll
-            for (int q = 0; q < P; ++q) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) x[q][e] = 0.f;
-                if (live && team.t + q * p.team < p.packs) ring.read(stage, kTensorBranch, add, q, x[q]);
-            }
-        }
+        Row x;
+        if constexpr (kBranch) read(stage, kTensorBranch, row_at<B>(p.in.branch, at), x);
         if constexpr (kFull) {
             if (post) {
-                float ss[1] = {0.f}, shrunk;
-#pragma unroll
-                for (int q = 0; q < P; ++q)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) ss[0] = fmaf(x[q][e], x[q][e], ss[0]);
+                float ss[1] = {x.dot(x)}, shrunk;
                 team.sum(ss);
                 const float f = unit_factor(team, x, ss[0], p.inv_d, p.eps, shrunk);
-#pragma unroll
-                for (int q = 0; q < P; ++q) {
-                    const int pack = team.t + q * p.team;
-                    if (pack >= p.packs) break;
-                    float u[V];
-                    if (!kHold) weight(p.in.post, p.in.post_dtype, pack, u);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) x[q][e] *= f * (kHold ? u_held[kHold ? q : 0][e] : u[e]);
-                }
+                if (!kHold) load(p.in.post, p.in.post_dtype, p.offset, u);
+                x *= f;
+                x *= u;
             }
-            if (gate) {
-                const int g = at / p.in.gate_span;
-                const unsigned char *const from = gate_at(at);
+            if (gate && live) {
+                const unsigned char *const from = gate_at(row);
+                if (gates) {
 #pragma unroll
-                for (int q = 0; q < P; ++q) {
-                    const int pack = team.t + q * p.team;
-                    if (pack >= p.packs || !live) break;
-                    float u[V];
-                    if (gates)
-                        ring.read_typed(stage, kTensorGate, from, p.in.gate_dtype, q, u);
-                    else if (!kHold)
-                        load_typed<V>(from, p.in.gate_dtype, pack * V, u);
-                    else if (g != gate_row)
-                        load_typed<V>(from, p.in.gate_dtype, pack * V, gate_held[kHold ? q : 0]);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) x[q][e] *= kHold && !gates ? gate_held[kHold ? q : 0][e] : u[e];
+                    for (int q = 0; q < P; ++q) {
+                        float f[V];
+                        ring.read_typed(stage, kTensorGate, from, p.in.gate_dtype, q, f);
+                        held.set(q * V, f);
+                    }
+                } else if (p.in.by_span.of(row) != gate_row) {
+                    gate_row = p.in.by_span.of(row);
+                    load(from, p.in.gate_dtype, 0.f, held);
                 }
-                if (live) gate_row = g;
+                x *= held;
             }
         }
-        R *const out = reinterpret_cast<R *>(p.h) + (int64_t)at * p.d;
-#pragma unroll
-        for (int q = 0; q < P; ++q) {
-            const int pack = team.t + q * p.team;
-            float r[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) r[e] = 0.f;
-            if (live && pack < p.packs) ring.read(stage, kTensorH, src, q, r);
-#pragma unroll
-            for (int e = 0; e < V; ++e) x[q][e] = kBranch ? fmaf(p.scale, x[q][e], r[e]) : r[e];
-            if (kBranch && live && pack < p.packs) Raw<R, V>::store(out + pack * V, x[q]);
+        if constexpr (kBranch) {
+            Row r;
+            read(stage, kTensorH, row_at<R>(p.in.h, at), r);
+            x.scale_add(p.scale, r);
+        } else {
+            read(stage, kTensorH, row_at<R>(p.in.h, at), x);
+        }
+        if (kBranch && live) {
+            R *const out = reinterpret_cast<R *>(p.h) + (int64_t)row * p.d;
+            each([&](int q, int pack) {
+                float f[V];
+                x.get(q * V, f);
+                Raw<R, V>::store(out + pack * V, f);
+            });
         }
         if (pre) {
-            float ss[1] = {0.f}, shrunk;
-#pragma unroll
-            for (int q = 0; q < P; ++q)
-#pragma unroll
-                for (int e = 0; e < V; ++e) ss[0] = fmaf(x[q][e], x[q][e], ss[0]);
+            float ss[1] = {x.dot(x)}, shrunk;
             team.sum(ss);
             const float f = unit_factor(team, x, ss[0], p.inv_d, p.eps, shrunk);
-            B *const normed = reinterpret_cast<B *>(p.y) + (int64_t)at * p.d;
-#pragma unroll
-            for (int q = 0; q < P; ++q) {
-                const int pack = team.t + q * p.team;
-                if (pack >= p.packs) break;
-                float w[V];
-                if (!kHold) weight(p.in.weight, p.in.weight_dtype, pack, w);
-#pragma unroll
-                for (int e = 0; e < V; ++e) w[e] = x[q][e] * f * (kHold ? w_held[kHold ? q : 0][e] : w[e]);
-                if (live) Raw<B, V>::store(normed + pack * V, w);
+            if (!kHold) load(p.in.weight, p.in.weight_dtype, p.offset, w);
+            x *= f;
+            x *= w;
+            if (live) {
+                B *const out = reinterpret_cast<B *>(p.y) + (int64_t)row * p.d;
+                each([&](int q, int pack) {
+                    float f[V];
+                    x.get(q * V, f);
+                    Raw<B, V>::store(out + pack * V, f);
+                });
             }
         }
+        stage = ring.after(stage), to = ring.after(to);
     }
 }
 
@@ -169,7 +157,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) norm_forward_wide_kernel(cons
     __shared__ alignas(16) float scratch[Team::kScratch];
     Team team(kWideThreads, scratch);
     for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const R *const src = row_at<R>(p.residual, row);
+        const R *const src = row_at<R>(p.in.h, row);
         const B *const add = row_at<B>(p.in.branch, kBranch ? row : 0);
         const int64_t g = (int64_t)(row / p.in.gate_span) * p.d;
         float shrunk, f = 1.f;
@@ -266,6 +254,7 @@ int norm_args_status(const lamq_norm_args *a, bool backward) {
     } else {
         LAMQ_REQUIRE(a->d_residual, "null pointer (d_residual)");
         LAMQ_REQUIRE(join || !a->dh.data, "the norm alone has no dh");
+        LAMQ_REQUIRE(join || a->dy.data, "null pointer (dy)");
         LAMQ_REQUIRE(join || !a->d_branch, "the norm alone has no d_branch");
         LAMQ_REQUIRE(a->weight || (!a->d_weight && !a->dy.data), "dy and d_weight belong to a weight");
         LAMQ_REQUIRE(a->post || !a->d_post, "d_post belongs to a post weight");
@@ -285,7 +274,7 @@ extern "C" int lamq_norm_forward(const lamq_norm_args *a, lamq_stream_t stream) 
     const NormShape &s = l.shape;
     const int mode = l.mode, shared = l.shared;
     ForwardParams p;
-    p.residual = a->residual, p.in = present(*a, false);
+    p.in = present(*a, false);
     p.h = a->h, p.y = a->y;
     p.rows = (int)a->rows, p.d = a->d;
     p.scale = a->scale, p.eps = a->eps, p.offset = a->offset, p.inv_d = 1.f / (float)a->d;

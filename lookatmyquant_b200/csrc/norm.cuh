@@ -129,11 +129,129 @@ __device__ __forceinline__ void store_typed(void *base, int dtype, int64_t i, co
         Raw<__nv_bfloat16, V>::store(reinterpret_cast<__nv_bfloat16 *>(base) + i, f);
 }
 
+// ---- what a thread holds of a row: E elements, worked on in pairs (one instruction for two)
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t &>(d))
+        : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)),
+          "l"(reinterpret_cast<const uint64_t &>(c)));
+    return d;
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t &>(d))
+        : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)));
+    return d;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t &>(d))
+        : "l"(reinterpret_cast<const uint64_t &>(a)), "l"(reinterpret_cast<const uint64_t &>(b)));
+    return d;
+}
+
+template <int E>
+struct Vec {
+    static constexpr int kPairs = (E + 1) / 2;
+    float2 v[kPairs];  // the last half of an odd E is zero
+
+    __device__ __forceinline__ Vec() {
+        if constexpr (E % 2) v[kPairs - 1].y = 0.f;
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) v[i] = make_float2(0.f, 0.f);
+    }
+    // N elements from the Ith on (pairs, or one element)
+    template <int N>
+    __device__ __forceinline__ void set(int at, const float (&f)[N]) {
+        if constexpr (N == 1) {
+            if (at & 1)
+                v[at / 2].y = f[0];
+            else
+                v[at / 2].x = f[0];
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i += 2) v[(at + i) / 2] = make_float2(f[i], f[i + 1]);
+        }
+    }
+    template <int N>
+    __device__ __forceinline__ void get(int at, float (&f)[N]) const {
+        if constexpr (N == 1) {
+            f[0] = at & 1 ? v[at / 2].y : v[at / 2].x;
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i += 2) f[i] = v[(at + i) / 2].x, f[i + 1] = v[(at + i) / 2].y;
+        }
+    }
+    __device__ __forceinline__ void operator*=(float f) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) v[i] = mul2(v[i], make_float2(f, f));
+    }
+    __device__ __forceinline__ void operator*=(const Vec &b) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) v[i] = mul2(v[i], b.v[i]);
+    }
+    __device__ __forceinline__ void operator+=(const Vec &b) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) v[i] = add2(v[i], b.v[i]);
+    }
+    // this + a·b
+    __device__ __forceinline__ void add(const Vec &a, const Vec &b) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) v[i] = fma2(a.v[i], b.v[i], v[i]);
+    }
+    // this·f + b
+    __device__ __forceinline__ void scale_add(float f, const Vec &b) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) v[i] = fma2(v[i], make_float2(f, f), b.v[i]);
+    }
+    // (this − f·b)·r
+    __device__ __forceinline__ void take(float f, const Vec &b, float r) {
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) v[i] = mul2(fma2(b.v[i], make_float2(-f, -f), v[i]), make_float2(r, r));
+    }
+    __device__ __forceinline__ float dot(const Vec &b) const {
+        float2 s = mul2(v[0], b.v[0]);
+#pragma unroll
+        for (int i = 1; i < kPairs; ++i) s = fma2(v[i], b.v[i], s);
+        return s.x + s.y;
+    }
+};
+
+// i / by for 0 <= i < 2^31 and by >= 1: with 2^(l-1) < by <= 2^l, the upper bits of i · ceil(2^(31+l) / by). (The product
+// exceeds i · 2^(31+l) / by by less than 2^31 · by / by <= 2^(31+l) / by, what the next multiple is away.)
+struct Divisor {
+    uint32_t times;
+    int shift;
+    __device__ __forceinline__ int of(int i) const { return (int)((uint64_t)(uint32_t)i * times >> shift); }
+};
+
+inline Divisor divisor(int64_t by) {
+    int l = 0;
+    while (((int64_t)1 << l) < by) ++l;
+    return {(uint32_t)((((uint64_t)1 << (31 + l)) + by - 1) / by), 31 + l};
+}
+
+// A tensor's rows: at one stride of `stride` bytes, or (stride < 0) at two.
+struct Rows {
+    const unsigned char *data;
+    int64_t row, outer;  // bytes
+    int stride, inner;
+    Divisor by_inner;
+};
+
 template <typename T>
-__device__ __forceinline__ const T *row_at(const lamq_rows &r, int i) {
-    const int inner = (int)r.inner;  // the host keeps it within an int
-    const int o = i / inner;
-    return reinterpret_cast<const T *>(r.data) + o * r.outer + (i - o * inner) * r.row;
+__device__ __forceinline__ const T *row_at(const Rows &r, int i) {
+    if (r.stride >= 0) return reinterpret_cast<const T *>(r.data + (int64_t)i * r.stride);
+    const int o = r.by_inner.of(i);
+    return reinterpret_cast<const T *>(r.data + o * r.outer + (i - o * r.inner) * r.row);
 }
 
 // ---- teams
@@ -169,34 +287,45 @@ struct Team {
     template <int K>
     __device__ __forceinline__ void sum(float (&v)[K]) {
         static_assert(K <= kNormSums, "the scratch holds kNormSums sums a team");
-        if (size >= 32) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-                for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
-        } else {
+        if (size <= 32) {
             for (int o = size >> 1; o > 0; o >>= 1)
 #pragma unroll
                 for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+            return;
         }
-        if (size <= 32) return;
+        // Half of the lanes go on with one sum, half with another: 6 exchanges for two sums (7 for three) instead of 10 (15).
+        const int lane = t & 31;
+        float s = v[0];
+        int mine = 0;
+        if constexpr (K == 3) {
+            const bool up = lane & 16;
+            const float keep = (up ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, up ? v[0] : v[1], 16);
+            const float last = v[2] + __shfl_xor_sync(0xffffffffu, v[2], 16);
+            const bool third = lane & 8;  // lanes 8 to 15 and 24 to 31 take the third sum
+            s = (third ? last : keep) + __shfl_xor_sync(0xffffffffu, third ? keep : last, 8);
+            mine = third ? 2 : up;
+        } else if constexpr (K == 2) {
+            const bool up = lane & 16;
+            s = (up ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, up ? v[0] : v[1], 16);
+            mine = up;
+        }
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1)
+            if (x <= (K == 3 ? 4 : K == 2 ? 8 : 16)) s += __shfl_xor_sync(0xffffffffu, s, x);
         float *const half = scratch + turn * kHalf + slot * (kNormSums * kNormWarps);
         turn ^= 1;
-        if ((t & 31) == 0)
-#pragma unroll
-            for (int k = 0; k < K; ++k) half[k * kNormWarps + (t >> 5)] = v[k];
+        if (lane == 0 || (K >= 2 && lane == 16) || (K == 3 && lane == 8)) half[mine * kNormWarps + (t >> 5)] = s;
         barrier();
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const float4 *const f = reinterpret_cast<const float4 *>(half + k * kNormWarps);
-            const float4 a = f[0];
-            v[k] = (a.x + a.y) + (a.z + a.w);
-            for (int w = 4; w < size >> 5; w += 4) {
-                const float4 b = f[w / 4];
-                v[k] += (b.x + b.y) + (b.z + b.w);
-            }
+            float2 a = four(f[0]);
+            if (size > 128) a = add2(a, four(f[1]));
+            if (size > 256) a = add2(a, add2(four(f[2]), four(f[3])));
+            v[k] = a.x + a.y;
         }
     }
+    __device__ __forceinline__ static float2 four(float4 f) { return add2(make_float2(f.x, f.y), make_float2(f.z, f.w)); }
 };
 
 // ---- rows on their way
@@ -211,6 +340,7 @@ enum { kTensorH, kTensorDy, kTensorDh, kTensorBranch, kTensorGate, kTensors };
 struct RingParams {
     int stages, stage_bytes;          // of a block
     int at[kTensors], image[kTensors];  // where a tensor's part of a stage begins; elements: bytes of a team's row
+    int size[kTensors];                 // of an element; 0: the call does not read the tensor
 };
 
 template <int V, int P>
@@ -221,10 +351,19 @@ struct Ring {
     int packs;
 
     __device__ Ring(void *shared, const RingParams &p_, const Team &team_, int packs_)
-        : base(reinterpret_cast<unsigned char *>(shared)), p(p_), team(team_), packs(packs_) {}
+        : base(reinterpret_cast<unsigned char *>(shared)), p(p_), team(team_), packs(packs_) {
+        if constexpr (V == 8)  // a thread's places behind the row's end hold zeros throughout, so that it reads all of its places
+            for (int s = 0; s < p.stages; ++s)
+                for (int k = 0; k < kTensors; ++k)
+                    for (int i = 0; i < P * (p.size[k] >> 1); ++i)
+                        if (team.t + i / (p.size[k] >> 1) * team.size >= packs)
+                            *reinterpret_cast<uint4 *>(part(s, k) + (i * blockDim.x + threadIdx.x) * 16) = make_uint4(0, 0, 0, 0);
+    }
 
-    __device__ __forceinline__ static void copy16(void *to, const void *from) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+    // 16 bytes, or (bytes = 0) as many zeros
+    __device__ __forceinline__ static void copy16(void *to, const void *from, int bytes) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from),
+                     "r"(bytes)
                      : "memory");
     }
     __device__ __forceinline__ static void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -246,9 +385,9 @@ struct Ring {
     }
     __device__ __forceinline__ int after(int stage) const { return stage + 1 == p.stages ? 0 : stage + 1; }
 
-    // Starts the copies of a tensor's row.
+    // Starts the copies of a tensor's row (bytes = 0: of a row of zeros).
     template <typename T>
-    __device__ __forceinline__ void fetch(int stage, int tensor, const T *row) const {
+    __device__ __forceinline__ void fetch(int stage, int tensor, const T *row, int bytes) const {
         unsigned char *const to = part(stage, tensor);
         if constexpr (V == 8) {
             constexpr int kPieces = sizeof(T) / 2;
@@ -258,13 +397,13 @@ struct Ring {
                 if (pack >= packs) break;
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i)
-                    copy16(to + ((q * kPieces + i) * blockDim.x + threadIdx.x) * 16, row + pack * 8 + i * (8 / kPieces));
+                    copy16(to + ((q * kPieces + i) * blockDim.x + threadIdx.x) * 16, row + pack * 8 + i * (8 / kPieces), bytes);
             }
         } else {
             const int shift = (int)(reinterpret_cast<uintptr_t>(row) & 15);
             const unsigned char *const from = reinterpret_cast<const unsigned char *>(row) - shift;
             const int pieces = (shift + packs * (int)sizeof(T) + 15) >> 4;
-            for (int i = team.t; i < pieces; i += team.size) copy16(to + i * 16, from + i * 16);
+            for (int i = team.t; i < pieces; i += team.size) copy16(to + i * 16, from + i * 16, bytes);
         }
     }
 
@@ -281,15 +420,16 @@ struct Ring {
             Raw<T, 8>::unpack(v, f);
         } else {
             const int shift = (int)(reinterpret_cast<uintptr_t>(row) & 15);
-            f[0] = to_float(*reinterpret_cast<const T *>(from + shift + (team.t + q * team.size) * (int)sizeof(T)));
+            const int pack = team.t + q * team.size;
+            f[0] = pack < packs ? to_float(*reinterpret_cast<const T *>(from + shift + pack * (int)sizeof(T))) : 0.f;
         }
     }
 
-    __device__ __forceinline__ void fetch_typed(int stage, int tensor, const void *row, int dtype) const {
+    __device__ __forceinline__ void fetch_typed(int stage, int tensor, const void *row, int dtype, int bytes) const {
         if (dtype == LAMQ_F32)
-            fetch(stage, tensor, reinterpret_cast<const float *>(row));
+            fetch(stage, tensor, reinterpret_cast<const float *>(row), bytes);
         else
-            fetch(stage, tensor, reinterpret_cast<const __nv_bfloat16 *>(row));
+            fetch(stage, tensor, reinterpret_cast<const __nv_bfloat16 *>(row), bytes);
     }
     __device__ __forceinline__ void read_typed(int stage, int tensor, const void *row, int dtype, int q, float (&f)[V]) const {
         if (dtype == LAMQ_F32)
@@ -311,20 +451,14 @@ constexpr float kShrink = 0x1p-80f;  // brings fp32's largest numbers where 1638
 // The factor (mean(x²) + eps)^-1/2 of a row, from the sum of squares, for x as it stands after the call: where the sum
 // overflowed, x is multiplied by kShrink and summed again (eps is then far below the mean's last bit). `shrunk` is
 // kShrink or 1: the factor of x as it was is the result times `shrunk`.
-template <int P, int V>
-__device__ __forceinline__ float unit_factor(Team &team, float (&x)[P][V], float ss, float inv_d, float eps, float &shrunk) {
+template <int E>
+__device__ __forceinline__ float unit_factor(Team &team, Vec<E> &x, float ss, float inv_d, float eps, float &shrunk) {
     shrunk = 1.f;
     const bool over = isinf(ss);
     if (team.size < 32 ? __any_sync(0xffffffffu, over) : over) {
         if (over) shrunk = kShrink;
-        float again[1] = {0.f};
-#pragma unroll
-        for (int q = 0; q < P; ++q)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                x[q][e] *= shrunk;
-                again[0] = fmaf(x[q][e], x[q][e], again[0]);
-            }
+        x *= shrunk;
+        float again[1] = {x.dot(x)};
         team.sum(again);
         ss = again[0];
         if (over) eps = 0.f;
@@ -335,8 +469,6 @@ __device__ __forceinline__ float unit_factor(Team &team, float (&x)[P][V], float
 // ---- the host's side
 
 enum { kNormAlone, kJoinPlain, kJoinFull };  // the norm alone; a join without post and gate; any join
-
-inline int element_size(int dtype) { return dtype == LAMQ_F32 ? 4 : 2; }
 
 // How many threads share a row, and P: what they hold of it each (kWide: nothing, norm_wide.cuh).
 constexpr int kWide = 1 << 20;
@@ -351,24 +483,38 @@ enum { kHasWeight = 1, kHasPost = 2, kHasGate = 4, kHasDh = 8, kHasDy = 16, kHas
 
 struct Present {
     int has;
-    lamq_rows branch, dh, dy;
+    Rows h, branch, dh, dy;  // h: the norm's input, or what the branch is added to
     const void *weight, *post, *gate;
     int weight_dtype, post_dtype, gate_dtype, gate_span;
+    Divisor by_span;
 };
+
+inline int element_size(int dtype) { return dtype == LAMQ_F32 ? 4 : 2; }
+
+inline Rows rows_of(const lamq_rows &r, int64_t rows, int size) {
+    Rows x;
+    x.data = reinterpret_cast<const unsigned char *>(r.data);
+    x.row = r.row * size, x.outer = r.outer * size, x.inner = (int)r.inner, x.by_inner = divisor(r.inner);
+    const bool flat = r.inner >= rows || r.outer == r.inner * r.row;
+    x.stride = flat && x.row >= 0 && x.row <= INT_MAX ? (int)x.row : -1;
+    return x;
+}
 
 inline Present present(const lamq_norm_args &a, bool backward) {
     const void *const out = backward ? a.d_residual : a.branch.data ? a.h : a.y;
     const lamq_rows rows{const_cast<void *>(out), INT_MAX, a.d, 0};
+    const int r = element_size(a.residual_dtype), b = element_size(a.branch_dtype);
     Present p;
     p.has = (a.weight ? kHasWeight : 0) | (a.post ? kHasPost : 0) | (a.gate ? kHasGate : 0) |
             (a.branch.data ? kHasBranch : 0) | (backward && a.dh.data ? kHasDh : 0) | (backward && a.dy.data ? kHasDy : 0);
-    p.branch = a.branch.data ? a.branch : rows;
-    p.dh = p.has & kHasDh ? a.dh : rows;
-    p.dy = p.has & kHasDy ? a.dy : rows;
+    p.h = rows_of(a.residual, a.rows, r);
+    p.branch = rows_of(a.branch.data ? a.branch : rows, a.rows, b);
+    p.dh = rows_of(p.has & kHasDh ? a.dh : rows, a.rows, r);
+    p.dy = rows_of(p.has & kHasDy ? a.dy : rows, a.rows, b);
     p.weight = a.weight ? a.weight : out, p.weight_dtype = a.weight ? a.weight_dtype : a.residual_dtype;
     p.post = a.post ? a.post : out, p.post_dtype = a.post ? a.post_dtype : a.residual_dtype;
     p.gate = a.gate ? a.gate : out, p.gate_dtype = a.gate ? a.gate_dtype : a.residual_dtype;
-    p.gate_span = a.gate ? (int)a.gate_span : 1;
+    p.gate_span = a.gate ? (int)a.gate_span : 1, p.by_span = divisor(p.gate_span);
     return p;
 }
 
@@ -455,7 +601,7 @@ inline NormLayout norm_layout(const lamq_norm_args &a, bool backward, bool sums,
         const int threads = s.team * l.slots;
         RingParams &g = l.ring;
         for (int k = 0; k < kTensors; ++k) {
-            g.at[k] = g.stage_bytes;
+            g.at[k] = g.stage_bytes, g.size[k] = size[k];
             g.image[k] = (a.d * size[k] + 15) / 16 * 16 + 16;
             g.stage_bytes += size[k] == 0 ? 0 : s.V == 8 ? s.P * 8 * size[k] * threads : g.image[k] * l.slots;
         }

@@ -116,7 +116,7 @@ extern "C" int lamq_norm_backward(const lamq_norm_args *a, void *workspace, size
     const int mode = l.mode;
     const bool sums = a->d_weight || a->d_post || a->d_gate;
     BackwardParams p;
-    p.h = a->residual, p.in = present(*a, true);
+    p.in = present(*a, true);
     p.d_residual = a->d_residual, p.d_branch = a->d_branch, p.d_gate = a->d_gate;
     char *const ws = reinterpret_cast<char *>(workspace);
     p.w_part = a->d_weight ? reinterpret_cast<float *>(ws + q.w_at) : nullptr;

@@ -16,7 +16,6 @@ namespace lamq {
 namespace {
 
 struct BackwardParams {
-    lamq_rows h;
     Present in;
     void *d_residual, *d_branch, *d_gate;
     float *w_part, *u_part, *g_part;  // partial sums of d_weight, d_post and a shared d_gate (NULL: not wanted)
@@ -36,325 +35,263 @@ enum { kGateNone, kGateOne, kGateInside, kGateAcross };
 
 // What a thread has summed of its columns: in registers where these are few, else in shared memory that no other thread
 // touches (three sums of 16384 columns take 196608 bytes).
-template <int P, int V, bool kRegisters = P * V <= kNormShared>
+template <int E, bool kRegisters>
 struct Columns {
-    float v[P][V];
-    __device__ __forceinline__ Columns(float *) { clear(); }
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int q = 0; q < P; ++q)
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[q][e] = 0.f;
-    }
-    __device__ __forceinline__ void add(int q, int e, float a, float b) { v[q][e] = fmaf(a, b, v[q][e]); }
-    __device__ __forceinline__ void get(int q, float (&f)[V]) const {
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = v[q][e];
-    }
+    Vec<E> v;
+    __device__ __forceinline__ Columns(float *) { v.clear(); }
+    __device__ __forceinline__ void clear() { v.clear(); }
+    __device__ __forceinline__ void add(const Vec<E> &a, const Vec<E> &b) { v.add(a, b); }
+    __device__ __forceinline__ Vec<E> all() const { return v; }
 };
 
-template <int P, int V>
-struct Columns<P, V, false> {
-    float *at;
-    __device__ __forceinline__ Columns(float *shared) : at(shared + threadIdx.x) { clear(); }
-    __device__ __forceinline__ float &of(int q, int e) { return at[(q * V + e) * blockDim.x]; }
+template <int E>
+struct Columns<E, false> {
+    float2 *at;  // pair i of this thread: at[i * blockDim.x]
+    __device__ __forceinline__ Columns(float *shared) : at(reinterpret_cast<float2 *>(shared) + threadIdx.x) { clear(); }
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int q = 0; q < P; ++q)
-#pragma unroll
-            for (int e = 0; e < V; ++e) of(q, e) = 0.f;
+        for (int i = 0; i < Vec<E>::kPairs; ++i) at[i * blockDim.x] = make_float2(0.f, 0.f);
     }
-    __device__ __forceinline__ void add(int q, int e, float a, float b) { of(q, e) = fmaf(a, b, of(q, e)); }
-    __device__ __forceinline__ void get(int q, float (&f)[V]) {
+    __device__ __forceinline__ void add(const Vec<E> &a, const Vec<E> &b) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = of(q, e);
+        for (int i = 0; i < Vec<E>::kPairs; ++i) at[i * blockDim.x] = fma2(a.v[i], b.v[i], at[i * blockDim.x]);
+    }
+    __device__ __forceinline__ Vec<E> all() const {
+        Vec<E> x;
+#pragma unroll
+        for (int i = 0; i < Vec<E>::kPairs; ++i) x.v[i] = at[i * blockDim.x];
+        return x;
     }
 };
 
 // The block's teams' sums added in order and written as the block's partial row.
 template <int P, int V>
-__device__ __forceinline__ void write_partial(const BackwardParams &p, const Team &team, Columns<P, V> &sums, float *part,
-                                              float *shared) {
-    float acc[P][V];
-#pragma unroll
-    for (int q = 0; q < P; ++q) sums.get(q, acc[q]);
+__device__ __forceinline__ void write_partial(const BackwardParams &p, const Team &team, Vec<P * V> acc, float *part,
+                                              float2 *shared) {
     if constexpr (P * V <= kNormShared) {
+        constexpr int kPairs = Vec<P * V>::kPairs;
         if (p.slots > 1) {
             __syncthreads();
 #pragma unroll
-            for (int q = 0; q < P; ++q)
-#pragma unroll
-                for (int e = 0; e < V; ++e) shared[(q * V + e) * kNormThreads + threadIdx.x] = acc[q][e];
+            for (int i = 0; i < kPairs; ++i) shared[i * kNormThreads + threadIdx.x] = acc.v[i];
             __syncthreads();
             if (team.slot != 0) return;
             for (int s = 1; s < p.slots; ++s)
 #pragma unroll
-                for (int q = 0; q < P; ++q)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) acc[q][e] += shared[(q * V + e) * kNormThreads + s * p.team + team.t];
+                for (int i = 0; i < kPairs; ++i) acc.v[i] = add2(acc.v[i], shared[i * kNormThreads + s * p.team + team.t]);
         }
     }
     float *const row = part + (int64_t)blockIdx.x * p.columns;
 #pragma unroll
     for (int q = 0; q < P; ++q) {
         const int pack = team.t + q * p.team;
-        if (pack < p.packs) Raw<float, V>::store(row + pack * V, acc[q]);
+        float f[V];
+        acc.get(q * V, f);
+        if (pack < p.packs) Raw<float, V>::store(row + pack * V, f);
     }
 }
 
-// Threads that hold few packs keep the weights and gates of their columns in registers.
+// Threads that hold few elements keep the weights and the gate of their columns in registers.
 template <typename R, typename B, int V, int P, int kMode, bool kSums>
 __global__ void __launch_bounds__(kNormThreads, kMode != kJoinFull && P * V <= kNormShared ? 2 : 1)
     norm_backward_kernel(const __grid_constant__ BackwardParams p) {
     extern __shared__ uint4 stages[];
     __shared__ alignas(16) float scratch[Team::kScratch];
-    __shared__ float shared[kSums && P * V <= kNormShared ? kNormThreads * P * V : 1];
     constexpr bool kFull = kMode == kJoinFull, kJoin = kMode != kNormAlone, kHold = P * V <= kNormShared;
+    using Row = Vec<P * V>;
+    __shared__ float2 shared[kSums && kHold ? kNormThreads * Row::kPairs : 1];
     Team team(p.team, scratch);
     const Ring<V, P> ring(stages, p.ring, team, p.packs);
     float *const columns = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(stages) + p.sums_at);
     constexpr int kStep = kSums && !kHold ? P * V : 0;
-    Columns<P, V, !kStep> dw(columns), du(columns + (kFull ? 1 : 0) * kStep * p.team), dg(columns + (kFull ? 2 : 0) * kStep * p.team);
+    Columns<P * V, !kStep> dw(columns), du(columns + (kFull ? 1 : 0) * kStep * p.team),
+        dg(columns + (kFull ? 2 : 0) * kStep * p.team);
 
-    const bool has_dy = p.in.has & kHasDy, has_dh = kJoin && (p.in.has & kHasDh), post = kFull && (p.in.has & kHasPost),
+    const bool has_dy = kMode == kNormAlone || (p.in.has & kHasDy), has_dh = kJoin && (p.in.has & kHasDh), post = kFull && (p.in.has & kHasPost),
                gate = kFull && (p.in.has & kHasGate), gates = gate && p.in.gate_span == 1,
                gate_sums = kSums && kFull && p.gate_mode != kGateNone, branch = post || gate_sums;
-    const auto weight = [&](const void *from, int dtype, int pack, float (&w)[V]) {
-        load_typed<V>(from, dtype, pack * V, w);
-#pragma unroll
-        for (int e = 0; e < V; ++e) w[e] += p.offset;
-    };
-    float w_held[kHold ? P : 1][V], u_held[kHold && kFull ? P : 1][V], gate_held[kHold && kFull ? P : 1][V];
-    int gate_of = -1;  // the gate row that is held
-    if constexpr (kHold)
+    const auto each = [&](auto f) {  // this thread's packs
 #pragma unroll
         for (int q = 0; q < P; ++q) {
             const int pack = team.t + q * p.team;
-            if (pack >= p.packs) break;
-            if (has_dy) weight(p.in.weight, p.in.weight_dtype, pack, w_held[q]);
-            if constexpr (kFull)
-                if (post) weight(p.in.post, p.in.post_dtype, pack, u_held[q]);
+            if (pack < p.packs) f(q, pack);
         }
-    // a pack's weights: held, or loaded into `w`
-    const auto w_of = [&](int q, int pack, float (&w)[V]) {
-        if constexpr (kHold)
-#pragma unroll
-            for (int e = 0; e < V; ++e) w[e] = w_held[q][e];
-        else
-            weight(p.in.weight, p.in.weight_dtype, pack, w);
     };
-    const auto u_of = [&](int q, int pack, float (&u)[V]) {
-        if constexpr (kHold && kFull)
+    const auto load = [&](const void *from, int dtype, float add, Row &w) {  // a weight, or a row of the gate
+        w.clear();
+        each([&](int q, int pack) {
+            float f[V];
+            load_typed<V>(from, dtype, pack * V, f);
 #pragma unroll
-            for (int e = 0; e < V; ++e) u[e] = u_held[q][e];
-        else
-            weight(p.in.post, p.in.post_dtype, pack, u);
+            for (int e = 0; e < V; ++e) f[e] += add;
+            w.set(q * V, f);
+        });
     };
     const auto gate_at = [&](int row) {
         return reinterpret_cast<const unsigned char *>(p.in.gate) +
-               (int64_t)(row / p.in.gate_span) * p.d * (p.in.gate_dtype == LAMQ_F32 ? 4 : 2);
+               (int64_t)p.in.by_span.of(row) * p.d * (p.in.gate_dtype == LAMQ_F32 ? 4 : 2);
     };
+    Row w, u, held;
+    int gate_of = -1;  // the gate row that is held
+    if (kHold) {
+        if (has_dy) load(p.in.weight, p.in.weight_dtype, p.offset, w);
+        if (kFull && post) load(p.in.post, p.in.post_dtype, p.offset, u);
+    }
 
     const int worker = blockIdx.x * p.slots + team.slot;
     const bool ranges = kFull && p.gate_mode >= kGateInside;  // each team its own range of rows
     const int first = ranges ? worker * p.per : blockIdx.x * p.slots * p.per + team.slot, step = ranges ? 1 : p.slots;
-    const auto fetch = [&](int k, int stage) {
-        const int row = first + k * step;
-        if (k < p.per && row < p.rows) {
+    int fetched = 0;
+    const auto fetch = [&](int stage) {
+        const int row = first + fetched * step;
+        const bool there = fetched < p.per && row < p.rows;
+        if (there || p.team < 32) {  // a team that has no row beside others of its warp that do: zeros
+            const int at = there ? row : 0, bytes = there ? 16 : 0;
             if (has_dy) {
-                ring.fetch(stage, kTensorH, row_at<R>(p.h, row));
-                ring.fetch(stage, kTensorDy, row_at<B>(p.in.dy, row));
+                ring.fetch(stage, kTensorH, row_at<R>(p.in.h, at), bytes);
+                ring.fetch(stage, kTensorDy, row_at<B>(p.in.dy, at), bytes);
             }
-            if (has_dh) ring.fetch(stage, kTensorDh, row_at<R>(p.in.dh, row));
-            if (branch) ring.fetch(stage, kTensorBranch, row_at<B>(p.in.branch, row));
-            if (gates) ring.fetch_typed(stage, kTensorGate, gate_at(row), p.in.gate_dtype);
+            if (has_dh) ring.fetch(stage, kTensorDh, row_at<R>(p.in.dh, at), bytes);
+            if (branch) ring.fetch(stage, kTensorBranch, row_at<B>(p.in.branch, at), bytes);
+            if (gates) ring.fetch_typed(stage, kTensorGate, gate_at(at), p.in.gate_dtype, bytes);
         }
+        ++fetched;
         ring.commit();
     };
+    const auto read = [&](int stage, int tensor, const auto *row, Row &x) {
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+            float f[V];
+            ring.read(stage, tensor, row, q, f);
+            x.set(q * V, f);
+        }
+    };
     int stage = 0, to = 0;
-    for (int i = 1; i < p.ring.stages; ++i, to = ring.after(to)) fetch(i - 1, to);
-    for (int k = 0; k < p.per; ++k, stage = ring.after(stage), to = ring.after(to)) {
+    for (int i = 1; i < p.ring.stages; ++i, to = ring.after(to)) fetch(to);
+    for (int k = 0; k < p.per; ++k) {
         const int row = first + k * step;
         const bool live = row < p.rows;
         if (p.team < 32 ? !__any_sync(0xffffffffu, live) : !live) break;
-        if (p.ring.stages == 1) {
-            fetch(k, 0);
+        if (V == 1 && p.ring.stages > 1) {  // all have read the stage that is filled next
             ring.wait();
-        } else if (V == 1) {  // all have read the stage that is filled next
-            ring.wait();
-            fetch(k + p.ring.stages - 1, to);
+            fetch(to);
         } else {
-            fetch(k + p.ring.stages - 1, to);
+            fetch(to);
             ring.wait();
         }
         const int at = live ? row : 0;
-        float g[P][V], b[kFull ? P : 1][V];  // dy, then the gradient at h, then at the branch; the branch
-        float s[kFull ? 3 : 2] = {};         // Σ h², Σ t h, Σ b²
-        float x[P][V];
-        const R *const h_row = row_at<R>(p.h, at), *const dh_row = row_at<R>(p.in.dh, at);
-        const B *const dy_row = row_at<B>(p.in.dy, at), *const b_row = row_at<B>(p.in.branch, at);
-#pragma unroll
-        for (int q = 0; q < P; ++q) {
-            const int pack = team.t + q * p.team;
-            const bool in = live && pack < p.packs;
-#pragma unroll
-            for (int e = 0; e < V; ++e) x[q][e] = g[q][e] = 0.f;
-            if (has_dy && in) {
-                float w[V];
-                ring.read(stage, kTensorH, h_row, q, x[q]);
-                ring.read(stage, kTensorDy, dy_row, q, g[q]);
-                w_of(q, pack, w);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    s[0] = fmaf(x[q][e], x[q][e], s[0]);
-                    s[1] = fmaf(g[q][e] * w[e], x[q][e], s[1]);
-                }
-            }
-            if constexpr (kFull) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) b[q][e] = 0.f;
-                if (branch && in) ring.read(stage, kTensorBranch, b_row, q, b[q]);
-#pragma unroll
-                for (int e = 0; e < V; ++e) s[2] = fmaf(b[q][e], b[q][e], s[2]);
-            }
+        Row g, x, b;  // dy, then the gradient at h, then at the branch; h; the branch
+        if (has_dy) {
+            read(stage, kTensorH, row_at<R>(p.in.h, at), x);
+            read(stage, kTensorDy, row_at<B>(p.in.dy, at), g);
+        } else {
+            x.clear(), g.clear();
         }
+        if constexpr (kFull) {
+            if (branch)
+                read(stage, kTensorBranch, row_at<B>(p.in.branch, at), b);
+            else
+                b.clear();
+        }
+        Row t = g;
+        if (!kHold && has_dy) load(p.in.weight, p.in.weight_dtype, p.offset, w);
+        if (has_dy) t *= w;
+        float s[kFull ? 3 : 2];  // Σ h², Σ t h, Σ b²
+        s[0] = x.dot(x), s[1] = t.dot(x);
+        if constexpr (kFull) s[2] = b.dot(b);
         if (has_dy || post) team.sum(s);
         if (has_dy) {
             float shrunk;
             const float f = unit_factor(team, x, s[0], p.inv_d, p.eps, shrunk);
             if (p.team < 32 ? __any_sync(0xffffffffu, shrunk != 1.f) : shrunk != 1.f) {
-                float again[1] = {0.f};  // x changed, and the sum may have overflowed
-#pragma unroll
-                for (int q = 0; q < P; ++q) {
-                    const int pack = team.t + q * p.team;
-                    if (pack >= p.packs) break;
-                    float w[V];
-                    w_of(q, pack, w);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) again[0] = fmaf(g[q][e] * w[e], x[q][e], again[0]);
-                }
+                float again[1] = {t.dot(x)};  // x changed, and the sum may have overflowed
                 team.sum(again);
                 s[1] = again[0];
             }
             // f is the factor of x as it stands, f · shrunk that of x as it was
-            const float r = f * shrunk, c = s[1] * f * p.inv_d;
-#pragma unroll
-            for (int q = 0; q < P; ++q) {
-                const int pack = team.t + q * p.team;
-                if (pack >= p.packs) break;
-                float w[V];
-                w_of(q, pack, w);
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const float unit = x[q][e] * f;
-                    if (kSums) dw.add(q, e, g[q][e], unit);
-                    g[q][e] = r * fmaf(-unit, c, g[q][e] * w[e]);
+            x *= f;
+            if (kSums) dw.add(g, x);
+            t.take(s[1] * f * p.inv_d, x, f * shrunk);
+            g = t;
+        }
+        if (has_dh) {
+            read(stage, kTensorDh, row_at<R>(p.in.dh, at), x);
+            g += x;
+        }
+        if (live) {
+            R *const out = reinterpret_cast<R *>(p.d_residual) + (int64_t)row * p.d;
+            each([&](int q, int pack) {
+                float f[V];
+                g.get(q * V, f);
+                Raw<R, V>::store(out + pack * V, f);
+            });
+        }
+        if constexpr (kJoin) {
+            g *= p.scale;
+            if constexpr (kFull) {
+                float f = 1.f, shrunk = 1.f;
+                if (post) {
+                    f = unit_factor(team, b, s[2], p.inv_d, p.eps, shrunk);
+                    b *= f;
+                    if (!kHold) load(p.in.post, p.in.post_dtype, p.offset, u);
                 }
-            }
-        }
-        R *const out = reinterpret_cast<R *>(p.d_residual) + (int64_t)at * p.d;
+                if (gate && live) {
+                    const int gate_row = p.in.by_span.of(row);
+                    if (gates) {
+                        const unsigned char *const from = gate_at(row);
 #pragma unroll
-        for (int q = 0; q < P; ++q) {
-            const int pack = team.t + q * p.team;
-            if (pack >= p.packs || !live) break;
-            if (has_dh) {
-                float x[V];
-                ring.read(stage, kTensorDh, dh_row, q, x);
-#pragma unroll
-                for (int e = 0; e < V; ++e) g[q][e] += x[e];
-            }
-            Raw<R, V>::store(out + pack * V, g[q]);
-        }
-        if (!kJoin) continue;
-#pragma unroll
-        for (int q = 0; q < P; ++q)
-#pragma unroll
-            for (int e = 0; e < V; ++e) g[q][e] *= p.scale;
-        if constexpr (kFull) {
-            float f = 1.f, shrunk = 1.f;
-            if (post) {
-                f = unit_factor(team, b, s[2], p.inv_d, p.eps, shrunk);
-#pragma unroll
-                for (int q = 0; q < P; ++q)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) b[q][e] *= f;
-            }
-            if (gate) {
-                const int gate_row = at / p.in.gate_span;
-                const unsigned char *const from = gate_at(at);
-#pragma unroll
-                for (int q = 0; q < P; ++q) {
-                    const int pack = team.t + q * p.team;
-                    if (pack >= p.packs || !live) break;
-                    float v[V];
-                    if (gates)
-                        ring.read_typed(stage, kTensorGate, from, p.in.gate_dtype, q, v);
-                    else if (!kHold)
-                        load_typed<V>(from, p.in.gate_dtype, pack * V, v);
-                    else if (gate_row != gate_of)
-                        load_typed<V>(from, p.in.gate_dtype, pack * V, gate_held[kHold ? q : 0]);
+                        for (int q = 0; q < P; ++q) {
+                            float f[V];
+                            ring.read_typed(stage, kTensorGate, from, p.in.gate_dtype, q, f);
+                            held.set(q * V, f);
+                        }
+                    } else if (gate_row != gate_of) {
+                        gate_of = gate_row;
+                        load(gate_at(row), p.in.gate_dtype, 0.f, held);
+                    }
                     if (gate_sums) {
-                        float u[V];
-                        if (post) u_of(q, pack, u);
-#pragma unroll
-                        for (int e = 0; e < V; ++e) dg.add(q, e, g[q][e], post ? b[q][e] * u[e] : b[q][e]);
+                        Row q = b;
+                        if (post) q *= u;
+                        dg.add(g, q);
                     }
-#pragma unroll
-                    for (int e = 0; e < V; ++e) g[q][e] *= kHold && !gates ? gate_held[kHold ? q : 0][e] : v[e];
+                    g *= held;
+                    if (gate_sums && p.gate_mode >= kGateInside &&
+                        (k + 1 == p.per || row + 1 == (gate_row + 1) * p.in.gate_span)) {
+                        const Row sums = dg.all();
+                        each([&](int q, int pack) {
+                            float f[V];
+                            sums.get(q * V, f);
+                            if (p.gate_mode == kGateInside)
+                                store_typed<V>(p.d_gate, p.in.gate_dtype, (int64_t)gate_row * p.d + pack * V, f);
+                            else  // a worker and a gate row, both growing row by row: their sum names the pair
+                                Raw<float, V>::store(p.g_part + (int64_t)(worker + gate_row) * p.columns + pack * V, f);
+                        });
+                        dg.clear();
+                    }
                 }
-                if (live) gate_of = gate_row;
-                if (gate_sums && p.gate_mode >= kGateInside && live &&
-                    (k + 1 == p.per || (at + 1) % p.in.gate_span == 0 || at + 1 == p.rows)) {
-#pragma unroll
-                    for (int q = 0; q < P; ++q) {
-                        const int pack = team.t + q * p.team;
-                        if (pack >= p.packs) break;
-                        float sum[V];
-                        dg.get(q, sum);
-                        if (p.gate_mode == kGateInside)
-                            store_typed<V>(p.d_gate, p.in.gate_dtype, (int64_t)gate_row * p.d + pack * V, sum);
-                        else  // a worker and a gate row, both growing row by row: their sum names the pair
-                            Raw<float, V>::store(p.g_part + (int64_t)(worker + gate_row) * p.columns + pack * V, sum);
-                    }
-                    dg.clear();
+                if (post) {
+                    if (kSums) du.add(g, b);
+                    g *= u;
+                    float c[1] = {g.dot(b)};
+                    team.sum(c);
+                    g.take(c[0] * p.inv_d, b, f * shrunk);
                 }
             }
-            if (post) {
-                float t[1] = {0.f};
-#pragma unroll
-                for (int q = 0; q < P; ++q) {
-                    const int pack = team.t + q * p.team;
-                    if (pack >= p.packs) break;
-                    float u[V];
-                    u_of(q, pack, u);
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        if (kSums) du.add(q, e, g[q][e], b[q][e]);
-                        g[q][e] *= u[e];
-                        t[0] = fmaf(g[q][e], b[q][e], t[0]);
-                    }
-                }
-                team.sum(t);
-                const float r = f * shrunk, c = t[0] * p.inv_d;
-#pragma unroll
-                for (int q = 0; q < P; ++q)
-#pragma unroll
-                    for (int e = 0; e < V; ++e) g[q][e] = r * fmaf(-b[q][e], c, g[q][e]);
+            if (p.d_branch && live) {
+                B *const out = reinterpret_cast<B *>(p.d_branch) + (int64_t)row * p.d;
+                each([&](int q, int pack) {
+                    float f[V];
+                    g.get(q * V, f);
+                    Raw<B, V>::store(out + pack * V, f);
+                });
             }
         }
-        if (p.d_branch) {
-            B *const out = reinterpret_cast<B *>(p.d_branch) + (int64_t)at * p.d;
-#pragma unroll
-            for (int q = 0; q < P; ++q) {
-                const int pack = team.t + q * p.team;
-                if (live && pack < p.packs) Raw<B, V>::store(out + pack * V, g[q]);
-            }
-        }
+        stage = ring.after(stage), to = ring.after(to);
     }
     if constexpr (kSums) {
-        if (p.w_part) write_partial(p, team, dw, p.w_part, shared);
-        if (kFull && p.u_part) write_partial(p, team, du, p.u_part, shared);
-        if (kFull && p.gate_mode == kGateOne) write_partial(p, team, dg, p.g_part, shared);
+        if (p.w_part) write_partial<P, V>(p, team, dw.all(), p.w_part, shared);
+        if (kFull && p.u_part) write_partial<P, V>(p, team, du.all(), p.u_part, shared);
+        if (kFull && p.gate_mode == kGateOne) write_partial<P, V>(p, team, dg.all(), p.g_part, shared);
     }
 }
 

@@ -18,7 +18,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) norm_backward_wide_kernel(con
     const int first = blockIdx.x * p.per, end = min(p.rows, first + p.per);
     for (int row = first; row < end; ++row) {
         const int64_t out = (int64_t)row * p.d;
-        const R *const h = row_at<R>(p.h, row), *const dh = row_at<R>(p.in.dh, row);
+        const R *const h = row_at<R>(p.in.h, row), *const dh = row_at<R>(p.in.dh, row);
         const B *const dy = row_at<B>(p.in.dy, row), *const branch = row_at<B>(p.in.branch, row);
         const bool pre = (p.in.has & kHasDy);
         float f = 0.f, shrunk = 1.f, r = 0.f, c = 0.f;

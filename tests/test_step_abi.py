@@ -44,6 +44,7 @@ INVALID = [("lamq_norm_forward", (a, N), text) for a, text in BOTH + [(norm(h=0)
                                                                       (norm(y=0), b"null pointer (y)")]]
 INVALID += [("lamq_norm_backward", (a, P, 1 << 40, N), text) for a, text in BOTH + [
     (norm(dr=0), b"null pointer (d_residual)"), (norm(branch=NO, db=0), b"no dh"), (norm(branch=NO, dh=NO), b"no d_branch"),
+    (norm(branch=NO, dh=NO, dy=NO), b"null pointer (dy)"),
     (norm(weight=0), b"belong to a weight"), (norm(weight=0, dy=NO, dw=P), b"belong to a weight"),
     (norm(du=P), b"belongs to a post weight"), (norm(dg=P), b"belongs to a gate"), (norm(dy=rows(inner=-1)), b"inner count")]]
 INVALID += [("lamq_norm_backward", (norm(dw=P), P, 0, N), b"workspace of"),

@@ -16,7 +16,7 @@ extern "C" {
 
 /*
  * Rows of d contiguous elements: row i begins (i / inner)·outer + (i % inner)·row elements behind `data` (the heads of a
- * projection's output have an inner count; plain matrices have inner >= their number of rows).
+ * projection's output have an inner count; plain matrices have inner >= their number of rows, and so have a join's).
  */
 typedef struct lamq_rows {
     void *data;

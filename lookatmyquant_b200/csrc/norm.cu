@@ -20,12 +20,13 @@ struct ForwardParams {
     RingParams ring;
 };
 
-// Threads that hold few elements keep the weights and the gate of their columns in registers.
-template <typename R, typename B, int V, int P, int kMode>
-__global__ void __launch_bounds__(kNormThreads, P * V <= 8 ? 2 : 1) norm_forward_kernel(const __grid_constant__ ForwardParams p) {
+// Threads of blocks that are not too large (kHold) keep the weights and the gate of their columns in registers.
+template <typename R, typename B, NormKernel kKernel, int kMode>
+__global__ void __launch_bounds__(resident(kKernel, kMode, false), 1) norm_forward_kernel(const __grid_constant__ ForwardParams p) {
     extern __shared__ uint4 stages[];
     __shared__ alignas(16) float scratch[Team::kScratch];
-    constexpr bool kBranch = kMode != kNormAlone, kFull = kMode == kJoinFull, kHold = P * V <= kNormShared;
+    constexpr int V = NormSizes<kKernel>::V, P = NormSizes<kKernel>::P;
+    constexpr bool kBranch = kMode != kNormAlone, kFull = kMode == kJoinFull, kHold = NormSizes<kKernel>::kHold;
     using Row = Vec<P * V>;
     Team team(p.team, scratch);
     const Ring<V, P> ring(stages, p.ring, team, p.packs);
@@ -62,8 +63,8 @@ __global__ void __launch_bounds__(kNormThreads, P * V <= 8 ? 2 : 1) norm_forward
     const auto fetch = [&](int row, int stage) {
         if (row < p.rows || p.team < 32) {  // a team that has no row beside others of its warp that do: zeros
             const int at = row < p.rows ? row : 0, bytes = row < p.rows ? 16 : 0;
-            ring.fetch(stage, kTensorH, row_at<R>(p.in.h, at), bytes);
-            if (kBranch) ring.fetch(stage, kTensorBranch, row_at<B>(p.in.branch, at), bytes);
+            ring.fetch(stage, kTensorH, row_at<R, kBranch>(p.in.h, at), bytes);
+            if (kBranch) ring.fetch(stage, kTensorBranch, row_at<B, true>(p.in.branch, at), bytes);
             if (gates) ring.fetch_typed(stage, kTensorGate, gate_at(at), p.in.gate_dtype, bytes);
         }
         ring.commit();
@@ -91,7 +92,7 @@ __global__ void __launch_bounds__(kNormThreads, P * V <= 8 ? 2 : 1) norm_forward
         const bool live = row < p.rows;
         const int at = live ? row : 0;
         Row x;
-        if constexpr (kBranch) read(stage, kTensorBranch, row_at<B>(p.in.branch, at), x);
+        if constexpr (kBranch) read(stage, kTensorBranch, row_at<B, true>(p.in.branch, at), x);
         if constexpr (kFull) {
             if (post) {
                 float ss[1] = {x.dot(x)}, shrunk;
@@ -119,10 +120,10 @@ __global__ void __launch_bounds__(kNormThreads, P * V <= 8 ? 2 : 1) norm_forward
         }
         if constexpr (kBranch) {
             Row r;
-            read(stage, kTensorH, row_at<R>(p.in.h, at), r);
+            read(stage, kTensorH, row_at<R, kBranch>(p.in.h, at), r);
             x.scale_add(p.scale, r);
         } else {
-            read(stage, kTensorH, row_at<R>(p.in.h, at), x);
+            read(stage, kTensorH, row_at<R, kBranch>(p.in.h, at), x);
         }
         if (kBranch && live) {
             R *const out = reinterpret_cast<R *>(p.h) + (int64_t)row * p.d;
@@ -198,31 +199,33 @@ void launch_wide(const ForwardParams &p, int grid, bool branch, cudaStream_t str
         norm_forward_wide_kernel<R, B, false><<<grid, kWideThreads, 0, stream>>>(p);
 }
 
-template <typename R, typename B, int V, int P, int kMode>
+template <typename R, typename B, NormKernel kKernel, int kMode>
 int launch_forward(const ForwardParams &p, int grid, int shared, cudaStream_t stream) {
-    const auto kernel = norm_forward_kernel<R, B, V, P, kMode>;
+    const auto kernel = norm_forward_kernel<R, B, kKernel, kMode>;
     if (const int st = allow_shared(reinterpret_cast<const void *>(kernel), shared)) return st;
     kernel<<<grid, p.team * p.slots, shared, stream>>>(p);
     return LAMQ_OK;
 }
 
-template <typename R, typename B, int V, int P>
+template <typename R, typename B, NormKernel kKernel>
 int launch_forward(const ForwardParams &p, int grid, int mode, int shared, cudaStream_t stream) {
-    if (mode == kJoinFull) return launch_forward<R, B, V, P, kJoinFull>(p, grid, shared, stream);
-    if (mode == kJoinPlain) return launch_forward<R, B, V, P, kJoinPlain>(p, grid, shared, stream);
-    if constexpr (std::is_same_v<R, B>) return launch_forward<R, B, V, P, kNormAlone>(p, grid, shared, stream);
+    if (mode == kJoinFull) return launch_forward<R, B, kKernel, kJoinFull>(p, grid, shared, stream);
+    if (mode == kJoinPlain) return launch_forward<R, B, kKernel, kJoinPlain>(p, grid, shared, stream);
+    if constexpr (std::is_same_v<R, B>) return launch_forward<R, B, kKernel, kNormAlone>(p, grid, shared, stream);
     return LAMQ_ERR_INVALID;  // the checks refuse a norm of two types
 }
 
 template <typename R, typename B>
-int launch_forward(const NormShape &s, const ForwardParams &p, int grid, int mode, int shared, cudaStream_t stream) {
-    if (s.V == 8)
-        return s.P == 1   ? launch_forward<R, B, 8, 1>(p, grid, mode, shared, stream)
-               : s.P == 2 ? launch_forward<R, B, 8, 2>(p, grid, mode, shared, stream)
-                          : launch_forward<R, B, 8, 4>(p, grid, mode, shared, stream);
-    if (s.P == 1) return launch_forward<R, B, 1, 1>(p, grid, mode, shared, stream);
-    if (s.P == 8) return launch_forward<R, B, 1, 8>(p, grid, mode, shared, stream);
-    launch_wide<R, B>(p, grid, mode != kNormAlone, stream);
+int launch_forward(NormKernel kernel, const ForwardParams &p, int grid, int mode, int shared, cudaStream_t stream) {
+    switch (kernel) {
+        case kVectors: return launch_forward<R, B, kVectors>(p, grid, mode, shared, stream);
+        case kElements: return launch_forward<R, B, kElements>(p, grid, mode, shared, stream);
+        case kVectorsWide: return launch_forward<R, B, kVectorsWide>(p, grid, mode, shared, stream);
+        case kVectorsWidest: return launch_forward<R, B, kVectorsWidest>(p, grid, mode, shared, stream);
+        case kVectors8:
+        case kElements8: return LAMQ_ERR_INVALID;  // backward only
+        case kWide: launch_wide<R, B>(p, grid, mode != kNormAlone, stream);
+    }
     return LAMQ_OK;
 }
 
@@ -248,6 +251,9 @@ int norm_args_status(const lamq_norm_args *a, bool backward) {
     for (int i = 0; i < (backward ? 4 : 2); ++i)
         LAMQ_REQUIRE(!rows[i]->data || (rows[i]->inner >= 1 && rows[i]->inner <= INT_MAX), "rows: an inner count of 1 to 2^31 - 1");
     LAMQ_REQUIRE(a->residual.data, "null pointer (residual)");
+    for (int i = 0; join && i < (backward ? 4 : 2); ++i)
+        LAMQ_REQUIRE(!rows[i]->data || (one_stride(*rows[i], a->rows) && rows[i]->row <= INT_MAX / 4),
+                     "rows: a join's lie at one stride, below 2^29");
     if (!backward) {
         LAMQ_REQUIRE(!join || a->h, "null pointer (h)");
         LAMQ_REQUIRE(!a->weight || a->y, "null pointer (y)");
@@ -283,9 +289,9 @@ extern "C" int lamq_norm_forward(const lamq_norm_args *a, lamq_stream_t stream) 
     const int grid = (int)std::min<int64_t>((a->rows + p.slots - 1) / p.slots, kSMs * l.blocks);
     const cudaStream_t st = (cudaStream_t)stream;
     const int launched = a->residual_dtype == LAMQ_BF16
-                             ? launch_forward<__nv_bfloat16, __nv_bfloat16>(s, p, grid, mode, shared, st)
-                         : a->branch_dtype == LAMQ_BF16 ? launch_forward<float, __nv_bfloat16>(s, p, grid, mode, shared, st)
-                                                        : launch_forward<float, float>(s, p, grid, mode, shared, st);
+                             ? launch_forward<__nv_bfloat16, __nv_bfloat16>(s.kernel, p, grid, mode, shared, st)
+                         : a->branch_dtype == LAMQ_BF16 ? launch_forward<float, __nv_bfloat16>(s.kernel, p, grid, mode, shared, st)
+                                                        : launch_forward<float, float>(s.kernel, p, grid, mode, shared, st);
     if (launched) return launched;
     LAMQ_CHECK_LAUNCH("lamq_norm_forward");
     return LAMQ_OK;

@@ -25,6 +25,25 @@ int norm_args_status(const lamq_norm_args *a, bool backward);
 namespace {
 
 constexpr int kNormThreads = 512;   // most threads of a block
+
+// The kernels: vectors or elements, 16 of a row a thread in teams of up to 256 (the full join's backward: 8 of a row in teams of
+// up to 512); vectors in teams of up to 512, with 16 elements a thread and with 32; rows of elements by blocks (norm_wide.cuh).
+enum NormKernel { kVectors, kElements, kVectors8, kElements8, kVectorsWide, kVectorsWidest, kWide };
+
+enum { kNormAlone, kJoinPlain, kJoinFull };  // the norm alone; a join without post and gate; any join
+
+// Threads that an SM holds: 85 registers each where the forward reads vectors and has no post norm and gate, else 128.
+constexpr int resident(NormKernel kernel, int mode, bool backward) {
+    return !backward && kernel == kVectors && mode != kJoinFull ? 768 : kNormThreads;
+}
+
+template <NormKernel kKernel>
+struct NormSizes {
+    static constexpr int E = kKernel == kVectorsWidest ? 32 : kKernel == kVectors8 || kKernel == kElements8 ? 8 : 16;
+    static constexpr int V = kKernel == kElements || kKernel == kElements8 ? 1 : 8, P = E / V;
+    static constexpr bool kHold = kKernel <= kElements8;  // weights and sums stay in registers
+    static constexpr int kThreads = kHold ? 4096 / E : kNormThreads;
+};
 constexpr int kNormMaxD = 16384;    // widest row
 constexpr int kNormSums = 3;        // sums exchanged at once
 constexpr int kSMs = 148;
@@ -247,9 +266,9 @@ struct Rows {
     Divisor by_inner;
 };
 
-template <typename T>
+template <typename T, bool kFlat = false>
 __device__ __forceinline__ const T *row_at(const Rows &r, int i) {
-    if (r.stride >= 0) return reinterpret_cast<const T *>(r.data + (int64_t)i * r.stride);
+    if (kFlat || r.stride >= 0) return reinterpret_cast<const T *>(r.data + (int64_t)i * r.stride);
     const int o = r.by_inner.of(i);
     return reinterpret_cast<const T *>(r.data + o * r.outer + (i - o * r.inner) * r.row);
 }
@@ -340,7 +359,6 @@ enum { kTensorH, kTensorDy, kTensorDh, kTensorBranch, kTensorGate, kTensors };
 struct RingParams {
     int stages, stage_bytes;          // of a block
     int at[kTensors], image[kTensors];  // where a tensor's part of a stage begins; elements: bytes of a team's row
-    int size[kTensors];                 // of an element; 0: the call does not read the tensor
 };
 
 template <int V, int P>
@@ -351,14 +369,7 @@ struct Ring {
     int packs;
 
     __device__ Ring(void *shared, const RingParams &p_, const Team &team_, int packs_)
-        : base(reinterpret_cast<unsigned char *>(shared)), p(p_), team(team_), packs(packs_) {
-        if constexpr (V == 8)  // a thread's places behind the row's end hold zeros throughout, so that it reads all of its places
-            for (int s = 0; s < p.stages; ++s)
-                for (int k = 0; k < kTensors; ++k)
-                    for (int i = 0; i < P * (p.size[k] >> 1); ++i)
-                        if (team.t + i / (p.size[k] >> 1) * team.size >= packs)
-                            *reinterpret_cast<uint4 *>(part(s, k) + (i * blockDim.x + threadIdx.x) * 16) = make_uint4(0, 0, 0, 0);
-    }
+        : base(reinterpret_cast<unsigned char *>(shared)), p(p_), team(team_), packs(packs_) {}
 
     // 16 bytes, or (bytes = 0) as many zeros
     __device__ __forceinline__ static void copy16(void *to, const void *from, int bytes) {
@@ -393,11 +404,11 @@ struct Ring {
             constexpr int kPieces = sizeof(T) / 2;
 #pragma unroll
             for (int q = 0; q < P; ++q) {
-                const int pack = team.t + q * team.size;
-                if (pack >= packs) break;
+                int pack = team.t + q * team.size, some = bytes;
+                if (pack >= packs) pack = 0, some = 0;  // zeros behind the row's end
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i)
-                    copy16(to + ((q * kPieces + i) * blockDim.x + threadIdx.x) * 16, row + pack * 8 + i * (8 / kPieces), bytes);
+                    copy16(to + ((q * kPieces + i) * blockDim.x + threadIdx.x) * 16, row + pack * 8 + i * (8 / kPieces), some);
             }
         } else {
             const int shift = (int)(reinterpret_cast<uintptr_t>(row) & 15);
@@ -468,14 +479,6 @@ __device__ __forceinline__ float unit_factor(Team &team, Vec<E> &x, float ss, fl
 
 // ---- the host's side
 
-enum { kNormAlone, kJoinPlain, kJoinFull };  // the norm alone; a join without post and gate; any join
-
-// How many threads share a row, and P: what they hold of it each (kWide: nothing, norm_wide.cuh).
-constexpr int kWide = 1 << 20;
-constexpr int kNormFull = 16;  // elements a thread of the backward kernel with post norms and gates: more would spill
-struct NormShape {
-    int V, P, team, packs;
-};
 
 // Which tensors a call has, and in the place of the others an output's memory of the same shape and no smaller a type: what
 // a kernel gets may be read whether or not it is there.
@@ -491,12 +494,15 @@ struct Present {
 
 inline int element_size(int dtype) { return dtype == LAMQ_F32 ? 4 : 2; }
 
+inline bool one_stride(const lamq_rows &r, int64_t rows) {
+    return r.row >= 0 && (r.inner >= rows || r.outer == r.inner * r.row);
+}
+
 inline Rows rows_of(const lamq_rows &r, int64_t rows, int size) {
     Rows x;
     x.data = reinterpret_cast<const unsigned char *>(r.data);
     x.row = r.row * size, x.outer = r.outer * size, x.inner = (int)r.inner, x.by_inner = divisor(r.inner);
-    const bool flat = r.inner >= rows || r.outer == r.inner * r.row;
-    x.stride = flat && x.row >= 0 && x.row <= INT_MAX ? (int)x.row : -1;
+    x.stride = one_stride(r, rows) && x.row <= INT_MAX ? (int)x.row : -1;
     return x;
 }
 
@@ -522,40 +528,48 @@ inline bool aligned_rows(const lamq_rows &r) {
     return !r.data || ((reinterpret_cast<uintptr_t>(r.data) & 15) == 0 && r.row % 8 == 0 && r.outer % 8 == 0);
 }
 
-// Vectors where every row and every array begins on 16 bytes, elements elsewhere. Up to 32 packs a team is a power of two
-// of lanes; wider rows take the fewest packs a thread that 512 threads can hold. (Elements: eight a thread, so that a
-// thread has as many bytes under way as it can.)
+// How many threads share a row, and P: the packs of V elements that each holds of it.
+struct NormShape {
+    int V, P, team, packs;
+    NormKernel kernel;
+};
+
+// Vectors where every row and every array begins on 16 bytes, elements elsewhere. A thread holds 16 elements of a row: what it
+// does for a row beside the arithmetic (places, waits, exchanges) costs as much as the arithmetic of 16 (16384 x 2560, the norm's
+// backward, us: 78 with 8, 61 with 16). The full join's backward holds three sums and three tensors of a row: 8 of each (8192 x
+// 4096: 152 with 8 and 16 warps an SM, 189 with 16 and 8 warps). Up to 32 threads a team is a power of two of lanes, else whole
+// warps. Wider rows take teams of up to 512 threads with 16 elements, then with 32; rows wider than 4096 that may begin
+// anywhere, a block each.
 inline NormShape norm_shape(const lamq_norm_args &a, bool backward) {
     const void *arrays[] = {a.weight, a.post, a.gate, a.h, a.y, a.d_residual, a.d_branch, a.d_weight, a.d_post, a.d_gate};
     bool vec = a.d % 8 == 0 && aligned_rows(a.residual) && aligned_rows(a.branch);
     if (backward) vec = vec && aligned_rows(a.dh) && aligned_rows(a.dy);
     for (const void *p : arrays) vec = vec && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+    const bool full = backward && (a.post || a.gate);
+    int e = full ? 8 : 16;
     NormShape s;
-    s.V = vec ? 8 : 1;
-    s.packs = a.d / s.V;
-    if (s.packs <= 32) {
-        s.P = 1;
-        s.team = 1;
-        while (s.team < s.packs) s.team *= 2;
-    } else {
-        if (vec)
-            s.P = s.packs <= 512 ? 1 : s.packs <= 1024 ? 2 : 4;
-        else
-            s.P = s.packs <= 4096 ? 8 : kWide;
-        if (backward && (a.post || a.gate) && s.P != kWide && s.P * s.V > kNormFull) s.V = 1, s.P = kWide, s.packs = a.d;
-        s.team = s.P == kWide ? kNormThreads : ((s.packs + s.P - 1) / s.P + 31) / 32 * 32;
+    s.kernel = full ? (vec ? kVectors8 : kElements8) : vec ? kVectors : kElements;
+    if (a.d > 4096) {
+        s.kernel = !vec ? kWide : a.d <= 8192 ? kVectorsWide : full ? kWide : kVectorsWidest;
+        e = s.kernel == kVectorsWidest ? 32 : 16;
     }
+    s.V = vec && s.kernel != kWide ? 8 : 1;
+    s.P = e / s.V;
+    s.packs = a.d / s.V;
+    const int threads = (a.d + e - 1) / e;
+    s.team = s.kernel == kWide ? kNormThreads : (threads + 31) / 32 * 32;
+    if (threads <= 32)
+        for (s.team = 1; s.team < threads;) s.team *= 2;
     return s;
 }
 
-// Teams whose threads hold more than this of a row have a block to themselves: the memory in which a block adds its teams'
-// sums holds no more.
-constexpr int kNormShared = 8;
+inline bool holds(NormKernel kernel) { return kernel <= kElements8; }
 
-// Teams of a block: blocks of about `threads` threads, fewer where there are few rows, whole warps always.
-inline int norm_slots(const NormShape &s, int64_t rows, int threads) {
-    if (s.P > kNormShared / s.V) return 1;
-    const int least = std::max(1, 32 / s.team), most = std::max(least, threads / s.team);
+// Teams of a block: blocks of about 256 threads, fewer where there are few rows, whole warps always. Threads of larger teams
+// keep their sums in shared memory, where a block's teams are not added up: one team a block.
+inline int norm_slots(const NormShape &s, int64_t rows) {
+    if (!holds(s.kernel)) return 1;
+    const int least = std::max(1, 32 / s.team), most = std::max(least, 256 / s.team);
     const int64_t wanted = (rows + 2 * kSMs - 1) / (2 * kSMs);
     return (int)std::min<int64_t>(most, std::max<int64_t>(least, (wanted + least - 1) / least * least));
 }
@@ -573,7 +587,6 @@ inline int allow_shared(const void *kernel, int dynamic) {
 struct NormLayout {
     NormShape shape;
     int mode, slots, blocks;  // blocks: of an SM
-    bool few;                 // a thread holds few elements (kNormShared)
     RingParams ring;
     int sums_bytes, shared;   // of the dynamic shared memory: the sums that registers do not hold, and all of it
 };
@@ -581,7 +594,7 @@ struct NormLayout {
 constexpr int kSmemSM = 220 * 1024;  // of 228 KB; each block takes 1 KB for itself
 
 // `gate_sums`: the gradient of the gate is wanted; `sums`: that of any parameter. Blocks are as many as their registers allow
-// (64 for a thread that holds few elements of few tensors, else 128), or as have room for two stages each, and stages fill
+//, or as have room for two stages each, and stages fill
 // the room, four at most. What has no room, or two stages of rows that begin anywhere, is left to the wide kernels.
 inline NormLayout norm_layout(const lamq_norm_args &a, bool backward, bool sums, bool gate_sums) {
     NormLayout l{};
@@ -595,20 +608,20 @@ inline NormLayout norm_layout(const lamq_norm_args &a, bool backward, bool sums,
         size[kTensorH] = a.dy.data ? r : 0, size[kTensorDy] = a.dy.data ? b : 0, size[kTensorDh] = a.dh.data ? r : 0;
         size[kTensorBranch] = a.post || gate_sums ? b : 0;
     }
-    if (s.P != kWide) {
-        l.few = s.P * s.V <= kNormShared;
-        l.slots = norm_slots(s, a.rows, backward ? kNormThreads : 256);
+    if (s.kernel != kWide) {
+        const bool hold = holds(s.kernel);
+        l.slots = norm_slots(s, a.rows);
         const int threads = s.team * l.slots;
         RingParams &g = l.ring;
         for (int k = 0; k < kTensors; ++k) {
-            g.at[k] = g.stage_bytes, g.size[k] = size[k];
+            g.at[k] = g.stage_bytes;
             g.image[k] = (a.d * size[k] + 15) / 16 * 16 + 16;
             g.stage_bytes += size[k] == 0 ? 0 : s.V == 8 ? s.P * 8 * size[k] * threads : g.image[k] * l.slots;
         }
-        l.sums_bytes = sums && !l.few ? (l.mode == kJoinFull ? 3 : 1) * s.P * s.V * threads * (int)sizeof(float) : 0;
+        l.sums_bytes = sums && !hold ? (l.mode == kJoinFull ? 3 : 1) * s.P * s.V * threads * (int)sizeof(float) : 0;
         const int own = Team::kScratch * (int)sizeof(float) + 1024 + l.sums_bytes +
-                        (backward && sums && l.few ? kNormThreads * kNormShared * (int)sizeof(float) : 0);
-        l.blocks = std::max(1, (!l.few || (backward && l.mode == kJoinFull) ? 512 : 1024) / threads);
+                        (backward && sums && hold ? 4096 * (int)sizeof(float) : 0);
+        l.blocks = std::max(1, resident(s.kernel, l.mode, backward) / threads);
         for (;; --l.blocks) {
             g.stages = std::min(4, (kSmemSM / l.blocks - own) / std::max(1, g.stage_bytes));
             if (g.stages >= 2 || l.blocks == 1) break;
@@ -616,8 +629,8 @@ inline NormLayout norm_layout(const lamq_norm_args &a, bool backward, bool sums,
         l.shared = g.stages * g.stage_bytes + l.sums_bytes;
         if (g.stages >= (s.V == 1 ? 2 : 1)) return l;
     }
-    s.V = 1, s.P = kWide, s.team = kNormThreads, s.packs = a.d;
-    l.slots = 1, l.blocks = 2, l.few = false, l.shared = 0;
+    s.V = 1, s.kernel = kWide, s.team = kNormThreads, s.packs = a.d;
+    l.slots = 1, l.blocks = 2, l.shared = 0;
     return l;
 }
 

@@ -25,7 +25,7 @@ Plan plan_of(const lamq_norm_args &a) {
             q.gate_mode = kGateOne;
         } else if (a.gate_span == 1) {
             q.gate_mode = kGateInside;
-        } else if (a.gate_span <= per && shape.P != kWide) {  // a wide row's sums have no place but the partial rows
+        } else if (a.gate_span <= per && shape.kernel != kWide) {  // a wide row's sums have no place but the partial rows
             q.gate_mode = kGateInside;
             per = (per + a.gate_span - 1) / a.gate_span * a.gate_span;
         } else {
@@ -130,10 +130,13 @@ extern "C" int lamq_norm_backward(const lamq_norm_args *a, void *workspace, size
     p.ring = l.ring;
     p.sums_at = l.shared - l.sums_bytes;
     const int shared = l.shared;
-    const int launched = l.shape.V == 1   ? launch_backward_elements(l.shape.P, *a, &p, q.grid, mode, sums, shared, st)
-                         : l.shape.P == 1 ? launch_backward<8, 1>(*a, p, q.grid, mode, sums, shared, st)
-                         : l.shape.P == 2 ? launch_backward<8, 2>(*a, p, q.grid, mode, sums, shared, st)
-                                          : launch_backward<8, 4>(*a, p, q.grid, mode, sums, shared, st);
+    const NormKernel kernel = l.shape.kernel;
+    const int launched = kernel == kVectors       ? launch_backward<kVectors>(*a, p, q.grid, mode, sums, shared, st)
+                         : kernel == kVectors8    ? launch_backward<kVectors8>(*a, p, q.grid, mode, sums, shared, st)
+                         : kernel == kVectorsWide ? launch_backward<kVectorsWide>(*a, p, q.grid, mode, sums, shared, st)
+                         : kernel == kVectorsWidest
+                             ? launch_backward<kVectorsWidest>(*a, p, q.grid, mode, sums, shared, st)
+                             : launch_backward_elements(kernel, *a, &p, q.grid, mode, sums, shared, st);
     if (launched) return launched;
     LAMQ_CHECK_LAUNCH("lamq_norm_backward");
     if (!q.bytes) return LAMQ_OK;

@@ -65,20 +65,20 @@ struct Columns<E, false> {
 };
 
 // The block's teams' sums added in order and written as the block's partial row.
-template <int P, int V>
+template <int P, int V, bool kHold>
 __device__ __forceinline__ void write_partial(const BackwardParams &p, const Team &team, Vec<P * V> acc, float *part,
                                               float2 *shared) {
-    if constexpr (P * V <= kNormShared) {
-        constexpr int kPairs = Vec<P * V>::kPairs;
+    if constexpr (kHold) {
+        constexpr int kPairs = Vec<P * V>::kPairs, kThreads = 4096 / (P * V);
         if (p.slots > 1) {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < kPairs; ++i) shared[i * kNormThreads + threadIdx.x] = acc.v[i];
+            for (int i = 0; i < kPairs; ++i) shared[i * kThreads + threadIdx.x] = acc.v[i];
             __syncthreads();
             if (team.slot != 0) return;
             for (int s = 1; s < p.slots; ++s)
 #pragma unroll
-                for (int i = 0; i < kPairs; ++i) acc.v[i] = add2(acc.v[i], shared[i * kNormThreads + s * p.team + team.t]);
+                for (int i = 0; i < kPairs; ++i) acc.v[i] = add2(acc.v[i], shared[i * kThreads + s * p.team + team.t]);
         }
     }
     float *const row = part + (int64_t)blockIdx.x * p.columns;
@@ -91,15 +91,16 @@ __device__ __forceinline__ void write_partial(const BackwardParams &p, const Tea
     }
 }
 
-// Threads that hold few elements keep the weights and the gate of their columns in registers.
-template <typename R, typename B, int V, int P, int kMode, bool kSums>
-__global__ void __launch_bounds__(kNormThreads, kMode != kJoinFull && P * V <= kNormShared ? 2 : 1)
+// Threads of blocks that are not too large (kHold) keep the weights and the gate of their columns in registers.
+template <typename R, typename B, NormKernel kKernel, int kMode, bool kSums>
+__global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
     norm_backward_kernel(const __grid_constant__ BackwardParams p) {
     extern __shared__ uint4 stages[];
     __shared__ alignas(16) float scratch[Team::kScratch];
-    constexpr bool kFull = kMode == kJoinFull, kJoin = kMode != kNormAlone, kHold = P * V <= kNormShared;
+    constexpr int V = NormSizes<kKernel>::V, P = NormSizes<kKernel>::P;
+    constexpr bool kFull = kMode == kJoinFull, kJoin = kMode != kNormAlone, kHold = NormSizes<kKernel>::kHold;
     using Row = Vec<P * V>;
-    __shared__ float2 shared[kSums && kHold ? kNormThreads * Row::kPairs : 1];
+    __shared__ float2 shared[kSums && kHold ? NormSizes<kKernel>::kThreads * Row::kPairs : 1];
     Team team(p.team, scratch);
     const Ring<V, P> ring(stages, p.ring, team, p.packs);
     float *const columns = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(stages) + p.sums_at);
@@ -148,11 +149,11 @@ __global__ void __launch_bounds__(kNormThreads, kMode != kJoinFull && P * V <= k
         if (there || p.team < 32) {  // a team that has no row beside others of its warp that do: zeros
             const int at = there ? row : 0, bytes = there ? 16 : 0;
             if (has_dy) {
-                ring.fetch(stage, kTensorH, row_at<R>(p.in.h, at), bytes);
-                ring.fetch(stage, kTensorDy, row_at<B>(p.in.dy, at), bytes);
+                ring.fetch(stage, kTensorH, row_at<R, kJoin>(p.in.h, at), bytes);
+                ring.fetch(stage, kTensorDy, row_at<B, kJoin>(p.in.dy, at), bytes);
             }
-            if (has_dh) ring.fetch(stage, kTensorDh, row_at<R>(p.in.dh, at), bytes);
-            if (branch) ring.fetch(stage, kTensorBranch, row_at<B>(p.in.branch, at), bytes);
+            if (has_dh) ring.fetch(stage, kTensorDh, row_at<R, kJoin>(p.in.dh, at), bytes);
+            if (branch) ring.fetch(stage, kTensorBranch, row_at<B, kJoin>(p.in.branch, at), bytes);
             if (gates) ring.fetch_typed(stage, kTensorGate, gate_at(at), p.in.gate_dtype, bytes);
         }
         ++fetched;
@@ -182,14 +183,14 @@ __global__ void __launch_bounds__(kNormThreads, kMode != kJoinFull && P * V <= k
         const int at = live ? row : 0;
         Row g, x, b;  // dy, then the gradient at h, then at the branch; h; the branch
         if (has_dy) {
-            read(stage, kTensorH, row_at<R>(p.in.h, at), x);
-            read(stage, kTensorDy, row_at<B>(p.in.dy, at), g);
+            read(stage, kTensorH, row_at<R, kJoin>(p.in.h, at), x);
+            read(stage, kTensorDy, row_at<B, kJoin>(p.in.dy, at), g);
         } else {
             x.clear(), g.clear();
         }
         if constexpr (kFull) {
             if (branch)
-                read(stage, kTensorBranch, row_at<B>(p.in.branch, at), b);
+                read(stage, kTensorBranch, row_at<B, kJoin>(p.in.branch, at), b);
             else
                 b.clear();
         }
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(kNormThreads, kMode != kJoinFull && P * V <= k
             g = t;
         }
         if (has_dh) {
-            read(stage, kTensorDh, row_at<R>(p.in.dh, at), x);
+            read(stage, kTensorDh, row_at<R, kJoin>(p.in.dh, at), x);
             g += x;
         }
         if (live) {
@@ -289,49 +290,52 @@ __global__ void __launch_bounds__(kNormThreads, kMode != kJoinFull && P * V <= k
         stage = ring.after(stage), to = ring.after(to);
     }
     if constexpr (kSums) {
-        if (p.w_part) write_partial<P, V>(p, team, dw.all(), p.w_part, shared);
-        if (kFull && p.u_part) write_partial<P, V>(p, team, du.all(), p.u_part, shared);
-        if (kFull && p.gate_mode == kGateOne) write_partial<P, V>(p, team, dg.all(), p.g_part, shared);
+        if (p.w_part) write_partial<P, V, kHold>(p, team, dw.all(), p.w_part, shared);
+        if (kFull && p.u_part) write_partial<P, V, kHold>(p, team, du.all(), p.u_part, shared);
+        if (kFull && p.gate_mode == kGateOne) write_partial<P, V, kHold>(p, team, dg.all(), p.g_part, shared);
     }
 }
 
-template <typename R, typename B, int V, int P, int kMode, bool kSums>
+template <typename R, typename B, NormKernel kKernel, int kMode, bool kSums>
 int launch_backward(const BackwardParams &p, int grid, int shared, cudaStream_t stream) {
-    const auto kernel = norm_backward_kernel<R, B, V, P, kMode, kSums>;
+    const auto kernel = norm_backward_kernel<R, B, kKernel, kMode, kSums>;
     if (const int st = allow_shared(reinterpret_cast<const void *>(kernel), shared)) return st;
     kernel<<<grid, p.team * p.slots, shared, stream>>>(p);
     return LAMQ_OK;
 }
 
-template <typename R, typename B, int V, int P>
+template <typename R, typename B, NormKernel kKernel>
 int launch_backward(const BackwardParams &p, int grid, int mode, bool sums, int shared, cudaStream_t stream) {
-    if constexpr (P * V <= kNormFull)
+    constexpr bool k8 = kKernel == kVectors8 || kKernel == kElements8;  // for full joins only
+    if constexpr (k8 || kKernel == kVectorsWide)
         if (mode == kJoinFull)
-            return sums ? launch_backward<R, B, V, P, kJoinFull, true>(p, grid, shared, stream)
-                        : launch_backward<R, B, V, P, kJoinFull, false>(p, grid, shared, stream);
-    if (mode == kJoinPlain)
-        return sums ? launch_backward<R, B, V, P, kJoinPlain, true>(p, grid, shared, stream)
-                    : launch_backward<R, B, V, P, kJoinPlain, false>(p, grid, shared, stream);
-    if constexpr (std::is_same_v<R, B>)
-        return sums ? launch_backward<R, B, V, P, kNormAlone, true>(p, grid, shared, stream)
-                    : launch_backward<R, B, V, P, kNormAlone, false>(p, grid, shared, stream);
-    return LAMQ_ERR_INVALID;  // no such call: the checks refuse a norm of two types, the shape a wider full join
+            return sums ? launch_backward<R, B, kKernel, kJoinFull, true>(p, grid, shared, stream)
+                        : launch_backward<R, B, kKernel, kJoinFull, false>(p, grid, shared, stream);
+    if constexpr (!k8)
+        if (mode == kJoinPlain)
+            return sums ? launch_backward<R, B, kKernel, kJoinPlain, true>(p, grid, shared, stream)
+                        : launch_backward<R, B, kKernel, kJoinPlain, false>(p, grid, shared, stream);
+    if constexpr (!k8 && std::is_same_v<R, B>)
+        return sums ? launch_backward<R, B, kKernel, kNormAlone, true>(p, grid, shared, stream)
+                    : launch_backward<R, B, kKernel, kNormAlone, false>(p, grid, shared, stream);
+    return LAMQ_ERR_INVALID;  // no such call: the checks refuse a norm of two types, the shapes are chosen by the mode
 }
 
 // By the call's types.
-template <int V, int P>
+template <NormKernel kKernel>
 int launch_backward(const lamq_norm_args &a, const BackwardParams &p, int grid, int mode, bool sums, int shared,
                     cudaStream_t stream) {
     if (a.residual_dtype == LAMQ_BF16)
-        return launch_backward<__nv_bfloat16, __nv_bfloat16, V, P>(p, grid, mode, sums, shared, stream);
-    if (a.branch_dtype == LAMQ_BF16) return launch_backward<float, __nv_bfloat16, V, P>(p, grid, mode, sums, shared, stream);
-    return launch_backward<float, float, V, P>(p, grid, mode, sums, shared, stream);
+        return launch_backward<__nv_bfloat16, __nv_bfloat16, kKernel>(p, grid, mode, sums, shared, stream);
+    if (a.branch_dtype == LAMQ_BF16)
+        return launch_backward<float, __nv_bfloat16, kKernel>(p, grid, mode, sums, shared, stream);
+    return launch_backward<float, float, kKernel>(p, grid, mode, sums, shared, stream);
 }
 
 }  // namespace
 
 // The kernels for rows that may begin anywhere (norm_backward_elements.cu). `params`: a BackwardParams.
-int launch_backward_elements(int P, const lamq_norm_args &a, const void *params, int grid, int mode, bool sums, int shared,
+int launch_backward_elements(int kernel, const lamq_norm_args &a, const void *params, int grid, int mode, bool sums, int shared,
                              cudaStream_t stream);
 
 }  // namespace lamq

@@ -85,12 +85,12 @@ int launch_wide(const lamq_norm_args &a, const BackwardParams &p, int grid, int 
 
 }  // namespace
 
-int launch_backward_elements(int P, const lamq_norm_args &a, const void *params, int grid, int mode, bool sums, int shared,
+int launch_backward_elements(int kernel, const lamq_norm_args &a, const void *params, int grid, int mode, bool sums, int shared,
                              cudaStream_t stream) {
     const BackwardParams &p = *reinterpret_cast<const BackwardParams *>(params);
-    return P == 1   ? launch_backward<1, 1>(a, p, grid, mode, sums, shared, stream)
-           : P == 8 ? launch_backward<1, 8>(a, p, grid, mode, sums, shared, stream)
-                    : launch_wide(a, p, grid, mode, stream);
+    return kernel == kElements    ? launch_backward<kElements>(a, p, grid, mode, sums, shared, stream)
+           : kernel == kElements8 ? launch_backward<kElements8>(a, p, grid, mode, sums, shared, stream)
+                                  : launch_wide(a, p, grid, mode, stream);
 }
 
 }  // namespace lamq

@@ -14,7 +14,7 @@ but for trailing axes of one before the last: (d,) for all rows, (batch, 1, d) f
 element. Tensors are fp32 or bf16: the norm's input and output share a type; the residual and h share one, branch and y one (an
 fp32 stream takes bf16 branches, not the other way round); weights and the gate have types of their own. Sums are fp32 and
 results are rounded once: y comes from h before its rounding. Rows have up to 16384 elements; inputs may be strided views
-with a contiguous last axis (the heads of a projection's output), outputs are contiguous. eps is positive.
+with a contiguous last axis (the norm's also the heads of a projection's output), outputs are contiguous. eps is positive.
 """
 
 from __future__ import annotations
@@ -36,8 +36,8 @@ def _code(x: torch.Tensor, what: str) -> int:
     return code
 
 
-def _rows(x: torch.Tensor):
-    """(x, the lamq_rows of its rows), x copied where its rows do not lie at one or two strides."""
+def _rows(x: torch.Tensor, strides: int = 1):
+    """(x, the lamq_rows of its rows), x copied where its rows do not lie at `strides` strides (one or two)."""
     d = x.shape[-1]
     if x.is_contiguous():
         return x, (x.data_ptr(), 1 << 30, d, 0)
@@ -52,7 +52,7 @@ def _rows(x: torch.Tensor):
                 axes.append((n, s))
         if len(axes) <= 1:
             return x, (x.data_ptr(), 1 << 30, axes[0][1] if axes else d, 0)
-        if len(axes) == 2:
+        if len(axes) == 2 and strides == 2:
             return x, (x.data_ptr(), axes[1][0], axes[1][1], axes[0][1])
     x = x.contiguous()
     return x, (x.data_ptr(), 1 << 30, d, 0)
@@ -105,7 +105,7 @@ def norm_forward(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, offse
     n = y.numel() // d if d else 0
     if not n:
         return y
-    x, xr = _rows(x)
+    x, xr = _rows(x, 2)
     args = NORM_ARGS.pack(n, 1, d, code, code, wcode, 0, 0, 1.0, eps, offset, 0, *xr, *_NONE, weight.data_ptr(), 0, 0, 0,
                           y.data_ptr(), *_NONE, *_NONE, 0, 0, 0, 0, 0)
     here, stream = launch_on(dev)
@@ -140,8 +140,8 @@ def norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: 
         dw = torch.empty(d, dtype=weight.dtype, device=dev)
     if not n:
         return dx, None if dw is None else dw.zero_()
-    x, xr = _rows(x)
-    dy, dyr = _rows(dy)
+    x, xr = _rows(x, 2)
+    dy, dyr = _rows(dy, 2)
     args = NORM_ARGS.pack(n, 1, d, code, code, wcode, 0, 0, 1.0, eps, offset, 0, *xr, *_NONE, weight.data_ptr(), 0, 0, 0, 0,
                           *_NONE, *dyr, dx.data_ptr(), 0, ptr(dw) or 0, 0, 0)
     _backward(n, args, dev, dw is not None)

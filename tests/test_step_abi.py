@@ -38,6 +38,7 @@ BOTH = [(N, b"null pointer (args)"), (norm(n=-1), b"bad shape"), (norm(d=-1), b"
         (norm(scale=float("inf")), b"finite"), (norm(offset=float("nan")), b"finite"), (norm(gate=P, span=4), b"divide"),
         (norm(gate=P, span=0), b"divide"), (norm(residual=rows(0)), b"null pointer (residual)"),
         (norm(residual=rows(inner=0)), b"inner count"), (norm(branch=rows(inner=2**31)), b"inner count"),
+        (norm(branch=rows(inner=2, outer=100)), b"one stride"), (norm(residual=rows(row=2**30)), b"one stride"),
         (norm(branch=NO, weight=0), b"the norm alone"), (norm(branch=NO, post=P), b"the norm alone"),
         (norm(branch=NO, gate=P, span=6), b"the norm alone")]
 INVALID = [("lamq_norm_forward", (a, N), text) for a, text in BOTH + [(norm(h=0), b"null pointer (h)"),

@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, false), 1) norm_forwa
         if (kFull && post) load(p.in.post, p.in.post_dtype, p.offset, u);
     }
     const int step = gridDim.x * p.slots, first = blockIdx.x * p.slots + team.slot;
-    const auto fetch = [&](int row, int stage) {
+    const auto fetch = [&](int row, uint32_t stage) {
         if (row < p.rows || p.team < 32) {  // a team that has no row beside others of its warp that do: zeros
             const int at = row < p.rows ? row : 0, bytes = row < p.rows ? 16 : 0;
             ring.fetch(stage, kTensorH, row_at<R, kBranch>(p.in.h, at), bytes);
@@ -69,15 +69,8 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, false), 1) norm_forwa
         }
         ring.commit();
     };
-    const auto read = [&](int stage, int tensor, const auto *row, Row &x) {
-#pragma unroll
-        for (int q = 0; q < P; ++q) {
-            float f[V];
-            ring.read(stage, tensor, row, q, f);
-            x.set(q * V, f);
-        }
-    };
-    int stage = 0, to = 0, ahead = first;
+    uint32_t stage = ring.first(), to = stage;
+    int ahead = first;
     for (int i = 1; i < p.ring.stages; ++i, ahead += step, to = ring.after(to)) fetch(ahead, to);
     // Teams of a warp take steps together: the loop ends when the first of them has no row.
     const int lead = p.team < 32 ? team.slot % (32 / p.team) : 0;
@@ -92,7 +85,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, false), 1) norm_forwa
         const bool live = row < p.rows;
         const int at = live ? row : 0;
         Row x;
-        if constexpr (kBranch) read(stage, kTensorBranch, row_at<B, true>(p.in.branch, at), x);
+        if constexpr (kBranch) ring.read(stage, kTensorBranch, row_at<B, true>(p.in.branch, at), x);
         if constexpr (kFull) {
             if (post) {
                 float ss[1] = {x.dot(x)}, shrunk;
@@ -105,12 +98,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, false), 1) norm_forwa
             if (gate && live) {
                 const unsigned char *const from = gate_at(row);
                 if (gates) {
-#pragma unroll
-                    for (int q = 0; q < P; ++q) {
-                        float f[V];
-                        ring.read_typed(stage, kTensorGate, from, p.in.gate_dtype, q, f);
-                        held.set(q * V, f);
-                    }
+                    ring.read_typed(stage, kTensorGate, from, p.in.gate_dtype, held);
                 } else if (p.in.by_span.of(row) != gate_row) {
                     gate_row = p.in.by_span.of(row);
                     load(from, p.in.gate_dtype, 0.f, held);
@@ -120,10 +108,10 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, false), 1) norm_forwa
         }
         if constexpr (kBranch) {
             Row r;
-            read(stage, kTensorH, row_at<R, kBranch>(p.in.h, at), r);
+            ring.read(stage, kTensorH, row_at<R, kBranch>(p.in.h, at), r);
             x.scale_add(p.scale, r);
         } else {
-            read(stage, kTensorH, row_at<R, kBranch>(p.in.h, at), x);
+            ring.read(stage, kTensorH, row_at<R, kBranch>(p.in.h, at), x);
         }
         if (kBranch && live) {
             R *const out = reinterpret_cast<R *>(p.h) + (int64_t)row * p.d;

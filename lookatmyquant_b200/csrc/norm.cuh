@@ -357,25 +357,49 @@ struct Team {
 enum { kTensorH, kTensorDy, kTensorDh, kTensorBranch, kTensorGate, kTensors };
 
 struct RingParams {
-    int stages, stage_bytes;          // of a block
+    int stages, stage_bytes, ring_bytes;  // of a block: of one stage, of all
     int at[kTensors], image[kTensors];  // where a tensor's part of a stage begins; elements: bytes of a team's row
 };
 
+__device__ __forceinline__ uint4 shared16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ float shared_one(uint32_t at) {
+    if constexpr (sizeof(T) == 4) {
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at));
+        return v;
+    } else {
+        uint16_t v;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+        return __uint_as_float((uint32_t)v << 16);
+    }
+}
+
+// Places in it are the bytes of the shared window at which a stage begins.
 template <int V, int P>
 struct Ring {
-    unsigned char *base;
+    uint32_t base;
     const RingParams &p;
     const Team &team;
     int packs;
 
-    __device__ Ring(void *shared, const RingParams &p_, const Team &team_, int packs_)
-        : base(reinterpret_cast<unsigned char *>(shared)), p(p_), team(team_), packs(packs_) {}
+    __device__ Ring(const void *shared, const RingParams &p_, const Team &team_, int packs_)
+        : base((uint32_t)__cvta_generic_to_shared(shared)), p(p_), team(team_), packs(packs_) {}
+
+    __device__ __forceinline__ uint32_t first() const { return base; }
+    __device__ __forceinline__ uint32_t after(uint32_t stage) const {
+        const uint32_t next = stage + p.stage_bytes;
+        return next == base + p.ring_bytes ? base : next;
+    }
 
     // 16 bytes, or (bytes = 0) as many zeros
-    __device__ __forceinline__ static void copy16(void *to, const void *from, int bytes) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from),
-                     "r"(bytes)
-                     : "memory");
+    __device__ __forceinline__ static void copy16(uint32_t to, const void *from, int bytes) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
     }
     __device__ __forceinline__ static void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
@@ -391,15 +415,14 @@ struct Ring {
         if (V == 1) team.barrier();
     }
 
-    __device__ __forceinline__ unsigned char *part(int stage, int tensor) const {
-        return base + stage * p.stage_bytes + p.at[tensor] + (V == 1 ? team.slot * p.image[tensor] : 0);
+    __device__ __forceinline__ uint32_t part(uint32_t stage, int tensor) const {
+        return stage + p.at[tensor] + (V == 1 ? team.slot * p.image[tensor] : threadIdx.x * 16);
     }
-    __device__ __forceinline__ int after(int stage) const { return stage + 1 == p.stages ? 0 : stage + 1; }
 
     // Starts the copies of a tensor's row (bytes = 0: of a row of zeros).
     template <typename T>
-    __device__ __forceinline__ void fetch(int stage, int tensor, const T *row, int bytes) const {
-        unsigned char *const to = part(stage, tensor);
+    __device__ __forceinline__ void fetch(uint32_t stage, int tensor, const T *row, int bytes) const {
+        const uint32_t to = part(stage, tensor);
         if constexpr (V == 8) {
             constexpr int kPieces = sizeof(T) / 2;
 #pragma unroll
@@ -408,7 +431,7 @@ struct Ring {
                 if (pack >= packs) pack = 0, some = 0;  // zeros behind the row's end
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i)
-                    copy16(to + ((q * kPieces + i) * blockDim.x + threadIdx.x) * 16, row + pack * 8 + i * (8 / kPieces), some);
+                    copy16(to + (q * kPieces + i) * blockDim.x * 16, row + pack * 8 + i * (8 / kPieces), some);
             }
         } else {
             const int shift = (int)(reinterpret_cast<uintptr_t>(row) & 15);
@@ -418,35 +441,44 @@ struct Ring {
         }
     }
 
-    // This thread's pack q of the row in a stage.
+    // This thread's elements of the row in a stage, zeros behind the row's end.
     template <typename T>
-    __device__ __forceinline__ void read(int stage, int tensor, const T *row, int q, float (&f)[V]) const {
-        const unsigned char *const from = part(stage, tensor);
+    __device__ __forceinline__ void read(uint32_t stage, int tensor, const T *row, Vec<P * V> &x) const {
+        uint32_t from = part(stage, tensor);
         if constexpr (V == 8) {
             constexpr int kPieces = sizeof(T) / 2;
-            uint4 v[kPieces];
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i)
-                v[i] = *reinterpret_cast<const uint4 *>(from + ((q * kPieces + i) * blockDim.x + threadIdx.x) * 16);
-            Raw<T, 8>::unpack(v, f);
+            for (int q = 0; q < P; ++q) {
+                uint4 v[kPieces];
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) v[i] = shared16(from + (q * kPieces + i) * blockDim.x * 16);
+                float f[8];
+                Raw<T, 8>::unpack(v, f);
+                x.set(q * 8, f);
+            }
         } else {
-            const int shift = (int)(reinterpret_cast<uintptr_t>(row) & 15);
-            const int pack = team.t + q * team.size;
-            f[0] = pack < packs ? to_float(*reinterpret_cast<const T *>(from + shift + pack * (int)sizeof(T))) : 0.f;
+            from += (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15) + team.t * (uint32_t)sizeof(T);
+            const int there = packs - team.t;
+#pragma unroll
+            for (int q = 0; q < P; ++q, from += team.size * (uint32_t)sizeof(T)) {
+                float f[1] = {shared_one<T>(from)};  // the image has room for all of the team's places
+                if (q * team.size >= there) f[0] = 0.f;
+                x.set(q, f);
+            }
         }
     }
 
-    __device__ __forceinline__ void fetch_typed(int stage, int tensor, const void *row, int dtype, int bytes) const {
+    __device__ __forceinline__ void fetch_typed(uint32_t stage, int tensor, const void *row, int dtype, int bytes) const {
         if (dtype == LAMQ_F32)
             fetch(stage, tensor, reinterpret_cast<const float *>(row), bytes);
         else
             fetch(stage, tensor, reinterpret_cast<const __nv_bfloat16 *>(row), bytes);
     }
-    __device__ __forceinline__ void read_typed(int stage, int tensor, const void *row, int dtype, int q, float (&f)[V]) const {
+    __device__ __forceinline__ void read_typed(uint32_t stage, int tensor, const void *row, int dtype, Vec<P * V> &x) const {
         if (dtype == LAMQ_F32)
-            read(stage, tensor, reinterpret_cast<const float *>(row), q, f);
+            read(stage, tensor, reinterpret_cast<const float *>(row), x);
         else
-            read(stage, tensor, reinterpret_cast<const __nv_bfloat16 *>(row), q, f);
+            read(stage, tensor, reinterpret_cast<const __nv_bfloat16 *>(row), x);
     }
 };
 
@@ -615,7 +647,7 @@ inline NormLayout norm_layout(const lamq_norm_args &a, bool backward, bool sums,
         RingParams &g = l.ring;
         for (int k = 0; k < kTensors; ++k) {
             g.at[k] = g.stage_bytes;
-            g.image[k] = (a.d * size[k] + 15) / 16 * 16 + 16;
+            g.image[k] = (s.team * s.P * size[k] + 15) / 16 * 16 + 16;  // of elements: a place for each, wherever the row begins
             g.stage_bytes += size[k] == 0 ? 0 : s.V == 8 ? s.P * 8 * size[k] * threads : g.image[k] * l.slots;
         }
         l.sums_bytes = sums && !hold ? (l.mode == kJoinFull ? 3 : 1) * s.P * s.V * threads * (int)sizeof(float) : 0;
@@ -626,7 +658,8 @@ inline NormLayout norm_layout(const lamq_norm_args &a, bool backward, bool sums,
             g.stages = std::min(4, (kSmemSM / l.blocks - own) / std::max(1, g.stage_bytes));
             if (g.stages >= 2 || l.blocks == 1) break;
         }
-        l.shared = g.stages * g.stage_bytes + l.sums_bytes;
+        g.ring_bytes = g.stages * g.stage_bytes;
+        l.shared = g.ring_bytes + l.sums_bytes;
         if (g.stages >= (s.V == 1 ? 2 : 1)) return l;
     }
     s.V = 1, s.kernel = kWide, s.team = kNormThreads, s.packs = a.d;

@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
     const bool ranges = kFull && p.gate_mode >= kGateInside;  // each team its own range of rows
     const int first = ranges ? worker * p.per : blockIdx.x * p.slots * p.per + team.slot, step = ranges ? 1 : p.slots;
     int fetched = 0;
-    const auto fetch = [&](int stage) {
+    const auto fetch = [&](uint32_t stage) {
         const int row = first + fetched * step;
         const bool there = fetched < p.per && row < p.rows;
         if (there || p.team < 32) {  // a team that has no row beside others of its warp that do: zeros
@@ -159,15 +159,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
         ++fetched;
         ring.commit();
     };
-    const auto read = [&](int stage, int tensor, const auto *row, Row &x) {
-#pragma unroll
-        for (int q = 0; q < P; ++q) {
-            float f[V];
-            ring.read(stage, tensor, row, q, f);
-            x.set(q * V, f);
-        }
-    };
-    int stage = 0, to = 0;
+    uint32_t stage = ring.first(), to = stage;
     for (int i = 1; i < p.ring.stages; ++i, to = ring.after(to)) fetch(to);
     for (int k = 0; k < p.per; ++k) {
         const int row = first + k * step;
@@ -183,14 +175,14 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
         const int at = live ? row : 0;
         Row g, x, b;  // dy, then the gradient at h, then at the branch; h; the branch
         if (has_dy) {
-            read(stage, kTensorH, row_at<R, kJoin>(p.in.h, at), x);
-            read(stage, kTensorDy, row_at<B, kJoin>(p.in.dy, at), g);
+            ring.read(stage, kTensorH, row_at<R, kJoin>(p.in.h, at), x);
+            ring.read(stage, kTensorDy, row_at<B, kJoin>(p.in.dy, at), g);
         } else {
             x.clear(), g.clear();
         }
         if constexpr (kFull) {
             if (branch)
-                read(stage, kTensorBranch, row_at<B, kJoin>(p.in.branch, at), b);
+                ring.read(stage, kTensorBranch, row_at<B, kJoin>(p.in.branch, at), b);
             else
                 b.clear();
         }
@@ -216,7 +208,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
             g = t;
         }
         if (has_dh) {
-            read(stage, kTensorDh, row_at<R, kJoin>(p.in.dh, at), x);
+            ring.read(stage, kTensorDh, row_at<R, kJoin>(p.in.dh, at), x);
             g += x;
         }
         if (live) {
@@ -239,13 +231,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
                 if (gate && live) {
                     const int gate_row = p.in.by_span.of(row);
                     if (gates) {
-                        const unsigned char *const from = gate_at(row);
-#pragma unroll
-                        for (int q = 0; q < P; ++q) {
-                            float f[V];
-                            ring.read_typed(stage, kTensorGate, from, p.in.gate_dtype, q, f);
-                            held.set(q * V, f);
-                        }
+                        ring.read_typed(stage, kTensorGate, gate_at(row), p.in.gate_dtype, held);
                     } else if (gate_row != gate_of) {
                         gate_of = gate_row;
                         load(gate_at(row), p.in.gate_dtype, 0.f, held);

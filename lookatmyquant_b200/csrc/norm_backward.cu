@@ -46,8 +46,8 @@ Plan plan_of(const lamq_norm_args &a) {
     return q;
 }
 
-// Each output row is the sum of some partial rows: a block adds 32 columns of them, its warps every 16th row in order, then
-// the warps in order.
+// Each output row is the sum of some partial rows: a block adds 32 columns of them, its warps every 32nd row in order, then
+// the warps in order. Bound by the latency of its few loads, which are all on their way at once for up to 512 rows.
 struct ReduceParams {
     const float *w_part, *u_part, *g_part;
     void *d_weight, *d_post, *d_gate;
@@ -56,10 +56,11 @@ struct ReduceParams {
     int gate_one, gate_span, per, rows;
 };
 
-constexpr int kReduceWarps = 16;
+constexpr int kReduceWarps = 32;
 
 __global__ void __launch_bounds__(kReduceWarps * 32) norm_reduce_kernel(const __grid_constant__ ReduceParams p) {
     __shared__ float sums[kReduceWarps][32];
+    await_previous();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int blocks = (p.d + 31) / 32;  // of 32 columns each
     int job = blockIdx.x / blocks;
@@ -85,7 +86,7 @@ __global__ void __launch_bounds__(kReduceWarps * 32) norm_reduce_kernel(const __
     float s = 0.f;
     if (col < p.d) {
         const float *src = part + col;
-#pragma unroll 4
+#pragma unroll 16
         for (int k = warp; k < count; k += kReduceWarps) s += __ldcg(src + (int64_t)k * p.columns);
     }
     sums[warp][lane] = s;
@@ -149,7 +150,7 @@ extern "C" int lamq_norm_backward(const lamq_norm_args *a, void *workspace, size
     sum.gate_one = q.gate_mode == kGateOne, sum.gate_span = p.in.gate_span, sum.per = q.per, sum.rows = p.rows;
     const int64_t jobs = (a->d_weight ? 1 : 0) + (a->d_post ? 1 : 0) +
                          (q.gate_mode == kGateOne ? 1 : q.gate_mode == kGateAcross ? a->rows / a->gate_span : 0);
-    norm_reduce_kernel<<<(unsigned)(jobs * ((a->d + 31) / 32)), kReduceWarps * 32, 0, st>>>(sum);
+    launch_following(norm_reduce_kernel, (unsigned)(jobs * ((a->d + 31) / 32)), kReduceWarps * 32, st, sum);
     LAMQ_CHECK_LAUNCH("lamq_norm_backward (sums)");
     return LAMQ_OK;
 }

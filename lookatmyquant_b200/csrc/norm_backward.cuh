@@ -10,6 +10,7 @@
 // takes the rows of one range, blocks write one partial row each, and a second kernel adds the partials in order.
 #pragma once
 
+#include "dependent.cuh"
 #include "norm_wide.cuh"
 
 namespace lamq {
@@ -101,6 +102,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
     constexpr bool kFull = kMode == kJoinFull, kJoin = kMode != kNormAlone, kHold = NormSizes<kKernel>::kHold;
     using Row = Vec<P * V>;
     __shared__ float2 shared[kSums && kHold ? NormSizes<kKernel>::kThreads * Row::kPairs : 1];
+    if (kSums) let_follow();
     Team team(p.team, scratch);
     const Ring<V, P> ring(stages, p.ring, team, p.packs);
     float *const columns = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(stages) + p.sums_at);

@@ -8,6 +8,7 @@ namespace {
 template <typename R, typename B>
 __global__ void __launch_bounds__(kWideThreads, 1) norm_backward_wide_kernel(const __grid_constant__ BackwardParams p, int mode) {
     __shared__ alignas(16) float scratch[Team::kScratch];
+    let_follow();
     Team team(kWideThreads, scratch);
     const int64_t block_row = (int64_t)blockIdx.x * p.columns;
     const bool full = mode == kJoinFull;

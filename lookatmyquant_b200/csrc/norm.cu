@@ -21,21 +21,21 @@ struct ForwardParams {
 };
 
 // Threads of blocks that are not too large (kHold) keep the weights and the gate of their columns in registers.
-template <typename R, typename B, NormKernel kKernel, int kMode>
+template <typename R, typename B, NormKernel kKernel, int kMode, bool kSub>
 __global__ void __launch_bounds__(resident(kKernel, kMode, false), 1) norm_forward_kernel(const __grid_constant__ ForwardParams p) {
     extern __shared__ uint4 stages[];
-    __shared__ alignas(16) float scratch[Team::kScratch];
+    __shared__ alignas(16) float scratch[Team<false>::kScratch];
     constexpr int V = NormSizes<kKernel>::V, P = NormSizes<kKernel>::P;
     constexpr bool kBranch = kMode != kNormAlone, kFull = kMode == kJoinFull, kHold = NormSizes<kKernel>::kHold;
     using Row = Vec<P * V>;
-    Team team(p.team, scratch);
-    const Ring<V, P> ring(stages, p.ring, team, p.packs);
+    Team<kSub> team(p.team, P, scratch);
+    const Ring<V, P, kSub> ring(stages, p.ring, team, p.packs);
     const bool post = kFull && (p.in.has & kHasPost), gate = kFull && (p.in.has & kHasGate), pre = p.in.has & kHasWeight;
     const bool gates = gate && p.in.gate_span == 1;  // a gate row for each row
     const auto each = [&](auto f) {  // this thread's packs
 #pragma unroll
         for (int q = 0; q < P; ++q) {
-            const int pack = team.t + q * p.team;
+            const int pack = team.pack(q);
             if (pack < p.packs) f(q, pack);
         }
     };
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, false), 1) norm_forwa
     }
     const int step = gridDim.x * p.slots, first = blockIdx.x * p.slots + team.slot;
     const auto fetch = [&](int row, uint32_t stage) {
-        if (row < p.rows || p.team < 32) {  // a team that has no row beside others of its warp that do: zeros
+        if (row < p.rows || kSub) {  // a team that has no row beside others of its warp that do: zeros
             const int at = row < p.rows ? row : 0, bytes = row < p.rows ? 16 : 0;
             ring.fetch(stage, kTensorH, row_at<R, kBranch>(p.in.h, at), bytes);
             if (kBranch) ring.fetch(stage, kTensorBranch, row_at<B, true>(p.in.branch, at), bytes);
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, false), 1) norm_forwa
     int ahead = first;
     for (int i = 1; i < p.ring.stages; ++i, ahead += step, to = ring.after(to)) fetch(ahead, to);
     // Teams of a warp take steps together: the loop ends when the first of them has no row.
-    const int lead = p.team < 32 ? team.slot % (32 / p.team) : 0;
+    const int lead = kSub ? team.slot % (32 / p.team) : 0;
     for (int row = first; row - lead < p.rows; row += step, ahead += step) {
         if (V == 1 && p.ring.stages > 1) {  // all have read the stage that is filled next
             ring.wait();
@@ -142,54 +142,61 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, false), 1) norm_forwa
 }
 
 template <typename R, typename B, bool kBranch>
-__global__ void __launch_bounds__(kWideThreads, 1) norm_forward_wide_kernel(const __grid_constant__ ForwardParams p) {
-    __shared__ alignas(16) float scratch[Team::kScratch];
-    Team team(kWideThreads, scratch);
+__global__ void __launch_bounds__(kWideThreads) norm_forward_wide_kernel(const __grid_constant__ ForwardParams p) {
+    extern __shared__ float row_of_h[];
+    __shared__ float scratch[32];
     for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
         const R *const src = row_at<R>(p.in.h, row);
         const B *const add = row_at<B>(p.in.branch, kBranch ? row : 0);
-        const int64_t g = (int64_t)(row / p.in.gate_span) * p.d;
-        float shrunk, f = 1.f;
-        if (kBranch && (p.in.has & kHasPost)) {
-            f = wide_factor(team, p.d, [&](int j) { return load_one(add + j); }, p.inv_d, p.eps, shrunk);
-        } else {
-            shrunk = 1.f;
+        const int64_t g = (int64_t)p.in.by_span.of(row) * p.d, out = (int64_t)row * p.d;
+        const bool post = kBranch && (p.in.has & kHasPost), gate = kBranch && (p.in.has & kHasGate);
+        float shrunk = 1.f, f = 1.f, s[1] = {0.f};
+        if (post) {
+            wide_each(p.d, [&](int j) {
+                const float b = load_one(add + j);
+                s[0] = fmaf(b, b, s[0]);
+            });
+            wide_sum(s, scratch);
+            f = wide_factor(s[0], p.d, [&](int j) { return load_one(add + j); }, p.inv_d, p.eps, shrunk, scratch);
+            s[0] = 0.f;
         }
-        const auto h = [&](int j) {
-            const float r = load_one(src + j);
-            if (!kBranch) return r;
-            float x = load_one(add + j);
-            if (p.in.has & kHasPost) x = x * shrunk * (f * (p.offset + value_at(p.in.post, p.in.post_dtype, j)));
-            if (p.in.has & kHasGate) x *= value_at(p.in.gate, p.in.gate_dtype, g + j);
-            return fmaf(p.scale, x, r);
-        };
-        if (kBranch)
-            for (int j = threadIdx.x; j < p.d; j += kWideThreads) {
-                const float x[1] = {h(j)};
-                Raw<R, 1>::store(reinterpret_cast<R *>(p.h) + (int64_t)row * p.d + j, x);
+        wide_each(p.d, [&](int j) {
+            float h = load_one(src + j);
+            if (kBranch) {
+                float x = load_one(add + j);
+                if (post) x = x * shrunk * (f * (p.offset + value_at(p.in.post, p.in.post_dtype, j)));
+                if (gate) x *= value_at(p.in.gate, p.in.gate_dtype, g + j);
+                const float to[1] = {fmaf(p.scale, x, h)};
+                Raw<R, 1>::store(reinterpret_cast<R *>(p.h) + out + j, to);
+                h = to[0];
             }
+            row_of_h[j] = h;
+            s[0] = fmaf(h, h, s[0]);
+        });
         if (p.in.has & kHasWeight) {
-            float less;
-            const float factor = wide_factor(team, p.d, h, p.inv_d, p.eps, less);
-            for (int j = threadIdx.x; j < p.d; j += kWideThreads) {
-                const float y[1] = {h(j) * less * factor * (p.offset + value_at(p.in.weight, p.in.weight_dtype, j))};
-                Raw<B, 1>::store(reinterpret_cast<B *>(p.y) + (int64_t)row * p.d + j, y);
-            }
+            wide_sum(s, scratch);
+            const float factor = wide_factor(s[0], p.d, [&](int j) { return row_of_h[j]; }, p.inv_d, p.eps, shrunk, scratch);
+            wide_each(p.d, [&](int j) {
+                const float y[1] = {row_of_h[j] * shrunk * factor * (p.offset + value_at(p.in.weight, p.in.weight_dtype, j))};
+                Raw<B, 1>::store(reinterpret_cast<B *>(p.y) + out + j, y);
+            });
         }
     }
 }
 
-template <typename R, typename B>
-void launch_wide(const ForwardParams &p, int grid, bool branch, cudaStream_t stream) {
-    if (branch)
-        norm_forward_wide_kernel<R, B, true><<<grid, kWideThreads, 0, stream>>>(p);
-    else if constexpr (std::is_same_v<R, B>)
-        norm_forward_wide_kernel<R, B, false><<<grid, kWideThreads, 0, stream>>>(p);
+template <typename R, typename B, bool kBranch>
+int launch_wide(const ForwardParams &p, int grid, int shared, cudaStream_t stream) {
+    const auto kernel = norm_forward_wide_kernel<R, B, kBranch>;
+    if (const int st = allow_shared(reinterpret_cast<const void *>(kernel), shared)) return st;
+    kernel<<<grid, kWideThreads, shared, stream>>>(p);
+    return LAMQ_OK;
 }
 
 template <typename R, typename B, NormKernel kKernel, int kMode>
 int launch_forward(const ForwardParams &p, int grid, int shared, cudaStream_t stream) {
-    const auto kernel = norm_forward_kernel<R, B, kKernel, kMode>;
+    const bool sub = NormSizes<kKernel>::kHold && p.team < 32;
+    const auto kernel = sub ? norm_forward_kernel<R, B, kKernel, kMode, NormSizes<kKernel>::kHold>
+                            : norm_forward_kernel<R, B, kKernel, kMode, false>;
     if (const int st = allow_shared(reinterpret_cast<const void *>(kernel), shared)) return st;
     kernel<<<grid, p.team * p.slots, shared, stream>>>(p);
     return LAMQ_OK;
@@ -212,9 +219,11 @@ int launch_forward(NormKernel kernel, const ForwardParams &p, int grid, int mode
         case kVectorsWidest: return launch_forward<R, B, kVectorsWidest>(p, grid, mode, shared, stream);
         case kVectors8:
         case kElements8: return LAMQ_ERR_INVALID;  // backward only
-        case kWide: launch_wide<R, B>(p, grid, mode != kNormAlone, stream);
+        case kWide:
+            if (mode != kNormAlone) return launch_wide<R, B, true>(p, grid, shared, stream);
+            if constexpr (std::is_same_v<R, B>) return launch_wide<R, B, false>(p, grid, shared, stream);
     }
-    return LAMQ_OK;
+    return LAMQ_ERR_INVALID;  // the checks refuse a norm of two types
 }
 
 }  // namespace

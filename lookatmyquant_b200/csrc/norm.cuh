@@ -277,24 +277,34 @@ __device__ __forceinline__ const T *row_at(const Rows &r, int i) {
 
 constexpr int kNormWarps = kNormThreads / 32;
 
+// kSub: a team of less than a warp. Its thread t holds the packs t, t + size, ...; in larger ones a warp holds its threads' packs
+// one behind the other, 32 at a time, so that a thread's packs lie at a distance known to the compiler.
+template <bool kSub>
 struct Team {
     int size, t, slot;  // threads of a team; this one's place; the team's place in the block
+    int first;          // this thread's first pack
     int turn;           // which half of the scratch the next exchange uses
     float *scratch;     // kScratch floats, 16-byte aligned
 
     // Teams of more than a warp are at most half as many as the block's warps; each has kNormWarps floats for a sum.
     static constexpr int kSlots = kNormWarps / 2, kHalf = kSlots * kNormSums * kNormWarps, kScratch = 2 * kHalf;
 
-    __device__ Team(int size_, float *scratch_)
-        : size(size_), t(threadIdx.x % size_), slot(threadIdx.x / size_), turn(0), scratch(scratch_) {
-        if (size > 32) {  // the places of the warps that there are not add zeros
+    __device__ Team(int size_, int packs, float *scratch_)
+        : size(size_), t(threadIdx.x % size_), slot(threadIdx.x / size_), first(kSub ? t : (t >> 5) * 32 * packs + (t & 31)),
+          turn(0), scratch(scratch_) {
+        if (!kSub && size > 32) {  // the places of the warps that there are not add zeros
             for (int i = threadIdx.x; i < kScratch; i += blockDim.x) scratch[i] = 0.f;
             __syncthreads();
         }
     }
 
+    __device__ __forceinline__ int pack(int q) const { return first + q * (kSub ? size : 32); }
+
+    // Of the warp: whether any team's `x` holds; of a larger team, where all agree, x.
+    __device__ __forceinline__ static bool any(bool x) { return kSub ? __any_sync(0xffffffffu, x) : x; }
+
     __device__ __forceinline__ void barrier() const {
-        if (size <= 32)
+        if (kSub || size <= 32)
             __syncwarp();
         else
             asm volatile("bar.sync %0, %1;" ::"r"(slot + 1), "r"(size) : "memory");
@@ -306,7 +316,7 @@ struct Team {
     template <int K>
     __device__ __forceinline__ void sum(float (&v)[K]) {
         static_assert(K <= kNormSums, "the scratch holds kNormSums sums a team");
-        if (size <= 32) {
+        if constexpr (kSub) {
             for (int o = size >> 1; o > 0; o >>= 1)
 #pragma unroll
                 for (int k = 0; k < K; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
@@ -331,6 +341,12 @@ struct Team {
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1)
             if (x <= (K == 3 ? 4 : K == 2 ? 8 : 16)) s += __shfl_xor_sync(0xffffffffu, s, x);
+        if (size == 32) {
+            v[0] = __shfl_sync(0xffffffffu, s, 0);
+            if constexpr (K >= 2) v[1] = __shfl_sync(0xffffffffu, s, 16);
+            if constexpr (K == 3) v[2] = __shfl_sync(0xffffffffu, s, 8);
+            return;
+        }
         float *const half = scratch + turn * kHalf + slot * (kNormSums * kNormWarps);
         turn ^= 1;
         if (lane == 0 || (K >= 2 && lane == 16) || (K == 3 && lane == 8)) half[mine * kNormWarps + (t >> 5)] = s;
@@ -380,15 +396,16 @@ __device__ __forceinline__ float shared_one(uint32_t at) {
     }
 }
 
-// Places in it are the bytes of the shared window at which a stage begins.
-template <int V, int P>
+// Places in it are the bytes of the shared window at which a stage begins. Vectors: a warp's pieces lie together, 512 bytes for
+// each pack (fp32: two) of its threads.
+template <int V, int P, bool kSub>
 struct Ring {
     uint32_t base;
     const RingParams &p;
-    const Team &team;
+    const Team<kSub> &team;
     int packs;
 
-    __device__ Ring(const void *shared, const RingParams &p_, const Team &team_, int packs_)
+    __device__ Ring(const void *shared, const RingParams &p_, const Team<kSub> &team_, int packs_)
         : base((uint32_t)__cvta_generic_to_shared(shared)), p(p_), team(team_), packs(packs_) {}
 
     __device__ __forceinline__ uint32_t first() const { return base; }
@@ -416,22 +433,28 @@ struct Ring {
     }
 
     __device__ __forceinline__ uint32_t part(uint32_t stage, int tensor) const {
-        return stage + p.at[tensor] + (V == 1 ? team.slot * p.image[tensor] : threadIdx.x * 16);
+        return stage + p.at[tensor] + (V == 1 ? team.slot * p.image[tensor] : 0);
+    }
+    // of a thread's first piece among the vectors
+    template <typename T>
+    __device__ __forceinline__ static uint32_t own() {
+        return (threadIdx.x >> 5) * (P * (int)sizeof(T) / 2 * 512) + (threadIdx.x & 31) * 16;
     }
 
     // Starts the copies of a tensor's row (bytes = 0: of a row of zeros).
     template <typename T>
     __device__ __forceinline__ void fetch(uint32_t stage, int tensor, const T *row, int bytes) const {
-        const uint32_t to = part(stage, tensor);
+        uint32_t to = part(stage, tensor);
         if constexpr (V == 8) {
             constexpr int kPieces = sizeof(T) / 2;
+            to += own<T>();
 #pragma unroll
             for (int q = 0; q < P; ++q) {
-                int pack = team.t + q * team.size, some = bytes;
+                int pack = team.pack(q), some = bytes;
                 if (pack >= packs) pack = 0, some = 0;  // zeros behind the row's end
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i)
-                    copy16(to + (q * kPieces + i) * blockDim.x * 16, row + pack * 8 + i * (8 / kPieces), some);
+                    copy16(to + (q * kPieces + i) * 512, row + pack * 8 + i * (8 / kPieces), some);
             }
         } else {
             const int shift = (int)(reinterpret_cast<uintptr_t>(row) & 15);
@@ -447,22 +470,23 @@ struct Ring {
         uint32_t from = part(stage, tensor);
         if constexpr (V == 8) {
             constexpr int kPieces = sizeof(T) / 2;
+            from += own<T>();
 #pragma unroll
             for (int q = 0; q < P; ++q) {
                 uint4 v[kPieces];
 #pragma unroll
-                for (int i = 0; i < kPieces; ++i) v[i] = shared16(from + (q * kPieces + i) * blockDim.x * 16);
+                for (int i = 0; i < kPieces; ++i) v[i] = shared16(from + (q * kPieces + i) * 512);
                 float f[8];
                 Raw<T, 8>::unpack(v, f);
                 x.set(q * 8, f);
             }
         } else {
-            from += (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15) + team.t * (uint32_t)sizeof(T);
-            const int there = packs - team.t;
+            from += (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15) + team.first * (uint32_t)sizeof(T);
+            const int there = packs - team.first, step = kSub ? team.size : 32;
 #pragma unroll
-            for (int q = 0; q < P; ++q, from += team.size * (uint32_t)sizeof(T)) {
-                float f[1] = {shared_one<T>(from)};  // the image has room for all of the team's places
-                if (q * team.size >= there) f[0] = 0.f;
+            for (int q = 0; q < P; ++q) {
+                float f[1] = {shared_one<T>(from + q * step * (int)sizeof(T))};  // the image has room for all places
+                if (q * step >= there) f[0] = 0.f;
                 x.set(q, f);
             }
         }
@@ -494,11 +518,11 @@ constexpr float kShrink = 0x1p-80f;  // brings fp32's largest numbers where 1638
 // The factor (mean(x²) + eps)^-1/2 of a row, from the sum of squares, for x as it stands after the call: where the sum
 // overflowed, x is multiplied by kShrink and summed again (eps is then far below the mean's last bit). `shrunk` is
 // kShrink or 1: the factor of x as it was is the result times `shrunk`.
-template <int E>
-__device__ __forceinline__ float unit_factor(Team &team, Vec<E> &x, float ss, float inv_d, float eps, float &shrunk) {
+template <bool kSub, int E>
+__device__ __forceinline__ float unit_factor(Team<kSub> &team, Vec<E> &x, float ss, float inv_d, float eps, float &shrunk) {
     shrunk = 1.f;
     const bool over = isinf(ss);
-    if (team.size < 32 ? __any_sync(0xffffffffu, over) : over) {
+    if (team.any(over)) {
         if (over) shrunk = kShrink;
         x *= shrunk;
         float again[1] = {x.dot(x)};
@@ -608,7 +632,7 @@ inline int norm_slots(const NormShape &s, int64_t rows) {
 
 // Lets a kernel have `dynamic` bytes of shared memory beside its own. LAMQ_OK, or an error that is set.
 inline int allow_shared(const void *kernel, int dynamic) {
-    if (dynamic + Team::kScratch * (int)sizeof(float) + 32 * 1024 <= 48 * 1024) return LAMQ_OK;  // with any static array
+    if (dynamic + 24 * 1024 <= 48 * 1024) return LAMQ_OK;  // beside the kernels' static arrays, 20 KB at most
     const cudaError_t e = smem_limit_max_once(kernel);
     if (e == cudaSuccess) return LAMQ_OK;
     set_error("shared memory: %s", cudaGetErrorString(e));
@@ -651,7 +675,7 @@ inline NormLayout norm_layout(const lamq_norm_args &a, bool backward, bool sums,
             g.stage_bytes += size[k] == 0 ? 0 : s.V == 8 ? s.P * 8 * size[k] * threads : g.image[k] * l.slots;
         }
         l.sums_bytes = sums && !hold ? (l.mode == kJoinFull ? 3 : 1) * s.P * s.V * threads * (int)sizeof(float) : 0;
-        const int own = Team::kScratch * (int)sizeof(float) + 1024 + l.sums_bytes +
+        const int own = Team<false>::kScratch * (int)sizeof(float) + 1024 + l.sums_bytes +
                         (backward && sums && hold ? 4096 * (int)sizeof(float) : 0);
         l.blocks = std::max(1, resident(s.kernel, l.mode, backward) / threads);
         for (;; --l.blocks) {
@@ -663,7 +687,7 @@ inline NormLayout norm_layout(const lamq_norm_args &a, bool backward, bool sums,
         if (g.stages >= (s.V == 1 ? 2 : 1)) return l;
     }
     s.V = 1, s.kernel = kWide, s.team = kNormThreads, s.packs = a.d;
-    l.slots = 1, l.blocks = 2, l.shared = 0;
+    l.slots = 1, l.blocks = 2, l.shared = a.d * (int)sizeof(float);
     return l;
 }
 

@@ -129,7 +129,7 @@ extern "C" int lamq_norm_backward(const lamq_norm_args *a, void *workspace, size
     p.per = q.per, p.gate_mode = q.gate_mode;
     const cudaStream_t st = (cudaStream_t)stream;
     p.ring = l.ring;
-    p.sums_at = l.shared - l.sums_bytes;
+    p.sums_at = l.ring.ring_bytes;
     const int shared = l.shared;
     const NormKernel kernel = l.shape.kernel;
     const int launched = kernel == kVectors       ? launch_backward<kVectors>(*a, p, q.grid, mode, sums, shared, st)

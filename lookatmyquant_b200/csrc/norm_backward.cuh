@@ -66,8 +66,8 @@ struct Columns<E, false> {
 };
 
 // The block's teams' sums added in order and written as the block's partial row.
-template <int P, int V, bool kHold>
-__device__ __forceinline__ void write_partial(const BackwardParams &p, const Team &team, Vec<P * V> acc, float *part,
+template <int P, int V, bool kHold, bool kSub>
+__device__ __forceinline__ void write_partial(const BackwardParams &p, const Team<kSub> &team, Vec<P * V> acc, float *part,
                                               float2 *shared) {
     if constexpr (kHold) {
         constexpr int kPairs = Vec<P * V>::kPairs, kThreads = 4096 / (P * V);
@@ -85,7 +85,7 @@ __device__ __forceinline__ void write_partial(const BackwardParams &p, const Tea
     float *const row = part + (int64_t)blockIdx.x * p.columns;
 #pragma unroll
     for (int q = 0; q < P; ++q) {
-        const int pack = team.t + q * p.team;
+        const int pack = team.pack(q);
         float f[V];
         acc.get(q * V, f);
         if (pack < p.packs) Raw<float, V>::store(row + pack * V, f);
@@ -93,18 +93,18 @@ __device__ __forceinline__ void write_partial(const BackwardParams &p, const Tea
 }
 
 // Threads of blocks that are not too large (kHold) keep the weights and the gate of their columns in registers.
-template <typename R, typename B, NormKernel kKernel, int kMode, bool kSums>
+template <typename R, typename B, NormKernel kKernel, int kMode, bool kSums, bool kSub>
 __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
     norm_backward_kernel(const __grid_constant__ BackwardParams p) {
     extern __shared__ uint4 stages[];
-    __shared__ alignas(16) float scratch[Team::kScratch];
+    __shared__ alignas(16) float scratch[Team<false>::kScratch];
     constexpr int V = NormSizes<kKernel>::V, P = NormSizes<kKernel>::P;
     constexpr bool kFull = kMode == kJoinFull, kJoin = kMode != kNormAlone, kHold = NormSizes<kKernel>::kHold;
     using Row = Vec<P * V>;
     __shared__ float2 shared[kSums && kHold ? NormSizes<kKernel>::kThreads * Row::kPairs : 1];
     if (kSums) let_follow();
-    Team team(p.team, scratch);
-    const Ring<V, P> ring(stages, p.ring, team, p.packs);
+    Team<kSub> team(p.team, P, scratch);
+    const Ring<V, P, kSub> ring(stages, p.ring, team, p.packs);
     float *const columns = reinterpret_cast<float *>(reinterpret_cast<unsigned char *>(stages) + p.sums_at);
     constexpr int kStep = kSums && !kHold ? P * V : 0;
     Columns<P * V, !kStep> dw(columns), du(columns + (kFull ? 1 : 0) * kStep * p.team),
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
     const auto each = [&](auto f) {  // this thread's packs
 #pragma unroll
         for (int q = 0; q < P; ++q) {
-            const int pack = team.t + q * p.team;
+            const int pack = team.pack(q);
             if (pack < p.packs) f(q, pack);
         }
     };
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
     const auto fetch = [&](uint32_t stage) {
         const int row = first + fetched * step;
         const bool there = fetched < p.per && row < p.rows;
-        if (there || p.team < 32) {  // a team that has no row beside others of its warp that do: zeros
+        if (there || kSub) {  // a team that has no row beside others of its warp that do: zeros
             const int at = there ? row : 0, bytes = there ? 16 : 0;
             if (has_dy) {
                 ring.fetch(stage, kTensorH, row_at<R, kJoin>(p.in.h, at), bytes);
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
     for (int k = 0; k < p.per; ++k) {
         const int row = first + k * step;
         const bool live = row < p.rows;
-        if (p.team < 32 ? !__any_sync(0xffffffffu, live) : !live) break;
+        if (!team.any(live)) break;
         if (V == 1 && p.ring.stages > 1) {  // all have read the stage that is filled next
             ring.wait();
             fetch(to);
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
         if (has_dy) {
             float shrunk;
             const float f = unit_factor(team, x, s[0], p.inv_d, p.eps, shrunk);
-            if (p.team < 32 ? __any_sync(0xffffffffu, shrunk != 1.f) : shrunk != 1.f) {
+            if (team.any(shrunk != 1.f)) {
                 float again[1] = {t.dot(x)};  // x changed, and the sum may have overflowed
                 team.sum(again);
                 s[1] = again[0];
@@ -286,7 +286,9 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
 
 template <typename R, typename B, NormKernel kKernel, int kMode, bool kSums>
 int launch_backward(const BackwardParams &p, int grid, int shared, cudaStream_t stream) {
-    const auto kernel = norm_backward_kernel<R, B, kKernel, kMode, kSums>;
+    const bool sub = NormSizes<kKernel>::kHold && p.team < 32;
+    const auto kernel = sub ? norm_backward_kernel<R, B, kKernel, kMode, kSums, NormSizes<kKernel>::kHold>
+                            : norm_backward_kernel<R, B, kKernel, kMode, kSums, false>;
     if (const int st = allow_shared(reinterpret_cast<const void *>(kernel), shared)) return st;
     kernel<<<grid, p.team * p.slots, shared, stream>>>(p);
     return LAMQ_OK;

@@ -56,7 +56,7 @@ int lamq_norm_forward(const lamq_norm_args *args, lamq_stream_t stream);
  * its input), the statistics being computed again. d_residual is always written; d_branch (NULL: not wanted, as where it
  * equals d_residual), d_weight, d_post and d_gate where they are not NULL. The gradient of a weight or of a shared gate is
  * summed in fp32 in a fixed order: equal calls give equal bits. Workspace: lamq_norm_backward_workspace_size(args) bytes,
- * 16-byte aligned (0 where no such sum is wanted).
+ * 32-byte aligned (0 where no such sum is wanted).
  */
 size_t lamq_norm_backward_workspace_size(const lamq_norm_args *args);
 int lamq_norm_backward(const lamq_norm_args *args, void *workspace, size_t workspace_bytes, lamq_stream_t stream);

@@ -79,6 +79,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, false), 1) norm_forwa
             ring.wait();
             fetch(ahead, to);
         } else {
+            __syncwarp();  // all of the warp have read the stage that is filled next
             fetch(ahead, to);
             ring.wait();
         }

@@ -94,8 +94,10 @@ struct Raw<float, 8> {
         unpack(v, f);
     }
     __device__ __forceinline__ static void store(float *p, const float (&f)[8]) {
-        reinterpret_cast<float4 *>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-        reinterpret_cast<float4 *>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+        // 32 bytes at once: two stores of 16 would each fill half of every sector they touch
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]),
+                     "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
+                     : "memory");
     }
 };
 
@@ -366,7 +368,7 @@ struct Team {
 // ---- rows on their way
 //
 // A team's next rows are fetched into shared memory while it works on one: `stages` of them, a stage holding every tensor that
-// the call reads row by row. Vectors: a thread fetches its own packs and only it reads them. Elements: the team fetches the
+// the call reads row by row. Vectors: the threads of a warp fetch one another's packs. Elements: the team fetches the
 // 16-byte pieces that hold the row (whatever lies beside it in the first and the last of them comes along and is not used), and
 // meets before it reads them.
 
@@ -429,7 +431,10 @@ struct Ring {
             case 3: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
             default: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
         }
-        if (V == 1) team.barrier();
+        if (V == 1)
+            team.barrier();
+        else
+            __syncwarp();
     }
 
     __device__ __forceinline__ uint32_t part(uint32_t stage, int tensor) const {
@@ -441,21 +446,31 @@ struct Ring {
         return (threadIdx.x >> 5) * (P * (int)sizeof(T) / 2 * 512) + (threadIdx.x & 31) * 16;
     }
 
-    // Starts the copies of a tensor's row (bytes = 0: of a row of zeros).
+    // Starts the copies of a tensor's row (bytes = 0: of a row of zeros). Of fp32 packs, a pair of 16-byte pieces each, the threads
+    // of a warp (a smaller team) fetch neighbouring pieces, so that no sector is asked for twice.
     template <typename T>
     __device__ __forceinline__ void fetch(uint32_t stage, int tensor, const T *row, int bytes) const {
         uint32_t to = part(stage, tensor);
-        if constexpr (V == 8) {
-            constexpr int kPieces = sizeof(T) / 2;
+        if constexpr (V == 8 && sizeof(T) == 2) {
             to += own<T>();
 #pragma unroll
             for (int q = 0; q < P; ++q) {
                 int pack = team.pack(q), some = bytes;
                 if (pack >= packs) pack = 0, some = 0;  // zeros behind the row's end
-#pragma unroll
-                for (int i = 0; i < kPieces; ++i)
-                    copy16(to + (q * kPieces + i) * 512, row + pack * 8 + i * (8 / kPieces), some);
+                copy16(to + q * 512, row + pack * 8, some);
             }
+        } else if constexpr (V == 8) {
+            const int width = kSub ? team.size : 32, lane = kSub ? team.t : threadIdx.x & 31;
+            to += own<T>() - lane * 16;  // of the team's (the warp's) first thread
+#pragma unroll
+            for (int q = 0; q < P; ++q)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int piece = lane + i * width;
+                    int pack = team.pack(q) - lane + (piece >> 1), some = bytes;
+                    if (pack >= packs) pack = 0, some = 0;
+                    copy16(to + (2 * q + (piece & 1)) * 512 + (piece >> 1) * 16, row + pack * 8 + (piece & 1) * 4, some);
+                }
         } else {
             const int shift = (int)(reinterpret_cast<uintptr_t>(row) & 15);
             const unsigned char *const from = reinterpret_cast<const unsigned char *>(row) - shift;
@@ -590,7 +605,7 @@ struct NormShape {
     NormKernel kernel;
 };
 
-// Vectors where every row and every array begins on 16 bytes, elements elsewhere. A thread holds 16 elements of a row: what it
+// Vectors where every row begins on 16 bytes and every array on 32, elements elsewhere. A thread holds 16 elements of a row: what it
 // does for a row beside the arithmetic (places, waits, exchanges) costs as much as the arithmetic of 16 (16384 x 2560, the norm's
 // backward, us: 78 with 8, 61 with 16). The full join's backward holds three sums and three tensors of a row: 8 of each (8192 x
 // 4096: 152 with 8 and 16 warps an SM, 189 with 16 and 8 warps). Up to 32 threads a team is a power of two of lanes, else whole
@@ -600,7 +615,7 @@ inline NormShape norm_shape(const lamq_norm_args &a, bool backward) {
     const void *arrays[] = {a.weight, a.post, a.gate, a.h, a.y, a.d_residual, a.d_branch, a.d_weight, a.d_post, a.d_gate};
     bool vec = a.d % 8 == 0 && aligned_rows(a.residual) && aligned_rows(a.branch);
     if (backward) vec = vec && aligned_rows(a.dh) && aligned_rows(a.dy);
-    for (const void *p : arrays) vec = vec && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+    for (const void *p : arrays) vec = vec && (reinterpret_cast<uintptr_t>(p) & 31) == 0;  // 32 bytes are stored at once
     const bool full = backward && (a.post || a.gate);
     int e = full ? 8 : 16;
     NormShape s;

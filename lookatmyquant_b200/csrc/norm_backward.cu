@@ -113,6 +113,7 @@ extern "C" int lamq_norm_backward(const lamq_norm_args *a, void *workspace, size
     const Plan q = plan_of(*a);
     LAMQ_REQUIRE(workspace_bytes >= q.bytes, "a workspace of %zu bytes is needed", q.bytes);
     LAMQ_REQUIRE(q.bytes == 0 || workspace, "null pointer (workspace)");
+    LAMQ_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 31) == 0, "the workspace must be 32-byte aligned");
     const NormLayout &l = q.layout;
     const int mode = l.mode;
     const bool sums = a->d_weight || a->d_post || a->d_gate;

@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
             ring.wait();
             fetch(to);
         } else {
+            __syncwarp();  // all of the warp have read the stage that is filled next
             fetch(to);
             ring.wait();
         }

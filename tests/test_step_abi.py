@@ -49,7 +49,8 @@ INVALID += [("lamq_norm_backward", (a, P, 1 << 40, N), text) for a, text in BOTH
     (norm(weight=0), b"belong to a weight"), (norm(weight=0, dy=NO, dw=P), b"belong to a weight"),
     (norm(du=P), b"belongs to a post weight"), (norm(dg=P), b"belongs to a gate"), (norm(dy=rows(inner=-1)), b"inner count")]]
 INVALID += [("lamq_norm_backward", (norm(dw=P), P, 0, N), b"workspace of"),
-            ("lamq_norm_backward", (norm(dw=P), N, 1 << 40, N), b"null pointer (workspace)")]
+            ("lamq_norm_backward", (norm(dw=P), N, 1 << 40, N), b"null pointer (workspace)"),
+            ("lamq_norm_backward", (norm(dw=P), P + 16, 1 << 40, N), b"32-byte aligned")]
 
 
 def tensors(*entries):

@@ -1,10 +1,13 @@
 // What the norms' forward and backward kernels share: rows held in registers by teams of threads, their sums, and how a
 // call's sizes choose a kernel.
 //
-// A team of `team` threads owns a row at a time: thread t holds the packs t, t + team, ... of V elements, P of them at
-// most, so every row is read once and its sums need one exchange. Teams of 32 threads or less live in a warp (a power of
-// two of lanes); larger ones are whole warps that meet at a named barrier of their own, so a block's teams never wait for
-// one another.
+// A team of threads owns a row at a time: each thread holds P packs of V elements in registers, so every row is read once and
+// its sums need one exchange. Teams of 32 threads or less live in a warp (a power of two of lanes); larger ones are whole
+// warps that meet at a named barrier of their own, so a block's teams never wait for one another. The rows that come next
+// are on their way to shared memory meanwhile. Blocks stay on their SM and take row after row.
+//
+// Bound by memory in principle; what is reached is the rate of instructions and the latency of a row's two or three exchanges
+// (about half of the issue slots are used at 14 to 16 warps an SM, DRAM 36 to 54 %): see the kernels for the times.
 #pragma once
 
 #include <algorithm>
@@ -50,9 +53,9 @@ constexpr int kSMs = 148;
 
 // ---- loads
 //
-// As volatile assembly: the compiler runs none of them where the source does not. (Plain __ldg loads behind a condition were
-// executed ahead of it: kernels that tested a pointer for NULL before they read it faulted.) Absent tensors have a pointer
-// that may be read, too (the host's `present`).
+// As volatile assembly: the compiler runs none of them where the source does not. (With plain __ldg loads behind a test of their
+// pointer, kernels faulted in calls where it was NULL, though the source then reads nothing; with these they do not.) Absent
+// tensors have a pointer that may be read, too (the host's `present`).
 
 __device__ __forceinline__ uint4 load16(const void *p) {
     uint4 v;
@@ -550,7 +553,6 @@ __device__ __forceinline__ float unit_factor(Team<kSub> &team, Vec<E> &x, float 
 
 // ---- the host's side
 
-
 // Which tensors a call has, and in the place of the others an output's memory of the same shape and no smaller a type: what
 // a kernel gets may be read whether or not it is there.
 enum { kHasWeight = 1, kHasPost = 2, kHasGate = 4, kHasDh = 8, kHasDy = 16, kHasBranch = 32 };
@@ -607,7 +609,7 @@ struct NormShape {
 
 // Vectors where every row begins on 16 bytes and every array on 32, elements elsewhere. A thread holds 16 elements of a row: what it
 // does for a row beside the arithmetic (places, waits, exchanges) costs as much as the arithmetic of 16 (16384 x 2560, the norm's
-// backward, us: 78 with 8, 61 with 16). The full join's backward holds three sums and three tensors of a row: 8 of each (8192 x
+// backward, us: 78 with 8, 61 with 16; the forward of a join with both norms takes the same with either). The full join's backward holds three sums and three tensors of a row: 8 of each (8192 x
 // 4096: 152 with 8 and 16 warps an SM, 189 with 16 and 8 warps). Up to 32 threads a team is a power of two of lanes, else whole
 // warps. Wider rows take teams of up to 512 threads with 16 elements, then with 32; rows wider than 4096 that may begin
 // anywhere, a block each.
@@ -664,9 +666,10 @@ struct NormLayout {
 
 constexpr int kSmemSM = 220 * 1024;  // of 228 KB; each block takes 1 KB for itself
 
-// `gate_sums`: the gradient of the gate is wanted; `sums`: that of any parameter. Blocks are as many as their registers allow
-//, or as have room for two stages each, and stages fill
-// the room, four at most. What has no room, or two stages of rows that begin anywhere, is left to the wide kernels.
+// `gate_sums`: the gradient of the gate is wanted; `sums`: that of any parameter. Blocks are as many as their registers allow, or
+// as have room for two stages each; stages fill the room, four at most. What finds no room (rows that begin anywhere: for two
+// stages) is left to the wide kernels. More blocks with fewer registers are slower: the norm's backward of 16384 x 2560 at 96
+// registers, 4 blocks of 160 threads, 93 us against 55 at 122, 3 blocks (what spills, and one stage less).
 inline NormLayout norm_layout(const lamq_norm_args &a, bool backward, bool sums, bool gate_sums) {
     NormLayout l{};
     const bool join = a.branch.data, gates = a.gate && a.gate_span == 1;

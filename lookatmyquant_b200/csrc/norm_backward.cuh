@@ -8,6 +8,10 @@
 // Bound by memory. The statistics of h and b are computed again: their rows are read whole anyway, and nothing has to be
 // kept from the forward. The sums over rows stay in the registers of the threads that own the columns: a worker (a team)
 // takes the rows of one range, blocks write one partial row each, and a second kernel adds the partials in order.
+//
+// Measured (us; bytes at 6551 GB/s in brackets): the norm alone, 16384 x 2560 bf16 55 (38); a join with both norms and a gate for
+// all, 8192 x 4096 bf16 127 (62): 520 instructions a warp and row of 8 elements a thread at 2.0 a cycle, 122 registers, 16 warps;
+// the same with a gate of its own for each element, 3335 x 1337 fp32, rows that begin anywhere, 55 (22).
 #pragma once
 
 #include "dependent.cuh"
@@ -32,7 +36,6 @@ struct BackwardParams {
 // d_gate is not wanted; one gate row for all rows (summed like a weight's gradient); its rows are whole inside a worker's
 // range (written at once); its rows span workers (a partial for each worker and gate row that meet).
 enum { kGateNone, kGateOne, kGateInside, kGateAcross };
-
 
 // What a thread has summed of its columns: in registers where these are few, else in shared memory that no other thread
 // touches (three sums of 16384 columns take 196608 bytes).

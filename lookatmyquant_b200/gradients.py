@@ -89,14 +89,15 @@ def clip(tensors, max_norm: float, out=None, eps: float = 1e-6) -> torch.Tensor:
     """Scales `tensors` by min(1, max_norm / (norm + eps)), norm their `global_norm`, which is returned. In place, and then
     untouched where the norm is within the bound; or, with `out`, into its tensors (one for each, of its shape, fp32 or bf16).
     A norm that is NaN makes everything NaN, an infinite one zeros (infinite elements NaN), as in torch. Tensors that share
-    memory raise ValueError: they would be scaled twice."""
+    memory raise ValueError: they would be scaled twice (views with gaps, which go through copies, only where two are the
+    same)."""
     tensors = list(tensors)
     into = tensors if out is None else list(out)
     if len(into) != len(tensors):
         raise ValueError(f"{len(into)} outputs for {len(tensors)} gradients")
     device = _device(tensors)
     index, values, count, copies = device.index if device.type == "cuda" else -2, [], 0, []
-    late, written = [], []  # (tensor, what is copied into it afterwards); what changes
+    late, written, gaps = [], [], set()  # (tensor, what is copied into it afterwards); what changes; the views with gaps
     for x, o in zip(tensors, into):
         if x is None:
             continue
@@ -104,6 +105,10 @@ def clip(tensors, max_norm: float, out=None, eps: float = 1e-6) -> torch.Tensor:
         written.append(o)
         if o is x:
             if not x.is_contiguous() and not _dense(x):
+                place = (x.data_ptr(), x.shape, x.stride())
+                if place in gaps:
+                    raise ValueError("tensors of the list overlap where they are written")
+                gaps.add(place)
                 x = x.contiguous()
                 late.append((o, x))
             o = x
@@ -120,7 +125,7 @@ def clip(tensors, max_norm: float, out=None, eps: float = 1e-6) -> torch.Tensor:
         values += (x.data_ptr(), o.data_ptr(), x.numel(), code, to)
         count += 1
     norm = _call("lamq_gradient_clip", values, count, device, float(max_norm), float(eps))
-    torch.autograd.graph.increment_version(written)
+    torch.autograd.graph.increment_version([o for o in written if not o.is_inference()])
     for o, value in late:
         with torch.no_grad():
             o.copy_(value)

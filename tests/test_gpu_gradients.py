@@ -205,6 +205,12 @@ def test_clipping_is_a_change_that_autograd_sees(G):
         z.backward()
 
 
+def test_clipping_in_inference_mode(G):
+    with torch.inference_mode():
+        x = torch.full((100,), 2.0, device="cuda")
+        assert abs(float(G.clip([x], 10.0)) - 20.0) <= 1e-4 and bool(((x - 1.0).abs() <= 1e-6).all())
+
+
 def test_refusals(G):
     x = torch.ones(8, 8, device="cuda")
     for error, call in [
@@ -213,7 +219,7 @@ def test_refusals(G):
             (TypeError, lambda: G.global_norm([x.to_sparse()])), (TypeError, lambda: G.global_norm([1.0])),
             (ValueError, lambda: G.clip([x], -1.0)), (ValueError, lambda: G.clip([x], math.nan)),
             (ValueError, lambda: G.clip([x], 1.0, eps=-1.0)), (ValueError, lambda: G.clip([x, x], 1.0)),
-            (ValueError, lambda: G.clip([x, x[4:]], 1.0)), (ValueError, lambda: G.clip([x], 1.0, [x.flatten()])),
+            (ValueError, lambda: G.clip([x, x[4:]], 1.0)), (ValueError, lambda: G.clip([x[:, ::2], x[:, ::2]], 1.0)), (ValueError, lambda: G.clip([x], 1.0, [x.flatten()])),
             (ValueError, lambda: G.clip([x], 1.0, [])), (ValueError, lambda: G.clip([x[:4]], 1.0, [x[2:6]])),
             (TypeError, lambda: G.clip([x], 1.0, [x.half()])), (TypeError, lambda: G.clip([x], 1.0, [None]))]:
         with pytest.raises(error):

@@ -25,7 +25,7 @@ Plan plan_of(const lamq_norm_args &a) {
             q.gate_mode = kGateOne;
         } else if (a.gate_span == 1) {
             q.gate_mode = kGateInside;
-        } else if (a.gate_span <= per && shape.kernel != kWide) {  // a wide row's sums have no place but the partial rows
+        } else if (a.gate_span <= per) {
             q.gate_mode = kGateInside;
             per = (per + a.gate_span - 1) / a.gate_span * a.gate_span;
         } else {
@@ -36,8 +36,9 @@ Plan plan_of(const lamq_norm_args &a) {
     const int64_t workers = (a.rows + per - 1) / per;
     q.grid = (int)((workers + slots - 1) / slots);
     q.columns = (a.d + 7) / 8 * 8;
-    q.g_rows = q.gate_mode == kGateOne ? q.grid
-               : q.gate_mode == kGateAcross ? (int64_t)q.grid * slots + a.rows / a.gate_span : 0;
+    // the wide kernels sum every gate row in memory: one row for each block, where no worker shares a gate row
+    const bool block_rows = q.gate_mode == kGateOne || (q.gate_mode == kGateInside && shape.kernel == kWide && a.gate_span > 1);
+    q.g_rows = block_rows ? q.grid : q.gate_mode == kGateAcross ? (int64_t)q.grid * slots + a.rows / a.gate_span : 0;
     const size_t row = (size_t)q.columns * sizeof(float);
     q.w_at = 0;
     q.u_at = q.w_at + (a.d_weight ? (size_t)q.grid * row : 0);
@@ -151,6 +152,7 @@ extern "C" int lamq_norm_backward(const lamq_norm_args *a, void *workspace, size
     sum.gate_one = q.gate_mode == kGateOne, sum.gate_span = p.in.gate_span, sum.per = q.per, sum.rows = p.rows;
     const int64_t jobs = (a->d_weight ? 1 : 0) + (a->d_post ? 1 : 0) +
                          (q.gate_mode == kGateOne ? 1 : q.gate_mode == kGateAcross ? a->rows / a->gate_span : 0);
+    if (jobs == 0) return LAMQ_OK;
     launch_following(norm_reduce_kernel, (unsigned)(jobs * ((a->d + 31) / 32)), kReduceWarps * 32, st, sum);
     LAMQ_CHECK_LAUNCH("lamq_norm_backward (sums)");
     return LAMQ_OK;

@@ -50,31 +50,33 @@ __global__ void __launch_bounds__(kWideThreads) norm_backward_wide_kernel(const 
         if (post) fb = wide_factor(s[2], p.d, [&](int j) { return load_one(branch + j); }, p.inv_d, p.eps, less, scratch);
         const float c = s[1] * f * p.inv_d, r = f * shrunk;
         const int gate_row = p.in.by_span.of(row);
-        // one gate row for all: the block's partial row; else the pair's (a gate row of its own: written at once)
+        // a gate row is summed in the block's partial row, one that spans blocks in the pair's
         const bool begins = row == first || (p.gate_mode != kGateOne && row == gate_row * p.in.gate_span);
-        float *const part = p.g_part + (p.gate_mode == kGateOne ? (int64_t)blockIdx.x : (int64_t)blockIdx.x + gate_row) * p.columns;
+        const bool done = p.gate_mode == kGateInside && row + 1 == (gate_row + 1) * p.in.gate_span;
+        float *const part = p.g_part + (p.gate_mode == kGateAcross ? (int64_t)blockIdx.x + gate_row : (int64_t)blockIdx.x) * p.columns;
         float cb[1] = {0.f};
         wide_each(p.d, [&](int j) {
             float g[1] = {(p.in.has & kHasDh) ? load_one(dh + j) : 0.f};
             if (pre) {
                 const float unit = load_one(h + j) * shrunk * f, y = load_one(dy + j);
                 g[0] = fmaf(r, fmaf(-unit, c, y * weight(j)), g[0]);
-                if (p.w_part) p.w_part[block_row + j] = fmaf(y, unit, p.w_part[block_row + j]);
+                if (p.w_part) p.w_part[block_row + j] = fmaf(y, unit, own_at(p.w_part + block_row + j));
             }
             Raw<R, 1>::store(reinterpret_cast<R *>(p.d_residual) + out + j, g);
             float t[1] = {g[0] * p.scale};
             if (full) {
                 const float b = post || gate_sums ? load_one(branch + j) * less * fb : 0.f, u = post ? after(j) : 1.f;
                 if (gate_sums) {
-                    const float to[1] = {t[0] * (b * u)};
-                    if (p.gate_mode == kGateInside)
+                    float to[1] = {t[0] * (b * u)};
+                    if (!begins) to[0] += own_at(part + j);
+                    if (done)
                         store_typed<1>(p.d_gate, p.in.gate_dtype, (int64_t)gate_row * p.d + j, to);
                     else
-                        part[j] = begins ? to[0] : part[j] + to[0];
+                        part[j] = to[0];
                 }
                 if (gate) t[0] *= value_at(p.in.gate, p.in.gate_dtype, (int64_t)gate_row * p.d + j);
                 if (post) {
-                    if (p.u_part) p.u_part[block_row + j] = fmaf(t[0], b, p.u_part[block_row + j]);
+                    if (p.u_part) p.u_part[block_row + j] = fmaf(t[0], b, own_at(p.u_part + block_row + j));
                     t[0] *= u;
                     cb[0] = fmaf(t[0], b, cb[0]);
                     row_of_t[j] = t[0];

@@ -17,6 +17,13 @@ __device__ __forceinline__ float value_at(const void *p, int dtype, int64_t i) {
     return f[0];
 }
 
+// What this thread has written itself (not through the read-only path; volatile for the reason that all loads are).
+__device__ __forceinline__ float own_at(const float *p) {
+    float v;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+    return v;
+}
+
 // The sums over the block, in every thread, in a fixed order. scratch: K x 32 floats.
 template <int K>
 __device__ __forceinline__ void wide_sum(float (&v)[K], float *scratch) {

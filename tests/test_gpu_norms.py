@@ -96,6 +96,12 @@ def test_gates_of_texts_of_any_length(N, n, texts, d):
     check_join(N, t)
 
 
+@pytest.mark.parametrize("n,texts", [(1, 40), (2, 700), (3, 900), (5, 1), (600, 3), (400, 1)])
+@pytest.mark.parametrize("d,post", [(4097, True), (4099, False), (8200, True)])
+def test_gates_of_texts_in_wide_rows(N, n, texts, d, post):
+    check_join(N, case(n + d, n, d, FP, BF, post, "text", True, texts))
+
+
 def test_rows_at_strides(N):
     """Heads out of a joint projection, transposed and sliced tensors, expanded ones: read where they are, or copied."""
     g = generator(3)
@@ -130,8 +136,10 @@ def test_tensors_that_start_anywhere(N, shift):
     check_join(N, t)
 
 
-def test_what_is_not_wanted_is_none(N):
-    t = case(6, 20, 64, BF, BF, True, "text", True, 3)
+@pytest.mark.parametrize("d", [64, 37, 4104, 4097, 9728])
+@pytest.mark.parametrize("gate", ["text", "token", "channel"])
+def test_what_is_not_wanted_is_none(N, d, gate):
+    t = case(6, 20, d, BF, BF, True, gate, True, 3)
     h, y = N.join_forward(t["residual"], t["branch"], t["weight"], t["post"], t["gate"])
     args = (h, t["branch"], t["weight"], t["post"], t["gate"])
     every = N.join_backward(h, y, *args)
@@ -328,6 +336,24 @@ def test_many_rows(N):
     wx, ww = norm_gradient(y[-3:].double(), torch.zeros(3, d, device="cuda").double(), x[-3:].double(), w, 1e-6, 0.0)
     assert_close(dx[-3:], wx)
     assert_close(dw, ww)
+
+
+def test_another_stream_and_device_context(N):
+    """On a stream of its own, beside work on the default one; the results belong to that stream."""
+    t = case(3, 300, 256, BF, BF, True, "text", True, 4)
+    args = (t["weight"], t["post"], t["gate"], 0.3)
+    h, y = N.join_forward(t["residual"], t["branch"], *args)
+    want = (h, y, *N.join_backward(h, y, h, t["branch"], *args))
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(10):
+        with torch.cuda.stream(s):
+            h2, y2 = N.join_forward(t["residual"], t["branch"], *args)
+            got = (h2, y2, *N.join_backward(h2, y2, h2, t["branch"], *args))
+        N.join_forward(t["residual"], t["branch"], *args)
+        s.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
 
 
 def test_refusals(N):

@@ -293,19 +293,11 @@ def join(residual: torch.Tensor, branch: torch.Tensor, weight: torch.Tensor | No
 
 
 def run_layers(model, x: torch.Tensor) -> torch.Tensor:
-    """The hidden states behind the final norm of a Hugging Face model of the Llama kind (model.model.layers with
-    input_layernorm, self_attn, post_attention_layernorm and mlp; model.model.norm) for the embedded whole windows x (batch,
-    length, d): its own attention and MLP modules, and `norm` and `join` in the place of its norms and residual additions, each
-    of which goes into the join with the norm behind it, across the layers too. No cache, padding or other mask."""
-    inner = model.model
-    positions = torch.arange(x.shape[1], device=x.device)[None]
-    rotary = inner.rotary_emb(x, position_ids=positions)
-    after = [layer.input_layernorm for layer in inner.layers[1:]] + [inner.norm]
-    first = inner.layers[0].input_layernorm if len(inner.layers) else inner.norm
-    h, y = x, norm(x, first.weight, first.variance_epsilon)
-    for layer, following in zip(inner.layers, after):
-        a = layer.self_attn(hidden_states=y, position_embeddings=rotary, attention_mask=None)[0]
-        mid = layer.post_attention_layernorm
-        h, y = join(h, a, mid.weight, eps=mid.variance_epsilon)
-        h, y = join(h, layer.mlp(y), following.weight, eps=following.variance_epsilon)
-    return y
+    """What model.model(inputs_embeds=x) gives behind its final norm, for a Hugging Face causal model and the embedded whole
+    windows x (batch, length, d): the model's own masks, positions, attention and MLP modules, and `norm` and `join` in the
+    place of its decoder layers' norms and residual additions, each of which goes into the join with the norm behind it, across
+    the layers too (a layer's norms behind its blocks and a multiplier of their results included). Layers that do anything else, and
+    other norms than x · (mean(x²) + eps)^-1/2 · w, raise TypeError; hooks on the layers and norms that are not called, active
+    dropout between them and gradient checkpointing raise ValueError. No cache and no padding."""
+    from .decoder import joined  # it calls this module
+    return joined(model).model(inputs_embeds=x, use_cache=False).last_hidden_state

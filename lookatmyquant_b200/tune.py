@@ -1,8 +1,8 @@
 """Fine-tuning a model around its coded matrices, end to end on this package's kernels: the scaled embedding lookup and
 its gradient (embedding.scaled_embedding), attention forwards and backwards (attention.attention, as the model's
 attention implementation) and Muon updates (orthogonal.Muon) of the matrices that are still free; on request the layers'
-norms joined with their residual additions (norms.run_layers) and the gradients clipped by their global norm
-(gradients.clip).
+norms joined with their residual additions (decoder.joined, as norms.run_layers does) and the gradients clipped by their
+global norm (gradients.clip).
 
 The student is the model with some of its matrices replaced by their trellis words (here: every down_proj, as `measure`
 codes a piece); those stay. The loss is the mean cross-entropy of the windows' next tokens; Muon moves the free matrices,
@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import torch
 
-from . import attention, codes, embedding, gradients, norms, orthogonal
+from . import attention, codes, decoder, embedding, gradients, orthogonal
 from .measure import BLOCK_SEED, build_model, capture, zipf_tokens
 
 FREE = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj")
@@ -40,8 +40,8 @@ def coded(model, option: str, chunks: list) -> list:
 
 
 class Tuner:
-    """A student model, the free parameters and their optimisers; `step(ids)` is one update. `fused_norms` runs the layers
-    through norms.run_layers; with `max_norm` the gradients of all free parameters together are clipped to it, and
+    """A student model, the free parameters and their optimisers; `step(ids)` is one update. `fused_norms` runs the model
+    through decoder.joined; with `max_norm` the gradients of all free parameters together are clipped to it, and
     `grad_norm` is their norm before (a scalar on the device)."""
 
     def __init__(self, model, lr: float = 0.02, table_lr: float = 0.02, scale: float = 1.0, fused_norms: bool = False,
@@ -58,11 +58,10 @@ class Tuner:
         self.muon = orthogonal.Muon(free, lr=lr)
 
     def logits(self, ids: torch.Tensor) -> torch.Tensor:
-        """The student's logits: the table's rows looked up (scaled), the layers, the tied head."""
+        """The student's logits: the table's rows looked up (scaled), the layers, the model's own head."""
         x = embedding.scaled_embedding(self.table, ids, self.scale)
-        if self.fused_norms:
-            return self.model.lm_head(norms.run_layers(self.model, x))
-        return self.model(inputs_embeds=x, use_cache=False).logits
+        model = decoder.joined(self.model) if self.fused_norms else self.model
+        return model(inputs_embeds=x, use_cache=False).logits
 
     def loss(self, ids: torch.Tensor) -> torch.Tensor:
         """The mean cross-entropy of the windows' next tokens."""

@@ -3,7 +3,7 @@
  * backward pass: the norms before and after a block joined with the block's gate, its scale and the residual addition,
  * and the global norm of many gradients with its clipping. The conventions are lamq_b200.h's: plain device pointers and
  * sizes, asynchronous on the given stream, an int status, buffers and workspaces owned by the caller, nothing allocated
- * by a call. No kernel waits on another block, so there are no status words.
+ * by a call. Pointers lie at a multiple of their element's size. No kernel waits on another block, so there are no status words.
  */
 #ifndef LAMQ_B200_STEP_H
 #define LAMQ_B200_STEP_H

@@ -327,6 +327,9 @@ int check_list(const lamq_gradient *list, int64_t count, bool clip) {
                          (!clip || g.out_dtype == LAMQ_F32 || g.out_dtype == LAMQ_BF16),
                      "dtype: LAMQ_F32 or LAMQ_BF16");
         LAMQ_REQUIRE(g.n == 0 || (g.data && (!clip || g.out)), "null pointer (tensor %lld)", (long long)i);
+        LAMQ_REQUIRE(g.n == 0 || (aligned_to(g.data, g.dtype == LAMQ_BF16 ? 2 : 4) &&
+                                  (!clip || aligned_to(g.out, g.out_dtype == LAMQ_BF16 ? 2 : 4))),
+                     "tensor %lld: not aligned to its elements", (long long)i);
         LAMQ_REQUIRE(!clip || g.n == 0 || g.out != g.data || g.out_dtype == g.dtype, "dtype: in place it stays");
     }
     if (!clip) return LAMQ_OK;
@@ -410,9 +413,11 @@ int all_squares(const lamq_gradient *list, int64_t count, double *part, int &par
 int check_call(const lamq_gradient *list, int64_t count, bool clip, const float *norm, const void *workspace, size_t bytes) {
     if (const int st = check_list(list, count, clip)) return st;
     LAMQ_REQUIRE(norm, "null pointer (norm)");
+    LAMQ_REQUIRE(aligned_to(norm, sizeof(float)), "norm: not aligned to its elements");
     const size_t need = lamq_gradient_workspace_size(count);
     LAMQ_REQUIRE(bytes >= need, "a workspace of %zu bytes is needed", need);
     LAMQ_REQUIRE(need == 0 || workspace, "null pointer (workspace)");
+    LAMQ_REQUIRE(aligned_to(workspace, sizeof(double)), "the workspace must be 8-byte aligned");
     return LAMQ_OK;
 }
 

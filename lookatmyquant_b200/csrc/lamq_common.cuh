@@ -20,6 +20,9 @@ cudaError_t smem_limit_max_once(const void *kernel);
 // Counts one kernel launch of this library (lamq_kernel_launches()).
 void count_launch();
 
+// Whether a pointer is NULL or lies at a multiple of `bytes`, a power of two.
+inline bool aligned_to(const void *p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
+
 #define LAMQ_CHECK_LAUNCH(what)                                                         \
     do {                                                                                \
         cudaError_t _e = cudaGetLastError();                                            \

@@ -265,6 +265,20 @@ int norm_args_status(const lamq_norm_args *a, bool backward) {
         LAMQ_REQUIRE(a->post || !a->d_post, "d_post belongs to a post weight");
         LAMQ_REQUIRE(a->gate || !a->d_gate, "d_gate belongs to a gate");
     }
+    const struct {
+        const char *what;
+        const void *at;
+        int dtype;
+        bool used;
+    } pointers[] = {{"residual", a->residual.data, a->residual_dtype, true}, {"branch", a->branch.data, a->branch_dtype, true},
+                    {"weight", a->weight, a->weight_dtype, true}, {"post", a->post, a->post_dtype, true},
+                    {"gate", a->gate, a->gate_dtype, true}, {"h", a->h, a->residual_dtype, !backward},
+                    {"y", a->y, a->branch_dtype, !backward}, {"dh", a->dh.data, a->residual_dtype, backward},
+                    {"dy", a->dy.data, a->branch_dtype, backward}, {"d_residual", a->d_residual, a->residual_dtype, backward},
+                    {"d_branch", a->d_branch, a->branch_dtype, backward}, {"d_weight", a->d_weight, a->weight_dtype, backward},
+                    {"d_post", a->d_post, a->post_dtype, backward}, {"d_gate", a->d_gate, a->gate_dtype, backward}};
+    for (const auto &p : pointers)
+        LAMQ_REQUIRE(!p.used || aligned_to(p.at, element_size(p.dtype)), "%s: not aligned to its elements", p.what);
     return LAMQ_OK;
 }
 

@@ -103,25 +103,22 @@ def clip(tensors, max_norm: float, out=None, eps: float = 1e-6) -> torch.Tensor:
             continue
         code = to = _code(x, index, device, "gradients")
         written.append(o)
-        if o is x:
-            if not x.is_contiguous() and not _dense(x):
-                place = (x.data_ptr(), x.shape, x.stride())
-                if place in gaps:
-                    raise ValueError("tensors of the list overlap where they are written")
-                gaps.add(place)
-                x = x.contiguous()
-                late.append((o, x))
-            o = x
-        else:
+        same = o is x
+        if not same:
             to = _code(o, index, device, "outputs")
             if o.shape != x.shape:
                 raise ValueError(f"an output {tuple(o.shape)} for a gradient {tuple(x.shape)}")
-            if not (x.is_contiguous() and o.is_contiguous()) and not (_dense(x) and x.stride() == o.stride()):
-                x = x.contiguous()
-                copies.append(x)
-                if not o.is_contiguous():
-                    late.append((o, torch.empty(o.shape, dtype=o.dtype, device=device)))
-                    o = late[-1][1]
+        if not o.is_contiguous() and not _dense(o):
+            place = (o.data_ptr(), o.shape, o.stride())
+            if place in gaps:
+                raise ValueError("tensors of the list overlap where they are written")
+            gaps.add(place)
+            x = x.contiguous()
+            late.append((o, x if same else torch.empty(o.shape, dtype=o.dtype, device=device)))
+            o = late[-1][1]
+        elif not same and not (x.is_contiguous() and o.is_contiguous()) and not (_dense(x) and x.stride() == o.stride()):
+            x = torch.empty_strided(o.shape, o.stride(), dtype=x.dtype, device=device).copy_(x.detach())
+        copies.append(x)  # alive until the launch
         values += (x.data_ptr(), o.data_ptr(), x.numel(), code, to)
         count += 1
     norm = _call("lamq_gradient_clip", values, count, device, float(max_norm), float(eps))

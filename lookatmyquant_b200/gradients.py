@@ -110,7 +110,7 @@ def clip(tensors, max_norm: float, out=None, eps: float = 1e-6) -> torch.Tensor:
                 raise ValueError(f"an output {tuple(o.shape)} for a gradient {tuple(x.shape)}")
         if not o.is_contiguous() and not _dense(o):
             place = (o.data_ptr(), o.shape, o.stride())
-            if place in gaps:
+            if place in gaps or any(n != 1 and step == 0 for n, step in zip(o.shape, o.stride())):
                 raise ValueError("tensors of the list overlap where they are written")
             gaps.add(place)
             x = x.contiguous()

@@ -53,3 +53,16 @@ def test_outputs_in_another_order_of_the_axes_are_seen_where_they_lie(G):
     assert float(out.abs().sum()) == 0
     G.clip(xs, 1.0, [out.t(), torch.zeros(3, 4)])
     assert torch.allclose(out, torch.full((3, 4), 60**-0.5), rtol=1e-5)
+
+
+def test_tensors_that_overlap_themselves_are_refused_before_anything_changes(G):
+    x, wide = torch.full((8,), 3.0), torch.ones(3, 1).expand(3, 4)
+    for call in (lambda: G.clip([x, wide], 1.0), lambda: G.clip([x, torch.ones(3, 4)], 1.0, [x, wide]),
+                 lambda: G.clip([x, torch.ones(2, 3)], 1.0, [x, torch.zeros(3).expand(2, 3)])):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+        assert bool((x == 3).all()) and bool((wide == 1).all())
+    G.clip([x, torch.ones(3, 1).expand(3, 1)], 1.0)  # one entry along the axis
+    out = torch.zeros(3, 4)
+    G.clip([wide], 1.0, [out])  # read only
+    assert torch.allclose(out, torch.full((3, 4), 12**-0.5), rtol=1e-5)

@@ -124,6 +124,6 @@ def clip(tensors, max_norm: float, out=None, eps: float = 1e-6) -> torch.Tensor:
     norm = _call("lamq_gradient_clip", values, count, device, float(max_norm), float(eps))
     torch.autograd.graph.increment_version([o for o in written if not o.is_inference()])
     for o, value in late:
-        with torch.no_grad():
+        with torch.inference_mode() if o.is_inference() else torch.no_grad():
             o.copy_(value)
     return norm

@@ -66,3 +66,14 @@ def test_tensors_that_overlap_themselves_are_refused_before_anything_changes(G):
     out = torch.zeros(3, 4)
     G.clip([wide], 1.0, [out])  # read only
     assert torch.allclose(out, torch.full((3, 4), 12**-0.5), rtol=1e-5)
+
+
+def test_views_of_inference_mode_are_written_outside_it(G):
+    with torch.inference_mode():
+        base = torch.full((4, 6), 2.0)
+        view = base[:, :3]
+    x = torch.full((5,), 1.0)
+    G.clip([x, view], 1.0)
+    norm = 53.0**0.5
+    assert torch.allclose(view, torch.full((4, 3), 2 / norm), rtol=1e-5) and bool((base[:, 3:] == 2).all())
+    assert torch.allclose(x, torch.full((5,), 1 / norm), rtol=1e-5)

@@ -26,6 +26,7 @@ from ._lib import NORM_ARGS, check, launch_on, ptr
 
 _DTYPES = {torch.float32: _lib.LAMQ_F32, torch.bfloat16: _lib.LAMQ_BF16}
 _NONE = (0, 1, 0, 0)  # the lamq_rows of no tensor
+_FAR = 1 << 29  # elements between the rows of a join that the library does not take
 PARAMETERS = ("weight", "post_weight", "gate")
 
 
@@ -50,7 +51,7 @@ def _rows(x: torch.Tensor, strides: int = 1):
                 axes[-1] = (axes[-1][0] * n, s)
             else:
                 axes.append((n, s))
-        if len(axes) <= 1:
+        if len(axes) <= 1 and (strides == 2 or not axes or axes[0][1] < _FAR):
             return x, (x.data_ptr(), 1 << 30, axes[0][1] if axes else d, 0)
         if len(axes) == 2 and strides == 2:
             return x, (x.data_ptr(), axes[1][0], axes[1][1], axes[0][1])

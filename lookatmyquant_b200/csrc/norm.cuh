@@ -551,6 +551,14 @@ __device__ __forceinline__ float unit_factor(Team<kSub> &team, Vec<E> &x, float 
     return reciprocal_root(fmaf(ss, inv_d, eps));
 }
 
+// Whether of a row's Σ h² and Σ t·h, taken of the row as it is, one may have lost something to fp32's range: past its end; or, of
+// rows so small that the factor passes 2^20, products of 2^-126 and less, which are rounded to multiples of 2^-149. (Of others
+// that is 2^-103 in the result at most: the mean of roundings of 2^-150, times the factor twice and ĥ <= 128.) Σ t·h is then taken
+// of the normed row: an exchange more, so not for all.
+__device__ __forceinline__ bool sums_lost(float hh, float th, float eps) {
+    return isinf(hh) || !(fabsf(th) <= 0x1p126f) || (eps < 0x1p-40f && hh < 0x1p-26f && fabsf(th) < 0x1p-60f);
+}
+
 // ---- the host's side
 
 // Which tensors a call has, and in the place of the others an output's memory of the same shape and no smaller a type: what

@@ -200,17 +200,21 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
         if constexpr (kFull) s[2] = b.dot(b);
         if (has_dy || post) team.sum(s);
         if (has_dy) {
-            float shrunk;
-            const float f = unit_factor(team, x, s[0], p.inv_d, p.eps, shrunk);
-            if (team.any(shrunk != 1.f)) {
-                float again[1] = {t.dot(x)};  // x changed, and the sum may have overflowed
-                team.sum(again);
-                s[1] = again[0];
+            float shrunk = 1.f, f, c;  // f: the factor of x as it stood, f · shrunk that of h
+            const bool lost = sums_lost(s[0], s[1], p.eps);
+            if (team.any(lost)) {
+                f = unit_factor(team, x, s[0], p.inv_d, p.eps, shrunk);
+                x *= f;
+                float unit[1] = {t.dot(x)};
+                team.sum(unit);
+                c = lost ? unit[0] : s[1] * f;
+            } else {
+                f = reciprocal_root(fmaf(s[0], p.inv_d, p.eps));
+                x *= f;
+                c = s[1] * f;
             }
-            // f is the factor of x as it stands, f · shrunk that of x as it was
-            x *= f;
             if (kSums) dw.add(g, x);
-            t.take(s[1] * f * p.inv_d, x, f * shrunk);
+            t.take(c * p.inv_d, x, f * shrunk);
             g = t;
         }
         if (has_dh) {

@@ -37,18 +37,20 @@ __global__ void __launch_bounds__(kWideThreads) norm_backward_wide_kernel(const 
             }
         });
         if (pre || post) wide_sum(s, scratch);
-        float f = 0.f, shrunk = 1.f, fb = 1.f, less = 1.f;
+        float f = 0.f, shrunk = 1.f, fb = 1.f, less = 1.f, c = 0.f;
         if (pre) {
             f = wide_factor(s[0], p.d, [&](int j) { return load_one(h + j); }, p.inv_d, p.eps, shrunk, scratch);
-            if (shrunk != 1.f) {  // that sum may have overflowed, too
-                float again[1] = {0.f};
-                wide_each(p.d, [&](int j) { again[0] = fmaf(load_one(dy + j) * weight(j), load_one(h + j) * shrunk, again[0]); });
-                wide_sum(again, scratch);
-                s[1] = again[0];
+            c = s[1] * f;
+            if (sums_lost(s[0], s[1], p.eps)) {
+                float unit[1] = {0.f};
+                wide_each(p.d, [&](int j) { unit[0] = fmaf(load_one(dy + j) * weight(j), load_one(h + j) * shrunk * f, unit[0]); });
+                wide_sum(unit, scratch);
+                c = unit[0];
             }
+            c *= p.inv_d;
         }
         if (post) fb = wide_factor(s[2], p.d, [&](int j) { return load_one(branch + j); }, p.inv_d, p.eps, less, scratch);
-        const float c = s[1] * f * p.inv_d, r = f * shrunk;
+        const float r = f * shrunk;
         const int gate_row = p.in.by_span.of(row);
         // a gate row is summed in the block's partial row, one that spans blocks in the pair's
         const bool begins = row == first || (p.gate_mode != kGateOne && row == gate_row * p.in.gate_span);

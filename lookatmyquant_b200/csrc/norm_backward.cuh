@@ -200,19 +200,17 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
         if constexpr (kFull) s[2] = b.dot(b);
         if (has_dy || post) team.sum(s);
         if (has_dy) {
-            float shrunk = 1.f, f, c;  // f: the factor of x as it stood, f · shrunk that of h
             const bool lost = sums_lost(s[0], s[1], p.eps);
+            float shrunk;
+            const float f = unit_factor(team, x, s[0], p.inv_d, p.eps, shrunk);  // of x as it stands; f · shrunk is that of h
+            float c = s[1] * f, by = f;
             if (team.any(lost)) {
-                f = unit_factor(team, x, s[0], p.inv_d, p.eps, shrunk);
-                x *= f;
+                x *= f, by = 1.f;
                 float unit[1] = {t.dot(x)};
                 team.sum(unit);
-                c = lost ? unit[0] : s[1] * f;
-            } else {
-                f = reciprocal_root(fmaf(s[0], p.inv_d, p.eps));
-                x *= f;
-                c = s[1] * f;
+                if (lost) c = unit[0];
             }
+            x *= by;
             if (kSums) dw.add(g, x);
             t.take(c * p.inv_d, x, f * shrunk);
             g = t;

@@ -34,7 +34,10 @@ typedef struct lamq_rows {
  * residual, h and their gradients have residual_dtype; branch, y and theirs branch_dtype; weight, post and gate types of
  * their own, which their gradients share. Types are LAMQ_F32 and LAMQ_BF16; a bf16 residual takes bf16 branches only.
  * All sums are fp32 and results are rounded once (y comes from the unrounded h). Outputs (h, y and the gradients) are
- * contiguous rows x d and overlap no input. 264 bytes, no padding (`reserved` is ignored).
+ * contiguous rows x d and overlap no input. Rows that do not begin and end on 16 bytes are
+ * read in the aligned 16-byte pieces that hold them: up to 14 bytes in front of a tensor's first row and behind its last come along,
+ * are not used, and may change meanwhile. A suballocator that lets tensors begin anywhere needs a pool of whole 16-byte pieces
+ * (cudaMalloc's are). 264 bytes, no padding (`reserved` is ignored).
  */
 typedef struct lamq_norm_args {
     int64_t rows, gate_span;

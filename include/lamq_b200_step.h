@@ -66,7 +66,7 @@ int lamq_norm_backward(const lamq_norm_args *args, void *workspace, size_t works
 
 /*
  * One tensor of a list: n contiguous elements of dtype (LAMQ_F32 or LAMQ_BF16), and where its clipped values go
- * (out_dtype; data itself, in its own type, to clip in place).
+ * (out_dtype; data itself, in its own type, to clip in place). 32 bytes, no padding.
  */
 typedef struct lamq_gradient {
     void *data, *out;

@@ -94,6 +94,9 @@ ATTENTION_ARGS = struct.Struct("=q4i2qfi2Q16qQ16q")
 # lamq_rows is a pointer, an inner count and two strides)
 NORM_ARGS = struct.Struct("=2q6i3fi8q5Q8q5Q")
 
+# lamq_gradient (32 bytes): data, out; n; dtype, out_dtype
+GRADIENT = struct.Struct("=2Qq2i")
+
 
 class ProductGroup(_c.Structure):
     """lamq_product_group: one packed row group of a grouped product (64 bytes, the header's field order)."""

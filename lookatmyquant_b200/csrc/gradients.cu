@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstddef>
 #include <cstdint>
 #include <new>
 #include <vector>
@@ -290,6 +291,9 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // ---- the host's side
+
+static_assert(sizeof(lamq_gradient) == 32 && offsetof(lamq_gradient, n) == 16 && offsetof(lamq_gradient, out_dtype) == 28,
+              "the bindings pack 32 bytes an entry");
 
 int64_t tiles_of(const lamq_gradient &g) {
     const int64_t size = kTileBytes / (g.dtype == LAMQ_BF16 ? 2 : 4);

@@ -7,6 +7,8 @@
 // the row's threads. Measured (us; bytes at 6551 GB/s in brackets): 262144 heads of 128 out of a wider projection, bf16, 28 (20);
 // a join with both norms, a gate for each text and an fp32 stream, 8192 x 2560, 57 (38). y is made from h in fp32, before h is rounded to its type: one rounding fewer than a norm that reads
 // the stored h.
+#include <cstddef>
+
 #include "norm_wide.cuh"
 
 namespace lamq {
@@ -229,6 +231,12 @@ int launch_forward(NormKernel kernel, const ForwardParams &p, int grid, int mode
 }
 
 }  // namespace
+
+static_assert(sizeof(lamq_norm_args) == 264 && sizeof(lamq_rows) == 32, "the bindings pack 264 bytes");
+static_assert(offsetof(lamq_norm_args, d) == 16 && offsetof(lamq_norm_args, scale) == 40 && offsetof(lamq_norm_args, residual) == 56 &&
+                  offsetof(lamq_norm_args, weight) == 120 && offsetof(lamq_norm_args, dh) == 160 &&
+                  offsetof(lamq_norm_args, d_residual) == 224,
+              "the header's field order, without padding");
 
 int norm_args_status(const lamq_norm_args *a, bool backward) {
     LAMQ_REQUIRE(a, "null pointer (args)");

@@ -57,7 +57,7 @@ def _call(name, values, count, device, *rest):
     """A C call over `count` tensors, whose `values` are (pointer, pointer of the output, elements, type, type of the output)
     one behind the other. The norm."""
     lib = _lib.load()
-    table = struct.pack("=" + "2Qq2i" * count, *values)
+    table = struct.pack("=" + _lib.GRADIENT.format[1:] * count, *values)
     norm = torch.empty_strided((), (), dtype=torch.float32, device=device)
     size = lib.lamq_gradient_workspace_size(count)
     ws = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=device)

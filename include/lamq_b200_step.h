@@ -34,10 +34,10 @@ typedef struct lamq_rows {
  * residual, h and their gradients have residual_dtype; branch, y and theirs branch_dtype; weight, post and gate types of
  * their own, which their gradients share. Types are LAMQ_F32 and LAMQ_BF16; a bf16 residual takes bf16 branches only.
  * All sums are fp32 and results are rounded once (y comes from the unrounded h). Outputs (h, y and the gradients) are
- * contiguous rows x d and overlap no input. Rows that do not begin and end on 16 bytes are
- * read in the aligned 16-byte pieces that hold them: up to 14 bytes in front of a tensor's first row and behind its last come along,
- * are not used, and may change meanwhile. A suballocator that lets tensors begin anywhere needs a pool of whole 16-byte pieces
- * (cudaMalloc's are). 264 bytes, no padding (`reserved` is ignored).
+ * contiguous rows x d and overlap no input. Rows that do not begin and end on 16 bytes are read in the aligned 16-byte pieces that
+ * hold them: up to 14 bytes in front of a tensor's first row and behind its last come along, are not used, and may change
+ * meanwhile. A suballocator that lets tensors begin anywhere needs a pool of whole 16-byte pieces (cudaMalloc's are).
+ * 264 bytes, no padding (`reserved` is ignored).
  */
 typedef struct lamq_norm_args {
     int64_t rows, gate_span;
@@ -51,13 +51,15 @@ typedef struct lamq_norm_args {
     void *d_residual, *d_branch, *d_weight, *d_post, *d_gate;
 } lamq_norm_args;
 
-/* Writes h and y; nothing where there are no rows or no elements. `args` is host memory, read before the call returns (here and below). */
+/* Writes h and y; nothing where there are no rows or no elements. `args` is host memory, read before the call returns (here and
+ * below). */
 int lamq_norm_forward(const lamq_norm_args *args, lamq_stream_t stream);
 
 /*
- * The gradients, from dh and dy (data NULL: zero; the norm alone has a dy) and from `residual`, which here holds the forward's h (the norm alone:
- * its input), the statistics being computed again. d_residual is always written; d_branch (NULL: not wanted, as where it
- * equals d_residual), d_weight, d_post and d_gate where they are not NULL. The gradient of a weight or of a shared gate is
+ * The gradients, from dh and dy (data NULL: zero; the norm alone has a dy) and from `residual`, which here holds the forward's
+ * h (the norm alone: its input), the statistics being computed again. d_residual is always written (whoever wants the others alone
+ * pays for it, too); d_branch (NULL: not wanted, as where it equals d_residual), d_weight, d_post and d_gate where they are not
+ * NULL. The gradient of a weight or of a shared gate is
  * summed in fp32 in a fixed order: equal calls give equal bits. Workspace: lamq_norm_backward_workspace_size(args) bytes,
  * 32-byte aligned (0 where no such sum is wanted).
  */

@@ -5,8 +5,8 @@
 //
 // and N(x; w) alone. Bound by memory: each row is read once into registers and written once; a norm is one exchange among
 // the row's threads. Measured (us; bytes at 6551 GB/s in brackets): 262144 heads of 128 out of a wider projection, bf16, 28 (20);
-// a join with both norms, a gate for each text and an fp32 stream, 8192 x 2560, 57 (38). y is made from h in fp32, before h is rounded to its type: one rounding fewer than a norm that reads
-// the stored h.
+// a join with both norms, a gate for each text and an fp32 stream, 8192 x 2560, 57 (38); a plain join, 16384 x 2560 bf16 62 (51).
+// y is made from h in fp32, before h is rounded to its type: one rounding fewer than a norm that reads the stored h.
 #include <cstddef>
 
 #include "norm_wide.cuh"

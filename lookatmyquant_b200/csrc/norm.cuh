@@ -7,7 +7,8 @@
 // are on their way to shared memory meanwhile. Blocks stay on their SM and take row after row.
 //
 // Bound by memory in principle; what is reached is the rate of instructions and the latency of a row's two or three exchanges
-// (about half of the issue slots are used at 14 to 16 warps an SM, DRAM 36 to 54 %): see the kernels for the times.
+// (the profiled kernels issue 1.05 to 2.0 of 4 instructions a cycle at 11 to 16 warps an SM, DRAM at 27 to 54 %): see the kernels
+// for the times.
 #pragma once
 
 #include <algorithm>
@@ -53,9 +54,10 @@ constexpr int kSMs = 148;
 
 // ---- loads
 //
-// As volatile assembly: the compiler runs none of them where the source does not. (With plain __ldg loads behind a test of their
-// pointer, kernels faulted in calls where it was NULL, though the source then reads nothing; with these they do not.) Absent
-// tensors have a pointer that may be read, too (the host's `present`).
+// As volatile assembly, which the compiler runs only where the source does. What was seen: earlier kernels, with plain loads and
+// __ldg behind a test of their pointer, faulted in two calls where tensors were absent (NULL), though the source then reads none
+// of them; which load it was, and why, was not found. Since then all loads are these, absent tensors have a pointer that may be
+// read (the host's `present`), and the kernels were written anew; every load of an absent tensor stands behind its flag.
 
 __device__ __forceinline__ uint4 load16(const void *p) {
     uint4 v;
@@ -74,9 +76,6 @@ __device__ __forceinline__ float load_one(const __nv_bfloat16 *p) {
     asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(v) : "l"(p));
     return __uint_as_float((uint32_t)v << 16);
 }
-
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 // ---- V elements of T: 16 bytes (bf16) or 32 (fp32) where V is 8, one element where rows may begin anywhere
 
@@ -563,7 +562,7 @@ __device__ __forceinline__ bool sums_lost(float hh, float th, float eps) {
 
 // Which tensors a call has, and in the place of the others an output's memory of the same shape and no smaller a type: what
 // a kernel gets may be read whether or not it is there.
-enum { kHasWeight = 1, kHasPost = 2, kHasGate = 4, kHasDh = 8, kHasDy = 16, kHasBranch = 32 };
+enum { kHasWeight = 1, kHasPost = 2, kHasGate = 4, kHasDh = 8, kHasDy = 16 };
 
 struct Present {
     int has;
@@ -593,7 +592,7 @@ inline Present present(const lamq_norm_args &a, bool backward) {
     const int r = element_size(a.residual_dtype), b = element_size(a.branch_dtype);
     Present p;
     p.has = (a.weight ? kHasWeight : 0) | (a.post ? kHasPost : 0) | (a.gate ? kHasGate : 0) |
-            (a.branch.data ? kHasBranch : 0) | (backward && a.dh.data ? kHasDh : 0) | (backward && a.dy.data ? kHasDy : 0);
+            (backward && a.dh.data ? kHasDh : 0) | (backward && a.dy.data ? kHasDy : 0);
     p.h = rows_of(a.residual, a.rows, r);
     p.branch = rows_of(a.branch.data ? a.branch : rows, a.rows, b);
     p.dh = rows_of(p.has & kHasDh ? a.dh : rows, a.rows, r);
@@ -615,10 +614,11 @@ struct NormShape {
     NormKernel kernel;
 };
 
-// Vectors where every row begins on 16 bytes and every array on 32, elements elsewhere. A thread holds 16 elements of a row: what it
-// does for a row beside the arithmetic (places, waits, exchanges) costs as much as the arithmetic of 16 (16384 x 2560, the norm's
-// backward, us: 78 with 8, 61 with 16; the forward of a join with both norms takes the same with either). The full join's backward holds three sums and three tensors of a row: 8 of each (8192 x
-// 4096: 152 with 8 and 16 warps an SM, 189 with 16 and 8 warps). Up to 32 threads a team is a power of two of lanes, else whole
+// Vectors where every row begins on 16 bytes and every array on 32, elements elsewhere. A thread holds 16 elements of a row:
+// what it does for a row beside the arithmetic (places, waits, exchanges) costs as much as the arithmetic of 16 (16384 x 2560,
+// the norm's backward, us: 78 with 8, 61 with 16; the forward of a join with both norms takes the same with either). The full
+// join's backward holds three sums and three tensors of a row: 8 of each (8192 x 4096: 152 with 8 and 16 warps an SM, 189 with
+// 16 and 8 warps). Up to 32 threads a team is a power of two of lanes, else whole
 // warps. Wider rows take teams of up to 512 threads with 16 elements, then with 32; rows wider than 4096 that may begin
 // anywhere, a block each.
 inline NormShape norm_shape(const lamq_norm_args &a, bool backward) {
@@ -675,8 +675,10 @@ struct NormLayout {
 constexpr int kSmemSM = 220 * 1024;  // of 228 KB; each block takes 1 KB for itself
 
 // `gate_sums`: the gradient of the gate is wanted; `sums`: that of any parameter. Blocks are as many as their registers allow, or
-// as have room for two stages each; stages fill the room, four at most. What finds no room (rows that begin anywhere: for two
-// stages) is left to the wide kernels. More blocks with fewer registers are slower: the norm's backward of 16384 x 2560 at 96
+// as have room for two stages each; stages fill the room, four at most (a block alone on its SM may have one). What finds no
+// room (rows that begin anywhere: for two stages) is left to the wide kernels: the full join's backward of fp32 rows from 7688
+// elements on with parameters' gradients (from 6664 with a gate in fp32 for each element), the plain join's from 13320 (of an
+// fp32 stream with bf16 branches, 15368). More blocks with fewer registers are slower: the norm's backward of 16384 x 2560 at 96
 // registers, 4 blocks of 160 threads, 93 us against 55 at 122, 3 blocks (what spills, and one stage less).
 inline NormLayout norm_layout(const lamq_norm_args &a, bool backward, bool sums, bool gate_sums) {
     NormLayout l{};

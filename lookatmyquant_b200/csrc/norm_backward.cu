@@ -54,7 +54,7 @@ struct ReduceParams {
     void *d_weight, *d_post, *d_gate;
     int weight_dtype, post_dtype, gate_dtype;
     int d, columns, grid;
-    int gate_one, gate_span, per, rows;
+    int gate_one, gate_span, per;
 };
 
 constexpr int kReduceWarps = 32;
@@ -149,7 +149,7 @@ extern "C" int lamq_norm_backward(const lamq_norm_args *a, void *workspace, size
     sum.d_weight = a->d_weight, sum.d_post = a->d_post, sum.d_gate = gates ? a->d_gate : nullptr;
     sum.weight_dtype = a->weight_dtype, sum.post_dtype = a->post_dtype, sum.gate_dtype = a->gate_dtype;
     sum.d = a->d, sum.columns = q.columns, sum.grid = q.grid;
-    sum.gate_one = q.gate_mode == kGateOne, sum.gate_span = p.in.gate_span, sum.per = q.per, sum.rows = p.rows;
+    sum.gate_one = q.gate_mode == kGateOne, sum.gate_span = p.in.gate_span, sum.per = q.per;
     const int64_t jobs = (a->d_weight ? 1 : 0) + (a->d_post ? 1 : 0) +
                          (q.gate_mode == kGateOne ? 1 : q.gate_mode == kGateAcross ? a->rows / a->gate_span : 0);
     if (jobs == 0) return LAMQ_OK;

@@ -1,5 +1,5 @@
-// Rows of more elements than the teams' registers hold, where they may begin anywhere, and the full join's backward of more than
-// 8192: a block for each row, its threads taking every 1024th element. What a later pass needs of a row stays in shared memory as
+// Rows of more elements than the teams' registers hold, where they may begin anywhere, the full join's backward of more than
+// 8192, and what finds no room for its stages (norm_layout): a block for each row, its threads taking every 1024th element. What a later pass needs of a row stays in shared memory as
 // fp32; each thread reads there what it wrote itself. Sums over rows are added up in the block's partial row, each column by the
 // thread that owns it. Bound by the latency of the passes over a row (three in the join's forward, three in its backward).
 #pragma once

@@ -103,8 +103,7 @@ def clip(tensors, max_norm: float, out=None, eps: float = 1e-6) -> torch.Tensor:
             continue
         code = to = _code(x, index, device, "gradients")
         written.append(o)
-        same = o is x
-        if not same:
+        if o is not x:
             to = _code(o, index, device, "outputs")
             if o.shape != x.shape:
                 raise ValueError(f"an output {tuple(o.shape)} for a gradient {tuple(x.shape)}")
@@ -113,12 +112,12 @@ def clip(tensors, max_norm: float, out=None, eps: float = 1e-6) -> torch.Tensor:
             if place in gaps or any(n != 1 and step == 0 for n, step in zip(o.shape, o.stride())):
                 raise ValueError("tensors of the list overlap where they are written")
             gaps.add(place)
-            x = x.contiguous()
-            late.append((o, x if same else torch.empty(o.shape, dtype=o.dtype, device=device)))
-            o = late[-1][1]
-        elif not same and not (x.is_contiguous() and o.is_contiguous()) and not (_dense(x) and x.stride() == o.stride()):
+            copies.append(x.contiguous())  # alive until the launch
+            late.append((o, copies[-1] if o is x else torch.empty(o.shape, dtype=o.dtype, device=device)))
+            x, o = copies[-1], late[-1][1]
+        elif o is not x and not (x.is_contiguous() and o.is_contiguous()) and not (_dense(x) and x.stride() == o.stride()):
             x = torch.empty_strided(o.shape, o.stride(), dtype=x.dtype, device=device).copy_(x.detach())
-        copies.append(x)  # alive until the launch
+            copies.append(x)
         values += (x.data_ptr(), o.data_ptr(), x.numel(), code, to)
         count += 1
     norm = _call("lamq_gradient_clip", values, count, device, float(max_norm), float(eps))

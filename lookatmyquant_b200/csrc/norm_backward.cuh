@@ -9,8 +9,8 @@
 // kept from the forward. The sums over rows stay in the registers of the threads that own the columns: a worker (a team)
 // takes the rows of one range, blocks write one partial row each, and a second kernel adds the partials in order.
 //
-// Measured (us; bytes at 6551 GB/s in brackets): the norm alone, 16384 x 2560 bf16 55 (38); a plain join of that size 62 (51); a
-// join with both norms and a gate for all, 8192 x 4096 bf16 127 (62): 520 instructions a warp and row of 8 elements a thread at
+// Measured (us; bytes at 6551 GB/s in brackets): the norm alone, 16384 x 2560 bf16 53 (38); a plain join of that size 63 (51); a
+// join with both norms and a gate for all, 8192 x 4096 bf16 125 (62): 520 instructions a warp and row of 8 elements a thread at
 // 2.0 a cycle, 122 registers, 16 warps; the same with a gate of its own for each element, 3335 x 1337 fp32, rows that begin anywhere, 55 (22).
 #pragma once
 
@@ -201,10 +201,10 @@ __global__ void __launch_bounds__(resident(kKernel, kMode, true), 1)
         if (has_dy || post) team.sum(s);
         if (has_dy) {
             const bool lost = sums_lost(s[0], s[1], p.eps);
-            float shrunk;
-            const float f = unit_factor(team, x, s[0], p.inv_d, p.eps, shrunk);  // of x as it stands; f · shrunk is that of h
-            float c = s[1] * f, by = f;
+            // f: the factor of x as it stands, f · shrunk that of h
+            float shrunk = 1.f, f = reciprocal_root(fmaf(s[0], p.inv_d, p.eps)), c = s[1] * f, by = f;
             if (team.any(lost)) {
+                f = unit_factor(team, x, s[0], p.inv_d, p.eps, shrunk);
                 x *= f, by = 1.f;
                 float unit[1] = {t.dot(x)};
                 team.sum(unit);

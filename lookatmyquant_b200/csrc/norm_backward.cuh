@@ -11,7 +11,8 @@
 //
 // Measured (us; bytes at 6551 GB/s in brackets): the norm alone, 16384 x 2560 bf16 53 (38); a plain join of that size 63 (51); a
 // join with both norms and a gate for all, 8192 x 4096 bf16 125 (62): 520 instructions a warp and row of 8 elements a thread at
-// 2.0 a cycle, 122 registers, 16 warps; the same with a gate of its own for each element, 3335 x 1337 fp32, rows that begin anywhere, 55 (22).
+// 2.0 a cycle, 122 registers, 16 warps; the same with a gate of its own for each element, 3335 x 1337 fp32, rows that begin
+// anywhere, 55 (22).
 #pragma once
 
 #include "dependent.cuh"

@@ -94,8 +94,9 @@ def _is_rms(cls, forward) -> bool:
     try:
         module = cls.__new__(cls)
         torch.nn.Module.__init__(module)
-        x = torch.tensor([[1.0, -2.0, 0.5, 3.0], [0.25, 0.5, -0.125, 0.0625]], device="cpu")
-        w = torch.tensor([0.5, -2.0, 3.0, 1.25], device="cpu")
+        host = {"dtype": torch.float32, "device": "cpu"}
+        x = torch.tensor([[1.0, -2.0, 0.5, 3.0], [0.25, 0.5, -0.125, 0.0625]], **host)
+        w = torch.tensor([0.5, -2.0, 3.0, 1.25], **host)
         module.weight, module.variance_epsilon = torch.nn.Parameter(w, requires_grad=False), 0.25
         with torch.no_grad():
             got = forward(module, x)
@@ -206,8 +207,8 @@ class _Layer:
     def __getattr__(self, name):
         return getattr(self._layer, name)
 
-    def __call__(self, x, *args, **kwargs):
-        stream = x if isinstance(x, _Stream) else _Stream(x)
+    def __call__(self, hidden_states, *args, **kwargs):
+        stream = hidden_states if isinstance(hidden_states, _Stream) else _Stream(hidden_states)
         for step in _steps(self._layer, args, kwargs):
             y = stream.normed(step.norm)
             stream.branch, stream.step = step.run(y), step

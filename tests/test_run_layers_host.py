@@ -85,6 +85,36 @@ def test_the_model_is_left_as_it_was(N):
     assert before == {n: id(m) for n, m in model.named_modules()} and keys == [set(vars(m)) for m in model.modules()]
 
 
+def test_a_default_type_changes_no_norm(N):
+    """A class's formula is found out once, in fp32 whatever torch's default is then."""
+    from lookatmyquant_b200 import decoder
+    decoder._is_rms.cache_clear()
+    model, x = build("Llama"), torch.randn(1, 5, 32)
+    want = model.model(inputs_embeds=x, use_cache=False).last_hidden_state
+    torch.set_default_dtype(torch.bfloat16)
+    try:
+        got = N.run_layers(model, x)
+    finally:
+        torch.set_default_dtype(torch.float32)
+        decoder._is_rms.cache_clear()
+    assert torch.equal(got, want)
+
+
+def test_a_model_may_name_the_states(N):
+    model = build("Llama")
+
+    class Named(type(model.model)):
+        def forward(self, inputs_embeds=None, use_cache=None):
+            h = inputs_embeds
+            kw = dict(attention_mask=None, position_embeddings=self.rotary_emb(h, torch.arange(h.shape[1])[None]))
+            for layer in self.layers:
+                h = layer(hidden_states=h, **kw)
+            return transformers.modeling_outputs.BaseModelOutputWithPast(last_hidden_state=self.norm(h))
+    model.model.__class__ = Named
+    x = torch.randn(2, 5, 32)
+    assert torch.equal(N.run_layers(model, x), model.model(inputs_embeds=x).last_hidden_state)
+
+
 def test_hooks_of_what_still_runs_are_called(N):
     model, seen = build("Llama"), []
     for n, m in model.named_modules():

@@ -30,3 +30,17 @@ def test_what_lies_beside_a_tensor(N, d, dtype):  # noqa: F811
                             N.norm_forward(x, w), *N.norm_backward(b, x, w)))
         for a, c in zip(*results):
             assert a is None and c is None or torch.equal(a, c) and bool(a.isfinite().all())
+
+
+def test_rows_far_apart(N):  # noqa: F811
+    """The last tokens of two long texts: rows 2^29 + 64 elements apart, in place in the norm, through a copy in a join."""
+    stride = 2**29 + 64
+    base = torch.empty(stride + 64, dtype=BF, device="cuda")
+    x = torch.as_strided(base, (2, 64), (stride, 1))
+    x.copy_(values(generator(1), 2, 64))
+    w = values(generator(2), 64, dtype=BF)
+    near = x.contiguous()
+    assert torch.equal(N.norm_forward(x, w), N.norm_forward(near, w))
+    for a, b in zip((*N.join_forward(x, x, w), *N.join_backward(x, x, x, x, w), *N.norm_backward(x, x, w)),
+                    (*N.join_forward(near, near, w), *N.join_backward(near, near, near, near, w), *N.norm_backward(near, near, w))):
+        assert a is None and b is None or torch.equal(a, b)
